@@ -399,6 +399,80 @@ typedef struct gs_adam_group {
 int gs_adam_step(const gs_adam_group* groups, int n_groups, double beta1, double beta2, float eps,
                  int bias_correction, int64_t step, void* stream);
 
+/* ---------------------------------------------------------------------
+ * Feature fields: class logits distilled from a 2D network.  No counterpart
+ * in the reference, which composites arbitrary per-Gaussian features
+ * (src/mlx3d/splatting/rasterize.py:449-545) and leaves their training to
+ * the caller.
+ *
+ * Element types of the tensors below. */
+#define GS_F32 0
+#define GS_F16 1
+#define GS_BF16 2
+
+/* A teacher's largest logits of n rows (pixels), either as two arrays or as
+ * rows of a teacher cache (gs_teacher_write):
+ *   arrays:  values (n, k) of values_dtype, index (n, k) int32
+ *   cache:   records (n_records records of gs_teacher_record_bytes(k, bits)
+ *            bytes, 16-byte aligned), row r of the call is record rows[r]
+ *            (int64, device), or first_row + r where rows is NULL.
+ * An entry is absent if its index is outside [0, classes) or its value is
+ * -inf; a row outside [0, n_records) has no entries. */
+typedef struct gs_teacher {
+  const void* values;
+  const int32_t* index;
+  const void* records;
+  const int64_t* rows;
+  int64_t first_row;
+  int64_t n_records;
+  int32_t values_dtype;
+  int32_t k;    /* 1 .. GS_TEACHER_MAX_K (arrays), 1 .. GS_CACHE_MAX_K (cache) */
+  int32_t bits; /* 8 or 4: cache; 0: arrays */
+} gs_teacher;
+#define GS_TEACHER_MAX_K 256
+#define GS_CACHE_MAX_K 32
+#define GS_CACHE_MAX_CLASSES 32767
+
+/* Distillation from a teacher's largest logits.  Row r of the student's
+ * logits s (n, classes), contiguous, of type dtype, and its present teacher
+ * entries (z_k, i_k):
+ *   p = softmax_k(z / T), q = softmax(s / T) over all classes
+ *   L = weight T^2 sum_k p_k (log p_k - log q_{i_k})
+ *   dL/ds_c = weight T (q_c - sum_{k: i_k = c} p_k)
+ * (0 log 0 = 0; a row without entries has L = 0 and gradient 0; weight (n) or
+ * NULL for 1.)  Writes what is not NULL of
+ *   row_loss (n)   L
+ *   loss     (1)   scale * sum L, summed in a fixed order in 64 bits
+ *   grad     (n, classes) of type dtype: g * scale * dL/ds, with g = 1 if
+ *            cotangent is NULL, cotangent[r] if cotangent_per_row, else
+ *            cotangent[0] (device float).
+ * workspace (gs_distill_workspace_bytes()) is needed only for loss. */
+size_t gs_distill_workspace_bytes(void);
+int gs_distill(const void* logits, int dtype, int64_t n, int64_t classes, const gs_teacher* teacher,
+               float temperature, const float* weight, double scale, const float* cotangent,
+               int cotangent_per_row, float* row_loss, float* loss, void* grad, void* workspace,
+               size_t workspace_bytes, void* stream);
+
+/* Teacher cache: one record per row (pixel), holding the k largest usable
+ * logits of the row in 8 or 4 bits:
+ *   float offset (the largest), float scale, int16 index[k] (-1: absent),
+ *   k codes of `bits` bits (low nibble first), padding to 16 bytes;
+ *   value_k = offset - code_k * scale.
+ * gs_teacher_write fills records [first_row, first_row + n) from logits
+ * (n, classes), contiguous, of type dtype: the largest first, ties to the
+ * lowest index; +-inf, NaN and the type's lowest value are never taken.
+ *   scale = (z_1 - z_last) / (2^bits - 1), code_k = the quotient
+ *   (2^bits - 1) (z_1 - z_k) / (z_1 - z_last) rounded to nearest, ties to
+ *   even (the quotient of the exact differences).
+ * gs_teacher_read writes values (n, k) float (-inf where absent) and index
+ * (n, k) int32 (-1 where absent) of the records rows[r], or first_row + r
+ * where rows is NULL; a row outside [0, n_records) reads as all absent. */
+size_t gs_teacher_record_bytes(int k, int bits);
+int gs_teacher_write(const void* logits, int dtype, int64_t n, int64_t classes, void* records,
+                     int64_t n_records, int64_t first_row, int k, int bits, void* stream);
+int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows, int64_t first_row, int64_t n,
+                    int k, int bits, float* values, int32_t* index, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

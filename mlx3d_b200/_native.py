@@ -68,6 +68,29 @@ class GsAdamGroup(ctypes.Structure):
 
 GS_ADAM_MAX_GROUPS = 8
 
+# Element types of the feature-field entry points.
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+GS_TEACHER_MAX_K = 256
+GS_CACHE_MAX_K = 32
+GS_CACHE_MAX_CLASSES = 32767
+
+
+class GsTeacher(ctypes.Structure):
+    """Mirror of ``gs_teacher`` in include/gsplat_b200.h."""
+
+    _fields_ = [
+        ("values", c_void_p),
+        ("index", c_void_p),
+        ("records", c_void_p),
+        ("rows", c_void_p),
+        ("first_row", c_int64),
+        ("n_records", c_int64),
+        ("values_dtype", c_int32),
+        ("k", c_int32),
+        ("bits", c_int32),
+    ]
+
+
 # name -> (restype, argtypes)
 _P = c_void_p
 _SIGS = {
@@ -149,6 +172,15 @@ _SIGS = {
     "gs_l1_forward": (c_int, [_P, _P, c_int64, _P, c_size_t, _P, _P]),
     "gs_l1_backward": (c_int, [_P, _P, c_int64, _P, _P, _P]),
     "gs_adam_step": (c_int, [POINTER(GsAdamGroup), c_int, ctypes.c_double, ctypes.c_double, c_float, c_int, c_int64, _P]),
+    "gs_distill_workspace_bytes": (c_size_t, []),
+    "gs_distill": (
+        c_int,
+        [_P, c_int, c_int64, c_int64, POINTER(GsTeacher), c_float, _P, ctypes.c_double, _P, c_int, _P, _P, _P, _P,
+         c_size_t, _P],
+    ),
+    "gs_teacher_record_bytes": (c_size_t, [c_int, c_int]),
+    "gs_teacher_write": (c_int, [_P, c_int, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int, _P]),
+    "gs_teacher_read": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int, c_int, _P, _P, _P]),
     "gs_rasterize_forward": (
         c_int,
         [_P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P],
@@ -196,6 +228,16 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed (status {status}): {msg}")
 
 
+def call_on(device: torch.device, name: str, *args) -> None:
+    """:func:`call` on ``device`` (which need not be the current one), with
+    that device's current stream as the last argument."""
+    if device.index == torch.cuda.current_device():
+        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -215,6 +257,22 @@ def require_cuda(name: str, t: torch.Tensor, dtype=torch.float32) -> torch.Tenso
     if t.dtype != dtype:
         t = t.to(dtype)
     return t.contiguous()
+
+
+def require_float(name: str, t: torch.Tensor) -> torch.Tensor:
+    """Return ``t`` as a contiguous CUDA tensor of float32, float16 or
+    bfloat16, kept in its type (other floating types become float32)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_floating_point():
+        raise TypeError(f"{name} must be a floating-point tensor (got {t.dtype})")
+    return require_cuda(name, t, t.dtype if t.dtype in DTYPES else torch.float32)
+
+
+def same_device(device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} must be on {device} (got {t.device})")
 
 
 class _CudaArray:

@@ -5,15 +5,24 @@
 five windowed statistics, the SSIM and L1 sums, one backward kernel for the
 gradient of both terms.  ``l1_loss`` runs on ``gs_l1_forward`` /
 ``gs_l1_backward``; ``psnr`` is a one-line reduction.
+
+``distill_loss`` (an addition to the reference's losses) trains rendered or
+decoded class logits against a 2D teacher's largest logits, given as arrays
+or kept in a :class:`~mlx3d_b200.staging.TeacherCache`, on ``gs_distill``.
 """
 
 from __future__ import annotations
 
+import ctypes
+import math
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
+from .staging import TeacherRows
 
-__all__ = ["ssim", "l1_loss", "psnr", "l1_dssim_loss"]
+__all__ = ["ssim", "l1_loss", "psnr", "l1_dssim_loss", "distill_loss", "distill_loss_and_grad"]
 
 
 def _prep(pred, target):
@@ -115,3 +124,130 @@ def l1_loss(pred: torch.Tensor, target: torch.Tensor) -> torch.Tensor:
 def psnr(pred: torch.Tensor, target: torch.Tensor, max_val: float = 1.0) -> torch.Tensor:
     mse = ((pred - target) ** 2).mean()
     return 10.0 * torch.log10((max_val * max_val) / torch.clamp(mse, min=1e-12))
+
+
+class _DistillArgs:
+    """Checked arguments of one distillation call; keeps the tensors alive."""
+
+    def __init__(self, logits, teacher, temperature, weight, reduction):
+        if reduction not in ("mean", "sum", "none"):
+            raise ValueError("reduction must be 'mean', 'sum' or 'none'.")
+        temperature = float(temperature)
+        if not (temperature > 0.0 and math.isfinite(temperature)):
+            raise ValueError("temperature must be positive and finite.")
+        if not isinstance(logits, torch.Tensor) or logits.ndim < 1 or logits.shape[-1] < 1:
+            raise ValueError("logits must have shape (..., C) with C >= 1.")
+        lead = logits.shape[:-1]
+        self.rows = math.prod(lead)
+        if reduction == "mean" and self.rows == 0:
+            raise ValueError("reduction='mean' needs at least one row of logits.")
+        self.records = self.row_ids = self.values = self.index = None
+        if isinstance(teacher, TeacherRows):
+            if teacher.count != self.rows:
+                raise ValueError(f"teacher has {teacher.count} rows, logits {self.rows}.")
+            if teacher.cache.num_classes != logits.shape[-1]:
+                raise ValueError(f"the teacher cache holds {teacher.cache.num_classes} classes, "
+                                 f"logits have {logits.shape[-1]}.")
+        elif isinstance(teacher, (tuple, list)) and len(teacher) == 2:
+            values, index = teacher
+            if not isinstance(values, torch.Tensor) or not isinstance(index, torch.Tensor):
+                raise TypeError("teacher must be (values, index) tensors or TeacherCache.at(rows).")
+            if values.ndim != logits.ndim or values.shape[:-1] != lead or values.shape != index.shape:
+                raise ValueError("teacher values and index must both have shape (..., K) with the logits' rows.")
+            if not 1 <= values.shape[-1] <= nat.GS_TEACHER_MAX_K:
+                raise ValueError(f"the teacher must have 1 to {nat.GS_TEACHER_MAX_K} entries a row.")
+            if index.dtype not in (torch.int32, torch.int64, torch.int16):
+                raise TypeError("teacher index must be int16, int32 or int64.")
+        else:
+            raise TypeError("teacher must be (values, index) tensors or TeacherCache.at(rows).")
+        if weight is not None and (not isinstance(weight, torch.Tensor) or weight.shape != lead):
+            raise ValueError("weight must have the shape of the logits' rows.")
+        logits = nat.require_float("logits", logits)
+        dev = logits.device
+        if isinstance(teacher, TeacherRows):
+            cache = teacher.cache
+            self.records, self.row_ids = cache.records, teacher.rows
+            self.native = nat.GsTeacher(None, None, cache.records.data_ptr(), nat.ptr(teacher.rows), teacher.first,
+                                        cache.num_rows, 0, cache.k, cache.bits)
+        else:
+            self.values = nat.require_float("teacher values", teacher[0].detach())
+            index = teacher[1]
+            if index.dtype == torch.int64:  # out of int32's range is out of the classes' range
+                index = index.clamp(-1, 2**31 - 1)
+            self.index = nat.require_cuda("teacher index", index, torch.int32)
+            self.native = nat.GsTeacher(self.values.data_ptr(), self.index.data_ptr(), None, None, 0, 0,
+                                        nat.DTYPES[self.values.dtype], self.values.shape[-1], 0)
+        self.weight = None if weight is None else nat.require_cuda("weight", weight.detach())
+        nat.same_device(dev, **{"teacher values": self.values, "teacher index": self.index,
+                                "the teacher cache": self.records, "teacher rows": self.row_ids,
+                                "weight": self.weight})
+        self.logits = logits
+        self.lead = lead
+        self.temperature = temperature
+        self.reduction = reduction
+        self.scale = 1.0 / self.rows if reduction == "mean" else 1.0
+
+    def run(self, logits, want_loss=True, grad=None, cotangent=None):
+        """One launch: the loss (row losses for 'none') and / or the gradient into ``grad``."""
+        dev = logits.device
+        row_loss = loss = ws = None
+        if want_loss:
+            if self.reduction == "none":
+                row_loss = torch.empty(self.lead, device=dev, dtype=torch.float32)
+            else:
+                loss = torch.empty((), device=dev, dtype=torch.float32)
+                ws = torch.empty((nat.load().gs_distill_workspace_bytes(),), device=dev, dtype=torch.uint8)
+        nat.call_on(dev, "gs_distill", nat.ptr(logits), nat.DTYPES[logits.dtype], self.rows, logits.shape[-1],
+                    ctypes.byref(self.native), self.temperature, nat.ptr(self.weight), self.scale,
+                    nat.ptr(cotangent), int(self.reduction == "none"), nat.ptr(row_loss), nat.ptr(loss),
+                    nat.ptr(grad), nat.ptr(ws), 0 if ws is None else ws.numel())
+        return row_loss if self.reduction == "none" else loss
+
+
+class _Distill(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, args):
+        ctx.args = args
+        ctx.save_for_backward(logits, args.records, args.row_ids, args.values, args.index, args.weight)
+        args.logits = None  # saved above
+        return args.run(logits)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        logits = ctx.saved_tensors[0]
+        grad = torch.empty_like(logits)
+        ctx.args.run(logits, want_loss=False, grad=grad, cotangent=g.to(torch.float32).contiguous())
+        return grad, None
+
+
+def distill_loss(logits: torch.Tensor, teacher, temperature: float = 1.0, weight: torch.Tensor | None = None,
+                 reduction: str = "mean") -> torch.Tensor:
+    """Distillation from a teacher's largest logits; differentiable in ``logits``.
+
+    ``logits`` (..., C), float32, float16 or bfloat16: class logits of rendered pixels (for instance
+    ``render_features(...)["logits"]``).  ``teacher`` is ``(values, index)``, both (..., K) with K <= 256, or
+    ``TeacherCache.at(rows)``.  Per row, with p the softmax of the teacher's values / T over its entries and q
+    the softmax of logits / T over all C classes::
+
+        L = weight * T^2 * sum_k p_k (log p_k - log q[index_k])
+
+    An entry whose index is outside [0, C) or whose value is -inf is absent; a row without entries (an unlabelled
+    pixel) has loss and gradient 0.  Entries of one class add up.  ``reduction`` is "mean" (over all rows), "sum"
+    or "none" (a float32 loss per row).  With float16 logits take "sum": a mean's gradients, of the order of
+    1 / rows, fall below float16's range.  No gradient flows to the teacher or to ``weight``."""
+    args = _DistillArgs(logits, teacher, temperature, weight, reduction)
+    return _Distill.apply(args.logits, args)
+
+
+def distill_loss_and_grad(logits: torch.Tensor, teacher, temperature: float = 1.0,
+                          weight: torch.Tensor | None = None,
+                          reduction: str = "mean") -> tuple[torch.Tensor, torch.Tensor]:
+    """``distill_loss`` and its gradient with respect to ``logits`` (their shape and type) in one pass over the
+    logits, outside autograd: hand the gradient on with ``logits.backward(grad)``.  With ``reduction="none"``
+    each row's gradient is its own loss's."""
+    args = _DistillArgs(logits.detach() if isinstance(logits, torch.Tensor) else logits, teacher, temperature, weight,
+                        reduction)
+    grad = torch.empty_like(args.logits)
+    loss = args.run(args.logits, grad=grad)
+    return loss, grad

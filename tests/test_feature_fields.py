@@ -1,0 +1,135 @@
+"""Feature-field operators without a GPU: refusals of the Python entry points
+and of the C ABI, and the plain forms the GPU tests compare against."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from feature_helpers import distill64
+from mlx3d_b200 import _native as nat
+from mlx3d_b200.losses import distill_loss, distill_loss_and_grad
+from mlx3d_b200.staging import TeacherCache
+
+
+def _teacher(n=3, k=2):
+    return torch.zeros(n, k), torch.zeros(n, k, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("fn", [distill_loss, distill_loss_and_grad])
+def test_distill_refusals(fn):
+    s = torch.zeros(3, 5)
+    v, i = _teacher()
+    with pytest.raises(ValueError, match="CUDA"):
+        fn(s, (v, i))
+    with pytest.raises(ValueError, match="reduction"):
+        fn(s, (v, i), reduction="batchmean")
+    for t in (0.0, -1.0, math.nan, math.inf):
+        with pytest.raises(ValueError, match="temperature"):
+            fn(s, (v, i), temperature=t)
+    with pytest.raises(ValueError, match="shape"):
+        fn(torch.zeros(3, 0), (v, i))
+    with pytest.raises(ValueError, match="shape"):
+        fn(s, (v[:2], i[:2]))
+    with pytest.raises(ValueError, match="shape"):
+        fn(s, (v, i[:, :1]))
+    with pytest.raises(ValueError, match="entries"):
+        fn(s, (v[:, :0], i[:, :0]))
+    with pytest.raises(ValueError, match="entries"):
+        fn(s, _teacher(3, nat.GS_TEACHER_MAX_K + 1))
+    with pytest.raises(TypeError, match="index"):
+        fn(s, (v, i.float()))
+    with pytest.raises(TypeError, match="teacher"):
+        fn(s, v)
+    with pytest.raises(ValueError, match="weight"):
+        fn(s, (v, i), weight=torch.ones(2))
+    with pytest.raises(ValueError, match="at least one row"):
+        fn(s[:0], (v[:0], i[:0]))
+    with pytest.raises(TypeError, match="floating"):
+        fn(s.int(), (v, i))
+
+
+def test_teacher_cache_refusals():
+    for bad in (dict(k=0), dict(k=33), dict(num_classes=0), dict(num_classes=32768), dict(bits=2), dict(rows=-1)):
+        with pytest.raises(ValueError):
+            TeacherCache(**{**dict(rows=4, k=8, num_classes=20), **bad})
+    with pytest.raises(ValueError, match="CUDA"):
+        TeacherCache(4, 8, 20, device="cpu")
+
+
+def _native_teacher(**kw):
+    t = nat.GsTeacher(None, None, None, None, 0, 0, 0, 4, 8)
+    for name, v in kw.items():
+        setattr(t, name, v)
+    return t
+
+
+def test_native_distill_rejects_bad_arguments_before_the_device():
+    lib = nat.load()
+
+    def call(dtype=0, n=2, classes=5, t=None, temp=1.0, loss=None, ws=0):
+        t = _native_teacher() if t is None else t
+        return lib.gs_distill(None, dtype, n, classes, ctypes.byref(t), temp, None, 1.0, None, 0, None, loss, None,
+                              None, ws, None)
+
+    assert call(dtype=3) == nat.GS_ERR_INVALID_ARG
+    assert call(n=-1) == nat.GS_ERR_INVALID_ARG
+    assert call(classes=0) == nat.GS_ERR_INVALID_ARG
+    assert call(classes=1 << 31) == nat.GS_ERR_INVALID_ARG
+    assert call(t=_native_teacher(k=0)) == nat.GS_ERR_INVALID_ARG
+    assert call(t=_native_teacher(k=33)) == nat.GS_ERR_INVALID_ARG  # a cache's limit
+    assert call(t=_native_teacher(bits=0, k=257)) == nat.GS_ERR_INVALID_ARG
+    assert call(t=_native_teacher(bits=5)) == nat.GS_ERR_INVALID_ARG
+    assert call(t=_native_teacher(records=8, n_records=4)) == nat.GS_ERR_INVALID_ARG
+    assert b"aligned" in lib.gs_last_error()
+    for temp in (0.0, -2.0, math.nan, math.inf, 1e-39):
+        assert call(temp=temp) == nat.GS_ERR_INVALID_ARG
+        assert b"temperature" in lib.gs_last_error()
+    assert call() == nat.GS_ERR_INVALID_ARG  # NULL logits
+    assert call(t=_native_teacher(bits=0)) == nat.GS_ERR_INVALID_ARG
+    assert b"NULL" in lib.gs_last_error()
+    assert call(n=0, loss=16, ws=8) == nat.GS_ERR_CAPACITY
+    assert lib.gs_distill(None, 0, 2, 5, None, 1.0, None, 1.0, None, 0, None, None, None, None, 0,
+                          None) == nat.GS_ERR_INVALID_ARG
+
+
+def test_native_cache_rejects_bad_arguments_before_the_device():
+    lib = nat.load()
+    assert lib.gs_teacher_record_bytes(8, 8) == 32
+    assert lib.gs_teacher_record_bytes(32, 4) == 96
+    assert [lib.gs_teacher_record_bytes(k, b) for k, b in ((0, 8), (33, 8), (8, 3))] == [0, 0, 0]
+
+    def write(dtype=0, n=2, classes=5, records=16, held=4, first=0, k=4, bits=8):
+        return lib.gs_teacher_write(None, dtype, n, classes, records, held, first, k, bits, None)
+
+    for bad in (dict(dtype=9), dict(n=-1), dict(classes=0), dict(classes=32768), dict(records=8), dict(k=0),
+                dict(k=33), dict(bits=16), dict(first=-1), dict(first=3), dict(first=5, n=0), dict(records=None),
+                dict(n=1 << 62, held=4)):
+        assert write(**bad) == nat.GS_ERR_INVALID_ARG, bad
+    assert write() == nat.GS_ERR_INVALID_ARG  # NULL logits
+    assert write(n=0) == nat.GS_OK
+
+    def read(n=2, records=16, held=4, k=4, bits=8):
+        return lib.gs_teacher_read(records, held, None, 0, n, k, bits, None, None, None)
+
+    for bad in (dict(n=-1), dict(records=24), dict(k=0), dict(k=40), dict(bits=0), dict(held=-2), {}):
+        assert read(**bad) == nat.GS_ERR_INVALID_ARG, bad
+    assert read(n=0) == nat.GS_OK
+
+
+def test_plain_distillation_gradient_against_differences():
+    g = torch.Generator().manual_seed(3)
+    s = torch.randn(6, 9, generator=g, dtype=torch.float64)
+    v = torch.randn(6, 4, generator=g, dtype=torch.float64)
+    i = torch.randint(-1, 10, (6, 4), generator=g)  # absent ones, one past the end, repeats
+    i[2] = -1
+    loss, grad = distill64(s, v, i, t=1.7)
+    assert loss[2] == 0 and (grad[2] == 0).all()
+    h = 1e-6
+    for c in range(9):
+        d = torch.zeros_like(s)
+        d[:, c] = h
+        diff = (distill64(s + d, v, i, t=1.7)[0] - distill64(s - d, v, i, t=1.7)[0]) / (2 * h)
+        # third-order remainder h^2 / 6 * |L'''| <= 1e-11, cancellation 2^-52 * |L| / h <= 1e-8
+        assert torch.allclose(diff, grad[:, c], rtol=0, atol=1e-8)

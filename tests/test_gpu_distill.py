@@ -1,0 +1,337 @@
+"""Distillation loss and teacher cache on the GPU against plain 64-bit forms."""
+
+import math
+
+import pytest
+import torch
+
+from feature_helpers import DTYPES, distill64, distill_tolerance, half_step, read64, write64
+from mlx3d_b200 import _native as nat
+from mlx3d_b200.losses import distill_loss, distill_loss_and_grad
+from mlx3d_b200.staging import TeacherCache
+
+pytestmark = pytest.mark.gpu
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _inputs(n, c, k, dtype, vdtype="fp16", seed=0):
+    g = _gen(seed)
+    s = (torch.randn((n, c), device="cuda", generator=g) * 2).to(DTYPES[dtype])
+    v = (torch.randn((n, k), device="cuda", generator=g) * 2 + 3).to(DTYPES[vdtype])
+    i = torch.randint(-1, c + 1, (n, k), device="cuda", generator=g, dtype=torch.int32)  # absent and repeated ones
+    w = torch.rand((n,), device="cuda", generator=g)
+    return s, v, i, w
+
+
+def _check(s, v, i, w, t, loss, grad, g_row=1.0):
+    want_l, want_g = distill64(s, v, i, t, w)
+    tol_l, rel = distill_tolerance(s, v, t, v.shape[-1])
+    ww = torch.ones(s.shape[:-1], device="cuda", dtype=torch.float64) if w is None else w.double()
+    tol = ww * t * t * tol_l + 2.0 ** -22 * want_l.abs()
+    assert ((loss.double() - want_l).abs() <= tol).all()
+    if grad is not None:
+        # q and p are at most 1 and each off by rel: 2 rel (w T); factors and the final rounding
+        want_g = want_g * g_row
+        size = (ww * t * g_row if not isinstance(g_row, float) else ww * t * abs(g_row))[..., None]
+        tiny = 2.0 ** -25 if s.dtype == torch.float16 else 0.0  # half a subnormal step
+        tol = size * 2 * rel[..., None] + want_g.abs() * (half_step(s.dtype) + 2.0 ** -21) + tiny
+        assert ((grad.double() - want_g).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,c,k,t", [
+    (1, 1, 1, 1.0), (1, 2, 3, 1.0), (3, 7, 1, 2.0), (257, 20, 5, 1.0), (64, 32, 32, 0.5), (1000, 133, 8, 2.0),
+    (515, 150, 8, 4.0), (130, 151, 33, 1.0), (33, 1024, 64, 1.0), (17, 1201, 256, 1.0), (9, 4099, 16, 2.0),
+    (5, 32001, 32, 1.0), (2, 70001, 7, 1.0), (4097, 16, 4, 1.0), (2049, 8, 8, 1.0),
+])
+def test_distill_matches_the_definition(n, c, k, t, dtype):
+    vdtype = {"fp32": "fp32", "fp16": "fp16", "bf16": "bf16"}[dtype]
+    s, v, i, w = _inputs(n, c, k, dtype, vdtype, seed=n + c)
+    loss, grad = distill_loss_and_grad(s, (v, i), temperature=t, weight=w, reduction="none")
+    assert loss.dtype == torch.float32 and grad.dtype == s.dtype and grad.shape == s.shape
+    _check(s, v, i, w, t, loss, grad)
+    # the loss alone, and autograd's gradient, are the same numbers
+    leaf = s.clone().requires_grad_(True)
+    alone = distill_loss(leaf, (v, i), temperature=t, weight=w, reduction="none")
+    assert torch.equal(alone, loss)
+    alone.backward(torch.ones_like(alone))
+    assert torch.equal(leaf.grad, grad)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_reductions_and_cotangents(reduction):
+    n, c, k = 1031, 77, 6
+    s, v, i, w = _inputs(n, c, k, "fp32")
+    rows, _ = distill64(s, v, i, 2.0, w)
+    div = n if reduction == "mean" else 1
+    leaf = s.clone().requires_grad_(True)
+    loss = distill_loss(leaf, (v, i), 2.0, w, reduction)
+    tol_l, _ = distill_tolerance(s, v, 2.0, k)
+    got = float(loss.detach())
+    assert abs(got - float(rows.sum() / div)) <= float((w * 4.0 * tol_l).sum() / div) + 1e-6 * got
+    (loss * -3.0).backward()
+    _check(s, v, i, w, 2.0, distill_loss(s, (v, i), 2.0, w, "none"), leaf.grad, g_row=-3.0 / div)
+    l2, g2 = distill_loss_and_grad(s, (v, i), 2.0, w, reduction)
+    assert torch.equal(l2, loss.detach())
+    _check(s, v, i, w, 2.0, distill_loss(s, (v, i), 2.0, w, "none"), g2, g_row=1.0 / div)
+
+
+def test_per_row_cotangents_and_no_weight():
+    s, v, i, _ = _inputs(300, 41, 5, "bf16", "bf16")
+    leaf = s.clone().requires_grad_(True)
+    loss = distill_loss(leaf, (v, i), reduction="none")
+    g = torch.linspace(0.0, 2.0, 300, device="cuda")
+    loss.backward(g)
+    _check(s, v, i, None, 1.0, loss.detach(), leaf.grad, g_row=g.double()[:, None])
+
+
+def test_images_strides_and_unaligned_bases():
+    s, v, i, w = _inputs(24 * 20, 30, 4, "fp32")
+    want = distill_loss(s, (v, i), weight=w, reduction="none")
+    img = s.reshape(24, 20, 30)
+    got = distill_loss(img, (v.reshape(24, 20, 4), i.reshape(24, 20, 4)), weight=w.reshape(24, 20), reduction="none")
+    assert got.shape == (24, 20) and torch.equal(got.reshape(-1), want)
+    wide = torch.zeros((480, 37), device="cuda")
+    wide[:, 3:33] = s
+    assert torch.equal(distill_loss(wide[:, 3:33], (v, i), weight=w, reduction="none"), want)
+    for dtype in ("fp32", "fp16", "bf16"):  # contiguous, but off every vector boundary
+        x = s.to(DTYPES[dtype])
+        flat = torch.zeros((480 * 30 + 1,), device="cuda", dtype=x.dtype)
+        flat[1:] = x.reshape(-1)
+        off = flat[1:].reshape(480, 30)
+        a = distill_loss_and_grad(x, (v, i), weight=w)
+        b = distill_loss_and_grad(off, (v, i), weight=w)
+        tol = 2.0 ** -20 * float(a[0].abs()) if dtype == "fp32" else 2.0 ** -18 * float(a[0].abs())
+        assert abs(float(a[0]) - float(b[0])) <= tol
+        assert torch.allclose(a[1].float(), b[1].float(), rtol=2 * half_step(x.dtype) + 2.0 ** -18, atol=1e-9)
+
+
+def test_masked_values():
+    inf, low = math.inf, torch.finfo(torch.float32).min
+    s = torch.tensor([[0.0, 1.0, 2.0, -1.0]] * 8, device="cuda")
+    s[3, 1] = -inf  # a student class masked out, not among the teacher's
+    s[4, 0] = -inf  # ... among the teacher's: infinite loss, finite gradient
+    s[5, 1] = low
+    v = torch.tensor([[1.0, 0.0]] * 8, device="cuda")
+    i = torch.tensor([[0, 2]] * 8, device="cuda", dtype=torch.int32)
+    i[0] = -1  # nothing left
+    v[1] = -inf  # nothing left
+    v[2, 1] = -inf  # one entry left
+    v[6] = low  # two equal entries
+    v[7, 1] = low  # an entry with probability 0
+    i[7, 1] = 3
+    s[7, 3] = -inf  # ... on a masked class: contributes nothing
+    loss, grad = distill_loss_and_grad(s, (v, i), reduction="none")
+    want_l, want_g = distill64(s, v, i)
+    assert loss[4] == inf
+    keep = [0, 1, 2, 3, 5, 6, 7]
+    assert torch.allclose(loss[keep].double(), want_l[keep], rtol=1e-6, atol=1e-6)
+    assert torch.allclose(grad.double(), want_g, rtol=1e-6, atol=1e-6)
+    assert (loss[:2] == 0).all() and (grad[:2] == 0).all()
+    # NaN stays NaN in its row only
+    s[3, 0] = math.nan
+    v[2, 0] = math.nan
+    loss, grad = distill_loss_and_grad(s, (v, i), reduction="none")
+    assert loss[[2, 3]].isnan().all() and not loss[[0, 1, 5, 6, 7]].isnan().any()
+    assert not grad[[0, 1, 5, 6, 7]].isnan().any()
+
+
+def test_no_rows():
+    s = torch.zeros((0, 5), device="cuda", requires_grad=True)
+    v, i = torch.zeros((0, 2), device="cuda"), torch.zeros((0, 2), device="cuda", dtype=torch.int32)
+    loss = distill_loss(s, (v, i), reduction="sum")
+    assert float(loss) == 0.0
+    loss.backward()
+    assert s.grad.shape == (0, 5)
+    assert distill_loss(s, (v, i), reduction="none").shape == (0,)
+
+
+def test_wide_index_types():
+    s, v, i, _ = _inputs(50, 11, 3, "fp32")
+    want = distill_loss(s, (v, i))
+    assert torch.equal(distill_loss(s, (v, i.short())), want)
+    far = i.long()
+    far[i < 0] = (1 << 33) + 2  # 2 if cut to 32 bits
+    far[i >= 11] = -(1 << 40)
+    assert torch.equal(distill_loss(s, (v, far)), want)
+
+
+# ---------------------------------------------------------------- the cache
+def _cache_logits(n, c, dtype, seed):
+    g = _gen(seed)
+    z = (torch.randn((n, c), device="cuda", generator=g) * 3).to(DTYPES[dtype])
+    return z
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,c,k", [
+    (1, 1, 1), (1, 5, 8), (3, 2, 2), (100, 20, 5), (257, 32, 32), (300, 33, 31), (1000, 150, 8), (515, 133, 7),
+    (64, 1201, 32), (31, 4096, 16), (9, 32767, 32), (4100, 64, 3), (70, 257, 1),
+])
+def test_write_and_read_match_the_definition(n, c, k, dtype, bits):
+    z = _cache_logits(n, c, dtype, n * 7 + c)
+    if c > 4:
+        z[:, 1] = -math.inf
+        z[:, 3] = torch.finfo(z.dtype).min
+        z[n // 2] = -math.inf  # a row with nothing
+        z[n // 3, 2:] = math.nan  # a row with one usable class
+        z[0, 2] = math.inf
+    cache = TeacherCache(n + 5, k, c, bits=bits)
+    before = cache.records.clone()
+    cache.write(3, z)
+    values, index = cache.read(slice(3, 3 + n))
+    first, scale, want_i, code = write64(z, k, bits)
+    assert torch.equal(index.cpu(), want_i)
+    assert torch.equal(values.cpu(), read64(first, scale, want_i, code))  # the codes exactly
+    assert torch.equal(cache.records[:3], before[:3]) and torch.equal(cache.records[3 + n:], before[3 + n:])
+
+
+def test_write_equal_logits_take_the_lowest_indices():
+    z = torch.zeros((4, 100), device="cuda")
+    z[1] = -0.0
+    z[2, ::3] = -0.0
+    z[3, 50:] = 1.0
+    cache = TeacherCache(4, 6, 100)
+    cache.write(0, z)
+    values, index = cache.read(slice(None))
+    assert index[:3].tolist() == [[0, 1, 2, 3, 4, 5]] * 3
+    assert index[3].tolist() == [50, 51, 52, 53, 54, 55]
+    assert (values[:3] == 0).all() and (values[3] == 1).all()
+
+
+def test_write_extreme_ranges():
+    big = torch.finfo(torch.float32).max
+    z = torch.tensor([[big, -1e38, 0.0, 5.0], [1e-44, 0.0, -1e-44, -3e-44], [big, big, big, big],
+                      [3.0, 3.0, 3.0, 2.0]], device="cuda")
+    for bits in (8, 4):
+        cache = TeacherCache(4, 4, 4, bits=bits)
+        cache.write(0, z)
+        values, index = cache.read(slice(None))
+        first, scale, want_i, code = write64(z, 4, bits)
+        assert torch.equal(index.cpu(), want_i)
+        assert torch.equal(values.cpu(), read64(first, scale, want_i, code))
+
+
+def test_read_rows_in_any_order():
+    z = _cache_logits(500, 40, "fp32", 1)
+    cache = TeacherCache(500, 7, 40)
+    cache.write(0, z)
+    all_v, all_i = cache.read(slice(None))
+    rows = torch.tensor([[3, 499, 3], [0, -1, 500], [250, 1 << 40, -(1 << 50)]], device="cuda")
+    v, i = cache.read(rows)
+    assert v.shape == (3, 3, 7)
+    inside = (rows >= 0) & (rows < 500)
+    assert torch.equal(v[inside], all_v[rows[inside]]) and torch.equal(i[inside], all_i[rows[inside]])
+    assert (v[~inside] == -math.inf).all() and (i[~inside] == -1).all()
+    v32, i32 = cache.read(rows[:2].int())
+    assert torch.equal(v32, v[:2]) and torch.equal(i32, i[:2])
+    assert cache.read(slice(7, 7))[0].shape == (0, 7)
+    assert cache.read(rows[:0])[0].shape == (0, 3, 7)
+
+
+def test_cache_starts_empty_and_saves():
+    cache = TeacherCache(10, 3, 9, bits=4)
+    v, i = cache.read(slice(None))
+    assert (v == -math.inf).all() and (i == -1).all()
+    cache.write(2, _cache_logits(4, 9, "bf16", 2).reshape(2, 2, 9))
+    other = TeacherCache(10, 3, 9, bits=4)
+    other.load_state_dict(cache.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(cache.read(slice(None)), other.read(slice(None))))
+    with pytest.raises(ValueError, match="bits"):
+        TeacherCache(10, 3, 9, bits=8).load_state_dict(cache.state_dict())
+    with pytest.raises(ValueError, match="shape"):
+        TeacherCache(11, 3, 9, bits=4).load_state_dict(cache.state_dict())
+
+
+def test_cache_argument_checks():
+    cache = TeacherCache(10, 3, 9)
+    z = torch.zeros((4, 9), device="cuda")
+    with pytest.raises(ValueError, match="outside"):
+        cache.write(7, z)
+    with pytest.raises(ValueError, match="outside"):
+        cache.write(-1, z)
+    with pytest.raises(ValueError, match="shape"):
+        cache.write(0, z[:, :8])
+    with pytest.raises(ValueError, match="CUDA"):
+        cache.write(0, z.cpu())
+    for bad in (slice(0, 11), slice(-2, 3), slice(5, 2)):
+        with pytest.raises(ValueError, match="outside"):
+            cache.read(bad)
+    with pytest.raises(ValueError, match="step"):
+        cache.read(slice(0, 4, 2))
+    with pytest.raises(TypeError):
+        cache.read([1, 2])
+    with pytest.raises(TypeError):
+        cache.read(torch.ones(3, device="cuda"))
+    with pytest.raises(ValueError, match="rows"):
+        distill_loss(z, cache.at(slice(0, 3)))
+    with pytest.raises(ValueError, match="classes"):
+        distill_loss(torch.zeros((3, 8), device="cuda"), cache.at(slice(0, 3)))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("n,c,k,dtype", [(1, 5, 2, "fp32"), (300, 20, 5, "fp32"), (999, 133, 8, "fp16"),
+                                         (65, 1201, 32, "bf16"), (3, 20011, 17, "fp32")])
+def test_loss_from_the_cache_is_the_loss_of_what_it_reads(n, c, k, dtype, bits):
+    cache = TeacherCache(n + 40, k, c, bits=bits)
+    cache.write(40, _cache_logits(n, c, "fp32", 9))  # the first 40 rows stay empty
+    rows = torch.randint(-2, n + 43, (n,), device="cuda", generator=_gen(4))
+    s = _cache_logits(n, c, dtype, 11)
+    for at in (rows, slice(40, 40 + n)):
+        v, i = cache.read(at)
+        want = distill_loss_and_grad(s, (v, i), 2.0, reduction="none")
+        got = distill_loss_and_grad(s, cache.at(at), 2.0, reduction="none")
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        _check(s, v, i, None, 2.0, *got)
+
+
+def test_backward_refuses_rows_written_since_the_loss():
+    cache = TeacherCache(8, 2, 5)
+    cache.write(0, torch.randn((8, 5), device="cuda"))
+    s = torch.randn((8, 5), device="cuda", requires_grad=True)
+    loss = distill_loss(s, cache.at(slice(0, 8)))
+    cache.write(0, torch.randn((8, 5), device="cuda"))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_captured_and_on_another_stream():
+    z, s = _cache_logits(2000, 60, "fp32", 5), _cache_logits(2000, 60, "fp32", 6)
+    cache = TeacherCache(2000, 8, 60)
+
+    def work():
+        cache.write(0, z)
+        return distill_loss_and_grad(s, cache.at(slice(None)), 2.0)
+
+    want = work()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = work()
+        graphs, outs = [], []
+        for _ in range(2):  # two graphs, replayed in turn
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(work())
+            graphs.append(g)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    z.copy_(_cache_logits(2000, 60, "fp32", 7))
+    want = work()
+    for _ in range(2):
+        for g, out in zip(graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+def test_kernels_are_counted():
+    lib = nat.load()
+    before = lib.gs_kernel_launch_count()
+    cache = TeacherCache(4, 2, 5)
+    cache.write(0, torch.zeros((4, 5), device="cuda"))
+    assert lib.gs_kernel_launch_count() > before
