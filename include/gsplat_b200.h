@@ -473,6 +473,33 @@ int gs_teacher_write(const void* logits, int dtype, int64_t n, int64_t classes, 
 int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows, int64_t first_row, int64_t n,
                     int k, int bits, float* values, int32_t* index, void* stream);
 
+/* Gated feature decoder: y = (act(x Wg^T) * (x Wu^T)) Wd^T over n rows
+ * (pixels); x (n, d), Wg and Wu (f, d), Wd (c, f), y (n, c), all contiguous and
+ * of one type, GS_F16 or GS_BF16.  1 <= d <= GS_DECODE_MAX_D, f >= 1,
+ * 1 <= c <= GS_DECODE_MAX_C.  Products are summed in 32 bits; the hidden
+ * values are rounded to the type as operands of the second product.
+ *
+ * gs_decode_prepare lays the weights out for the kernels in `image`
+ * (gs_decode_image_bytes, 16-byte aligned); forward and backward read only
+ * that.  gs_decode_backward writes dx (n, d) unless NULL, and d_gate, d_up
+ * (f, d), d_down (c, f) unless all three are NULL, from dy (n, c); its workspace
+ * (gs_decode_workspace_bytes) is needed for the weight gradients only.  The
+ * sums over rows are taken in a fixed order. */
+#define GS_ACT_SILU 0
+#define GS_ACT_GELU 1 /* the error-function form */
+#define GS_DECODE_MAX_D 128
+#define GS_DECODE_MAX_C 256
+#define GS_DECODE_MAX_F 65536
+size_t gs_decode_image_bytes(int d, int f, int c);
+int gs_decode_prepare(const void* w_gate, const void* w_up, const void* w_down, int dtype, int d, int f, int c,
+                      void* image, size_t image_bytes, void* stream);
+int gs_decode_forward(const void* x, int dtype, int64_t n, int d, int f, int c, int activation, const void* image,
+                      size_t image_bytes, void* y, void* stream);
+size_t gs_decode_workspace_bytes(int64_t n, int d, int f, int c);
+int gs_decode_backward(const void* x, const void* dy, int dtype, int64_t n, int d, int f, int c, int activation,
+                       const void* image, size_t image_bytes, void* dx, void* d_gate, void* d_up, void* d_down,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

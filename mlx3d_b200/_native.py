@@ -73,6 +73,10 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 GS_TEACHER_MAX_K = 256
 GS_CACHE_MAX_K = 32
 GS_CACHE_MAX_CLASSES = 32767
+GS_DECODE_MAX_D = 128
+GS_DECODE_MAX_C = 256
+GS_DECODE_MAX_F = 65536
+GS_GATES = {"silu": 0, "gelu": 1}
 
 
 class GsTeacher(ctypes.Structure):
@@ -181,6 +185,14 @@ _SIGS = {
     "gs_teacher_record_bytes": (c_size_t, [c_int, c_int]),
     "gs_teacher_write": (c_int, [_P, c_int, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int, _P]),
     "gs_teacher_read": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int, c_int, _P, _P, _P]),
+    "gs_decode_image_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "gs_decode_prepare": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, c_size_t, _P]),
+    "gs_decode_forward": (c_int, [_P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P]),
+    "gs_decode_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "gs_decode_backward": (
+        c_int,
+        [_P, _P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P, _P, _P, _P, c_size_t, _P],
+    ),
     "gs_rasterize_forward": (
         c_int,
         [_P, _P, _P, c_int, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, _P, _P, _P, _P, _P],

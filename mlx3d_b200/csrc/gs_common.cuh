@@ -38,6 +38,7 @@ int binning_wait_failures(unsigned long long* out, int reset);
 // Sets the poll limit of the binning look-backs on the current device.
 int binning_set_wait_limit(int polls);
 int preprocess_wait_failures(unsigned long long* out, int reset);
+int decode_wait_failures(unsigned long long* out, int reset);
 
 // ------------------------------------------------ bulk (TMA) copies
 // One-shot shared-memory mbarrier tracking bulk global->shared copies

@@ -72,3 +72,67 @@ def read64(first, scale, index, code):
     """What the records stand for: the stored (float32) offset and step, one rounding at the end."""
     value = first - code * scale.float().double()
     return value.float().masked_fill(index < 0, -math.inf)
+
+
+def decode64(x, w_gate, w_up, w_down, act, dy=None):
+    """y, and with dy the gradients (dx, d w_gate, d w_up, d w_down), from the definition."""
+    x, wg, wu, wd = (t.double() for t in (x, w_gate, w_up, w_down))
+    g, u = x @ wg.T, x @ wu.T
+    if act == "silu":
+        gate = torch.sigmoid(g)
+        slope = gate * (1 + g * (1 - gate))
+    else:
+        gate = 0.5 * torch.erfc(-g / math.sqrt(2.0))
+        slope = gate + g * torch.exp(-0.5 * g * g) / math.sqrt(2.0 * math.pi)
+    a = g * gate
+    y = (a * u) @ wd.T
+    if dy is None:
+        return y
+    dy = dy.double()
+    dh = dy @ wd
+    dg, du = dh * u * slope, dh * a
+    return y, dg @ wg + du @ wu, dg.T @ x, du.T @ x, dy.T @ (a * u)
+
+
+def decode_tolerances(x, w_gate, w_up, w_down, act, dy=None):
+    """Absolute bounds of decode64's outputs, element by element.
+
+    Each second product sums terms of which one factor was rounded to 16 bits (half a step e), plus 32-bit
+    accumulation: an instruction sums 16 products and the accumulator, each sum off by at most 2^-23 of the
+    magnitudes (truncation).  First products g, u, dh: their 32-bit errors, carried through the activation
+    (|slope| <= 1.13, |slope'| <= 1), change h, dg, du by at most 4 * 2^-23 * (terms) of the magnitudes' products;
+    the hardware exponential and reciprocal add 2^-20.  All of it is below eps32 = 2^-17 (K + 16) / 16 relative to the
+    products of magnitudes; the final rounding adds half a step of the value."""
+    e = half_step(x.dtype)
+    ax, ag, au, ad = (t.double().abs() for t in (x, w_gate, w_up, w_down))
+    k1 = (x.shape[1] + 16) / 16
+    eps = 2.0 ** -17 * k1
+    mg, mu = ax @ ag.T, ax @ au.T  # magnitudes of the sums that give g and u
+    x64, wg, wu, wd = (t.double() for t in (x, w_gate, w_up, w_down))
+    g, u = x64 @ wg.T, x64 @ wu.T
+    gate = torch.sigmoid(g) if act == "silu" else 0.5 * torch.erfc(-g / math.sqrt(2.0))
+    a = (g * gate).abs()
+    # errors of a and u from the first products, of h = a u
+    ea, eu = 1.13 * eps * mg + 2.0 ** -20 * a, eps * mu
+    eh = (e + 2.0 ** -22) * a * u.abs() + ea * u.abs() + eu * a + ea * eu
+    sub = 2.0 ** -25 if x.dtype == torch.float16 else 0.0  # half a subnormal step of a rounded operand
+    y = decode64(x, w_gate, w_up, w_down, act)
+    acc = 2.0 ** -23 * (w_gate.shape[0] / 16 + 16)
+    out = [(eh + sub) @ ad.T + acc * ((a * u.abs()) @ ad.T) + e * y.abs() + sub]
+    if dy is None:
+        return out[0]
+    ady = dy.double().abs()
+    mdh = ady @ ad
+    _, dx, dwg, dwu, dwd = decode64(x, w_gate, w_up, w_down, act, dy)
+    edh = 2.0 ** -17 * (w_down.shape[0] + 16) / 16 * mdh
+    dh = (dy.double() @ wd).abs()
+    edg = 1.13 * ((e + 2.0 ** -19) * dh * u.abs() + edh * (u.abs() + eu) + dh * eu) + dh * u.abs() * eps * mg + sub
+    edu = (e + 2.0 ** -22) * dh * a + edh * (a + ea) + dh * ea + sub
+    mdg, mdu = 1.13 * mdh * mu, mdh * (1.13 * mg)
+    acc_f = 2.0 ** -23 * (2 * w_gate.shape[0] / 16 + 16)
+    acc_n = 2.0 ** -23 * (x.shape[0] / 16 + 160)
+    out.append(edg @ ag + edu @ au + acc_f * (mdg @ ag + mdu @ au) + e * dx.abs() + sub)
+    out.append(edg.T @ ax + acc_n * (mdg.T @ ax) + e * dwg.abs() + sub)
+    out.append(edu.T @ ax + acc_n * (mdu.T @ ax) + e * dwu.abs() + sub)
+    out.append(ady.T @ (eh + sub) + acc_n * (ady.T @ (a * u.abs())) + e * dwd.abs() + sub)
+    return out

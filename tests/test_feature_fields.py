@@ -7,9 +7,10 @@ import math
 import pytest
 import torch
 
-from feature_helpers import distill64
+from feature_helpers import decode64, distill64
 from mlx3d_b200 import _native as nat
 from mlx3d_b200.losses import distill_loss, distill_loss_and_grad
+from mlx3d_b200.splatting import FeatureDecoder, decode_features
 from mlx3d_b200.staging import TeacherCache
 
 
@@ -133,3 +134,84 @@ def test_plain_distillation_gradient_against_differences():
         diff = (distill64(s + d, v, i, t=1.7)[0] - distill64(s - d, v, i, t=1.7)[0]) / (2 * h)
         # third-order remainder h^2 / 6 * |L'''| <= 1e-11, cancellation 2^-52 * |L| / h <= 1e-8
         assert torch.allclose(diff, grad[:, c], rtol=0, atol=1e-8)
+
+
+def _weights(d=4, f=8, c=3, dtype=torch.bfloat16):
+    return torch.zeros(f, d, dtype=dtype), torch.zeros(f, d, dtype=dtype), torch.zeros(c, f, dtype=dtype)
+
+
+def test_decode_refusals():
+    x = torch.zeros(5, 4, dtype=torch.bfloat16)
+    wg, wu, wd = _weights()
+    with pytest.raises(ValueError, match="CUDA"):
+        decode_features(x, wg, wu, wd)
+    with pytest.raises(ValueError, match="activation"):
+        decode_features(x, wg, wu, wd, activation="relu")
+    for bad in ((x[:, :3], wg, wu, wd), (x, wg[:7], wu, wd), (x, wg, wu, wd[:, :7]), (x, wg[0], wu, wd),
+                (x[0, 0], wg, wu, wd)):
+        with pytest.raises(ValueError):
+            decode_features(*bad)
+    with pytest.raises(ValueError, match="channels"):
+        decode_features(torch.zeros(5, 129), *_weights(129))
+    with pytest.raises(ValueError, match="channels"):
+        decode_features(torch.zeros(5, 0), *_weights(0))
+    with pytest.raises(ValueError, match="outputs"):
+        decode_features(x, *_weights(c=257))
+    with pytest.raises(ValueError, match="hidden"):
+        decode_features(x, *_weights(f=0))
+    with pytest.raises(TypeError, match="float16"):
+        decode_features(x, *_weights(dtype=torch.float32))
+    with pytest.raises(TypeError, match="float16"):
+        decode_features(x, wg, wu.half(), wd)
+    with pytest.raises(TypeError, match="floating"):
+        decode_features(x.int(), wg, wu, wd)
+    with pytest.raises(ValueError, match="params"):
+        FeatureDecoder({"w_gate": wg})
+    with pytest.raises(TypeError, match="dtype"):
+        FeatureDecoder(dict(w_gate=wg, w_up=wu, w_down=wd), dtype=torch.float32)
+
+
+def test_native_decode_rejects_bad_arguments_before_the_device():
+    lib = nat.load()
+    size = lib.gs_decode_image_bytes(32, 100, 20)
+    assert size == 2 * (16384 + 32 * 128)
+    for d, f, c in ((0, 8, 8), (129, 8, 8), (8, 0, 8), (8, 65537, 8), (8, 8, 0), (8, 8, 257)):
+        assert lib.gs_decode_image_bytes(d, f, c) == 0
+        assert lib.gs_decode_workspace_bytes(10, d, f, c) == 0
+        assert lib.gs_decode_prepare(16, 16, 16, 1, d, f, c, 16, 1 << 30, None) == nat.GS_ERR_INVALID_ARG
+        assert lib.gs_decode_forward(16, 1, 4, d, f, c, 0, 16, 1 << 30, 16, None) == nat.GS_ERR_INVALID_ARG
+        assert lib.gs_decode_backward(16, 16, 1, 4, d, f, c, 0, 16, 1 << 30, 16, None, None, None, None, 0,
+                                      None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_prepare(16, 16, 16, 0, 32, 100, 20, 16, size, None) == nat.GS_ERR_INVALID_ARG  # float32
+    assert lib.gs_decode_prepare(16, 16, 16, 1, 32, 100, 20, 16, size - 1, None) == nat.GS_ERR_CAPACITY
+    assert lib.gs_decode_prepare(16, 16, 16, 1, 32, 100, 20, 8, size, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_prepare(None, 16, 16, 1, 32, 100, 20, 16, size, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(16, 1, -1, 32, 100, 20, 0, 16, size, 16, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(16, 1, 4, 32, 100, 20, 2, 16, size, 16, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(None, 1, 4, 32, 100, 20, 0, 16, size, 16, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(16, 1, 4, 32, 100, 20, 0, 16, size - 16, 16, None) == nat.GS_ERR_CAPACITY
+    assert lib.gs_decode_forward(None, 1, 0, 32, 100, 20, 0, None, 0, None, None) == nat.GS_OK
+    need = lib.gs_decode_workspace_bytes(1000, 32, 100, 20)
+    assert need >= 4 * (2 * 32 * 100 + 20 * 100)
+    args = (16, 16, 1, 1000, 32, 100, 20, 0, 16, size, None, 16, 16)
+    assert lib.gs_decode_backward(*args, None, 16, need, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_backward(*args, 16, 16, need - 1, None) == nat.GS_ERR_CAPACITY
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_plain_decoder_gradients_against_differences(act):
+    g = torch.Generator().manual_seed(5)
+    leaves = [torch.randn(*s, generator=g, dtype=torch.float64) for s in ((4, 3), (5, 3), (5, 3), (2, 5))]
+    dy = torch.randn(4, 2, generator=g, dtype=torch.float64)
+    grads = decode64(*leaves, act, dy)[1:]
+    h = 1e-6
+    for t, grad in zip(leaves, grads):
+        for i in range(t.numel()):
+            keep = float(t.view(-1)[i])
+            t.view(-1)[i] = keep + h
+            up = (decode64(*leaves, act) * dy).sum()
+            t.view(-1)[i] = keep - h
+            down = (decode64(*leaves, act) * dy).sum()
+            t.view(-1)[i] = keep
+            # third derivatives are below 1e3 here: remainder 2e-10; cancellation 2^-52 * 100 / h = 2e-8
+            assert abs(float((up - down) / (2 * h) - grad.view(-1)[i])) < 1e-7

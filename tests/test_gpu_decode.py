@@ -1,0 +1,197 @@
+"""Gated feature decoder on the GPU against the plain 64-bit form."""
+
+import ctypes
+import math
+
+import pytest
+import torch
+
+from feature_helpers import DTYPES, decode64, decode_tolerances
+from mlx3d_b200 import _native as nat
+from mlx3d_b200.splatting import FeatureDecoder, decode_features
+
+pytestmark = pytest.mark.gpu
+
+
+def _inputs(n, d, f, c, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    ty = DTYPES[dtype]
+    x = rnd(n, d)
+    x[: n // 10] = 0.0  # uncovered pixels
+    return (x.to(ty), (rnd(f, d) / math.sqrt(d)).to(ty), (rnd(f, d) / math.sqrt(d)).to(ty),
+            (rnd(c, f) * 2 / math.sqrt(f)).to(ty), (rnd(n, c) * 0.1).to(ty))
+
+
+def _wait_failures():
+    cnt = ctypes.c_uint64(0)
+    nat.call("gs_wait_failures", ctypes.byref(cnt), 0)
+    return cnt.value
+
+
+def _within(got, want, tol):
+    assert torch.isfinite(got).all()
+    worst = ((got.double() - want).abs() / tol.clamp(min=1e-30)).max()
+    assert float(worst) <= 1.0, float(worst)
+
+
+SIZES = [
+    (1, 1, 1, 1), (1, 32, 64, 20), (2, 3, 5, 7), (127, 16, 64, 16), (128, 64, 64, 64), (129, 17, 65, 33),
+    (300, 47, 171, 133), (1000, 128, 256, 256), (513, 64, 200, 150), (260, 65, 40, 129), (130, 8, 600, 250),
+    (77, 120, 128, 2), (40000, 64, 128, 150), (20001, 33, 70, 31),
+]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,d,f,c", SIZES)
+def test_forward_matches_the_definition(n, d, f, c, dtype, act):
+    x, wg, wu, wd, _ = _inputs(n, d, f, c, dtype, seed=n + d)
+    y = decode_features(x, wg, wu, wd, act)
+    assert y.shape == (n, c) and y.dtype == x.dtype
+    _within(y, decode64(x, wg, wu, wd, act), decode_tolerances(x, wg, wu, wd, act))
+    assert _wait_failures() == 0
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,d,f,c", SIZES)
+def test_gradients_match_the_definition(n, d, f, c, dtype, act):
+    x, wg, wu, wd, dy = _inputs(n, d, f, c, dtype, seed=n + c)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = decode_features(*leaves, act)
+    grads = torch.autograd.grad(y, leaves, dy)
+    plain = [t.detach() for t in leaves]
+    want = decode64(*plain, act, dy)
+    tol = decode_tolerances(*plain, act, dy)
+    for got, w, t, leaf in zip((y.detach(), *grads), want, tol, (y, *leaves)):
+        assert got.shape == leaf.shape and got.dtype == leaf.dtype
+        _within(got, w, t)
+    assert _wait_failures() == 0
+
+
+def test_gradients_on_demand_are_the_same_numbers():
+    x, wg, wu, wd, dy = _inputs(700, 40, 100, 30, "bf16")
+    full = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    want = torch.autograd.grad(decode_features(*full), full, dy)
+    for need in ((True, False, False, False), (False, True, False, False), (False, False, False, True)):
+        leaves = [t.clone().requires_grad_(r) for t, r in zip((x, wg, wu, wd), need)]
+        decode_features(*leaves).backward(dy)
+        for leaf, w, r in zip(leaves, want, need):
+            assert (leaf.grad is None) if not r else torch.equal(leaf.grad, w)
+
+
+def test_repeated_calls_are_bitwise_equal():
+    x, wg, wu, wd, dy = _inputs(30000, 64, 256, 150, "bf16")
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    runs = []
+    for _ in range(3):
+        y = decode_features(*leaves)
+        runs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+def test_images_strides_types_and_unaligned_rows():
+    x, wg, wu, wd, _ = _inputs(20 * 30, 24, 50, 11, "fp16")
+    want = decode_features(x, wg, wu, wd)
+    assert torch.equal(decode_features(x.reshape(20, 30, 24), wg, wu, wd), want.reshape(20, 30, 11))
+    wide = torch.zeros((600, 40), device="cuda", dtype=x.dtype)
+    wide[:, 5:29] = x
+    assert torch.equal(decode_features(wide[:, 5:29], wg, wu, wd), want)
+    flat = torch.zeros((600 * 24 + 1,), device="cuda", dtype=x.dtype)
+    flat[1:] = x.reshape(-1)
+    assert torch.equal(decode_features(flat[1:].reshape(600, 24), wg, wu, wd), want)
+    assert torch.equal(decode_features(x.float(), wg, wu, wd), want)  # rounded to the weights' type
+    assert torch.equal(decode_features(x, wg.T.contiguous().T, wu, wd), want)
+    assert torch.equal(decode_features(x[0], wg, wu, wd), want[0])
+
+
+def test_gradient_through_float32_features():
+    x, wg, wu, wd, dy = _inputs(50, 8, 16, 5, "bf16")
+    a = x.float().requires_grad_(True)
+    b = x.clone().requires_grad_(True)
+    decode_features(a, wg, wu, wd).backward(dy)
+    decode_features(b, wg, wu, wd).backward(dy)
+    assert a.grad.dtype == torch.float32 and torch.equal(a.grad, b.grad.float())
+
+
+def test_no_rows():
+    x, wg, wu, wd, dy = _inputs(0, 8, 16, 5, "bf16")
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = decode_features(*leaves)
+    assert y.shape == (0, 5)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert grads[0].shape == (0, 8) and all((g == 0).all() for g in grads[1:])
+
+
+def test_one_bad_pixel_stays_alone():
+    x, wg, wu, wd, _ = _inputs(300, 16, 32, 9, "bf16")
+    want = decode_features(x, wg, wu, wd)
+    x[200] = math.nan
+    x[201, 0] = math.inf
+    got = decode_features(x, wg, wu, wd)
+    keep = [i for i in range(300) if i not in (200, 201)]
+    assert torch.equal(got[keep], want[keep]) and got[200].isnan().all()
+
+
+def test_large_gates_do_not_overflow():
+    x = torch.tensor([[300.0], [-300.0], [0.0]], device="cuda", dtype=torch.bfloat16)
+    one = torch.ones((1, 1), device="cuda", dtype=torch.bfloat16)
+    for act in ("silu", "gelu"):
+        a = x.clone().requires_grad_(True)
+        y = decode_features(a, one, one, one, act)
+        assert y[:, 0].tolist() == [90112.0, 0.0, 0.0]  # 300^2 rounded to bf16
+        y.sum().backward()
+        assert torch.isfinite(a.grad).all() and a.grad[1] == 0
+
+
+def test_weights_changed_before_the_backward_are_refused():
+    x, wg, wu, wd, dy = _inputs(10, 8, 16, 5, "bf16")
+    wg.requires_grad_(True)
+    y = decode_features(x, wg, wu, wd)
+    with torch.no_grad():
+        wg.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+
+
+def test_captured_and_on_another_stream():
+    x, wg, wu, wd, dy = _inputs(3000, 32, 96, 40, "bf16")
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+
+    def work():
+        y = decode_features(*leaves)
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = work()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = work()
+        graphs, outs = [], []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                outs.append(work())
+            graphs.append(g)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():
+        x.copy_(_inputs(3000, 32, 96, 40, "bf16", seed=8)[0])
+    want = work()
+    for _ in range(2):
+        for g, out in zip(graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_decoder_object_trains_float32_leaves():
+    dec = FeatureDecoder.create(16, 32, 7, generator=torch.Generator(device="cuda").manual_seed(1))
+    x = torch.randn((64, 16), device="cuda")
+    y = dec(x)
+    assert y.dtype == torch.bfloat16
+    y.float().square().sum().backward()
+    for p in dec.params.values():
+        assert p.grad is not None and p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all()
