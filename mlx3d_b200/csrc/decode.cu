@@ -10,7 +10,9 @@
 // same panel serves as a K-major and as an MN-major operand, so x, dy and each
 // weight are laid out once and never transposed.
 //
-// This form is sequential: load, first products, activation, second products.
+// Warps have roles: input loaders, a weight loader, one thread that issues the
+// matrix instructions, two warpgroups that apply the activation (alternating
+// chunks, or halves of one), and a warp that stores finished tiles.
 #include "feature_common.cuh"
 #include "tc_common.cuh"
 
@@ -19,10 +21,12 @@ namespace gs {
 constexpr int kTile = 128;              // rows of a tile (M of the matrix instructions)
 constexpr int kChunk = 64;              // hidden units of a chunk
 constexpr int kPanel = kTile * 128;     // bytes of a 128-row panel
-constexpr int kDecodeThreads = 256;
+constexpr int kDecodeThreads = 512;
+constexpr int kLoaders = 128;           // warps 4-7
+constexpr int kEpilogue = 256;          // warps 8-15, two warpgroups
+constexpr int kMaxXStages = 4, kMaxWStages = 16;
 constexpr uint32_t kTmemCols = 512;
-// TMEM columns
-constexpr uint32_t kColG = 0, kColU = 64, kColDh = 128, kColH = 192, kColOut = 256;
+constexpr size_t kMaxSmem = 232448;     // 227 KB
 
 enum { kFwd = 0, kDx = 1, kDw = 2 };
 
@@ -50,6 +54,10 @@ struct DecodeArgs {
   int chunks;
   int chunk_bytes;
   int act;
+  int x_stages, w_stages;  // shared-memory stages of inputs and weight chunks
+  int out_pitch;           // bytes of a row of the output stage, 0: rows stored from registers
+  int out_vec;             // bytes of a store to the output stage
+  int out_bulk;            // output rows can be written with bulk copies
 };
 
 __host__ __device__ __forceinline__ int round_up(int v, int m) { return (v + m - 1) / m * m; }
@@ -91,18 +99,44 @@ __global__ void k_decode_prepare(const T* __restrict__ wg, const T* __restrict__
   }
 }
 
-// act(g), and act'(g) where wanted.  exp and the reciprocal are the hardware
-// approximations (2 ulp): the results are rounded to 16 bits.
+
+// act and act' of two values.  The exponential and the reciprocal are the
+// hardware approximations (2 ulp; the results are rounded to 16 bits).  The
+// special-function unit (16 a clock and SM) bounds the activation, so silu's two
+// logistic functions share one reciprocal: 1 / a = b * (1 / ab).  Exponentials
+// stop at 2^63, so that ab stays finite; below that the logistic function is 0.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <int ACT, bool SLOPE>
-__device__ __forceinline__ void gate(float g, float& a, float& slope) {
+__device__ __forceinline__ void gate2(float g0, float g1, float& a0, float& a1, float& s0, float& s1) {
   if (ACT == GS_ACT_SILU) {
-    const float s = __frcp_rn(1.0f + __expf(-g));
-    a = g * s;
-    if (SLOPE) slope = s + a * (1.0f - s);
+    const float t0 = g0 * -1.4426950408889634f, t1 = g1 * -1.4426950408889634f;
+    const float p0 = 1.0f + ex2(fminf(t0, 63.0f)), p1 = 1.0f + ex2(fminf(t1, 63.0f));
+    const float inv = rcp(p0 * p1);
+    const float l0 = t0 > 63.0f ? 0.0f : inv * p1, l1 = t1 > 63.0f ? 0.0f : inv * p0;
+    a0 = g0 * l0;
+    a1 = g1 * l1;
+    if (SLOPE) {
+      s0 = __fmaf_rn(a0, 1.0f - l0, l0);
+      s1 = __fmaf_rn(a1, 1.0f - l1, l1);
+    }
   } else {
-    const float phi = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-    a = g * phi;
-    if (SLOPE) slope = phi + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+    const float f0 = 0.5f + 0.5f * erff(g0 * 0.70710678118654752f);
+    const float f1 = 0.5f + 0.5f * erff(g1 * 0.70710678118654752f);
+    a0 = g0 * f0;
+    a1 = g1 * f1;
+    if (SLOPE) {
+      s0 = __fmaf_rn(g0 * 0.39894228040143268f, ex2(g0 * g0 * -0.72134752044448170f), f0);
+      s1 = __fmaf_rn(g1 * 0.39894228040143268f, ex2(g1 * g1 * -0.72134752044448170f), f1);
+    }
   }
 }
 
@@ -119,218 +153,607 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// `rows` x `width` elements into panels; rows past the end of the input become
-// zero.  Columns past `width` were zeroed once and are never written.
+// ------------------------------------------------------------ shared pieces
+// Barriers of a CTA.  A wait that gives up raises `abort`, which makes every
+// other wait give up too; the roles then leave their loops, the CTA frees its
+// TMEM and returns, and the launch is counted in gs_wait_failures.
+struct Bars {
+  unsigned long long xfull[kMaxXStages], xempty[kMaxXStages];
+  unsigned long long wfull[kMaxWStages], wempty[kMaxWStages];
+  unsigned long long gfull[2], hfull[2], dhfull, sfree;  // sfree: dW's operand stage
+  unsigned long long yfull[2], yempty[2];
+  unsigned long long ofull, oempty;  // output stage
+  uint32_t tmem;
+  volatile int abort;
+};
+
+__device__ __forceinline__ bool wait_for(Bars* b, unsigned long long* bar, unsigned parity) {
+  for (int i = 0; i < (1 << 22); ++i) {
+    unsigned done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (b->abort) return false;
+  }
+  b->abort = 1;
+  return false;
+}
+__device__ __forceinline__ void arrive(unsigned long long* bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void init_bars(Bars* b) {
+  for (int i = 0; i < kMaxXStages; ++i) {
+    mbar_init(&b->xfull[i], kLoaders);
+    mbar_init(&b->xempty[i], 1);
+  }
+  for (int i = 0; i < kMaxWStages; ++i) {
+    mbar_init(&b->wfull[i], 1);
+    mbar_init(&b->wempty[i], 1);
+  }
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&b->gfull[i], 1);
+    mbar_init(&b->yfull[i], 1);
+    mbar_init(&b->yempty[i], 128);
+  }
+  mbar_init(&b->sfree, 1);
+  b->abort = 0;
+}
+
+// One tile of `rows` x `width` elements into panels, by the loader warps; rows
+// past the end of the input become zero.  Columns past `width` were zeroed
+// once and are never written.  16-byte units are copied asynchronously
+// (complete after cp.async.wait_group) where width and address allow.
 template <typename T>
-__device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows) {
-  if (width % 8 == 0 && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+__device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
+                                          bool vec) {
+  if (vec) {
     const int per_row = width >> 3;
-    for (int i = threadIdx.x; i < kTile * per_row; i += kDecodeThreads) {
-      const int row = i / per_row, unit = i - row * per_row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows) v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      *reinterpret_cast<uint4*>(panels + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7)) = v;
+    const uint32_t base = smem_addr(panels);
+    int row = l / per_row, unit = l - row * per_row;
+    const int drow = kLoaders / per_row, dunit = kLoaders - drow * per_row;
+    for (int i = l; i < kTile * per_row; i += kLoaders) {
+      const uint32_t dst = base + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
+      const int bytes = row < rows ? 16 : 0;  // 0: fill with zeros, nothing is read
+      const T* from = bytes ? src + (size_t)i * 8 : src;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+      row += drow;
+      unit += dunit;
+      if (unit >= per_row) {
+        unit -= per_row;
+        ++row;
+      }
     }
     return;
   }
-  for (int i = threadIdx.x; i < kTile * width; i += kDecodeThreads) {
-    const int row = i / width, col = i - row * width;
-    *reinterpret_cast<T*>(panels + (col >> 6) * kPanel + tc::panel_elem(row, col & 63)) =
-        row < rows ? src[i] : from_f32<T>(0.0f);
+  int row = l / width, col = l - row * width;
+  const int drow = kLoaders / width, dcol = kLoaders - drow * width;
+#pragma unroll 8
+  for (int i = l; i < kTile * width; i += kLoaders) {
+    const T v = row < rows ? src[i] : from_f32<T>(0.0f);
+    *reinterpret_cast<T*>(panels + (col >> 6) * kPanel + tc::panel_elem(row, col & 63)) = v;
+    row += drow;
+    col += dcol;
+    if (col >= width) {
+      col -= width;
+      ++row;
+    }
   }
 }
 
+// The loader warps' loop over this CTA's tiles.  With s stages, a tile is
+// handed over after the loads of the s - 2 following tiles have been issued.
+template <typename T, bool DY>
+__device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_t* stages, int stage_bytes,
+                                            int64_t first, int64_t step, int64_t tiles) {
+  const int l = threadIdx.x - 128;
+  const T* x = static_cast<const T*>(a.x);
+  const T* dy = static_cast<const T*>(a.dy);
+  const bool vx = a.d % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const bool vy = DY && a.c % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
+  const int lag = a.x_stages > 2 ? a.x_stages - 2 : 0;
+  int64_t it = 0, given = 0;
+  for (int64_t t = first; t < tiles; t += step, ++it) {
+    const int s = (int)(it % a.x_stages);
+    if (it >= a.x_stages && !wait_for(b, &b->xempty[s], (unsigned)(it / a.x_stages - 1) & 1)) break;
+    const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
+    uint8_t* xs = stages + s * stage_bytes;
+    load_tile<T>(xs, x + t * kTile * a.d, a.d, rows, l, vx);
+    if (DY) load_tile<T>(xs + a.nxp * kPanel, dy + t * kTile * a.c, a.c, rows, l, vy);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (it >= lag) {
+      if (lag == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else if (lag == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 2;" ::: "memory");
+      tc::fence_async_smem();
+      arrive(&b->xfull[given % a.x_stages]);
+      ++given;
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  tc::fence_async_smem();
+  for (; given < it; ++given) arrive(&b->xfull[given % a.x_stages]);
+}
+
+// --------------------------------------------------------- forward and dx
+// Per chunk q of the CTA's sequence of (tile, chunk):
+//   first products   [g | u] = x [Wg | Wu]^T  (and dh = dy Wd)  -> TMEM buffer q & 1
+//   activation       warpgroup q & 1: TMEM -> registers -> 16-bit operands,
+//                    written over the buffer's own columns
+//   second products  y += h Wd^T, or dx += [dg | du] [Wg ; Wu], A from TMEM
+// The first products of chunk q + 1 are issued before the second ones of q, so
+// the tensor core works while a warpgroup does.  Finished tiles are taken by
+// the warpgroups in turn, through shared memory to a bulk store: rows straight
+// from the registers would write one sector per thread and instruction.
 template <typename T, int MODE, int ACT>
 __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   extern __shared__ uint8_t raw[];
-  __shared__ unsigned long long bars[2];
-  __shared__ uint32_t tmem_slot;
-  uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  uint8_t* xs = smem;
-  uint8_t* ys = xs + a.nxp * kPanel;
-  uint8_t* ws = ys + (MODE == kFwd ? 0 : a.nyp * kPanel);
-  uint8_t* st = ws + a.chunk_bytes;  // dg, du, h panels (weight gradients)
-  unsigned long long* wbar = &bars[0];
-  unsigned long long* mbar = &bars[1];
+  __shared__ Bars bars;
+  Bars* b = &bars;
   constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+  constexpr uint32_t kBuf = MODE == kFwd ? 128 : 192;  // TMEM columns of a chunk: g, u (, dh)
+  constexpr uint32_t kOut = 2 * kBuf;
+  const int width = MODE == kFwd ? a.c : a.d, wp = MODE == kFwd ? a.cp : a.dp;
+  const int nout = wp <= (512 - (int)kOut) / 2 ? 2 : 1;  // accumulators of finished tiles
+  const uint32_t out_cols = (512 - kOut) / nout;
+  uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  const int stage_bytes = (a.nxp + (MODE == kFwd ? 0 : a.nyp)) * kPanel;
+  uint8_t* ws = smem + a.x_stages * stage_bytes;
+  uint8_t* os = ws + a.w_stages * a.chunk_bytes;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quarter = warp & 3, half = warp >> 2;
-  const int row = quarter * 32 + lane;
-  if (warp == 0) tc::tmem_alloc(&tmem_slot, kTmemCols);
+  if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
   if (threadIdx.x == 0) {
-    mbar_init(wbar, 1);
-    mbar_init(mbar, 1);
+    init_bars(b);
+    for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], 128);
+    mbar_init(&b->ofull, 128);
+    mbar_init(&b->oempty, 1);
   }
-  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - xs); i += kDecodeThreads * 16)
-    *reinterpret_cast<uint4*>(xs + i) = make_uint4(0, 0, 0, 0);
+  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDecodeThreads * 16)
+    *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
+  tc::fence_async_smem();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = tmem_slot;
-  const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-
+  const uint32_t tmem = b->tmem;
   const int64_t tiles = (a.n + kTile - 1) / kTile;
-  unsigned wphase = 0, mphase = 0;
-  bool ok = true, loaded = false;
-  const T* x = static_cast<const T*>(a.x);
-  const T* dy = static_cast<const T*>(a.dy);
+  const int64_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;  // tiles of this CTA
+  const int64_t total = mine * a.chunks;
+  const bool resident = a.w_stages >= a.chunks;
 
-  for (int64_t t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-    const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
-    load_tile<T>(xs, x + t * kTile * a.d, a.d, rows);
-    if (MODE != kFwd) load_tile<T>(ys, dy + t * kTile * a.c, a.c, rows);
-    tc::fence_async_smem();
-    __syncthreads();
-    const int j0 = MODE == kDw ? blockIdx.y : 0, j1 = MODE == kDw ? j0 + 1 : a.chunks;
-    for (int j = j0; j < j1; ++j) {
-      if (threadIdx.x == 0) {
-        if (!loaded || (MODE != kDw && a.chunks > 1)) {
-          mbar_arrive_expect_tx(wbar, a.chunk_bytes);
-          bulk_g2s(ws, a.image + (size_t)j * a.chunk_bytes, a.chunk_bytes, wbar);
-          ok = mbar_wait(wbar, wphase);
-          wphase ^= 1;
-        }
-        // first products: [g | u] = x [Wg | Wu]^T
-        const uint32_t wgu = smem_addr(ws), wdn = wgu + a.nxp * kPanel;
+  if (warp >= 4 && warp < 8) {
+    run_loaders<T, MODE != kFwd>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+  } else if (warp == 1) {
+    if (lane == 0) {  // weight chunks; all resident: loaded once
+      const int64_t loads = resident ? a.chunks : total;
+      for (int64_t q = 0; q < loads; ++q) {
+        const int s = (int)(q % a.w_stages);
+        if (q >= a.w_stages && !wait_for(b, &b->wempty[s], (unsigned)(q / a.w_stages - 1) & 1)) break;
+        mbar_arrive_expect_tx(&b->wfull[s], a.chunk_bytes);
+        bulk_g2s(ws + s * a.chunk_bytes, a.image + (q % a.chunks) * a.chunk_bytes, a.chunk_bytes, &b->wfull[s]);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 0) {
+    if (lane == 0) {
+      int64_t it1 = 0, it2 = 0;
+      int j1 = 0, j2 = 0;
+      bool ok = true;
+      const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
+      const uint32_t id2 = tc::instr_desc(kBf16, wp, false, MODE == kDx);
+      auto first_products = [&](int64_t q) {
+        const int xs = (int)(it1 % a.x_stages), s = (int)(q % a.w_stages);
+        if (j1 == 0) ok &= wait_for(b, &b->xfull[xs], (unsigned)(it1 / a.x_stages) & 1);
+        if (!resident || q < a.chunks) ok &= wait_for(b, &b->wfull[s], resident ? 0 : (unsigned)(q / a.w_stages) & 1);
+        if (!ok) return;
+        tc::fence_after();
+        const uint32_t xa = smem_addr(smem) + xs * stage_bytes, ya = xa + a.nxp * kPanel;
+        const uint32_t wgu = smem_addr(ws) + s * a.chunk_bytes, wdn = wgu + a.nxp * kPanel;
+        const uint32_t buf = tmem + (uint32_t)(q & 1) * kBuf;
         for (int k = 0; k < a.dp / 16; ++k) {
           const uint32_t at = (k >> 2) * kPanel + (k & 3) * 32;
-          tc::mma_ss(tmem + kColG, tc::desc_k(smem_addr(xs) + at), tc::desc_k(wgu + at),
-                     tc::instr_desc(kBf16, 128, false, false), k > 0);
+          tc::mma_ss(buf, tc::desc_k(xa + at), tc::desc_k(wgu + at), id1, k > 0);
         }
-        if (MODE != kFwd) {  // dh = dy Wd
+        if (MODE == kDx)
           for (int k = 0; k < a.cp / 16; ++k)
-            tc::mma_ss(tmem + kColDh, tc::desc_k(smem_addr(ys) + (k >> 2) * kPanel + (k & 3) * 32),
-                       tc::desc_mn(wdn + k * 2048, kPanel), tc::instr_desc(kBf16, 64, false, true), k > 0);
+            tc::mma_ss(buf + 128, tc::desc_k(ya + (k >> 2) * kPanel + (k & 3) * 32),
+                       tc::desc_mn(wdn + k * 2048, kPanel), idh, k > 0);
+        tc::commit(&b->gfull[q & 1]);
+        if (++j1 == a.chunks) {
+          tc::commit(&b->xempty[xs]);
+          j1 = 0;
+          ++it1;
         }
-        tc::commit(mbar);
-      }
-      loaded = true;
-      ok &= mbar_wait(mbar, mphase);
-      mphase ^= 1;
-      tc::fence_after();
-      uint32_t g[32], u[32], dh[32];
-      tc::tmem_ld32(lanes + kColG + half * 32, g);
-      tc::tmem_ld32(lanes + kColU + half * 32, u);
-      if (MODE != kFwd) tc::tmem_ld32(lanes + kColDh + half * 32, dh);
-      tc::tmem_wait_ld();
-      tc::after_wait(g);
-      tc::after_wait(u);
-      if (MODE != kFwd) tc::after_wait(dh);
-      uint32_t ph[16], pg[16], pu[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float a0, a1, s0, s1;
-        gate<ACT, MODE != kFwd>(__uint_as_float(g[2 * i]), a0, s0);
-        gate<ACT, MODE != kFwd>(__uint_as_float(g[2 * i + 1]), a1, s1);
-        const float u0 = __uint_as_float(u[2 * i]), u1 = __uint_as_float(u[2 * i + 1]);
-        if (MODE != kDx) ph[i] = pack2<T>(a0 * u0, a1 * u1);
-        if (MODE != kFwd) {
-          const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
-          pg[i] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
-          pu[i] = pack2<T>(d0 * a0, d1 * a1);
-        }
-      }
-      if (MODE == kFwd) {
-        tc::tmem_st16(lanes + kColH + half * 16, ph);
-        tc::tmem_wait_st();
-      } else if (MODE == kDx) {
-        tc::tmem_st16(lanes + kColH + half * 16, pg);
-        tc::tmem_st16(lanes + kColH + 32 + half * 16, pu);
-        tc::tmem_wait_st();
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t off = tc::panel_offset(row, half * 4 + q);
-          *reinterpret_cast<uint4*>(st + off) = make_uint4(pg[4 * q], pg[4 * q + 1], pg[4 * q + 2], pg[4 * q + 3]);
-          *reinterpret_cast<uint4*>(st + kPanel + off) =
-              make_uint4(pu[4 * q], pu[4 * q + 1], pu[4 * q + 2], pu[4 * q + 3]);
-          *reinterpret_cast<uint4*>(st + 2 * kPanel + off) =
-              make_uint4(ph[4 * q], ph[4 * q + 1], ph[4 * q + 2], ph[4 * q + 3]);
-        }
-        tc::fence_async_smem();
-      }
-      tc::fence_before();
-      ok = __syncthreads_and(ok);
-      if (!ok) break;
-      if (threadIdx.x == 0) {
+      };
+      if (total > 0) first_products(0);
+      for (int64_t q = 0; q < total && ok; ++q) {
+        if (q + 1 < total) first_products(q + 1);
+        const int s = (int)(q % a.w_stages), yb = (int)(it2 % nout);
+        if (j2 == 0 && it2 >= nout) ok &= wait_for(b, &b->yempty[yb], (unsigned)(it2 / nout - 1) & 1);
+        ok &= wait_for(b, &b->hfull[q & 1], (unsigned)(q >> 1) & 1);
+        if (!ok) break;
         tc::fence_after();
-        const uint32_t wgu = smem_addr(ws), wdn = wgu + a.nxp * kPanel;
-        if (MODE == kFwd) {  // y += h Wd^T
-          for (int k = 0; k < 4; ++k)
-            tc::mma_ts(tmem + kColOut, tmem + kColH + k * 8, tc::desc_k(wdn + k * 32),
-                       tc::instr_desc(kBf16, a.cp, false, false), j > 0 || k > 0);
-        } else if (MODE == kDx) {  // dx += [dg | du] [Wg ; Wu]
-          for (int k = 0; k < 8; ++k)
-            tc::mma_ts(tmem + kColOut, tmem + kColH + k * 8, tc::desc_mn(wgu + k * 2048, kPanel),
-                       tc::instr_desc(kBf16, a.dp, false, true), j > 0 || k > 0);
+        const uint32_t wgu = smem_addr(ws) + s * a.chunk_bytes, wdn = wgu + a.nxp * kPanel;
+        const uint32_t buf = tmem + (uint32_t)(q & 1) * kBuf, out = tmem + kOut + yb * out_cols;
+        if (MODE == kFwd) {
+          for (int k = 0; k < 4; ++k) tc::mma_ts(out, buf + k * 8, tc::desc_k(wdn + k * 32), id2, j2 > 0 || k > 0);
         } else {
-          const uint32_t sa = smem_addr(st);
-          const bool first = t == blockIdx.x;
-          for (int k = 0; k < 8; ++k)  // [dWg ; dWu] += [dg | du]^T x
-            tc::mma_ss(tmem + kColOut, tc::desc_mn(sa + k * 2048, kPanel), tc::desc_mn(smem_addr(xs) + k * 2048, kPanel),
-                       tc::instr_desc(kBf16, a.dp, true, true), !first || k > 0);
-          for (int m = 0; m < (a.c + 127) / 128; ++m)  // dWd += dy^T h
-            for (int k = 0; k < 8; ++k)
-              tc::mma_ss(tmem + kColOut + 128 + m * 64, tc::desc_mn(smem_addr(ys) + m * 2 * kPanel + k * 2048, kPanel),
-                         tc::desc_mn(sa + 2 * kPanel + k * 2048, kPanel), tc::instr_desc(kBf16, 64, true, true),
-                         !first || k > 0);
+          for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
+            tc::mma_ts(out, buf + (k >> 2) * 64 + (k & 3) * 8, tc::desc_mn(wgu + k * 2048, kPanel), id2,
+                       j2 > 0 || k > 0);
         }
-        tc::commit(mbar);
+        if (!resident) tc::commit(&b->wempty[s]);
+        if (++j2 == a.chunks) {
+          tc::commit(&b->yfull[yb]);
+          j2 = 0;
+          ++it2;
+        }
       }
-      ok &= mbar_wait(mbar, mphase);
-      mphase ^= 1;
-      tc::fence_after();
+      // Every issued instruction has finished when this phase completes.
+      if (!ok) tc::commit(&b->sfree);
     }
-    if (MODE != kDw && ok) {
-      const int width = MODE == kFwd ? a.c : a.d;
-      T* out = static_cast<T*>(a.out) + (t * kTile + row) * width;
-      for (int c0 = half * 32; c0 < width; c0 += 64) {
+    __syncwarp();
+  } else if (warp == 2) {
+    if (a.out_pitch && a.out_bulk) {  // finished tiles: output stage -> global memory
+      uint8_t* out = static_cast<uint8_t*>(a.out);
+      const int row_bytes = width * 2;
+      for (int64_t i = 0; i < mine; ++i) {
+        const int64_t t = blockIdx.x + i * gridDim.x;
+        if (!__all_sync(~0u, wait_for(b, &b->ofull, (unsigned)i & 1))) break;
+        const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
+        uint8_t* dst = out + t * kTile * row_bytes;
+        if (a.out_pitch != row_bytes) {  // padded rows, each a whole number of 16-byte units
+          for (int r = lane; r < rows; r += 32)
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)r * row_bytes),
+                         "r"(smem_addr(os + r * a.out_pitch)), "r"(row_bytes)
+                         : "memory");
+        } else {
+          const int bytes = rows * row_bytes & ~15;
+          if (lane == 0 && bytes > 0)
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(os)),
+                         "r"(bytes)
+                         : "memory");
+          for (int e = bytes + 2 * lane; e < rows * row_bytes; e += 64)
+            *reinterpret_cast<uint16_t*>(dst + e) = *reinterpret_cast<const uint16_t*>(os + e);
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive(&b->oempty);
+      }
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+  } else if (warp >= 8) {
+    const int wg = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    bool ok = true;
+    int64_t drained = wg;  // this warpgroup takes tiles wg, wg + 2, ...
+    auto drain = [&](int64_t i) {
+      const int yb = (int)(i % nout);
+      ok = wait_for(b, &b->yfull[yb], (unsigned)(i / nout) & 1);
+      if (ok && a.out_pitch && a.out_bulk && i > 0) ok = wait_for(b, &b->oempty, (unsigned)(i - 1) & 1);
+      ok = __all_sync(~0u, ok);
+      if (!ok) return;
+      tc::fence_after();
+      const int64_t t = blockIdx.x + i * gridDim.x;
+      const uint32_t src = lanes + kOut + yb * out_cols;
+      const bool staged = a.out_pitch && a.out_bulk;
+      const bool here = staged || t * kTile + row < a.n;
+      uint8_t* dst = staged ? os + row * a.out_pitch : static_cast<uint8_t*>(a.out) + (t * kTile + row) * width * 2;
+      for (int c0 = 0; c0 < width; c0 += 32) {
         uint32_t v[32];
-        tc::tmem_ld32(lanes + kColOut + c0, v);
+        __syncwarp();
+        tc::tmem_ld32(src + c0, v);
         tc::tmem_wait_ld();
         tc::after_wait(v);
-        if (row < rows)
+        uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c0 + i < width) out[c0 + i] = from_f32<T>(__uint_as_float(v[i]));
+        for (int e = 0; e < 16; ++e) w[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+        if (!here) continue;  // (rejoined by the __syncwarp above)
+        uint8_t* p = dst + c0 * 2;
+        const int left = width - c0;
+        if (a.out_vec == 16) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (8 * e < left)
+              *reinterpret_cast<uint4*>(p + 16 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        } else if (a.out_vec == 8) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (4 * e < left) *reinterpret_cast<uint2*>(p + 8 * e) = make_uint2(w[2 * e], w[2 * e + 1]);
+        } else if (a.out_vec == 4) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (2 * e < left) *reinterpret_cast<uint32_t*>(p + 4 * e) = w[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (e < left) *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+        }
+      }
+      __syncwarp();
+      tc::fence_before();
+      arrive(&b->yempty[yb]);
+      if (staged) {
+        tc::fence_async_smem();
+        arrive(&b->ofull);
+      }
+    };
+    for (int64_t q = wg; q < total && ok; q += 2) {
+      // A tile that ended two chunks ago is taken before this chunk, one that
+      // has only just ended after it (its last products are still running).
+      if (drained < mine && (drained + 1) * a.chunks < q) {
+        drain(drained);
+        drained += 2;
+        if (!ok) break;
+      }
+      ok = __all_sync(~0u, wait_for(b, &b->gfull[wg], (unsigned)(q >> 1) & 1));
+      if (!ok) break;
+      tc::fence_after();
+      const uint32_t buf = lanes + (uint32_t)wg * kBuf;
+      if (MODE == kFwd) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          uint32_t g[32], u[32], h[16];
+          tc::tmem_ld32(buf + p * 32, g);
+          tc::tmem_ld32(buf + 64 + p * 32, u);
+          tc::tmem_wait_ld();
+          tc::after_wait(g);
+          tc::after_wait(u);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a0, a1, s0, s1;
+            gate2<ACT, false>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, s0, s1);
+            h[i] = pack2<T>(a0 * __uint_as_float(u[2 * i]), a1 * __uint_as_float(u[2 * i + 1]));
+          }
+          tc::tmem_st16(buf + p * 16, h);
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          uint32_t g[16], u[16], dh[16], pg[8], pu[8];
+          tc::tmem_ld16(buf + p * 16, g);
+          tc::tmem_ld16(buf + 64 + p * 16, u);
+          tc::tmem_ld16(buf + 128 + p * 16, dh);
+          tc::tmem_wait_ld();
+          tc::after_wait(g);
+          tc::after_wait(u);
+          tc::after_wait(dh);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float a0, a1, s0, s1;
+            gate2<ACT, true>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, s0, s1);
+            const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
+            pg[i] = pack2<T>(d0 * __uint_as_float(u[2 * i]) * s0, d1 * __uint_as_float(u[2 * i + 1]) * s1);
+            pu[i] = pack2<T>(d0 * a0, d1 * a1);
+          }
+          tc::tmem_st8(buf + p * 8, pg);
+          tc::tmem_st8(buf + 64 + p * 8, pu);
+        }
+      }
+      tc::tmem_wait_st();
+      tc::fence_before();
+      arrive(&b->hfull[wg]);
+      if (drained < mine && (drained + 1) * a.chunks == q) {
+        drain(drained);
+        drained += 2;
       }
     }
-    tc::fence_before();
-    ok = __syncthreads_and(ok);
-    tc::fence_after();
-  }
-  if (MODE == kDw && ok) {
-    const size_t fd = (size_t)a.f * a.d;
-    float* part = a.partials + (size_t)blockIdx.x * (2 * fd + (size_t)a.c * a.f);
-    const int j = blockIdx.y;
-    const int h = j * kChunk + (row & 63);
-    float* gu = part + (row < 64 ? 0 : fd) + (size_t)h * a.d;
-    for (int c0 = half * 32; c0 < a.d; c0 += 64) {
-      uint32_t v[32];
-      tc::tmem_ld32(lanes + kColOut + c0, v);
-      tc::tmem_wait_ld();
-      tc::after_wait(v);
-      if (h < a.f)
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (c0 + i < a.d) gu[c0 + i] = __uint_as_float(v[i]);
+    while (ok && drained < mine) {
+      drain(drained);
+      drained += 2;
     }
-    for (int m = 0; m < (a.c + 127) / 128; ++m) {
-      uint32_t v[32];
-      tc::tmem_ld32(lanes + kColOut + 128 + m * 64 + half * 32, v);
-      tc::tmem_wait_ld();
-      tc::after_wait(v);
-      const int c = m * 128 + row, h0 = j * kChunk + half * 32;
-      if (c < a.c)
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (h0 + i < a.f) part[2 * fd + (size_t)c * a.f + h0 + i] = __uint_as_float(v[i]);
-    }
-    tc::fence_before();
   }
-  if (!ok && threadIdx.x == 0) atomicAdd(&g_decode_wait_failures, 1ull);
   __syncthreads();
+  if (b->abort) {  // what is in flight must end before the CTA does (bounded)
+    if (threadIdx.x == 0) {
+      atomicAdd(&g_decode_wait_failures, 1ull);
+      mbar_wait(&b->sfree, 0);
+      for (int i = 0; i < a.w_stages; ++i)
+        for (unsigned par = 0; par < 2; ++par) mbar_wait(&b->wfull[i], par);
+    }
+    __syncthreads();
+  }
+  if (warp == 0) tc::tmem_free(tmem, kTmemCols);
+}
+
+// --------------------------------------------------------- weight gradients
+// A CTA keeps one chunk's weights and walks tiles; per tile
+//   [g | u] = x [Wg | Wu]^T, dh = dy Wd         -> TMEM
+//   activation (both warpgroups, 32 hidden units each) -> dg, du, h panels in
+//                shared memory, rows = pixels
+//   [dWg ; dWu] += [dg | du]^T x,  dWd += dy^T h -> TMEM, summed over all tiles
+// The panels are K-major for nobody: both operands of the sums over pixels are
+// MN-major, x and dy from the same panels the first products read.  The next
+// tile's [g | u] is issued before this tile's sums.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
+  extern __shared__ uint8_t raw[];
+  __shared__ Bars bars;
+  Bars* b = &bars;
+  constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+  uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
+  const int stage_bytes = (a.nxp + a.nyp) * kPanel;
+  uint8_t* ws = smem + a.x_stages * stage_bytes;
+  uint8_t* st = ws + a.chunk_bytes;  // dg, du, h panels
+  const int mblocks = (a.c + 127) / 128;
+  const int acc_cols = (a.dp > 64 ? 128 : 64) + mblocks * 64;
+  const int nbuf = acc_cols <= 192 ? 2 : 1;  // [g | u] buffers
+  // TMEM: [g | u] at 0 (and 128), dh, the sums
+  const uint32_t col_dh = nbuf * 128, col_gu = col_dh + 64, col_dd = col_gu + (a.dp > 64 ? 128 : 64);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
+  if (threadIdx.x == 0) {
+    init_bars(b);
+    for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kEpilogue);
+    mbar_init(&b->dhfull, 1);
+  }
+  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDecodeThreads * 16)
+    *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
+  tc::fence_async_smem();
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = b->tmem;
+  const int64_t tiles = (a.n + kTile - 1) / kTile;
+  const int64_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;
+
+  if (warp >= 4 && warp < 8) {
+    run_loaders<T, true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+  } else if (warp == 0) {
+    if (lane == 0) {
+      bool ok = true;
+      mbar_arrive_expect_tx(&b->wfull[0], a.chunk_bytes);
+      bulk_g2s(ws, a.image + (size_t)blockIdx.y * a.chunk_bytes, a.chunk_bytes, &b->wfull[0]);
+      ok = wait_for(b, &b->wfull[0], 0);
+      const uint32_t wgu = smem_addr(ws), wdn = wgu + a.nxp * kPanel, sa = smem_addr(st);
+      const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
+      const uint32_t idg = tc::instr_desc(kBf16, a.dp, true, true), idd = tc::instr_desc(kBf16, 64, true, true);
+      auto gu_products = [&](int64_t i) {
+        const int xs = (int)(i % a.x_stages);
+        ok &= wait_for(b, &b->xfull[xs], (unsigned)(i / a.x_stages) & 1);
+        if (!ok) return;
+        tc::fence_after();
+        const uint32_t xa = smem_addr(smem) + xs * stage_bytes;
+        for (int k = 0; k < a.dp / 16; ++k) {
+          const uint32_t at = (k >> 2) * kPanel + (k & 3) * 32;
+          tc::mma_ss(tmem + (uint32_t)(i % nbuf) * 128, tc::desc_k(xa + at), tc::desc_k(wgu + at), id1, k > 0);
+        }
+      };
+      auto dh_products = [&](int64_t i) {
+        const uint32_t ya = smem_addr(smem) + (int)(i % a.x_stages) * stage_bytes + a.nxp * kPanel;
+        for (int k = 0; k < a.cp / 16; ++k)
+          tc::mma_ss(tmem + col_dh, tc::desc_k(ya + (k >> 2) * kPanel + (k & 3) * 32),
+                     tc::desc_mn(wdn + k * 2048, kPanel), idh, k > 0);
+        tc::commit(&b->dhfull);
+      };
+      if (mine > 0) {
+        gu_products(0);
+        if (ok) dh_products(0);
+      }
+      // nbuf = 2 needs the next tile's stage while this one's is in use
+      const bool ahead = nbuf == 2 && a.x_stages > 1;
+      for (int64_t i = 0; i < mine && ok; ++i) {
+        if (ahead && i + 1 < mine) gu_products(i + 1);
+        // tile i's g, u, dh have been read and its panels written
+        ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
+        if (!ok) break;
+        tc::fence_after();
+        if (ahead && i + 1 < mine) dh_products(i + 1);
+        const int xs = (int)(i % a.x_stages);
+        const uint32_t xa = smem_addr(smem) + xs * stage_bytes, ya = xa + a.nxp * kPanel;
+        for (int k = 0; k < 8; ++k)
+          tc::mma_ss(tmem + col_gu, tc::desc_mn(sa + k * 2048, kPanel), tc::desc_mn(xa + k * 2048, kPanel), idg,
+                     i > 0 || k > 0);
+        // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
+        for (int m = 0; m < mblocks; ++m)
+          for (int k = 0; k < 8; ++k)
+            tc::mma_ss(tmem + col_dd + m * 64, tc::desc_mn(ya + m * 2 * kPanel + k * 2048, kPanel),
+                       tc::desc_mn(sa + 2 * kPanel + k * 2048, kPanel), idd, i > 0 || k > 0);
+        tc::commit(&b->sfree);
+        tc::commit(&b->xempty[xs]);
+        if (!ahead && i + 1 < mine) {
+          gu_products(i + 1);
+          if (ok) dh_products(i + 1);
+        }
+      }
+      if (!ok) {
+        mbar_wait(&b->wfull[0], 0);
+        tc::commit(&b->yfull[0]);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    const int wg = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    bool ok = true;
+    for (int64_t i = 0; i < mine; ++i) {
+      ok = __all_sync(~0u, wait_for(b, &b->dhfull, (unsigned)i & 1));
+      if (!ok) break;
+      tc::fence_after();
+      const uint32_t buf = lanes + (uint32_t)(i % nbuf) * 128 + wg * 32;
+      uint32_t pg[16], pu[16], ph[16];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        uint32_t g[16], u[16], dh[16];
+        tc::tmem_ld16(buf + p * 16, g);
+        tc::tmem_ld16(buf + 64 + p * 16, u);
+        tc::tmem_ld16(lanes + col_dh + wg * 32 + p * 16, dh);
+        tc::tmem_wait_ld();
+        tc::after_wait(g);
+        tc::after_wait(u);
+        tc::after_wait(dh);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float a0, a1, s0, s1;
+          gate2<ACT, true>(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), a0, a1, s0, s1);
+          const float u0 = __uint_as_float(u[2 * e]), u1 = __uint_as_float(u[2 * e + 1]);
+          const float d0 = __uint_as_float(dh[2 * e]), d1 = __uint_as_float(dh[2 * e + 1]);
+          pg[8 * p + e] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
+          pu[8 * p + e] = pack2<T>(d0 * a0, d1 * a1);
+          ph[8 * p + e] = pack2<T>(a0 * u0, a1 * u1);
+        }
+      }
+      // the previous tile's sums have read the panels
+      if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
+      if (!ok) break;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t off = tc::panel_offset(row, wg * 4 + q);
+        *reinterpret_cast<uint4*>(st + off) = make_uint4(pg[4 * q], pg[4 * q + 1], pg[4 * q + 2], pg[4 * q + 3]);
+        *reinterpret_cast<uint4*>(st + kPanel + off) = make_uint4(pu[4 * q], pu[4 * q + 1], pu[4 * q + 2], pu[4 * q + 3]);
+        *reinterpret_cast<uint4*>(st + 2 * kPanel + off) =
+            make_uint4(ph[4 * q], ph[4 * q + 1], ph[4 * q + 2], ph[4 * q + 3]);
+      }
+      tc::fence_async_smem();
+      tc::fence_before();
+      arrive(&b->hfull[0]);
+    }
+    if (ok && mine > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(mine - 1) & 1));
+    if (ok && mine > 0) {
+      tc::fence_after();
+      const size_t fd = (size_t)a.f * a.d;
+      float* part = a.partials + (size_t)blockIdx.x * (2 * fd + (size_t)a.c * a.f);
+      const int h = blockIdx.y * kChunk + (row & 63);
+      float* gu = part + (row < 64 ? 0 : fd) + (size_t)h * a.d;
+      for (int c0 = wg * 32; c0 < a.d; c0 += 64) {
+        uint32_t v[32];
+        __syncwarp();
+        tc::tmem_ld32(lanes + col_gu + c0, v);
+        tc::tmem_wait_ld();
+        tc::after_wait(v);
+        if (h < a.f)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (c0 + e < a.d) gu[c0 + e] = __uint_as_float(v[e]);
+      }
+      for (int m = 0; m < mblocks; ++m) {
+        uint32_t v[32];
+        __syncwarp();
+        tc::tmem_ld32(lanes + col_dd + m * 64 + wg * 32, v);
+        tc::tmem_wait_ld();
+        tc::after_wait(v);
+        const int c = m * 128 + row, h0 = blockIdx.y * kChunk + wg * 32;
+        if (c < a.c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            if (h0 + e < a.f) part[2 * fd + (size_t)c * a.f + h0 + e] = __uint_as_float(v[e]);
+      }
+      tc::fence_before();
+    }
+  }
+  __syncthreads();
+  if (b->abort) {  // what is in flight must end before the CTA does (bounded)
+    if (threadIdx.x == 0) {
+      atomicAdd(&g_decode_wait_failures, 1ull);
+      mbar_wait(&b->yfull[0], 0);
+    }
+    __syncthreads();
+  }
   if (warp == 0) tc::tmem_free(tmem, kTmemCols);
 }
 
@@ -386,15 +809,58 @@ static DecodeArgs decode_args(const void* x, const void* dy, int64_t n, int d, i
   return a;
 }
 
+// Shared memory of a launch: input stages, weight stages, output stage.  Weight
+// chunks are kept resident if they all fit beside two input stages; else at
+// least two stages stream them.  What is left goes to further input stages.
+template <int MODE>
+static size_t plan_smem(DecodeArgs& a) {
+  const size_t fixed = 1024 + sizeof(Bars) + 64;
+  const size_t in = (size_t)(a.nxp + (MODE == kFwd ? 0 : a.nyp)) * kPanel;
+  if (MODE == kDw) {
+    const size_t own = fixed + a.chunk_bytes + 3 * (size_t)kPanel;
+    a.w_stages = 1;
+    a.x_stages = (int)std::min<size_t>(kMaxXStages, (kMaxSmem - own) / in);
+    return own + a.x_stages * in - sizeof(Bars);
+  }
+  const int width = MODE == kFwd ? a.c : a.d, row = width * 2;
+  // Stage rows are padded to an odd number of 16-byte units where that keeps
+  // 16-byte stores (width a multiple of 8, one bulk copy a row); otherwise the
+  // stage is the output's own layout (one bulk copy a tile), whose rows are an
+  // odd number of out_vec bytes apart: no bank conflicts either way.
+  a.out_vec = width % 8 == 0 ? 16 : width % 4 == 0 ? 8 : width % 2 == 0 ? 4 : 2;
+  a.out_pitch = width % 8 == 0 ? (row / 16 | 1) * 16 : row;
+  a.out_bulk = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  size_t out = a.out_bulk ? ((size_t)kTile * a.out_pitch + 15) & ~(size_t)15 : 0;
+  const int need = std::min(a.chunks, 2);
+  a.x_stages = 2;
+  if (fixed + out + 2 * in + (size_t)need * a.chunk_bytes > kMaxSmem) a.x_stages = 1;
+  if (fixed + out + in + (size_t)need * a.chunk_bytes > kMaxSmem) {
+    out = 0;
+    a.x_stages = fixed + 2 * in + (size_t)need * a.chunk_bytes > kMaxSmem ? 1 : 2;
+  }
+  if (!out) {
+    a.out_pitch = 0;
+    a.out_bulk = 0;
+    // rows of the caller's own output: its alignment bounds the store size
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.out);
+    while (a.out_vec > 2 && at % a.out_vec) a.out_vec /= 2;
+  }
+  const size_t left = kMaxSmem - fixed - out - a.x_stages * in;
+  a.w_stages = (int)std::min<size_t>(std::min(a.chunks, kMaxWStages), left / a.chunk_bytes);
+  while (a.x_stages >= 2 && a.x_stages < kMaxXStages &&
+         fixed + out + (a.x_stages + 1) * in + (size_t)a.w_stages * a.chunk_bytes <= kMaxSmem)
+    ++a.x_stages;
+  return fixed - sizeof(Bars) + out + a.x_stages * in + (size_t)a.w_stages * a.chunk_bytes;
+}
+
 template <typename T, int MODE, int ACT>
-static int launch_decode_as(const DecodeArgs& a, dim3 grid, cudaStream_t s) {
-  size_t smem = 1024 + (size_t)a.nxp * kPanel + a.chunk_bytes;
-  if (MODE != kFwd) smem += (size_t)a.nyp * kPanel;
-  if (MODE == kDw) smem += 3 * (size_t)kPanel;
-  smem = std::max<size_t>(smem, 120 * 1024);  // one CTA per SM: each takes all of TMEM
-  cudaError_t e = cudaFuncSetAttribute(k_decode<T, MODE, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+static int launch_decode_as(DecodeArgs a, dim3 grid, cudaStream_t s) {
+  // one CTA per SM: each takes all of TMEM
+  const size_t smem = std::max<size_t>(plan_smem<MODE>(a), 120 * 1024);
+  auto* kernel = MODE == kDw ? k_decode_dw<T, ACT> : k_decode<T, MODE == kDx ? kDx : kFwd, ACT>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_decode: %s", cudaGetErrorString(e));
-  k_decode<T, MODE, ACT><<<grid, kDecodeThreads, smem, s>>>(a);
+  kernel<<<grid, kDecodeThreads, smem, s>>>(a);
   return check_launch("k_decode");
 }
 
