@@ -181,6 +181,19 @@ __device__ __forceinline__ bool wait_for(Bars* b, unsigned long long* bar, unsig
   b->abort = 1;
   return false;
 }
+// Position in a ring of stages: the stage, and the parity of the phase that
+// fills it (a consumer waits for `parity`, a producer for its complement, which
+// the first round passes at once).
+struct Ring {
+  int at = 0;
+  unsigned parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++at == stages) {
+      at = 0;
+      parity ^= 1;
+    }
+  }
+};
 __device__ __forceinline__ void arrive(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
@@ -205,43 +218,89 @@ __device__ __forceinline__ void init_bars(Bars* b) {
 
 // One tile of `rows` x `width` elements into panels, by the loader warps; rows
 // past the end of the input become zero.  Columns past `width` were zeroed
-// once and are never written.  16-byte units are copied asynchronously
-// (complete after cp.async.wait_group) where width and address allow.
-template <typename T>
-__device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
-                                          bool vec) {
-  if (vec) {
-    const int per_row = width >> 3;
-    const uint32_t base = smem_addr(panels);
-    int row = l / per_row, unit = l - row * per_row;
-    const int drow = kLoaders / per_row, dunit = kLoaders - drow * per_row;
-    for (int i = l; i < kTile * per_row; i += kLoaders) {
-      const uint32_t dst = base + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
-      const int bytes = row < rows ? 16 : 0;  // 0: fill with zeros, nothing is read
-      const T* from = bytes ? src + (size_t)i * 8 : src;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
-      row += drow;
-      unit += dunit;
-      if (unit >= per_row) {
-        unit -= per_row;
-        ++row;
-      }
-    }
-    return;
-  }
-  int row = l / width, col = l - row * width;
-  const int drow = kLoaders / width, dcol = kLoaders - drow * width;
-#pragma unroll 8
-  for (int i = l; i < kTile * width; i += kLoaders) {
-    const T v = row < rows ? src[i] : from_f32<T>(0.0f);
-    *reinterpret_cast<T*>(panels + (col >> 6) * kPanel + tc::panel_elem(row, col & 63)) = v;
+// once and are never written.  Units of UNIT bytes (16, 8 or 4, the largest
+// that divides a row and the address) are copied asynchronously (complete after
+// cp.async.wait_group): a unit never straddles a row or a 16-byte unit of the
+// panel, and nothing waits for memory.
+template <int UNIT, typename T>
+__device__ __forceinline__ void copy_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l) {
+  constexpr int kElems = UNIT / 2;
+  const int per_row = width / kElems;
+  const uint32_t base = smem_addr(panels);
+  int row = l / per_row, unit = l - row * per_row;
+  const int drow = kLoaders / per_row, dunit = kLoaders - drow * per_row;
+  const char* from = reinterpret_cast<const char*>(src) + l * UNIT;
+#pragma unroll 4
+  for (int i = l; i < kTile * per_row; i += kLoaders) {
+    const int col = unit * kElems;
+    const uint32_t dst = base + (col >> 6) * kPanel + tc::panel_elem(row, col & 63);
+    const int bytes = row < rows ? UNIT : 0;  // 0: fill with zeros, nothing is read
+    const char* at = bytes ? from : reinterpret_cast<const char*>(src);
+    if (UNIT == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(at), "r"(bytes) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(at), "r"(bytes), "n"(UNIT)
+                   : "memory");
+    from += kLoaders * UNIT;
     row += drow;
-    col += dcol;
-    if (col >= width) {
-      col -= width;
+    unit += dunit;
+    if (unit >= per_row) {
+      unit -= per_row;
       ++row;
     }
   }
+}
+
+// Odd widths: 16 bytes are read at once (the tile is one contiguous block;
+// `aligned`: it starts on a 16-byte boundary) and stored element by element.
+template <typename T>
+__device__ __forceinline__ void scatter_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
+                                             bool aligned16) {
+  constexpr int kBatch = 4;
+  const int total = kTile * width, have = rows * width;  // a multiple of 8
+  const T zero = from_f32<T>(0.0f);
+  for (int i0 = l * 8; i0 < total; i0 += kLoaders * 8 * kBatch) {
+    __align__(16) T v[kBatch][8];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int i = i0 + q * kLoaders * 8;
+      if (aligned16 && i + 8 <= have) {
+        *reinterpret_cast<uint4*>(v[q]) = __ldg(reinterpret_cast<const uint4*>(src + i));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[q][e] = i + e < have ? src[i + e] : zero;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const int i = i0 + q * kLoaders * 8;
+      if (i >= total) break;
+      int row = i / width, col = i - row * width;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        *reinterpret_cast<T*>(panels + (col >> 6) * kPanel + tc::panel_elem(row, col & 63)) = v[q][e];
+        if (++col == width) {
+          col = 0;
+          ++row;
+        }
+      }
+    }
+  }
+}
+
+// The largest copy unit of rows of `width` elements at p: 16, 8, 4 or 2 bytes.
+__device__ __forceinline__ int copy_unit(const void* p, int width) {
+  const uintptr_t m = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(width * 2);
+  return (m & 15) == 0 ? 16 : (m & 7) == 0 ? 8 : (m & 3) == 0 ? 4 : 2;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
+                                          int unit) {
+  if (unit == 16) copy_tile<16>(panels, src, width, rows, l);
+  else if (unit == 8) copy_tile<8>(panels, src, width, rows, l);
+  else if (unit == 4) copy_tile<4>(panels, src, width, rows, l);
+  else scatter_tile(panels, src, width, rows, l, (reinterpret_cast<uintptr_t>(src) & 15) == 0);
 }
 
 // The loader warps' loop over this CTA's tiles.  With s stages, a tile is
@@ -252,30 +311,34 @@ __device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_
   const int l = threadIdx.x - 128;
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
-  const bool vx = a.d % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  const bool vy = DY && a.c % 8 == 0 && (reinterpret_cast<uintptr_t>(dy) & 15) == 0;
+  const int vx = copy_unit(x, a.d), vy = DY ? copy_unit(dy, a.c) : 0;
   const int lag = a.x_stages > 2 ? a.x_stages - 2 : 0;
-  int64_t it = 0, given = 0;
-  for (int64_t t = first; t < tiles; t += step, ++it) {
-    const int s = (int)(it % a.x_stages);
-    if (it >= a.x_stages && !wait_for(b, &b->xempty[s], (unsigned)(it / a.x_stages - 1) & 1)) break;
+  Ring fill, give;
+  int pending = 0;  // tiles issued and not handed over
+  for (int64_t t = first; t < tiles; t += step) {
+    if (!wait_for(b, &b->xempty[fill.at], fill.parity ^ 1)) break;
     const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
-    uint8_t* xs = stages + s * stage_bytes;
+    uint8_t* xs = stages + fill.at * stage_bytes;
     load_tile<T>(xs, x + t * kTile * a.d, a.d, rows, l, vx);
     if (DY) load_tile<T>(xs + a.nxp * kPanel, dy + t * kTile * a.c, a.c, rows, l, vy);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    if (it >= lag) {
+    fill.next(a.x_stages);
+    if (++pending > lag) {
       if (lag == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
       else if (lag == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
       else asm volatile("cp.async.wait_group 2;" ::: "memory");
       tc::fence_async_smem();
-      arrive(&b->xfull[given % a.x_stages]);
-      ++given;
+      arrive(&b->xfull[give.at]);
+      give.next(a.x_stages);
+      --pending;
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   tc::fence_async_smem();
-  for (; given < it; ++given) arrive(&b->xfull[given % a.x_stages]);
+  for (; pending > 0; --pending) {
+    arrive(&b->xfull[give.at]);
+    give.next(a.x_stages);
+  }
 }
 
 // --------------------------------------------------------- forward and dx
@@ -329,68 +392,84 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   } else if (warp == 1) {
     if (lane == 0) {  // weight chunks; all resident: loaded once
       const int64_t loads = resident ? a.chunks : total;
+      Ring w;
+      int j = 0;
       for (int64_t q = 0; q < loads; ++q) {
-        const int s = (int)(q % a.w_stages);
-        if (q >= a.w_stages && !wait_for(b, &b->wempty[s], (unsigned)(q / a.w_stages - 1) & 1)) break;
-        mbar_arrive_expect_tx(&b->wfull[s], a.chunk_bytes);
-        bulk_g2s(ws + s * a.chunk_bytes, a.image + (q % a.chunks) * a.chunk_bytes, a.chunk_bytes, &b->wfull[s]);
+        if (!wait_for(b, &b->wempty[w.at], w.parity ^ 1)) break;
+        mbar_arrive_expect_tx(&b->wfull[w.at], a.chunk_bytes);
+        bulk_g2s(ws + w.at * a.chunk_bytes, a.image + (size_t)j * a.chunk_bytes, a.chunk_bytes, &b->wfull[w.at]);
+        w.next(a.w_stages);
+        if (++j == a.chunks) j = 0;
       }
     }
     __syncwarp();
   } else if (warp == 0) {
     if (lane == 0) {
-      int64_t it1 = 0, it2 = 0;
+      // This thread's instructions bound short tiles: counters instead of
+      // divisions, descriptors advanced by adding to their address field.
+      Ring x, w1, w2, y;
       int j1 = 0, j2 = 0;
-      bool ok = true;
+      bool ok = true, wait_w = true;
       const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
       const uint32_t id2 = tc::instr_desc(kBf16, wp, false, MODE == kDx);
-      auto first_products = [&](int64_t q) {
-        const int xs = (int)(it1 % a.x_stages), s = (int)(q % a.w_stages);
-        if (j1 == 0) ok &= wait_for(b, &b->xfull[xs], (unsigned)(it1 / a.x_stages) & 1);
-        if (!resident || q < a.chunks) ok &= wait_for(b, &b->wfull[s], resident ? 0 : (unsigned)(q / a.w_stages) & 1);
+      const uint64_t x0 = tc::desc_k(smem_addr(smem)), wk0 = tc::desc_k(smem_addr(ws));
+      const uint64_t wn0 = tc::desc_mn(smem_addr(ws), kPanel);
+      const uint32_t xstep = stage_bytes >> 4, wstep = a.chunk_bytes >> 4, wdn = a.nxp * (kPanel >> 4);
+      const int k1 = a.dp / 16, kh = a.cp / 16;
+      auto first_products = [&](uint32_t buf, unsigned long long* done) {
+        if (j1 == 0) ok &= wait_for(b, &b->xfull[x.at], x.parity);
+        if (wait_w) ok &= wait_for(b, &b->wfull[w1.at], w1.parity);
         if (!ok) return;
         tc::fence_after();
-        const uint32_t xa = smem_addr(smem) + xs * stage_bytes, ya = xa + a.nxp * kPanel;
-        const uint32_t wgu = smem_addr(ws) + s * a.chunk_bytes, wdn = wgu + a.nxp * kPanel;
-        const uint32_t buf = tmem + (uint32_t)(q & 1) * kBuf;
-        for (int k = 0; k < a.dp / 16; ++k) {
-          const uint32_t at = (k >> 2) * kPanel + (k & 3) * 32;
-          tc::mma_ss(buf, tc::desc_k(xa + at), tc::desc_k(wgu + at), id1, k > 0);
+        const uint64_t xd = x0 + x.at * xstep, wk = wk0 + w1.at * wstep;
+#pragma unroll 4
+        for (int k = 0; k < k1; ++k) {
+          const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
+          tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
         }
-        if (MODE == kDx)
-          for (int k = 0; k < a.cp / 16; ++k)
-            tc::mma_ss(buf + 128, tc::desc_k(ya + (k >> 2) * kPanel + (k & 3) * 32),
-                       tc::desc_mn(wdn + k * 2048, kPanel), idh, k > 0);
-        tc::commit(&b->gfull[q & 1]);
+        if (MODE == kDx) {
+          const uint64_t yd = xd + wdn, wn = wn0 + w1.at * wstep + wdn;
+#pragma unroll 4
+          for (int k = 0; k < kh; ++k)
+            tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+        }
+        tc::commit(done);
+        w1.next(a.w_stages);
         if (++j1 == a.chunks) {
-          tc::commit(&b->xempty[xs]);
+          tc::commit(&b->xempty[x.at]);
+          x.next(a.x_stages);
           j1 = 0;
-          ++it1;
+          if (resident) wait_w = false;
         }
       };
-      if (total > 0) first_products(0);
+      first_products(tmem, &b->gfull[0]);
+      unsigned qb = 0, qphase = 0;  // chunk's buffer and its phase
       for (int64_t q = 0; q < total && ok; ++q) {
-        if (q + 1 < total) first_products(q + 1);
-        const int s = (int)(q % a.w_stages), yb = (int)(it2 % nout);
-        if (j2 == 0 && it2 >= nout) ok &= wait_for(b, &b->yempty[yb], (unsigned)(it2 / nout - 1) & 1);
-        ok &= wait_for(b, &b->hfull[q & 1], (unsigned)(q >> 1) & 1);
+        if (q + 1 < total) first_products(tmem + (qb ^ 1) * kBuf, &b->gfull[qb ^ 1]);
+        if (j2 == 0) ok &= wait_for(b, &b->yempty[y.at], y.parity ^ 1);
+        ok &= wait_for(b, &b->hfull[qb], qphase);
         if (!ok) break;
         tc::fence_after();
-        const uint32_t wgu = smem_addr(ws) + s * a.chunk_bytes, wdn = wgu + a.nxp * kPanel;
-        const uint32_t buf = tmem + (uint32_t)(q & 1) * kBuf, out = tmem + kOut + yb * out_cols;
+        const uint32_t buf = tmem + qb * kBuf, out = tmem + kOut + y.at * out_cols;
         if (MODE == kFwd) {
-          for (int k = 0; k < 4; ++k) tc::mma_ts(out, buf + k * 8, tc::desc_k(wdn + k * 32), id2, j2 > 0 || k > 0);
+          const uint64_t wk = wk0 + w2.at * wstep + wdn;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc::mma_ts(out, buf + k * 8, wk + k * 2, id2, j2 > 0 || k > 0);
         } else {
+          const uint64_t wn = wn0 + w2.at * wstep;
+#pragma unroll
           for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
-            tc::mma_ts(out, buf + (k >> 2) * 64 + (k & 3) * 8, tc::desc_mn(wgu + k * 2048, kPanel), id2,
-                       j2 > 0 || k > 0);
+            tc::mma_ts(out, buf + (k >> 2) * 64 + (k & 3) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
         }
-        if (!resident) tc::commit(&b->wempty[s]);
+        if (!resident) tc::commit(&b->wempty[w2.at]);
+        w2.next(a.w_stages);
         if (++j2 == a.chunks) {
-          tc::commit(&b->yfull[yb]);
+          tc::commit(&b->yfull[y.at]);
+          y.next(nout);
           j2 = 0;
-          ++it2;
         }
+        qb ^= 1;
+        if (qb == 0) qphase ^= 1;
       }
       // Every issued instruction has finished when this phase completes.
       if (!ok) tc::commit(&b->sfree);
@@ -431,9 +510,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     bool ok = true;
     int64_t drained = wg;  // this warpgroup takes tiles wg, wg + 2, ...
+    int64_t ends = (int64_t)(wg + 1) * a.chunks;  // the chunk after that tile's last
     auto drain = [&](int64_t i) {
-      const int yb = (int)(i % nout);
-      ok = wait_for(b, &b->yfull[yb], (unsigned)(i / nout) & 1);
+      const int yb = nout == 2 ? (int)(i & 1) : 0;
+      ok = wait_for(b, &b->yfull[yb], (unsigned)(nout == 2 ? i >> 1 : i) & 1);
       if (ok && a.out_pitch && a.out_bulk && i > 0) ok = wait_for(b, &b->oempty, (unsigned)(i - 1) & 1);
       ok = __all_sync(~0u, ok);
       if (!ok) return;
@@ -485,9 +565,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
     for (int64_t q = wg; q < total && ok; q += 2) {
       // A tile that ended two chunks ago is taken before this chunk, one that
       // has only just ended after it (its last products are still running).
-      if (drained < mine && (drained + 1) * a.chunks < q) {
+      if (drained < mine && ends < q) {
         drain(drained);
         drained += 2;
+        ends += 2 * a.chunks;
         if (!ok) break;
       }
       ok = __all_sync(~0u, wait_for(b, &b->gfull[wg], (unsigned)(q >> 1) & 1));
@@ -537,9 +618,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
       tc::tmem_wait_st();
       tc::fence_before();
       arrive(&b->hfull[wg]);
-      if (drained < mine && (drained + 1) * a.chunks == q) {
+      if (drained < mine && ends == q) {
         drain(drained);
         drained += 2;
+        ends += 2 * a.chunks;
       }
     }
     while (ok && drained < mine) {
@@ -610,55 +692,61 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
       mbar_arrive_expect_tx(&b->wfull[0], a.chunk_bytes);
       bulk_g2s(ws, a.image + (size_t)blockIdx.y * a.chunk_bytes, a.chunk_bytes, &b->wfull[0]);
       ok = wait_for(b, &b->wfull[0], 0);
-      const uint32_t wgu = smem_addr(ws), wdn = wgu + a.nxp * kPanel, sa = smem_addr(st);
       const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
       const uint32_t idg = tc::instr_desc(kBf16, a.dp, true, true), idd = tc::instr_desc(kBf16, 64, true, true);
-      auto gu_products = [&](int64_t i) {
-        const int xs = (int)(i % a.x_stages);
-        ok &= wait_for(b, &b->xfull[xs], (unsigned)(i / a.x_stages) & 1);
+      const uint32_t xstep = stage_bytes >> 4, ypart = a.nxp * (kPanel >> 4);
+      const uint64_t xk0 = tc::desc_k(smem_addr(smem)), xn0 = tc::desc_mn(smem_addr(smem), kPanel);
+      const uint64_t wk = tc::desc_k(smem_addr(ws)), wn = tc::desc_mn(smem_addr(ws), kPanel) + ypart;
+      const uint64_t gn = tc::desc_mn(smem_addr(st), kPanel), hn = gn + 2 * (kPanel >> 4);
+      const int k1 = a.dp / 16, kh = a.cp / 16;
+      Ring xg, xh, xs;  // stages of the next [g | u], dh and sums
+      unsigned gb = 0;
+      auto gu_products = [&]() {
+        ok &= wait_for(b, &b->xfull[xg.at], xg.parity);
         if (!ok) return;
         tc::fence_after();
-        const uint32_t xa = smem_addr(smem) + xs * stage_bytes;
-        for (int k = 0; k < a.dp / 16; ++k) {
-          const uint32_t at = (k >> 2) * kPanel + (k & 3) * 32;
-          tc::mma_ss(tmem + (uint32_t)(i % nbuf) * 128, tc::desc_k(xa + at), tc::desc_k(wgu + at), id1, k > 0);
+        const uint64_t xd = xk0 + xg.at * xstep;
+#pragma unroll 4
+        for (int k = 0; k < k1; ++k) {
+          const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
+          tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
         }
+        xg.next(a.x_stages);
+        if (nbuf == 2) gb ^= 1;
       };
-      auto dh_products = [&](int64_t i) {
-        const uint32_t ya = smem_addr(smem) + (int)(i % a.x_stages) * stage_bytes + a.nxp * kPanel;
-        for (int k = 0; k < a.cp / 16; ++k)
-          tc::mma_ss(tmem + col_dh, tc::desc_k(ya + (k >> 2) * kPanel + (k & 3) * 32),
-                     tc::desc_mn(wdn + k * 2048, kPanel), idh, k > 0);
+      auto dh_products = [&]() {
+        const uint64_t yd = xk0 + xh.at * xstep + ypart;
+#pragma unroll 4
+        for (int k = 0; k < kh; ++k)
+          tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
         tc::commit(&b->dhfull);
+        xh.next(a.x_stages);
       };
-      if (mine > 0) {
-        gu_products(0);
-        if (ok) dh_products(0);
-      }
+      gu_products();
+      if (ok) dh_products();
       // nbuf = 2 needs the next tile's stage while this one's is in use
       const bool ahead = nbuf == 2 && a.x_stages > 1;
       for (int64_t i = 0; i < mine && ok; ++i) {
-        if (ahead && i + 1 < mine) gu_products(i + 1);
+        if (ahead && i + 1 < mine) gu_products();
         // tile i's g, u, dh have been read and its panels written
         ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
         if (!ok) break;
         tc::fence_after();
-        if (ahead && i + 1 < mine) dh_products(i + 1);
-        const int xs = (int)(i % a.x_stages);
-        const uint32_t xa = smem_addr(smem) + xs * stage_bytes, ya = xa + a.nxp * kPanel;
-        for (int k = 0; k < 8; ++k)
-          tc::mma_ss(tmem + col_gu, tc::desc_mn(sa + k * 2048, kPanel), tc::desc_mn(xa + k * 2048, kPanel), idg,
-                     i > 0 || k > 0);
+        if (ahead && i + 1 < mine) dh_products();
+        const uint64_t xd = xn0 + xs.at * xstep, yd = xd + ypart;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) tc::mma_ss(tmem + col_gu, gn + k * 128, xd + k * 128, idg, i > 0 || k > 0);
         // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
         for (int m = 0; m < mblocks; ++m)
+#pragma unroll
           for (int k = 0; k < 8; ++k)
-            tc::mma_ss(tmem + col_dd + m * 64, tc::desc_mn(ya + m * 2 * kPanel + k * 2048, kPanel),
-                       tc::desc_mn(sa + 2 * kPanel + k * 2048, kPanel), idd, i > 0 || k > 0);
+            tc::mma_ss(tmem + col_dd + m * 64, yd + m * 2 * (kPanel >> 4) + k * 128, hn + k * 128, idd, i > 0 || k > 0);
         tc::commit(&b->sfree);
-        tc::commit(&b->xempty[xs]);
+        tc::commit(&b->xempty[xs.at]);
+        xs.next(a.x_stages);
         if (!ahead && i + 1 < mine) {
-          gu_products(i + 1);
-          if (ok) dh_products(i + 1);
+          gu_products();
+          if (ok) dh_products();
         }
       }
       if (!ok) {
@@ -675,7 +763,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
       ok = __all_sync(~0u, wait_for(b, &b->dhfull, (unsigned)i & 1));
       if (!ok) break;
       tc::fence_after();
-      const uint32_t buf = lanes + (uint32_t)(i % nbuf) * 128 + wg * 32;
+      const uint32_t buf = lanes + (nbuf == 2 ? (uint32_t)(i & 1) * 128 : 0) + wg * 32;
       uint32_t pg[16], pu[16], ph[16];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
