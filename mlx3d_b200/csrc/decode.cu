@@ -216,74 +216,63 @@ __device__ __forceinline__ void init_bars(Bars* b) {
   b->abort = 0;
 }
 
-// One tile of `rows` x `width` elements into panels, by the loader warps; rows
-// past the end of the input become zero.  Columns past `width` were zeroed
-// once and are never written.  Units of UNIT bytes (16, 8 or 4, the largest
-// that divides a row and the address) are copied asynchronously (complete after
-// cp.async.wait_group): a unit never straddles a row or a 16-byte unit of the
-// panel, and nothing waits for memory.
-template <int UNIT, typename T>
-__device__ __forceinline__ void copy_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l) {
-  constexpr int kElems = UNIT / 2;
-  const int per_row = width / kElems;
+// One tile of `rows` x `width` elements into panels, by the loader warps, one
+// 16-byte unit of a panel row at a time: consecutive lanes read consecutive
+// addresses.  Rows past the end of the input become zero; columns past `width`
+// were zeroed once and are never written.  A unit is 16 / PART asynchronous
+// copies (complete after cp.async.wait_group) of PART bytes, the largest power
+// of two that divides a row and the address, so nothing waits for memory; rows
+// of odd width (PART = 2) go through registers.
+template <int PART, typename T>
+__device__ __forceinline__ void load_tile_by(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l) {
+  const int per_row = (width + 7) >> 3;
   const uint32_t base = smem_addr(panels);
   int row = l / per_row, unit = l - row * per_row;
   const int drow = kLoaders / per_row, dunit = kLoaders - drow * per_row;
-  const char* from = reinterpret_cast<const char*>(src) + l * UNIT;
-#pragma unroll 4
-  for (int i = l; i < kTile * per_row; i += kLoaders) {
-    const int col = unit * kElems;
-    const uint32_t dst = base + (col >> 6) * kPanel + tc::panel_elem(row, col & 63);
-    const int bytes = row < rows ? UNIT : 0;  // 0: fill with zeros, nothing is read
-    const char* at = bytes ? from : reinterpret_cast<const char*>(src);
-    if (UNIT == 16)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(at), "r"(bytes) : "memory");
-    else
-      asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(at), "r"(bytes), "n"(UNIT)
-                   : "memory");
-    from += kLoaders * UNIT;
-    row += drow;
-    unit += dunit;
-    if (unit >= per_row) {
-      unit -= per_row;
-      ++row;
-    }
-  }
-}
-
-// Odd widths: 16 bytes are read at once (the tile is one contiguous block;
-// `aligned`: it starts on a 16-byte boundary) and stored element by element.
-template <typename T>
-__device__ __forceinline__ void scatter_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
-                                             bool aligned16) {
-  constexpr int kBatch = 4;
-  const int total = kTile * width, have = rows * width;  // a multiple of 8
-  const T zero = from_f32<T>(0.0f);
-  for (int i0 = l * 8; i0 < total; i0 += kLoaders * 8 * kBatch) {
-    __align__(16) T v[kBatch][8];
+  constexpr int kBatch = PART == 2 ? 4 : 1;
+  while (row < kTile) {
+    if (PART > 2) {
+      const uint32_t dst = base + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
+      const T* from = src + (row < rows ? row * width + unit * 8 : 0);
+      const int bytes = row < rows ? PART : 0;  // 0: fill with zeros, nothing is read
+      const int left = width - unit * 8;
 #pragma unroll
-    for (int q = 0; q < kBatch; ++q) {
-      const int i = i0 + q * kLoaders * 8;
-      if (aligned16 && i + 8 <= have) {
-        *reinterpret_cast<uint4*>(v[q]) = __ldg(reinterpret_cast<const uint4*>(src + i));
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[q][e] = i + e < have ? src[i + e] : zero;
+      for (int e = 0; e < 16 / PART; ++e) {
+        if (PART < 16 && e * (PART / 2) >= left) break;
+        if (PART == 16)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst + e * PART),
+                       "l"(from + (bytes ? e * (PART / 2) : 0)), "r"(bytes), "n"(PART)
+                       : "memory");
       }
-    }
+      row += drow;
+      unit += dunit;
+      if (unit >= per_row) {
+        unit -= per_row;
+        ++row;
+      }
+    } else {
+      __align__(16) T v[kBatch][8];
+      uint32_t off[kBatch];
+      int left[kBatch];
 #pragma unroll
-    for (int q = 0; q < kBatch; ++q) {
-      const int i = i0 + q * kLoaders * 8;
-      if (i >= total) break;
-      int row = i / width, col = i - row * width;
+      for (int q = 0; q < kBatch; ++q) {
+        left[q] = row < kTile ? width - unit * 8 : 0;
+        off[q] = (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
+        const T* from = src + row * width + unit * 8;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        *reinterpret_cast<T*>(panels + (col >> 6) * kPanel + tc::panel_elem(row, col & 63)) = v[q][e];
-        if (++col == width) {
-          col = 0;
+        for (int e = 0; e < 8; ++e) v[q][e] = row < rows && e < left[q] ? from[e] : from_f32<T>(0.0f);
+        row += drow;
+        unit += dunit;
+        if (unit >= per_row) {
+          unit -= per_row;
           ++row;
         }
       }
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q)
+        if (left[q] > 0) *reinterpret_cast<uint4*>(panels + off[q]) = *reinterpret_cast<const uint4*>(v[q]);
     }
   }
 }
@@ -297,10 +286,10 @@ __device__ __forceinline__ int copy_unit(const void* p, int width) {
 template <typename T>
 __device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
                                           int unit) {
-  if (unit == 16) copy_tile<16>(panels, src, width, rows, l);
-  else if (unit == 8) copy_tile<8>(panels, src, width, rows, l);
-  else if (unit == 4) copy_tile<4>(panels, src, width, rows, l);
-  else scatter_tile(panels, src, width, rows, l, (reinterpret_cast<uintptr_t>(src) & 15) == 0);
+  if (unit == 16) load_tile_by<16>(panels, src, width, rows, l);
+  else if (unit == 8) load_tile_by<8>(panels, src, width, rows, l);
+  else if (unit == 4) load_tile_by<4>(panels, src, width, rows, l);
+  else load_tile_by<2>(panels, src, width, rows, l);
 }
 
 // The loader warps' loop over this CTA's tiles.  With s stages, a tile is
@@ -367,7 +356,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   uint8_t* ws = smem + a.x_stages * stage_bytes;
   uint8_t* os = ws + a.w_stages * a.chunk_bytes;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
   if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
   if (threadIdx.x == 0) {
     init_bars(b);
@@ -404,9 +393,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
     }
     __syncwarp();
   } else if (warp == 0) {
-    if (lane == 0) {
-      // This thread's instructions bound short tiles: counters instead of
-      // divisions, descriptors advanced by adding to their address field.
+    {
+      // This warp's instructions bound short tiles: counters instead of
+      // divisions, descriptors advanced by adding to their address field.  All
+      // lanes run the loop, one issues.
       Ring x, w1, w2, y;
       int j1 = 0, j2 = 0;
       bool ok = true, wait_w = true;
@@ -419,24 +409,30 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
       auto first_products = [&](uint32_t buf, unsigned long long* done) {
         if (j1 == 0) ok &= wait_for(b, &b->xfull[x.at], x.parity);
         if (wait_w) ok &= wait_for(b, &b->wfull[w1.at], w1.parity);
+        ok = __all_sync(~0u, ok);
         if (!ok) return;
         tc::fence_after();
         const uint64_t xd = x0 + x.at * xstep, wk = wk0 + w1.at * wstep;
+        const bool last = j1 + 1 == a.chunks;
+        if (tc::elect_one()) {
 #pragma unroll 4
-        for (int k = 0; k < k1; ++k) {
-          const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-          tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
-        }
-        if (MODE == kDx) {
-          const uint64_t yd = xd + wdn, wn = wn0 + w1.at * wstep + wdn;
+          for (int k = 0; k < k1; ++k) {
+            const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
+            tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
+          }
+          if (MODE == kDx) {
+            const uint64_t yd = xd + wdn, wn = wn0 + w1.at * wstep + wdn;
 #pragma unroll 4
-          for (int k = 0; k < kh; ++k)
-            tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+            for (int k = 0; k < kh; ++k)
+              tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+          }
+          tc::commit(done);
+          if (last) tc::commit(&b->xempty[x.at]);
         }
-        tc::commit(done);
+        __syncwarp();
         w1.next(a.w_stages);
-        if (++j1 == a.chunks) {
-          tc::commit(&b->xempty[x.at]);
+        ++j1;
+        if (last) {
           x.next(a.x_stages);
           j1 = 0;
           if (resident) wait_w = false;
@@ -448,23 +444,29 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         if (q + 1 < total) first_products(tmem + (qb ^ 1) * kBuf, &b->gfull[qb ^ 1]);
         if (j2 == 0) ok &= wait_for(b, &b->yempty[y.at], y.parity ^ 1);
         ok &= wait_for(b, &b->hfull[qb], qphase);
+        ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
         const uint32_t buf = tmem + qb * kBuf, out = tmem + kOut + y.at * out_cols;
-        if (MODE == kFwd) {
-          const uint64_t wk = wk0 + w2.at * wstep + wdn;
+        const bool last = j2 + 1 == a.chunks;
+        if (tc::elect_one()) {
+          if (MODE == kFwd) {
+            const uint64_t wk = wk0 + w2.at * wstep + wdn;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc::mma_ts(out, buf + k * 8, wk + k * 2, id2, j2 > 0 || k > 0);
-        } else {
-          const uint64_t wn = wn0 + w2.at * wstep;
+            for (int k = 0; k < 4; ++k) tc::mma_ts(out, buf + k * 8, wk + k * 2, id2, j2 > 0 || k > 0);
+          } else {
+            const uint64_t wn = wn0 + w2.at * wstep;
 #pragma unroll
-          for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
-            tc::mma_ts(out, buf + (k >> 2) * 64 + (k & 3) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
+            for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
+              tc::mma_ts(out, buf + (k >> 2) * 64 + (k & 3) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
+          }
+          if (!resident) tc::commit(&b->wempty[w2.at]);
+          if (last) tc::commit(&b->yfull[y.at]);
         }
-        if (!resident) tc::commit(&b->wempty[w2.at]);
+        __syncwarp();
         w2.next(a.w_stages);
-        if (++j2 == a.chunks) {
-          tc::commit(&b->yfull[y.at]);
+        ++j2;
+        if (last) {
           y.next(nout);
           j2 = 0;
         }
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         if (qb == 0) qphase ^= 1;
       }
       // Every issued instruction has finished when this phase completes.
-      if (!ok) tc::commit(&b->sfree);
+      if (!ok && tc::elect_one()) tc::commit(&b->sfree);
     }
     __syncwarp();
   } else if (warp == 2) {
@@ -667,7 +669,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
   // TMEM: [g | u] at 0 (and 128), dh, the sums
   const uint32_t col_dh = nbuf * 128, col_gu = col_dh + 64, col_dd = col_gu + (a.dp > 64 ? 128 : 64);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
   if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
   if (threadIdx.x == 0) {
     init_bars(b);
@@ -687,10 +689,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
   if (warp >= 4 && warp < 8) {
     run_loaders<T, true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
   } else if (warp == 0) {
-    if (lane == 0) {
+    {
       bool ok = true;
-      mbar_arrive_expect_tx(&b->wfull[0], a.chunk_bytes);
-      bulk_g2s(ws, a.image + (size_t)blockIdx.y * a.chunk_bytes, a.chunk_bytes, &b->wfull[0]);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&b->wfull[0], a.chunk_bytes);
+        bulk_g2s(ws, a.image + (size_t)blockIdx.y * a.chunk_bytes, a.chunk_bytes, &b->wfull[0]);
+      }
+      __syncwarp();
       ok = wait_for(b, &b->wfull[0], 0);
       const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
       const uint32_t idg = tc::instr_desc(kBf16, a.dp, true, true), idd = tc::instr_desc(kBf16, 64, true, true);
@@ -703,23 +708,30 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
       unsigned gb = 0;
       auto gu_products = [&]() {
         ok &= wait_for(b, &b->xfull[xg.at], xg.parity);
+        ok = __all_sync(~0u, ok);
         if (!ok) return;
         tc::fence_after();
         const uint64_t xd = xk0 + xg.at * xstep;
+        if (tc::elect_one()) {
 #pragma unroll 4
-        for (int k = 0; k < k1; ++k) {
-          const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-          tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
+          for (int k = 0; k < k1; ++k) {
+            const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
+            tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
+          }
         }
+        __syncwarp();
         xg.next(a.x_stages);
         if (nbuf == 2) gb ^= 1;
       };
       auto dh_products = [&]() {
         const uint64_t yd = xk0 + xh.at * xstep + ypart;
+        if (tc::elect_one()) {
 #pragma unroll 4
-        for (int k = 0; k < kh; ++k)
-          tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
-        tc::commit(&b->dhfull);
+          for (int k = 0; k < kh; ++k)
+            tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+          tc::commit(&b->dhfull);
+        }
+        __syncwarp();
         xh.next(a.x_stages);
       };
       gu_products();
@@ -730,19 +742,24 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
         if (ahead && i + 1 < mine) gu_products();
         // tile i's g, u, dh have been read and its panels written
         ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
+        ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
         if (ahead && i + 1 < mine) dh_products();
         const uint64_t xd = xn0 + xs.at * xstep, yd = xd + ypart;
+        if (tc::elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) tc::mma_ss(tmem + col_gu, gn + k * 128, xd + k * 128, idg, i > 0 || k > 0);
-        // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
-        for (int m = 0; m < mblocks; ++m)
+          for (int k = 0; k < 8; ++k) tc::mma_ss(tmem + col_gu, gn + k * 128, xd + k * 128, idg, i > 0 || k > 0);
+          // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
+          for (int m = 0; m < mblocks; ++m)
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            tc::mma_ss(tmem + col_dd + m * 64, yd + m * 2 * (kPanel >> 4) + k * 128, hn + k * 128, idd, i > 0 || k > 0);
-        tc::commit(&b->sfree);
-        tc::commit(&b->xempty[xs.at]);
+            for (int k = 0; k < 8; ++k)
+              tc::mma_ss(tmem + col_dd + m * 64, yd + m * 2 * (kPanel >> 4) + k * 128, hn + k * 128, idd,
+                         i > 0 || k > 0);
+          tc::commit(&b->sfree);
+          tc::commit(&b->xempty[xs.at]);
+        }
+        __syncwarp();
         xs.next(a.x_stages);
         if (!ahead && i + 1 < mine) {
           gu_products();
@@ -751,7 +768,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
       }
       if (!ok) {
         mbar_wait(&b->wfull[0], 0);
-        tc::commit(&b->yfull[0]);
+        if (tc::elect_one()) tc::commit(&b->yfull[0]);
       }
     }
     __syncwarp();

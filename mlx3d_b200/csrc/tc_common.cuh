@@ -47,6 +47,15 @@ __host__ __device__ constexpr uint32_t instr_desc(bool bf16, int n, bool a_mn, b
          ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 
+// True in one lane of a converged warp.  Matrix instructions are issued under
+// this by warps whose control flow is uniform, so that their descriptors stay in
+// uniform registers; under `lane == 0` each costs about 110 cycles to issue.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(p));
+  return p != 0;
+}
+
 // D[128 x N] (TMEM) (+)= A (smem) B (smem), K = 16.  One thread issues.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
