@@ -21,9 +21,11 @@ namespace gs {
 constexpr int kTile = 128;              // rows of a tile (M of the matrix instructions)
 constexpr int kChunk = 64;              // hidden units of a chunk
 constexpr int kPanel = kTile * 128;     // bytes of a 128-row panel
-constexpr int kDecodeThreads = 512;
+constexpr int kDecodeThreads = 640;     // forward and dx; the weight gradients have no drain warps
+constexpr int kDwThreads = 512;
 constexpr int kLoaders = 128;           // warps 4-7
 constexpr int kEpilogue = 256;          // warps 8-15, two warpgroups
+constexpr int kDrain = 128;             // warps 16-19
 constexpr int kMaxXStages = 4, kMaxWStages = 16;
 constexpr uint32_t kTmemCols = 512;
 constexpr size_t kMaxSmem = 232448;     // 227 KB
@@ -210,7 +212,7 @@ __device__ __forceinline__ void init_bars(Bars* b) {
   for (int i = 0; i < 2; ++i) {
     mbar_init(&b->gfull[i], 1);
     mbar_init(&b->yfull[i], 1);
-    mbar_init(&b->yempty[i], 128);
+    mbar_init(&b->yempty[i], kDrain);
   }
   mbar_init(&b->sfree, 1);
   b->abort = 0;
@@ -219,60 +221,70 @@ __device__ __forceinline__ void init_bars(Bars* b) {
 // One tile of `rows` x `width` elements into panels, by the loader warps, one
 // 16-byte unit of a panel row at a time: consecutive lanes read consecutive
 // addresses.  Rows past the end of the input become zero; columns past `width`
-// were zeroed once and are never written.  A unit is 16 / PART asynchronous
-// copies (complete after cp.async.wait_group) of PART bytes, the largest power
-// of two that divides a row and the address, so nothing waits for memory; rows
-// of odd width (PART = 2) go through registers.
+// were zeroed once and are never written.  PART is the largest power of two
+// that divides a row's bytes and the address.  Whole units (PART = 16) are
+// copied asynchronously (complete after cp.async.wait_group); smaller parts are
+// gathered in registers, several units at a time: asynchronous copies of 4
+// bytes run at under two a cycle and SM (6000 cycles for 128 rows of 150).
+template <int PART>
+struct PartType {};
+template <>
+struct PartType<8> { using type = uint2; };
+template <>
+struct PartType<4> { using type = uint32_t; };
+template <>
+struct PartType<2> { using type = uint16_t; };
+
 template <int PART, typename T>
 __device__ __forceinline__ void load_tile_by(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l) {
   const int per_row = (width + 7) >> 3;
   const uint32_t base = smem_addr(panels);
   int row = l / per_row, unit = l - row * per_row;
   const int drow = kLoaders / per_row, dunit = kLoaders - drow * per_row;
-  constexpr int kBatch = PART == 2 ? 4 : 1;
-  while (row < kTile) {
-    if (PART > 2) {
+  auto advance = [&]() {
+    row += drow;
+    unit += dunit;
+    if (unit >= per_row) {
+      unit -= per_row;
+      ++row;
+    }
+  };
+  if constexpr (PART == 16) {
+#pragma unroll 4
+    while (row < kTile) {
       const uint32_t dst = base + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
       const T* from = src + (row < rows ? row * width + unit * 8 : 0);
-      const int bytes = row < rows ? PART : 0;  // 0: fill with zeros, nothing is read
-      const int left = width - unit * 8;
-#pragma unroll
-      for (int e = 0; e < 16 / PART; ++e) {
-        if (PART < 16 && e * (PART / 2) >= left) break;
-        if (PART == 16)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
-        else
-          asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst + e * PART),
-                       "l"(from + (bytes ? e * (PART / 2) : 0)), "r"(bytes), "n"(PART)
-                       : "memory");
-      }
-      row += drow;
-      unit += dunit;
-      if (unit >= per_row) {
-        unit -= per_row;
-        ++row;
-      }
-    } else {
-      __align__(16) T v[kBatch][8];
-      uint32_t off[kBatch];
-      int left[kBatch];
+      const int bytes = row < rows ? 16 : 0;  // 0: fill with zeros, nothing is read
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
+      advance();
+    }
+  } else {
+    using Part = typename PartType<PART>::type;
+    constexpr int kParts = 16 / PART, kBatch = PART == 2 ? 5 : 10;
+    while (row < kTile) {
+      union {
+        Part part[kParts];
+        uint4 all;
+      } v[kBatch];
+      const int row0 = row, unit0 = unit;
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
-        left[q] = row < kTile ? width - unit * 8 : 0;
-        off[q] = (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
-        const T* from = src + row * width + unit * 8;
+        v[q].all = make_uint4(0, 0, 0, 0);
+        const Part* from = reinterpret_cast<const Part*>(src + row * width + unit * 8);
+        const int left = row < rows ? width - unit * 8 : 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[q][e] = row < rows && e < left[q] ? from[e] : from_f32<T>(0.0f);
-        row += drow;
-        unit += dunit;
-        if (unit >= per_row) {
-          unit -= per_row;
-          ++row;
-        }
+        for (int e = 0; e < kParts; ++e)
+          if (e * (PART / 2) < left) v[q].part[e] = __ldg(from + e);
+        advance();
       }
+      row = row0;
+      unit = unit0;
 #pragma unroll
-      for (int q = 0; q < kBatch; ++q)
-        if (left[q] > 0) *reinterpret_cast<uint4*>(panels + off[q]) = *reinterpret_cast<const uint4*>(v[q]);
+      for (int q = 0; q < kBatch; ++q) {
+        if (row < kTile)
+          *reinterpret_cast<uint4*>(panels + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7)) = v[q].all;
+        advance();
+      }
     }
   }
 }
@@ -330,16 +342,38 @@ __device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_
   }
 }
 
+// 32 columns of an output row (or `left`, if fewer), in stores of `vec` bytes.
+__device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16], int left, int vec) {
+  if (vec == 16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (8 * e < left)
+        *reinterpret_cast<uint4*>(p + 16 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+  } else if (vec == 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (4 * e < left) *reinterpret_cast<uint2*>(p + 8 * e) = make_uint2(w[2 * e], w[2 * e + 1]);
+  } else if (vec == 4) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+      if (2 * e < left) *reinterpret_cast<uint32_t*>(p + 4 * e) = w[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      if (e < left) *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+  }
+}
+
 // --------------------------------------------------------- forward and dx
 // Per chunk q of the CTA's sequence of (tile, chunk):
 //   first products   [g | u] = x [Wg | Wu]^T  (and dh = dy Wd)  -> TMEM buffer q & 1
-//   activation       warpgroup q & 1: TMEM -> registers -> 16-bit operands,
-//                    written over the buffer's own columns
+//   activation       two warpgroups, 32 hidden units each: TMEM -> registers ->
+//                    16-bit operands, written over the buffer's own columns
 //   second products  y += h Wd^T, or dx += [dg | du] [Wg ; Wu], A from TMEM
 // The first products of chunk q + 1 are issued before the second ones of q, so
-// the tensor core works while a warpgroup does.  Finished tiles are taken by
-// the warpgroups in turn, through shared memory to a bulk store: rows straight
-// from the registers would write one sector per thread and instruction.
+// the tensor core works while the warpgroups do.  Finished tiles are taken by
+// four drain warps, through shared memory to a bulk store: rows straight from
+// the registers would write one sector per thread and instruction.
 template <typename T, int MODE, int ACT>
 __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   extern __shared__ uint8_t raw[];
@@ -360,8 +394,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
   if (threadIdx.x == 0) {
     init_bars(b);
-    for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], 128);
-    mbar_init(&b->ofull, 128);
+    for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kEpilogue);
+    mbar_init(&b->ofull, kDrain);
     mbar_init(&b->oempty, 1);
   }
   for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDecodeThreads * 16)
@@ -415,16 +449,16 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         const uint64_t xd = x0 + x.at * xstep, wk = wk0 + w1.at * wstep;
         const bool last = j1 + 1 == a.chunks;
         if (tc::elect_one()) {
-#pragma unroll 4
-          for (int k = 0; k < k1; ++k) {
+#pragma unroll
+          for (int k = 0; k < GS_DECODE_MAX_D / 16; ++k) {
             const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-            tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
+            if (k < k1) tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
           }
           if (MODE == kDx) {
             const uint64_t yd = xd + wdn, wn = wn0 + w1.at * wstep + wdn;
-#pragma unroll 4
-            for (int k = 0; k < kh; ++k)
-              tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+#pragma unroll
+            for (int k = 0; k < GS_DECODE_MAX_C / 16; ++k)
+              if (k < kh) tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
           }
           tc::commit(done);
           if (last) tc::commit(&b->xempty[x.at]);
@@ -453,12 +487,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
           if (MODE == kFwd) {
             const uint64_t wk = wk0 + w2.at * wstep + wdn;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) tc::mma_ts(out, buf + k * 8, wk + k * 2, id2, j2 > 0 || k > 0);
+            for (int k = 0; k < 4; ++k)  // h in the columns of g, 16 of each 32
+              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wk + k * 2, id2, j2 > 0 || k > 0);
           } else {
             const uint64_t wn = wn0 + w2.at * wstep;
 #pragma unroll
             for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
-              tc::mma_ts(out, buf + (k >> 2) * 64 + (k & 3) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
+              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
           }
           if (!resident) tc::commit(&b->wempty[w2.at]);
           if (last) tc::commit(&b->yfull[y.at]);
@@ -507,128 +542,92 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
       }
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-  } else if (warp >= 8) {
-    const int wg = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+  } else if (warp >= 16) {  // finished tiles: TMEM -> output stage (or global memory)
+    const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    bool ok = true;
-    int64_t drained = wg;  // this warpgroup takes tiles wg, wg + 2, ...
-    int64_t ends = (int64_t)(wg + 1) * a.chunks;  // the chunk after that tile's last
-    auto drain = [&](int64_t i) {
-      const int yb = nout == 2 ? (int)(i & 1) : 0;
-      ok = wait_for(b, &b->yfull[yb], (unsigned)(nout == 2 ? i >> 1 : i) & 1);
-      if (ok && a.out_pitch && a.out_bulk && i > 0) ok = wait_for(b, &b->oempty, (unsigned)(i - 1) & 1);
-      ok = __all_sync(~0u, ok);
-      if (!ok) return;
+    const bool staged = a.out_pitch && a.out_bulk;
+    Ring y;
+    for (int64_t i = 0; i < mine; ++i) {
+      bool ok = wait_for(b, &b->yfull[y.at], y.parity);
+      if (ok && staged) ok = wait_for(b, &b->oempty, (unsigned)(i & 1) ^ 1);
+      if (!__all_sync(~0u, ok)) break;
       tc::fence_after();
       const int64_t t = blockIdx.x + i * gridDim.x;
-      const uint32_t src = lanes + kOut + yb * out_cols;
-      const bool staged = a.out_pitch && a.out_bulk;
+      const uint32_t src = lanes + kOut + y.at * out_cols;
       const bool here = staged || t * kTile + row < a.n;
-      uint8_t* dst = staged ? os + row * a.out_pitch : static_cast<uint8_t*>(a.out) + (t * kTile + row) * width * 2;
-      for (int c0 = 0; c0 < width; c0 += 32) {
-        uint32_t v[32];
-        __syncwarp();
-        tc::tmem_ld32(src + c0, v);
+      uint8_t* p = staged ? os + row * a.out_pitch : static_cast<uint8_t*>(a.out) + (t * kTile + row) * width * 2;
+      uint32_t v[32];
+      tc::tmem_ld32(src, v);
+      for (int c0 = 0; c0 < width; c0 += 32, p += 64) {
+        uint32_t w[16];
         tc::tmem_wait_ld();
         tc::after_wait(v);
-        uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) w[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
-        if (!here) continue;  // (rejoined by the __syncwarp above)
-        uint8_t* p = dst + c0 * 2;
-        const int left = width - c0;
-        if (a.out_vec == 16) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (8 * e < left)
-              *reinterpret_cast<uint4*>(p + 16 * e) = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
-        } else if (a.out_vec == 8) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (4 * e < left) *reinterpret_cast<uint2*>(p + 8 * e) = make_uint2(w[2 * e], w[2 * e + 1]);
-        } else if (a.out_vec == 4) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (2 * e < left) *reinterpret_cast<uint32_t*>(p + 4 * e) = w[e];
+        __syncwarp();
+        if (c0 + 32 < width) {
+          tc::tmem_ld32(src + c0 + 32, v);
         } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (e < left) *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+          tc::fence_before();
+          arrive(&b->yempty[y.at]);
         }
+        if (here) store_row32(p, w, width - c0, a.out_vec);
       }
       __syncwarp();
-      tc::fence_before();
-      arrive(&b->yempty[yb]);
       if (staged) {
         tc::fence_async_smem();
         arrive(&b->ofull);
       }
-    };
-    for (int64_t q = wg; q < total && ok; q += 2) {
-      // A tile that ended two chunks ago is taken before this chunk, one that
-      // has only just ended after it (its last products are still running).
-      if (drained < mine && ends < q) {
-        drain(drained);
-        drained += 2;
-        ends += 2 * a.chunks;
-        if (!ok) break;
-      }
-      ok = __all_sync(~0u, wait_for(b, &b->gfull[wg], (unsigned)(q >> 1) & 1));
-      if (!ok) break;
+      y.next(nout);
+    }
+  } else if (warp >= 8) {  // activation: each warpgroup half of a chunk's hidden units
+    const int wg = (warp >> 2) & 1;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    Ring q;
+    for (int64_t i = 0; i < total; ++i) {
+      if (!__all_sync(~0u, wait_for(b, &b->gfull[q.at], q.parity))) break;
       tc::fence_after();
-      const uint32_t buf = lanes + (uint32_t)wg * kBuf;
-      if (MODE == kFwd) {
+      const uint32_t buf = lanes + (uint32_t)q.at * kBuf + wg * 32;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          uint32_t g[32], u[32], h[16];
-          tc::tmem_ld32(buf + p * 32, g);
-          tc::tmem_ld32(buf + 64 + p * 32, u);
+      for (int p = 0; p < 2; ++p) {
+        uint32_t g[16], u[16], h[8];
+        tc::tmem_ld16(buf + p * 16, g);
+        tc::tmem_ld16(buf + 64 + p * 16, u);
+        if constexpr (MODE == kFwd) {
           tc::tmem_wait_ld();
           tc::after_wait(g);
           tc::after_wait(u);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int e = 0; e < 8; ++e) {
             float a0, a1, s0, s1;
-            gate2<ACT, false>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, s0, s1);
-            h[i] = pack2<T>(a0 * __uint_as_float(u[2 * i]), a1 * __uint_as_float(u[2 * i + 1]));
+            gate2<ACT, false>(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), a0, a1, s0, s1);
+            h[e] = pack2<T>(a0 * __uint_as_float(u[2 * e]), a1 * __uint_as_float(u[2 * e + 1]));
           }
-          tc::tmem_st16(buf + p * 16, h);
-        }
-      } else {
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          uint32_t g[16], u[16], dh[16], pg[8], pu[8];
-          tc::tmem_ld16(buf + p * 16, g);
-          tc::tmem_ld16(buf + 64 + p * 16, u);
+          // over columns of g that this warp has read: 32 wg .. 32 wg + 15
+          tc::tmem_st8(buf + p * 8, h);
+        } else {
+          uint32_t dh[16], du[8];
           tc::tmem_ld16(buf + 128 + p * 16, dh);
           tc::tmem_wait_ld();
           tc::after_wait(g);
           tc::after_wait(u);
           tc::after_wait(dh);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
+          for (int e = 0; e < 8; ++e) {
             float a0, a1, s0, s1;
-            gate2<ACT, true>(__uint_as_float(g[2 * i]), __uint_as_float(g[2 * i + 1]), a0, a1, s0, s1);
-            const float d0 = __uint_as_float(dh[2 * i]), d1 = __uint_as_float(dh[2 * i + 1]);
-            pg[i] = pack2<T>(d0 * __uint_as_float(u[2 * i]) * s0, d1 * __uint_as_float(u[2 * i + 1]) * s1);
-            pu[i] = pack2<T>(d0 * a0, d1 * a1);
+            gate2<ACT, true>(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), a0, a1, s0, s1);
+            const float d0 = __uint_as_float(dh[2 * e]), d1 = __uint_as_float(dh[2 * e + 1]);
+            h[e] = pack2<T>(d0 * __uint_as_float(u[2 * e]) * s0, d1 * __uint_as_float(u[2 * e + 1]) * s1);
+            du[e] = pack2<T>(d0 * a0, d1 * a1);
           }
-          tc::tmem_st8(buf + p * 8, pg);
-          tc::tmem_st8(buf + 64 + p * 8, pu);
+          tc::tmem_st8(buf + p * 8, h);        // dg over g
+          tc::tmem_st8(buf + 64 + p * 8, du);  // du over u
         }
       }
       tc::tmem_wait_st();
       tc::fence_before();
-      arrive(&b->hfull[wg]);
-      if (drained < mine && ends == q) {
-        drain(drained);
-        drained += 2;
-        ends += 2 * a.chunks;
-      }
-    }
-    while (ok && drained < mine) {
-      drain(drained);
-      drained += 2;
+      arrive(&b->hfull[q.at]);
+      q.next(2);
     }
   }
   __syncthreads();
@@ -654,7 +653,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
 // MN-major, x and dy from the same panels the first products read.  The next
 // tile's [g | u] is issued before this tile's sums.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
+__global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
   extern __shared__ uint8_t raw[];
   __shared__ Bars bars;
   Bars* b = &bars;
@@ -676,7 +675,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
     for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kEpilogue);
     mbar_init(&b->dhfull, 1);
   }
-  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDecodeThreads * 16)
+  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDwThreads * 16)
     *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
   tc::fence_async_smem();
   tc::fence_before();
@@ -713,10 +712,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
         tc::fence_after();
         const uint64_t xd = xk0 + xg.at * xstep;
         if (tc::elect_one()) {
-#pragma unroll 4
-          for (int k = 0; k < k1; ++k) {
+#pragma unroll
+          for (int k = 0; k < GS_DECODE_MAX_D / 16; ++k) {
             const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-            tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
+            if (k < k1) tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
           }
         }
         __syncwarp();
@@ -726,9 +725,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode_dw(DecodeArgs a) {
       auto dh_products = [&]() {
         const uint64_t yd = xk0 + xh.at * xstep + ypart;
         if (tc::elect_one()) {
-#pragma unroll 4
-          for (int k = 0; k < kh; ++k)
-            tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+#pragma unroll
+          for (int k = 0; k < GS_DECODE_MAX_C / 16; ++k)
+            if (k < kh) tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
           tc::commit(&b->dhfull);
         }
         __syncwarp();
@@ -965,7 +964,7 @@ static int launch_decode_as(DecodeArgs a, dim3 grid, cudaStream_t s) {
   auto* kernel = MODE == kDw ? k_decode_dw<T, ACT> : k_decode<T, MODE == kDx ? kDx : kFwd, ACT>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_decode: %s", cudaGetErrorString(e));
-  kernel<<<grid, kDecodeThreads, smem, s>>>(a);
+  kernel<<<grid, MODE == kDw ? kDwThreads : kDecodeThreads, smem, s>>>(a);
   return check_launch("k_decode");
 }
 
