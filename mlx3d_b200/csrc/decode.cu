@@ -102,11 +102,34 @@ __global__ void k_decode_prepare(const T* __restrict__ wg, const T* __restrict__
 }
 
 
-// act and act' of two values.  The exponential and the reciprocal are the
-// hardware approximations (2 ulp; the results are rounded to 16 bits).  The
-// special-function unit (16 a clock and SM) bounds the activation, so silu's two
-// logistic functions share one reciprocal: 1 / a = b * (1 / ab).  Exponentials
-// stop at 2^63, so that ab stays finite; below that the logistic function is 0.
+// Pairs of float32 values in 64-bit registers: sm_100 multiplies and adds two at
+// once, and the activation is bound by the instructions it issues.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ void split(F2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -117,28 +140,53 @@ __device__ __forceinline__ float rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float fma_sat(float a, float b, float c) {
+  float y;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// act(g) of two values and, where wanted, act'(g).  The exponential and the
+// reciprocal are the hardware approximations (2 ulp; the results are rounded to
+// 16 bits).  The special-function unit (16 a clock and SM) is the other bound,
+// so two values share one reciprocal: 1 / a = b * (1 / ab).
+//   silu: l = 1 / (1 + 2^t), t = -g log2 e up to 63 so that the product stays
+//         finite; 2^-62 is taken off and the result clamped to [0, 1], which
+//         makes l zero where t was cut.
+//   gelu: Phi(-|g|) = e^(-g^2 / 2) P(t) / 2, t = 1 / (1 + p |g| / sqrt 2), the
+//         five-term form of Abramowitz and Stegun, Handbook of Mathematical
+//         Functions, 7.1.26 (|error| of erf <= 1.5e-7); its exponential is the
+//         density's too.
 template <int ACT, bool SLOPE>
-__device__ __forceinline__ void gate2(float g0, float g1, float& a0, float& a1, float& s0, float& s1) {
+__device__ __forceinline__ void gate2(F2 g, F2& a, F2& slope) {
+  float g0, g1;
+  split(g, g0, g1);
   if (ACT == GS_ACT_SILU) {
-    const float t0 = g0 * -1.4426950408889634f, t1 = g1 * -1.4426950408889634f;
-    const float p0 = 1.0f + ex2(fminf(t0, 63.0f)), p1 = 1.0f + ex2(fminf(t1, 63.0f));
+    float t0, t1, p0, p1;
+    split(mul(g, f2(-1.4426950408889634f)), t0, t1);
+    const F2 p = add(f2(ex2(fminf(t0, 63.0f)), ex2(fminf(t1, 63.0f))), f2(1.0f));
+    split(p, p0, p1);
     const float inv = rcp(p0 * p1);
-    const float l0 = t0 > 63.0f ? 0.0f : inv * p1, l1 = t1 > 63.0f ? 0.0f : inv * p0;
-    a0 = g0 * l0;
-    a1 = g1 * l1;
-    if (SLOPE) {
-      s0 = __fmaf_rn(a0, 1.0f - l0, l0);
-      s1 = __fmaf_rn(a1, 1.0f - l1, l1);
-    }
+    const F2 l = f2(fma_sat(inv, p1, -0x1p-62f), fma_sat(inv, p0, -0x1p-62f));
+    a = mul(g, l);
+    if (SLOPE) slope = fma(a, fma(l, f2(-1.0f), f2(1.0f)), l);
   } else {
-    const float f0 = 0.5f + 0.5f * erff(g0 * 0.70710678118654752f);
-    const float f1 = 0.5f + 0.5f * erff(g1 * 0.70710678118654752f);
-    a0 = g0 * f0;
-    a1 = g1 * f1;
-    if (SLOPE) {
-      s0 = __fmaf_rn(g0 * 0.39894228040143268f, ex2(g0 * g0 * -0.72134752044448170f), f0);
-      s1 = __fmaf_rn(g1 * 0.39894228040143268f, ex2(g1 * g1 * -0.72134752044448170f), f1);
-    }
+    float d0, d1, e0, e1, q0, q1;
+    // |g| stops at 1e9 (Phi is 0 or 1 long before): the denominators' product stays finite
+    const F2 d = fma(f2(fminf(fabsf(g0), 1e9f), fminf(fabsf(g1), 1e9f)), f2(0.3275911f * 0.70710678118654752f), f2(1.0f));
+    split(d, d0, d1);
+    const float inv = rcp(d0 * d1);
+    const F2 t = f2(inv * d1, inv * d0);
+    split(mul(mul(g, g), f2(-0.72134752044448170f)), e0, e1);
+    const F2 e = f2(ex2(e0), ex2(e1));  // e^(-g^2 / 2)
+    F2 q = fma(t, f2(0.5f * 1.061405429f), f2(0.5f * -1.453152027f));
+    q = fma(t, q, f2(0.5f * 1.421413741f));
+    q = fma(t, q, f2(0.5f * -0.284496736f));
+    q = fma(t, q, f2(0.5f * 0.254829592f));
+    split(mul(mul(t, q), e), q0, q1);  // Phi(-|g|)
+    const F2 phi = f2(g0 < 0.0f ? q0 : 1.0f - q0, g1 < 0.0f ? q1 : 1.0f - q1);
+    a = mul(g, phi);
+    if (SLOPE) slope = fma(mul(g, e), f2(0.39894228040143268f), phi);
   }
 }
 
@@ -155,6 +203,13 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(F2 v) {
+  float lo, hi;
+  split(v, lo, hi);
+  return pack2<T>(lo, hi);
+}
+
 // ------------------------------------------------------------ shared pieces
 // Barriers of a CTA.  A wait that gives up raises `abort`, which makes every
 // other wait give up too; the roles then leave their loops, the CTA frees its
@@ -162,7 +217,7 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
 struct Bars {
   unsigned long long xfull[kMaxXStages], xempty[kMaxXStages];
   unsigned long long wfull[kMaxWStages], wempty[kMaxWStages];
-  unsigned long long gfull[2], hfull[2], dhfull, sfree;  // sfree: dW's operand stage
+  unsigned long long gfull[2], hfull[2], dhfull, dhread, sfree;  // sfree: dW's operand stage
   unsigned long long yfull[2], yempty[2];
   unsigned long long ofull, oempty;  // output stage
   uint32_t tmem;
@@ -178,11 +233,21 @@ __device__ __forceinline__ bool wait_for(Bars* b, unsigned long long* bar, unsig
         : "r"(smem_addr(bar)), "r"(parity)
         : "memory");
     if (done) return true;
-    if (b->abort) return false;
+    if ((i & 15) == 15 && b->abort) return false;
   }
   b->abort = 1;
   return false;
 }
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool passed(unsigned long long* bar, unsigned parity) {
+  unsigned done;
+  asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+               : "=r"(done)
+               : "r"(smem_addr(bar)), "r"(parity)
+               : "memory");
+  return done;
+}
+
 // Position in a ring of stages: the stage, and the parity of the phase that
 // fills it (a consumer waits for `parity`, a producer for its complement, which
 // the first round passes at once).
@@ -342,6 +407,39 @@ __device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_
   }
 }
 
+// COLS hidden units of a thread's row: g, u and (backward) dh from TMEM, then
+// h = act(g) u, dg = dh u act'(g), du = dh act(g) as pairs of 16-bit operands.
+template <int MODE, int COLS>
+struct GateIn {
+  uint32_t g[COLS], u[COLS], dh[MODE == kFwd ? 1 : COLS];
+  __device__ __forceinline__ void load(uint32_t at_g, uint32_t at_u, uint32_t at_dh) {
+    tc::tmem_ld(at_g, g);
+    tc::tmem_ld(at_u, u);
+    if constexpr (MODE != kFwd) tc::tmem_ld(at_dh, dh);
+  }
+  __device__ __forceinline__ void settle() {
+    tc::tmem_wait_ld();
+    tc::after_wait(g);
+    tc::after_wait(u);
+    if constexpr (MODE != kFwd) tc::after_wait(dh);
+  }
+  template <typename T, int ACT>
+  __device__ __forceinline__ void compute(uint32_t* h, uint32_t* dg, uint32_t* du) const {
+#pragma unroll
+    for (int e = 0; e < COLS / 2; ++e) {
+      F2 act, slope;
+      gate2<ACT, MODE != kFwd>(f2(g[2 * e], g[2 * e + 1]), act, slope);
+      const F2 uu = f2(u[2 * e], u[2 * e + 1]);
+      if constexpr (MODE != kDx) h[e] = pack2<T>(mul(act, uu));
+      if constexpr (MODE != kFwd) {
+        const F2 d = f2(dh[2 * e], dh[2 * e + 1]);
+        dg[e] = pack2<T>(mul(mul(d, uu), slope));
+        du[e] = pack2<T>(mul(d, act));
+      }
+    }
+  }
+};
+
 // 32 columns of an output row (or `left`, if fewer), in stores of `vec` bytes.
 __device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16], int left, int vec) {
   if (vec == 16) {
@@ -449,16 +547,16 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         const uint64_t xd = x0 + x.at * xstep, wk = wk0 + w1.at * wstep;
         const bool last = j1 + 1 == a.chunks;
         if (tc::elect_one()) {
-#pragma unroll
-          for (int k = 0; k < GS_DECODE_MAX_D / 16; ++k) {
+#pragma unroll 1
+          for (int k = 0; k < k1; ++k) {
             const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-            if (k < k1) tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
+            tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
           }
           if (MODE == kDx) {
             const uint64_t yd = xd + wdn, wn = wn0 + w1.at * wstep + wdn;
-#pragma unroll
-            for (int k = 0; k < GS_DECODE_MAX_C / 16; ++k)
-              if (k < kh) tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+#pragma unroll 1
+            for (int k = 0; k < kh; ++k)
+              tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
           }
           tc::commit(done);
           if (last) tc::commit(&b->xempty[x.at]);
@@ -486,12 +584,12 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         if (tc::elect_one()) {
           if (MODE == kFwd) {
             const uint64_t wk = wk0 + w2.at * wstep + wdn;
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 4; ++k)  // h in the columns of g, 16 of each 32
               tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wk + k * 2, id2, j2 > 0 || k > 0);
           } else {
             const uint64_t wn = wn0 + w2.at * wstep;
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
               tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
           }
@@ -556,22 +654,29 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
       const uint32_t src = lanes + kOut + y.at * out_cols;
       const bool here = staged || t * kTile + row < a.n;
       uint8_t* p = staged ? os + row * a.out_pitch : static_cast<uint8_t*>(a.out) + (t * kTile + row) * width * 2;
-      uint32_t v[32];
-      tc::tmem_ld32(src, v);
-      for (int c0 = 0; c0 < width; c0 += 32, p += 64) {
-        uint32_t w[16];
+      // The next columns are on their way while the current ones are stored; the
+      // accumulator is given back when the last ones have been read.
+      uint32_t v[2][32];
+      tc::tmem_ld(src, v[0]);
+      if (width > 32) tc::tmem_ld(src + 32, v[1]);
+      for (int c0 = 0; c0 < width; c0 += 64, p += 128) {
         tc::tmem_wait_ld();
-        tc::after_wait(v);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
-        __syncwarp();
-        if (c0 + 32 < width) {
-          tc::tmem_ld32(src + c0 + 32, v);
-        } else {
+        tc::after_wait(v[0]);
+        tc::after_wait(v[1]);
+        if (c0 + 64 >= width) {
           tc::fence_before();
           arrive(&b->yempty[y.at]);
         }
-        if (here) store_row32(p, w, width - c0, a.out_vec);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            w[e] = pack2<T>(__uint_as_float(v[half][2 * e]), __uint_as_float(v[half][2 * e + 1]));
+          __syncwarp();
+          if (c0 + 64 + 32 * half < width) tc::tmem_ld(src + c0 + 64 + 32 * half, v[half]);
+          if (here && c0 + 32 * half < width) store_row32(p + 64 * half, w, width - c0 - 32 * half, a.out_vec);
+        }
       }
       __syncwarp();
       if (staged) {
@@ -583,51 +688,46 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   } else if (warp >= 8) {  // activation: each warpgroup half of a chunk's hidden units
     const int wg = (warp >> 2) & 1;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    // TMEM loads take about 300 cycles: the next columns, of the next chunk
+    // too if it is ready, are on their way while the current ones are computed.
+    constexpr int kCols = MODE == kFwd ? 16 : 8, kPasses = 32 / kCols;
+    GateIn<MODE, kCols> v[2];
     Ring q;
+    bool have = false;
     for (int64_t i = 0; i < total; ++i) {
-      if (!__all_sync(~0u, wait_for(b, &b->gfull[q.at], q.parity))) break;
-      tc::fence_after();
       const uint32_t buf = lanes + (uint32_t)q.at * kBuf + wg * 32;
+      if (!have) {
+        if (!__all_sync(~0u, wait_for(b, &b->gfull[q.at], q.parity))) break;
+        tc::fence_after();
+        v[0].load(buf, buf + 64, buf + 128);
+      }
+      unsigned long long* full = &b->hfull[q.at];
+      q.next(2);
+      have = false;
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        uint32_t g[16], u[16], h[8];
-        tc::tmem_ld16(buf + p * 16, g);
-        tc::tmem_ld16(buf + 64 + p * 16, u);
+      for (int p = 0; p < kPasses; ++p) {
+        v[p & 1].settle();
+        if (p + 1 < kPasses) {
+          v[(p + 1) & 1].load(buf + (p + 1) * kCols, buf + 64 + (p + 1) * kCols, buf + 128 + (p + 1) * kCols);
+        } else if (i + 1 < total && __all_sync(~0u, passed(&b->gfull[q.at], q.parity))) {
+          tc::fence_after();
+          const uint32_t next = lanes + (uint32_t)q.at * kBuf + wg * 32;
+          v[0].load(next, next + 64, next + 128);
+          have = true;
+        }
+        // The results go over columns of g and u that this warp has read.
+        uint32_t h[kCols / 2], dg[kCols / 2], du[kCols / 2];
+        v[p & 1].template compute<T, ACT>(h, dg, du);
         if constexpr (MODE == kFwd) {
-          tc::tmem_wait_ld();
-          tc::after_wait(g);
-          tc::after_wait(u);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float a0, a1, s0, s1;
-            gate2<ACT, false>(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), a0, a1, s0, s1);
-            h[e] = pack2<T>(a0 * __uint_as_float(u[2 * e]), a1 * __uint_as_float(u[2 * e + 1]));
-          }
-          // over columns of g that this warp has read: 32 wg .. 32 wg + 15
-          tc::tmem_st8(buf + p * 8, h);
+          tc::tmem_st(buf + p * (kCols / 2), h);
         } else {
-          uint32_t dh[16], du[8];
-          tc::tmem_ld16(buf + 128 + p * 16, dh);
-          tc::tmem_wait_ld();
-          tc::after_wait(g);
-          tc::after_wait(u);
-          tc::after_wait(dh);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float a0, a1, s0, s1;
-            gate2<ACT, true>(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), a0, a1, s0, s1);
-            const float d0 = __uint_as_float(dh[2 * e]), d1 = __uint_as_float(dh[2 * e + 1]);
-            h[e] = pack2<T>(d0 * __uint_as_float(u[2 * e]) * s0, d1 * __uint_as_float(u[2 * e + 1]) * s1);
-            du[e] = pack2<T>(d0 * a0, d1 * a1);
-          }
-          tc::tmem_st8(buf + p * 8, h);        // dg over g
-          tc::tmem_st8(buf + 64 + p * 8, du);  // du over u
+          tc::tmem_st(buf + p * (kCols / 2), dg);
+          tc::tmem_st(buf + 64 + p * (kCols / 2), du);
         }
       }
       tc::tmem_wait_st();
       tc::fence_before();
-      arrive(&b->hfull[q.at]);
-      q.next(2);
+      arrive(full);
     }
   }
   __syncthreads();
@@ -674,6 +774,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
     init_bars(b);
     for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kEpilogue);
     mbar_init(&b->dhfull, 1);
+    mbar_init(&b->dhread, kEpilogue);
   }
   for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDwThreads * 16)
     *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
@@ -712,10 +813,10 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
         tc::fence_after();
         const uint64_t xd = xk0 + xg.at * xstep;
         if (tc::elect_one()) {
-#pragma unroll
-          for (int k = 0; k < GS_DECODE_MAX_D / 16; ++k) {
+#pragma unroll 1
+          for (int k = 0; k < k1; ++k) {
             const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-            if (k < k1) tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
+            tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
           }
         }
         __syncwarp();
@@ -725,9 +826,9 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       auto dh_products = [&]() {
         const uint64_t yd = xk0 + xh.at * xstep + ypart;
         if (tc::elect_one()) {
-#pragma unroll
-          for (int k = 0; k < GS_DECODE_MAX_C / 16; ++k)
-            if (k < kh) tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+#pragma unroll 1
+          for (int k = 0; k < kh; ++k)
+            tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
           tc::commit(&b->dhfull);
         }
         __syncwarp();
@@ -739,19 +840,24 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       const bool ahead = nbuf == 2 && a.x_stages > 1;
       for (int64_t i = 0; i < mine && ok; ++i) {
         if (ahead && i + 1 < mine) gu_products();
-        // tile i's g, u, dh have been read and its panels written
-        ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
+        // tile i's g, u and dh have been read
+        ok &= wait_for(b, &b->dhread, (unsigned)i & 1);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
         if (ahead && i + 1 < mine) dh_products();
+        // its panels are written
+        ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        tc::fence_after();
         const uint64_t xd = xn0 + xs.at * xstep, yd = xd + ypart;
         if (tc::elect_one()) {
-#pragma unroll
+#pragma unroll 1
           for (int k = 0; k < 8; ++k) tc::mma_ss(tmem + col_gu, gn + k * 128, xd + k * 128, idg, i > 0 || k > 0);
           // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
           for (int m = 0; m < mblocks; ++m)
-#pragma unroll
+#pragma unroll 1
             for (int k = 0; k < 8; ++k)
               tc::mma_ss(tmem + col_dd + m * 64, yd + m * 2 * (kPanel >> 4) + k * 128, hn + k * 128, idd,
                          i > 0 || k > 0);
@@ -775,32 +881,24 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
     const int wg = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     bool ok = true;
+    GateIn<kDw, 8> v[2];
     for (int64_t i = 0; i < mine; ++i) {
+      const uint32_t buf = lanes + (nbuf == 2 ? (uint32_t)(i & 1) * 128 : 0) + wg * 32, dhc = lanes + col_dh + wg * 32;
       ok = __all_sync(~0u, wait_for(b, &b->dhfull, (unsigned)i & 1));
       if (!ok) break;
       tc::fence_after();
-      const uint32_t buf = lanes + (nbuf == 2 ? (uint32_t)(i & 1) * 128 : 0) + wg * 32;
+      v[0].load(buf, buf + 64, dhc);
       uint32_t pg[16], pu[16], ph[16];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        uint32_t g[16], u[16], dh[16];
-        tc::tmem_ld16(buf + p * 16, g);
-        tc::tmem_ld16(buf + 64 + p * 16, u);
-        tc::tmem_ld16(lanes + col_dh + wg * 32 + p * 16, dh);
-        tc::tmem_wait_ld();
-        tc::after_wait(g);
-        tc::after_wait(u);
-        tc::after_wait(dh);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float a0, a1, s0, s1;
-          gate2<ACT, true>(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), a0, a1, s0, s1);
-          const float u0 = __uint_as_float(u[2 * e]), u1 = __uint_as_float(u[2 * e + 1]);
-          const float d0 = __uint_as_float(dh[2 * e]), d1 = __uint_as_float(dh[2 * e + 1]);
-          pg[8 * p + e] = pack2<T>(d0 * u0 * s0, d1 * u1 * s1);
-          pu[8 * p + e] = pack2<T>(d0 * a0, d1 * a1);
-          ph[8 * p + e] = pack2<T>(a0 * u0, a1 * u1);
+      for (int p = 0; p < 4; ++p) {
+        v[p & 1].settle();
+        if (p < 3) {
+          v[(p + 1) & 1].load(buf + 8 * (p + 1), buf + 64 + 8 * (p + 1), dhc + 8 * (p + 1));
+        } else {
+          tc::fence_before();
+          arrive(&b->dhread);
         }
+        v[p & 1].template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
       }
       // the previous tile's sums have read the panels
       if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
@@ -814,7 +912,6 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
             make_uint4(ph[4 * q], ph[4 * q + 1], ph[4 * q + 2], ph[4 * q + 3]);
       }
       tc::fence_async_smem();
-      tc::fence_before();
       arrive(&b->hfull[0]);
     }
     if (ok && mine > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(mine - 1) & 1));
@@ -827,7 +924,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       for (int c0 = wg * 32; c0 < a.d; c0 += 64) {
         uint32_t v[32];
         __syncwarp();
-        tc::tmem_ld32(lanes + col_gu + c0, v);
+        tc::tmem_ld(lanes + col_gu + c0, v);
         tc::tmem_wait_ld();
         tc::after_wait(v);
         if (h < a.f)
@@ -838,7 +935,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       for (int m = 0; m < mblocks; ++m) {
         uint32_t v[32];
         __syncwarp();
-        tc::tmem_ld32(lanes + col_dd + m * 64 + wg * 32, v);
+        tc::tmem_ld(lanes + col_dd + m * 64 + wg * 32, v);
         tc::tmem_wait_ld();
         tc::after_wait(v);
         const int c = m * 128 + row, h0 = blockIdx.y * kChunk + wg * 32;
