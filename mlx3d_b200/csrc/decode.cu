@@ -369,8 +369,9 @@ __device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__
   else load_tile_by<2>(panels, src, width, rows, l);
 }
 
-// The loader warps' loop over this CTA's tiles.  With s stages, a tile is
-// handed over after the loads of the s - 2 following tiles have been issued.
+// The loader warps' loop over this CTA's tiles.  A tile is handed over when its
+// loads have landed; with four stages, after the next tile's have been issued
+// (any later, and handing it over would wait for a stage still in use).
 template <typename T, bool DY>
 __device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_t* stages, int stage_bytes,
                                             int64_t first, int64_t step, int64_t tiles) {
@@ -378,7 +379,7 @@ __device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_
   const T* x = static_cast<const T*>(a.x);
   const T* dy = static_cast<const T*>(a.dy);
   const int vx = copy_unit(x, a.d), vy = DY ? copy_unit(dy, a.c) : 0;
-  const int lag = a.x_stages > 2 ? a.x_stages - 2 : 0;
+  const int lag = a.x_stages > 3 ? a.x_stages - 3 : 0;
   Ring fill, give;
   int pending = 0;  // tiles issued and not handed over
   for (int64_t t = first; t < tiles; t += step) {
@@ -391,8 +392,7 @@ __device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_
     fill.next(a.x_stages);
     if (++pending > lag) {
       if (lag == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-      else if (lag == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 2;" ::: "memory");
+      else asm volatile("cp.async.wait_group 1;" ::: "memory");
       tc::fence_async_smem();
       arrive(&b->xfull[give.at]);
       give.next(a.x_stages);
@@ -527,36 +527,40 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   } else if (warp == 0) {
     {
       // This warp's instructions bound short tiles: counters instead of
-      // divisions, descriptors advanced by adding to their address field.  All
-      // lanes run the loop, one issues.
+      // divisions, and all operands of the matrix instructions made uniform
+      // before the elected lane issues them.
       Ring x, w1, w2, y;
       int j1 = 0, j2 = 0;
       bool ok = true, wait_w = true;
       const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
       const uint32_t id2 = tc::instr_desc(kBf16, wp, false, MODE == kDx);
-      const uint64_t x0 = tc::desc_k(smem_addr(smem)), wk0 = tc::desc_k(smem_addr(ws));
-      const uint64_t wn0 = tc::desc_mn(smem_addr(ws), kPanel);
+      const uint32_t x0 = tc::desc_k(smem_addr(smem)), wk0 = tc::desc_k(smem_addr(ws));
+      const uint32_t wn0 = tc::desc_mn(smem_addr(ws), kPanel);
       const uint32_t xstep = stage_bytes >> 4, wstep = a.chunk_bytes >> 4, wdn = a.nxp * (kPanel >> 4);
       const int k1 = a.dp / 16, kh = a.cp / 16;
-      auto first_products = [&](uint32_t buf, unsigned long long* done) {
+      auto first_products = [&](uint32_t buf_, unsigned long long* done) {
         if (j1 == 0) ok &= wait_for(b, &b->xfull[x.at], x.parity);
         if (wait_w) ok &= wait_for(b, &b->wfull[w1.at], w1.parity);
         ok = __all_sync(~0u, ok);
         if (!ok) return;
         tc::fence_after();
-        const uint64_t xd = x0 + x.at * xstep, wk = wk0 + w1.at * wstep;
+        const uint32_t buf = tc::uniform(buf_), xd = tc::uniform(x0 + x.at * xstep);
+        const uint32_t wk = tc::uniform(wk0 + w1.at * wstep), wn = tc::uniform(wn0 + w1.at * wstep + wdn);
         const bool last = j1 + 1 == a.chunks;
         if (tc::elect_one()) {
-#pragma unroll 1
-          for (int k = 0; k < k1; ++k) {
-            const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-            tc::mma_ss(buf, xd + at, wk + at, id1, k > 0);
-          }
+          tc::mma_ss(buf, xd, wk, id1, false);
+#pragma unroll
+          for (int k = 1; k < GS_DECODE_MAX_D / 16; ++k)
+            if (k < k1)
+              tc::mma_ss(buf, xd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wk + (k >> 2) * (kPanel >> 4) + (k & 3) * 2,
+                         id1, true);
           if (MODE == kDx) {
-            const uint64_t yd = xd + wdn, wn = wn0 + w1.at * wstep + wdn;
-#pragma unroll 1
-            for (int k = 0; k < kh; ++k)
-              tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+            const uint32_t yd = xd + wdn;
+            tc::mma_ss(buf + 128, yd, wn, idh, false);
+#pragma unroll
+            for (int k = 1; k < GS_DECODE_MAX_C / 16; ++k)
+              if (k < kh)
+                tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, true);
           }
           tc::commit(done);
           if (last) tc::commit(&b->xempty[x.at]);
@@ -579,19 +583,20 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
-        const uint32_t buf = tmem + qb * kBuf, out = tmem + kOut + y.at * out_cols;
-        const bool last = j2 + 1 == a.chunks;
+        const uint32_t buf = tc::uniform(tmem + qb * kBuf), out = tc::uniform(tmem + kOut + y.at * out_cols);
+        const uint32_t wk = tc::uniform(wk0 + w2.at * wstep + wdn), wn = tc::uniform(wn0 + w2.at * wstep);
+        const bool last = j2 + 1 == a.chunks, more = __all_sync(~0u, j2 > 0);
         if (tc::elect_one()) {
           if (MODE == kFwd) {
-            const uint64_t wk = wk0 + w2.at * wstep + wdn;
-#pragma unroll 1
-            for (int k = 0; k < 4; ++k)  // h in the columns of g, 16 of each 32
-              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wk + k * 2, id2, j2 > 0 || k > 0);
+            tc::mma_ts(out, buf, wk, id2, more);
+#pragma unroll
+            for (int k = 1; k < 4; ++k)  // h in the columns of g, 16 of each 32
+              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wk + k * 2, id2, true);
           } else {
-            const uint64_t wn = wn0 + w2.at * wstep;
-#pragma unroll 1
-            for (int k = 0; k < 8; ++k)  // dg in the columns of g, du in those of u
-              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wn + k * 128, id2, j2 > 0 || k > 0);
+            tc::mma_ts(out, buf, wn, id2, more);
+#pragma unroll
+            for (int k = 1; k < 8; ++k)  // dg in the columns of g, du in those of u
+              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wn + k * 128, id2, true);
           }
           if (!resident) tc::commit(&b->wempty[w2.at]);
           if (last) tc::commit(&b->yfull[y.at]);
@@ -800,9 +805,9 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
       const uint32_t idg = tc::instr_desc(kBf16, a.dp, true, true), idd = tc::instr_desc(kBf16, 64, true, true);
       const uint32_t xstep = stage_bytes >> 4, ypart = a.nxp * (kPanel >> 4);
-      const uint64_t xk0 = tc::desc_k(smem_addr(smem)), xn0 = tc::desc_mn(smem_addr(smem), kPanel);
-      const uint64_t wk = tc::desc_k(smem_addr(ws)), wn = tc::desc_mn(smem_addr(ws), kPanel) + ypart;
-      const uint64_t gn = tc::desc_mn(smem_addr(st), kPanel), hn = gn + 2 * (kPanel >> 4);
+      const uint32_t xk0 = tc::desc_k(smem_addr(smem)), xn0 = tc::desc_mn(smem_addr(smem), kPanel);
+      const uint32_t wk = tc::uniform(tc::desc_k(smem_addr(ws))), sn = tc::uniform(tc::desc_mn(smem_addr(st), kPanel));
+      const uint32_t wn = tc::uniform(tc::desc_mn(smem_addr(ws), kPanel) + ypart);
       const int k1 = a.dp / 16, kh = a.cp / 16;
       Ring xg, xh, xs;  // stages of the next [g | u], dh and sums
       unsigned gb = 0;
@@ -811,24 +816,26 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
         ok = __all_sync(~0u, ok);
         if (!ok) return;
         tc::fence_after();
-        const uint64_t xd = xk0 + xg.at * xstep;
+        const uint32_t xd = tc::uniform(xk0 + xg.at * xstep), buf = tc::uniform(tmem + gb * 128);
         if (tc::elect_one()) {
-#pragma unroll 1
-          for (int k = 0; k < k1; ++k) {
-            const uint32_t at = (k >> 2) * (kPanel >> 4) + (k & 3) * 2;
-            tc::mma_ss(tmem + gb * 128, xd + at, wk + at, id1, k > 0);
-          }
+          tc::mma_ss(buf, xd, wk, id1, false);
+#pragma unroll
+          for (int k = 1; k < GS_DECODE_MAX_D / 16; ++k)
+            if (k < k1)
+              tc::mma_ss(buf, xd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wk + (k >> 2) * (kPanel >> 4) + (k & 3) * 2,
+                         id1, true);
         }
         __syncwarp();
         xg.next(a.x_stages);
         if (nbuf == 2) gb ^= 1;
       };
       auto dh_products = [&]() {
-        const uint64_t yd = xk0 + xh.at * xstep + ypart;
+        const uint32_t yd = tc::uniform(xk0 + xh.at * xstep + ypart), buf = tc::uniform(tmem + col_dh);
         if (tc::elect_one()) {
-#pragma unroll 1
-          for (int k = 0; k < kh; ++k)
-            tc::mma_ss(tmem + col_dh, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, k > 0);
+          tc::mma_ss(buf, yd, wn, idh, false);
+#pragma unroll
+          for (int k = 1; k < GS_DECODE_MAX_C / 16; ++k)
+            if (k < kh) tc::mma_ss(buf, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, true);
           tc::commit(&b->dhfull);
         }
         __syncwarp();
@@ -838,6 +845,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       if (ok) dh_products();
       // nbuf = 2 needs the next tile's stage while this one's is in use
       const bool ahead = nbuf == 2 && a.x_stages > 1;
+      const uint32_t tgu = tc::uniform(tmem + col_gu), tdd = tc::uniform(tmem + col_dd);
       for (int64_t i = 0; i < mine && ok; ++i) {
         if (ahead && i + 1 < mine) gu_products();
         // tile i's g, u and dh have been read
@@ -851,16 +859,22 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
-        const uint64_t xd = xn0 + xs.at * xstep, yd = xd + ypart;
+        const uint32_t xd = tc::uniform(xn0 + xs.at * xstep), yd = xd + ypart;
+        const bool more = __all_sync(~0u, i > 0);
         if (tc::elect_one()) {
-#pragma unroll 1
-          for (int k = 0; k < 8; ++k) tc::mma_ss(tmem + col_gu, gn + k * 128, xd + k * 128, idg, i > 0 || k > 0);
+          tc::mma_ss(tgu, sn, xd, idg, more);
+#pragma unroll
+          for (int k = 1; k < 8; ++k) tc::mma_ss(tgu, sn + k * 128, xd + k * 128, idg, true);
           // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
-          for (int m = 0; m < mblocks; ++m)
-#pragma unroll 1
-            for (int k = 0; k < 8; ++k)
-              tc::mma_ss(tmem + col_dd + m * 64, yd + m * 2 * (kPanel >> 4) + k * 128, hn + k * 128, idd,
-                         i > 0 || k > 0);
+          const uint32_t hn = sn + 2 * (kPanel >> 4);
+#pragma unroll
+          for (int m = 0; m < GS_DECODE_MAX_C / 128; ++m) {
+            if (m >= mblocks) break;
+            const uint32_t ym = yd + m * 2 * (kPanel >> 4);
+            tc::mma_ss(tdd + m * 64, ym, hn, idd, more);
+#pragma unroll
+            for (int k = 1; k < 8; ++k) tc::mma_ss(tdd + m * 64, ym + k * 128, hn + k * 128, idd, true);
+          }
           tc::commit(&b->sfree);
           tc::commit(&b->xempty[xs.at]);
         }

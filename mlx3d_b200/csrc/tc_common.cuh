@@ -26,18 +26,19 @@ __device__ __forceinline__ uint32_t panel_elem(int row, int col) {
 
 // Shared-memory matrix descriptor, 128-byte swizzle: bits 0-13 address / 16,
 // 16-29 leading byte offset / 16, 32-45 stride byte offset / 16, bits 46-48 =
-// 1, bits 61-63 = 2 (128-byte swizzle).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)((lbo & 0x3ffff) >> 4) << 16) |
-         ((uint64_t)((sbo & 0x3ffff) >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// 1, bits 61-63 = 2 (128-byte swizzle).  8-row groups are 1024 bytes apart in
+// every layout used here, so the upper word is a constant and a descriptor is
+// handled as its lower word; an offset of n bytes adds n / 16 to it.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+// K-major panel: 16 K elements = 32 bytes.
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return ((addr & 0x3ffff) >> 4) | (1u << 16); }
+// MN-major panels, `panel_bytes` apart; 16 K rows = 2048 bytes.
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr, uint32_t panel_bytes) {
+  return ((addr & 0x3ffff) >> 4) | ((panel_bytes >> 4) << 16);
 }
-// K-major panel: 8-row groups are 1024 bytes apart; 16 K elements = 32 bytes.
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return smem_desc(addr, 16, 1024); }
-// MN-major panels, `panel_bytes` apart; 8-row (K) groups are 1024 bytes apart;
-// 16 K rows = 2048 bytes.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t panel_bytes) {
-  return smem_desc(addr, panel_bytes, 1024);
-}
+// The value of lane 0, known to be the same in every lane: it can be kept in a
+// uniform register, which the matrix instructions take their operands from.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(~0u, v, 0); }
 
 // Instruction descriptor of kind::f16, float32 accumulators, M = 128:
 // bits 4-5 accumulator type (1 = f32), 7-9 / 10-12 A / B type (0 = f16, 1 =
@@ -57,19 +58,20 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // D[128 x N] (TMEM) (+)= A (smem) B (smem), K = 16.  One thread issues.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((int)accumulate)
+      "{\n .reg .pred p;\n .reg .b64 da, db;\n setp.ne.b32 p, %4, 0;\n"
+      " mov.b64 da, {%1, %5};\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((int)accumulate), "n"(kDescHigh)
       : "memory");
 }
 // As mma_ss with A in TMEM (two 16-bit elements a column, lane = row).
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((int)accumulate)
+      "{\n .reg .pred p;\n .reg .b64 db;\n setp.ne.b32 p, %4, 0;\n mov.b64 db, {%2, %5};\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((int)accumulate), "n"(kDescHigh)
       : "memory");
 }
 // The barrier completes a phase when every matrix instruction this thread
