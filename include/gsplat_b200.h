@@ -482,20 +482,25 @@ int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows,
  * gs_decode_prepare lays the weights out for the kernels in `image`
  * (gs_decode_image_bytes, 16-byte aligned); forward and backward read only
  * that.  gs_decode_backward writes dx (n, d) unless NULL, and d_gate, d_up
- * (f, d), d_down (c, f) unless all three are NULL, from dy (n, c); its workspace
- * (gs_decode_workspace_bytes) is needed for the weight gradients only.  The
- * sums over rows are taken in a fixed order. */
+ * (f, d), d_down (c, f) unless all three are NULL, from dy (n, c); sums over
+ * rows are taken in a fixed order.
+ * gs_decode_workspace_bytes is the scratch (16-byte aligned) of a forward call
+ * (dy NULL, weights 0) or a backward call (weights: whether the weight gradients
+ * are wanted).  It depends on the alignment of x and dy: rows that are no
+ * multiple of 16 bytes, or do not start on a 16-byte boundary, are copied to
+ * padded rows in it.  It may be 0. */
 #define GS_ACT_SILU 0
 #define GS_ACT_GELU 1 /* the error-function form */
 #define GS_DECODE_MAX_D 128
 #define GS_DECODE_MAX_C 256
 #define GS_DECODE_MAX_F 65536
+#define GS_DECODE_MAX_N 2147483391 /* rows are counted in 32 bits by the copy engine */
 size_t gs_decode_image_bytes(int d, int f, int c);
 int gs_decode_prepare(const void* w_gate, const void* w_up, const void* w_down, int dtype, int d, int f, int c,
                       void* image, size_t image_bytes, void* stream);
+size_t gs_decode_workspace_bytes(const void* x, const void* dy, int64_t n, int d, int f, int c, int weights);
 int gs_decode_forward(const void* x, int dtype, int64_t n, int d, int f, int c, int activation, const void* image,
-                      size_t image_bytes, void* y, void* stream);
-size_t gs_decode_workspace_bytes(int64_t n, int d, int f, int c);
+                      size_t image_bytes, void* y, void* workspace, size_t workspace_bytes, void* stream);
 int gs_decode_backward(const void* x, const void* dy, int dtype, int64_t n, int d, int f, int c, int activation,
                        const void* image, size_t image_bytes, void* dx, void* d_gate, void* d_up, void* d_down,
                        void* workspace, size_t workspace_bytes, void* stream);

@@ -76,6 +76,7 @@ GS_CACHE_MAX_CLASSES = 32767
 GS_DECODE_MAX_D = 128
 GS_DECODE_MAX_C = 256
 GS_DECODE_MAX_F = 65536
+GS_DECODE_MAX_N = 2147483391
 GS_GATES = {"silu": 0, "gelu": 1}
 
 
@@ -187,8 +188,10 @@ _SIGS = {
     "gs_teacher_read": (c_int, [_P, c_int64, _P, c_int64, c_int64, c_int, c_int, _P, _P, _P]),
     "gs_decode_image_bytes": (c_size_t, [c_int, c_int, c_int]),
     "gs_decode_prepare": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, _P, c_size_t, _P]),
-    "gs_decode_forward": (c_int, [_P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P]),
-    "gs_decode_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
+    "gs_decode_forward": (
+        c_int, [_P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P, c_size_t, _P]
+    ),
+    "gs_decode_workspace_bytes": (c_size_t, [_P, _P, c_int64, c_int, c_int, c_int, c_int]),
     "gs_decode_backward": (
         c_int,
         [_P, _P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P, _P, _P, _P, c_size_t, _P],

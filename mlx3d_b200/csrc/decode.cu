@@ -10,9 +10,10 @@
 // same panel serves as a K-major and as an MN-major operand, so x, dy and each
 // weight are laid out once and never transposed.
 //
-// Warps have roles: input loaders, a weight loader, one thread that issues the
-// matrix instructions, two warpgroups that apply the activation (alternating
-// chunks, or halves of one), and a warp that stores finished tiles.
+// Warps have roles: one fetches inputs, one weights, one issues the matrix
+// instructions, warpgroups apply the activation, drain and store finished tiles.
+#include <cuda.h>
+
 #include "feature_common.cuh"
 #include "tc_common.cuh"
 
@@ -21,11 +22,12 @@ namespace gs {
 constexpr int kTile = 128;              // rows of a tile (M of the matrix instructions)
 constexpr int kChunk = 64;              // hidden units of a chunk
 constexpr int kPanel = kTile * 128;     // bytes of a 128-row panel
-constexpr int kDecodeThreads = 640;     // forward and dx; the weight gradients have no drain warps
-constexpr int kDwThreads = 512;
-constexpr int kLoaders = 128;           // warps 4-7
-constexpr int kEpilogue = 256;          // warps 8-15, two warpgroups
-constexpr int kDrain = 128;             // warps 16-19
+// Warps of the forward and dx kernel: 0 issues matrix instructions, 1 fetches
+// weights, 2 stores tiles, 3 fetches inputs, 4-11 (two warpgroups) activate,
+// 12-15 drain finished tiles.  Of the weight-gradient kernel: 0 issues, 1
+// fetches, 4-19 (four warpgroups) activate.
+constexpr int kDecodeThreads = 512, kEpilogue = 256, kDrain = 128;
+constexpr int kDwThreads = 640, kDwEpilogue = 512;
 constexpr int kMaxXStages = 4, kMaxWStages = 16;
 constexpr uint32_t kTmemCols = 512;
 constexpr size_t kMaxSmem = 232448;     // 227 KB
@@ -44,8 +46,7 @@ int decode_wait_failures(unsigned long long* out, int reset) {
 }
 
 struct DecodeArgs {
-  const void* x;
-  const void* dy;
+  CUtensorMap map_x, map_dy;  // x and dy in boxes of 128 rows of one panel
   const uint8_t* image;
   void* out;        // y or dx
   float* partials;  // weight gradients: [split][gate f*d | up f*d | down c*f]
@@ -59,7 +60,7 @@ struct DecodeArgs {
   int x_stages, w_stages;  // shared-memory stages of inputs and weight chunks
   int out_pitch;           // bytes of a row of the output stage, 0: rows stored from registers
   int out_vec;             // bytes of a store to the output stage
-  int out_bulk;            // output rows can be written with bulk copies
+  int out_bulk;            // the output stage is stored by one bulk copy
 };
 
 __host__ __device__ __forceinline__ int round_up(int v, int m) { return (v + m - 1) / m * m; }
@@ -267,7 +268,7 @@ __device__ __forceinline__ void arrive(unsigned long long* bar) {
 
 __device__ __forceinline__ void init_bars(Bars* b) {
   for (int i = 0; i < kMaxXStages; ++i) {
-    mbar_init(&b->xfull[i], kLoaders);
+    mbar_init(&b->xfull[i], 1);
     mbar_init(&b->xempty[i], 1);
   }
   for (int i = 0; i < kMaxWStages; ++i) {
@@ -283,127 +284,36 @@ __device__ __forceinline__ void init_bars(Bars* b) {
   b->abort = 0;
 }
 
-// One tile of `rows` x `width` elements into panels, by the loader warps, one
-// 16-byte unit of a panel row at a time: consecutive lanes read consecutive
-// addresses.  Rows past the end of the input become zero; columns past `width`
-// were zeroed once and are never written.  PART is the largest power of two
-// that divides a row's bytes and the address.  Whole units (PART = 16) are
-// copied asynchronously (complete after cp.async.wait_group); smaller parts are
-// gathered in registers, several units at a time: asynchronous copies of 4
-// bytes run at under two a cycle and SM (6000 cycles for 128 rows of 150).
-template <int PART>
-struct PartType {};
-template <>
-struct PartType<8> { using type = uint2; };
-template <>
-struct PartType<4> { using type = uint32_t; };
-template <>
-struct PartType<2> { using type = uint16_t; };
-
-template <int PART, typename T>
-__device__ __forceinline__ void load_tile_by(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l) {
-  const int per_row = (width + 7) >> 3;
-  const uint32_t base = smem_addr(panels);
-  int row = l / per_row, unit = l - row * per_row;
-  const int drow = kLoaders / per_row, dunit = kLoaders - drow * per_row;
-  auto advance = [&]() {
-    row += drow;
-    unit += dunit;
-    if (unit >= per_row) {
-      unit -= per_row;
-      ++row;
-    }
-  };
-  if constexpr (PART == 16) {
-#pragma unroll 4
-    while (row < kTile) {
-      const uint32_t dst = base + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7);
-      const T* from = src + (row < rows ? row * width + unit * 8 : 0);
-      const int bytes = row < rows ? 16 : 0;  // 0: fill with zeros, nothing is read
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(bytes) : "memory");
-      advance();
-    }
-  } else {
-    using Part = typename PartType<PART>::type;
-    constexpr int kParts = 16 / PART, kBatch = PART == 2 ? 5 : 10;
-    while (row < kTile) {
-      union {
-        Part part[kParts];
-        uint4 all;
-      } v[kBatch];
-      const int row0 = row, unit0 = unit;
-#pragma unroll
-      for (int q = 0; q < kBatch; ++q) {
-        v[q].all = make_uint4(0, 0, 0, 0);
-        const Part* from = reinterpret_cast<const Part*>(src + row * width + unit * 8);
-        const int left = row < rows ? width - unit * 8 : 0;
-#pragma unroll
-        for (int e = 0; e < kParts; ++e)
-          if (e * (PART / 2) < left) v[q].part[e] = __ldg(from + e);
-        advance();
-      }
-      row = row0;
-      unit = unit0;
-#pragma unroll
-      for (int q = 0; q < kBatch; ++q) {
-        if (row < kTile)
-          *reinterpret_cast<uint4*>(panels + (unit >> 3) * kPanel + tc::panel_offset(row, unit & 7)) = v[q].all;
-        advance();
-      }
-    }
-  }
+// Inputs are fetched by the copy engine, one box of 128 rows x 64 columns per
+// panel, with zeros past the last row and column.  It needs rows of a multiple of
+// 16 bytes from a 16-byte boundary; other inputs are copied to padded rows first
+// (k_pad_rows).  Cutting panel units out of misaligned rows inside this kernel
+// cost more than that copy: gathered by loader warps from 4-byte words, from
+// shifted 16-byte chunks of a row per thread or exchanged between lanes, 128 rows
+// of 150 took 5600 to 10000 cycles, against 1900 for the weight gradients' matrix
+// instructions.
+__device__ __forceinline__ void fetch_panels(uint8_t* panels, const CUtensorMap* map, int count, int row,
+                                             unsigned long long* bar) {
+  for (int p = 0; p < count; ++p)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+        ::"r"(smem_addr(panels + p * kPanel)), "l"(map), "r"(p * 64), "r"(row), "r"(smem_addr(bar))
+        : "memory");
 }
 
-// The largest copy unit of rows of `width` elements at p: 16, 8, 4 or 2 bytes.
-__device__ __forceinline__ int copy_unit(const void* p, int width) {
-  const uintptr_t m = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(width * 2);
-  return (m & 15) == 0 ? 16 : (m & 7) == 0 ? 8 : (m & 3) == 0 ? 4 : 2;
-}
-
-template <typename T>
-__device__ __forceinline__ void load_tile(uint8_t* panels, const T* __restrict__ src, int width, int rows, int l,
-                                          int unit) {
-  if (unit == 16) load_tile_by<16>(panels, src, width, rows, l);
-  else if (unit == 8) load_tile_by<8>(panels, src, width, rows, l);
-  else if (unit == 4) load_tile_by<4>(panels, src, width, rows, l);
-  else load_tile_by<2>(panels, src, width, rows, l);
-}
-
-// The loader warps' loop over this CTA's tiles.  A tile is handed over when its
-// loads have landed; with four stages, after the next tile's have been issued
-// (any later, and handing it over would wait for a stage still in use).
-template <typename T, bool DY>
-__device__ __forceinline__ void run_loaders(const DecodeArgs& a, Bars* b, uint8_t* stages, int stage_bytes,
-                                            int64_t first, int64_t step, int64_t tiles) {
-  const int l = threadIdx.x - 128;
-  const T* x = static_cast<const T*>(a.x);
-  const T* dy = static_cast<const T*>(a.dy);
-  const int vx = copy_unit(x, a.d), vy = DY ? copy_unit(dy, a.c) : 0;
-  const int lag = a.x_stages > 3 ? a.x_stages - 3 : 0;
-  Ring fill, give;
-  int pending = 0;  // tiles issued and not handed over
+// One lane's loop over this CTA's tiles.
+template <bool DY>
+__device__ __forceinline__ void fetch_inputs(const DecodeArgs& a, Bars* b, uint8_t* stages, int stage_bytes,
+                                             int64_t first, int64_t step, int64_t tiles) {
+  Ring fill;
   for (int64_t t = first; t < tiles; t += step) {
     if (!wait_for(b, &b->xempty[fill.at], fill.parity ^ 1)) break;
-    const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
+    unsigned long long* full = &b->xfull[fill.at];
     uint8_t* xs = stages + fill.at * stage_bytes;
-    load_tile<T>(xs, x + t * kTile * a.d, a.d, rows, l, vx);
-    if (DY) load_tile<T>(xs + a.nxp * kPanel, dy + t * kTile * a.c, a.c, rows, l, vy);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    mbar_arrive_expect_tx(full, stage_bytes);
+    fetch_panels(xs, &a.map_x, a.nxp, (int)(t * kTile), full);
+    if (DY) fetch_panels(xs + a.nxp * kPanel, &a.map_dy, a.nyp, (int)(t * kTile), full);
     fill.next(a.x_stages);
-    if (++pending > lag) {
-      if (lag == 0) asm volatile("cp.async.wait_group 0;" ::: "memory");
-      else asm volatile("cp.async.wait_group 1;" ::: "memory");
-      tc::fence_async_smem();
-      arrive(&b->xfull[give.at]);
-      give.next(a.x_stages);
-      --pending;
-    }
-  }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  tc::fence_async_smem();
-  for (; pending > 0; --pending) {
-    arrive(&b->xfull[give.at]);
-    give.next(a.x_stages);
   }
 }
 
@@ -473,7 +383,7 @@ __device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16],
 // four drain warps, through shared memory to a bulk store: rows straight from
 // the registers would write one sector per thread and instruction.
 template <typename T, int MODE, int ACT>
-__global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
+__global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_constant__ DecodeArgs a) {
   extern __shared__ uint8_t raw[];
   __shared__ Bars bars;
   Bars* b = &bars;
@@ -494,11 +404,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
     init_bars(b);
     for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kEpilogue);
     mbar_init(&b->ofull, kDrain);
-    mbar_init(&b->oempty, 1);
+    mbar_init(&b->oempty, a.out_bulk ? 1 : kDrain);
   }
-  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDecodeThreads * 16)
-    *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
-  tc::fence_async_smem();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -508,8 +415,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
   const int64_t total = mine * a.chunks;
   const bool resident = a.w_stages >= a.chunks;
 
-  if (warp >= 4 && warp < 8) {
-    run_loaders<T, MODE != kFwd>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+  if (warp == 3) {
+    if (lane == 0) fetch_inputs<MODE != kFwd>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+    __syncwarp();
   } else if (warp == 1) {
     if (lane == 0) {  // weight chunks; all resident: loaded once
       const int64_t loads = resident ? a.chunks : total;
@@ -616,7 +524,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
     }
     __syncwarp();
   } else if (warp == 2) {
-    if (a.out_pitch && a.out_bulk) {  // finished tiles: output stage -> global memory
+    if (a.out_bulk) {  // finished tiles: output stage -> global memory
       uint8_t* out = static_cast<uint8_t*>(a.out);
       const int row_bytes = width * 2;
       for (int64_t i = 0; i < mine; ++i) {
@@ -624,12 +532,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         if (!__all_sync(~0u, wait_for(b, &b->ofull, (unsigned)i & 1))) break;
         const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
         uint8_t* dst = out + t * kTile * row_bytes;
-        if (a.out_pitch != row_bytes) {  // padded rows, each a whole number of 16-byte units
-          for (int r = lane; r < rows; r += 32)
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst + (size_t)r * row_bytes),
-                         "r"(smem_addr(os + r * a.out_pitch)), "r"(row_bytes)
-                         : "memory");
-        } else {
+        {
           const int bytes = rows * row_bytes & ~15;
           if (lane == 0 && bytes > 0)
             asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(os)),
@@ -645,14 +548,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
       }
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
-  } else if (warp >= 16) {  // finished tiles: TMEM -> output stage (or global memory)
+  } else if (warp >= 12) {  // finished tiles: TMEM -> output stage (or global memory)
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const bool staged = a.out_pitch && a.out_bulk;
+    const bool staged = a.out_pitch > 0;
     Ring y;
     for (int64_t i = 0; i < mine; ++i) {
       bool ok = wait_for(b, &b->yfull[y.at], y.parity);
-      if (ok && staged) ok = wait_for(b, &b->oempty, (unsigned)(i & 1) ^ 1);
+      if (ok && a.out_bulk) ok = wait_for(b, &b->oempty, (unsigned)(i & 1) ^ 1);
       if (!__all_sync(~0u, ok)) break;
       tc::fence_after();
       const int64_t t = blockIdx.x + i * gridDim.x;
@@ -684,14 +587,34 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
         }
       }
       __syncwarp();
-      if (staged) {
+      if (a.out_bulk) {
         tc::fence_async_smem();
         arrive(&b->ofull);
+      } else if (staged) {  // padded rows, written by the drain warps themselves in 16-byte units
+        arrive(&b->ofull);
+        if (!__all_sync(~0u, wait_for(b, &b->ofull, (unsigned)i & 1))) break;
+        const int per_row = width >> 3, l = threadIdx.x - 384;
+        const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.out) + t * kTile * width * 2);
+        int r = l / per_row, u = l - r * per_row;
+        const int dr = kDrain / per_row, du = kDrain - dr * per_row;
+#pragma unroll 4
+        for (int e = l; e < rows * per_row; e += kDrain) {
+          dst[e] = *reinterpret_cast<const uint4*>(os + r * a.out_pitch + u * 16);
+          r += dr;
+          u += du;
+          if (u >= per_row) {
+            u -= per_row;
+            ++r;
+          }
+        }
+        arrive(&b->oempty);
+        if (!__all_sync(~0u, wait_for(b, &b->oempty, (unsigned)i & 1))) break;
       }
       y.next(nout);
     }
-  } else if (warp >= 8) {  // activation: each warpgroup half of a chunk's hidden units
-    const int wg = (warp >> 2) & 1;
+  } else if (warp >= 4) {  // activation: each warpgroup half of a chunk's hidden units
+    const int wg = (warp >> 2) - 1;
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     // TMEM loads take about 300 cycles: the next columns, of the next chunk
     // too if it is ready, are on their way while the current ones are computed.
@@ -740,8 +663,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
     if (threadIdx.x == 0) {
       atomicAdd(&g_decode_wait_failures, 1ull);
       mbar_wait(&b->sfree, 0);
-      for (int i = 0; i < a.w_stages; ++i)
-        for (unsigned par = 0; par < 2; ++par) mbar_wait(&b->wfull[i], par);
+      for (unsigned par = 0; par < 2; ++par) {
+        for (int i = 0; i < a.w_stages; ++i) mbar_wait(&b->wfull[i], par);
+        for (int i = 0; i < a.x_stages; ++i) mbar_wait(&b->xfull[i], par);
+      }
     }
     __syncthreads();
   }
@@ -751,14 +676,14 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(DecodeArgs a) {
 // --------------------------------------------------------- weight gradients
 // A CTA keeps one chunk's weights and walks tiles; per tile
 //   [g | u] = x [Wg | Wu]^T, dh = dy Wd         -> TMEM
-//   activation (both warpgroups, 32 hidden units each) -> dg, du, h panels in
+//   activation (four warpgroups, 16 hidden units each) -> dg, du, h panels in
 //                shared memory, rows = pixels
 //   [dWg ; dWu] += [dg | du]^T x,  dWd += dy^T h -> TMEM, summed over all tiles
 // The panels are K-major for nobody: both operands of the sums over pixels are
 // MN-major, x and dy from the same panels the first products read.  The next
 // tile's [g | u] is issued before this tile's sums.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
+__global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_constant__ DecodeArgs a) {
   extern __shared__ uint8_t raw[];
   __shared__ Bars bars;
   Bars* b = &bars;
@@ -777,13 +702,10 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
   if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
   if (threadIdx.x == 0) {
     init_bars(b);
-    for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kEpilogue);
+    for (int i = 0; i < 2; ++i) mbar_init(&b->hfull[i], kDwEpilogue);
     mbar_init(&b->dhfull, 1);
-    mbar_init(&b->dhread, kEpilogue);
+    mbar_init(&b->dhread, kDwEpilogue);
   }
-  for (uint32_t i = threadIdx.x * 16; i < (uint32_t)(ws - smem); i += kDwThreads * 16)
-    *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
-  tc::fence_async_smem();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -791,8 +713,9 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
   const int64_t tiles = (a.n + kTile - 1) / kTile;
   const int64_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;
 
-  if (warp >= 4 && warp < 8) {
-    run_loaders<T, true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+  if (warp == 1) {
+    if (lane == 0) fetch_inputs<true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+    __syncwarp();
   } else if (warp == 0) {
     {
       bool ok = true;
@@ -843,17 +766,17 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       };
       gu_products();
       if (ok) dh_products();
-      // nbuf = 2 needs the next tile's stage while this one's is in use
-      const bool ahead = nbuf == 2 && a.x_stages > 1;
       const uint32_t tgu = tc::uniform(tmem + col_gu), tdd = tc::uniform(tmem + col_dd);
       for (int64_t i = 0; i < mine && ok; ++i) {
-        if (ahead && i + 1 < mine) gu_products();
+        // The next tile's first products go before this one's sums if its inputs are there.
+        const bool ahead = i + 1 < mine && nbuf == 2 && __all_sync(~0u, passed(&b->xfull[xg.at], xg.parity));
+        if (ahead) gu_products();
         // tile i's g, u and dh have been read
         ok &= wait_for(b, &b->dhread, (unsigned)i & 1);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
-        if (ahead && i + 1 < mine) dh_products();
+        if (ahead) dh_products();
         // its panels are written
         ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
         ok = __all_sync(~0u, ok);
@@ -891,35 +814,33 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       }
     }
     __syncwarp();
-  } else if (warp >= 8) {
-    const int wg = (warp >> 2) & 1, row = (warp & 3) * 32 + lane;
+  } else if (warp >= 4) {
+    const int wg = (warp >> 2) - 1, row = (warp & 3) * 32 + lane;  // 16 hidden units a thread
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     bool ok = true;
-    GateIn<kDw, 8> v[2];
     for (int64_t i = 0; i < mine; ++i) {
-      const uint32_t buf = lanes + (nbuf == 2 ? (uint32_t)(i & 1) * 128 : 0) + wg * 32, dhc = lanes + col_dh + wg * 32;
+      const uint32_t buf = lanes + (nbuf == 2 ? (uint32_t)(i & 1) * 128 : 0) + wg * 16, dhc = lanes + col_dh + wg * 16;
       ok = __all_sync(~0u, wait_for(b, &b->dhfull, (unsigned)i & 1));
       if (!ok) break;
       tc::fence_after();
-      v[0].load(buf, buf + 64, dhc);
-      uint32_t pg[16], pu[16], ph[16];
+      uint32_t pg[8], pu[8], ph[8];
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        v[p & 1].settle();
-        if (p < 3) {
-          v[(p + 1) & 1].load(buf + 8 * (p + 1), buf + 64 + 8 * (p + 1), dhc + 8 * (p + 1));
-        } else {
+      for (int p = 0; p < 2; ++p) {
+        GateIn<kDw, 8> v;
+        v.load(buf + 8 * p, buf + 64 + 8 * p, dhc + 8 * p);
+        v.settle();
+        if (p == 1) {
           tc::fence_before();
           arrive(&b->dhread);
         }
-        v[p & 1].template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
+        v.template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
       }
       // the previous tile's sums have read the panels
       if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
       if (!ok) break;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t off = tc::panel_offset(row, wg * 4 + q);
+      for (int q = 0; q < 2; ++q) {
+        const uint32_t off = tc::panel_offset(row, wg * 2 + q);
         *reinterpret_cast<uint4*>(st + off) = make_uint4(pg[4 * q], pg[4 * q + 1], pg[4 * q + 2], pg[4 * q + 3]);
         *reinterpret_cast<uint4*>(st + kPanel + off) = make_uint4(pu[4 * q], pu[4 * q + 1], pu[4 * q + 2], pu[4 * q + 3]);
         *reinterpret_cast<uint4*>(st + 2 * kPanel + off) =
@@ -935,27 +856,27 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
       float* part = a.partials + (size_t)blockIdx.x * (2 * fd + (size_t)a.c * a.f);
       const int h = blockIdx.y * kChunk + (row & 63);
       float* gu = part + (row < 64 ? 0 : fd) + (size_t)h * a.d;
-      for (int c0 = wg * 32; c0 < a.d; c0 += 64) {
-        uint32_t v[32];
+      for (int c0 = wg * 16; c0 < a.d; c0 += 64) {
+        uint32_t v[16];
         __syncwarp();
         tc::tmem_ld(lanes + col_gu + c0, v);
         tc::tmem_wait_ld();
         tc::after_wait(v);
         if (h < a.f)
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
+          for (int e = 0; e < 16; ++e)
             if (c0 + e < a.d) gu[c0 + e] = __uint_as_float(v[e]);
       }
       for (int m = 0; m < mblocks; ++m) {
-        uint32_t v[32];
+        uint32_t v[16];
         __syncwarp();
-        tc::tmem_ld(lanes + col_dd + m * 64 + wg * 32, v);
+        tc::tmem_ld(lanes + col_dd + m * 64 + wg * 16, v);
         tc::tmem_wait_ld();
         tc::after_wait(v);
-        const int c = m * 128 + row, h0 = blockIdx.y * kChunk + wg * 32;
+        const int c = m * 128 + row, h0 = blockIdx.y * kChunk + wg * 16;
         if (c < a.c)
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
+          for (int e = 0; e < 16; ++e)
             if (h0 + e < a.f) part[2 * fd + (size_t)c * a.f + h0 + e] = __uint_as_float(v[e]);
       }
       tc::fence_before();
@@ -966,6 +887,8 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(DecodeArgs a) {
     if (threadIdx.x == 0) {
       atomicAdd(&g_decode_wait_failures, 1ull);
       mbar_wait(&b->yfull[0], 0);
+      for (unsigned par = 0; par < 2; ++par)
+        for (int i = 0; i < a.x_stages; ++i) mbar_wait(&b->xfull[i], par);
     }
     __syncthreads();
   }
@@ -994,13 +917,20 @@ static int decode_splits(int64_t n, int f) {
 static int check_dims(const char* who, int64_t n, int dtype, int d, int f, int c) {
   if (dtype != GS_F16 && dtype != GS_BF16)
     return set_error(GS_ERR_INVALID_ARG, "%s: dtype must be GS_F16 or GS_BF16 (got %d)", who, dtype);
-  if (n < 0) return set_error(GS_ERR_INVALID_ARG, "%s: n is negative", who);
+  if (n < 0 || n > GS_DECODE_MAX_N)
+    return set_error(GS_ERR_INVALID_ARG, "%s: n must be in [0, %d]", who, GS_DECODE_MAX_N);
   if (d < 1 || d > GS_DECODE_MAX_D)
     return set_error(GS_ERR_INVALID_ARG, "%s: d must be in [1, %d] (got %d)", who, GS_DECODE_MAX_D, d);
   if (c < 1 || c > GS_DECODE_MAX_C)
     return set_error(GS_ERR_INVALID_ARG, "%s: c must be in [1, %d] (got %d)", who, GS_DECODE_MAX_C, c);
   if (f < 1 || f > GS_DECODE_MAX_F)
     return set_error(GS_ERR_INVALID_ARG, "%s: f must be in [1, %d] (got %d)", who, GS_DECODE_MAX_F, f);
+  return GS_OK;
+}
+
+static int check_workspace(const char* who, const void* ws, size_t have, size_t need) {
+  if (need > 0 && (!ws || have < need)) return set_error(GS_ERR_CAPACITY, "%s: workspace too small", who);
+  if (!aligned(ws, 16)) return set_error(GS_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", who);
   return GS_OK;
 }
 
@@ -1011,10 +941,75 @@ static int check_image(const char* who, const void* image, size_t image_bytes, i
   return GS_OK;
 }
 
-static DecodeArgs decode_args(const void* x, const void* dy, int64_t n, int d, int f, int c, int act,
-                              const void* image) {
+// Rows of `width` elements to rows of `padded` (a multiple of 8), zeros behind:
+// one thread per 16 bytes written, reading `PART` bytes at a time (the largest
+// power of two that divides a row and the address).
+template <typename Part>
+__global__ void k_pad_rows(const Part* __restrict__ src, int64_t n, int width, int per_row, uint4* __restrict__ dst) {
+  constexpr int kParts = 16 / sizeof(Part), kElems = sizeof(Part) / 2;
+  const int parts = width / kElems;  // of a row
+  const int64_t total = n * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t row = i / per_row;
+    const int p0 = (int)(i - row * per_row) * kParts;
+    union {
+      Part part[kParts];
+      uint4 all;
+    } v;
+    v.all = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int e = 0; e < kParts; ++e)
+      if (p0 + e < parts) v.part[e] = __ldg(src + row * parts + p0 + e);
+    dst[i] = v.all;
+  }
+}
+
+static bool fetchable(const void* p, int width) { return width % 8 == 0 && aligned(p, 16); }
+
+static size_t padded_bytes(int64_t n, int width) { return ((size_t)n * round_up(width, 8) * 2 + 255) & ~(size_t)255; }
+
+// Returns rows the copy engine can fetch: p itself, or its padded copy at *ws
+// (which is moved past it).
+static const void* fetchable_rows(const void* p, int64_t n, int width, uint8_t** ws, cudaStream_t s) {
+  if (fetchable(p, width)) return p;
+  uint4* out = reinterpret_cast<uint4*>(*ws);
+  *ws += padded_bytes(n, width);
+  const int per_row = round_up(width, 8) / 8;
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * per_row, 256), 148 * 64);
+  const uintptr_t m = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(width * 2);
+  if (m % 16 == 0) k_pad_rows<uint4><<<grid, 256, 0, s>>>(static_cast<const uint4*>(p), n, width, per_row, out);
+  else if (m % 8 == 0) k_pad_rows<uint2><<<grid, 256, 0, s>>>(static_cast<const uint2*>(p), n, width, per_row, out);
+  else if (m % 4 == 0) k_pad_rows<uint32_t><<<grid, 256, 0, s>>>(static_cast<const uint32_t*>(p), n, width, per_row, out);
+  else k_pad_rows<uint16_t><<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(p), n, width, per_row, out);
+  return out;
+}
+
+// A map of (n, width) 16-bit elements, rows round_up(width, 8) apart, in boxes of
+// 128 rows x 64 columns with the panels' swizzle.
+static bool panel_map(CUtensorMap* map, const void* base, int dtype, int64_t n, int width) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess)
+      fn = nullptr;
+    return reinterpret_cast<Encode>(fn);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)n}, strides[1] = {(cuuint64_t)round_up(width, 8) * 2};
+  const cuuint32_t box[2] = {64, kTile}, step[2] = {1, 1};
+  return encode(map, dtype == GS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static DecodeArgs decode_args(int64_t n, int d, int f, int c, int act, const void* image) {
   DecodeArgs a{};
-  a.x = x; a.dy = dy; a.image = static_cast<const uint8_t*>(image);
+  a.image = static_cast<const uint8_t*>(image);
   a.n = n; a.d = d; a.f = f; a.c = c;
   a.dp = round_up(d, 16); a.cp = round_up(c, 16);
   a.nxp = (d + 63) / 64; a.nyp = (c + 63) / 64;
@@ -1038,14 +1033,16 @@ static size_t plan_smem(DecodeArgs& a) {
     return own + a.x_stages * in - sizeof(Bars);
   }
   const int width = MODE == kFwd ? a.c : a.d, row = width * 2;
-  // Stage rows are padded to an odd number of 16-byte units where that keeps
-  // 16-byte stores (width a multiple of 8, one bulk copy a row); otherwise the
-  // stage is the output's own layout (one bulk copy a tile), whose rows are an
-  // odd number of out_vec bytes apart: no bank conflicts either way.
+  // The stage has the output's own layout where its rows are an odd number of
+  // out_vec bytes apart, so that a column's stores hit all banks: one bulk copy
+  // a tile.  An even number of 16-byte units is padded by one, and the drain
+  // warps copy the rows themselves (128 bulk copies a tile, one a row, took
+  // 5000 cycles: 64 classes 498 us for 1600x1060 instead of DRAIN_US).
   a.out_vec = width % 8 == 0 ? 16 : width % 4 == 0 ? 8 : width % 2 == 0 ? 4 : 2;
   a.out_pitch = width % 8 == 0 ? (row / 16 | 1) * 16 : row;
-  a.out_bulk = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-  size_t out = a.out_bulk ? ((size_t)kTile * a.out_pitch + 15) & ~(size_t)15 : 0;
+  const bool fits = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  a.out_bulk = fits && a.out_pitch == row;
+  size_t out = fits ? ((size_t)kTile * a.out_pitch + 15) & ~(size_t)15 : 0;
   const int need = std::min(a.chunks, 2);
   a.x_stages = 2;
   if (fixed + out + 2 * in + (size_t)need * a.chunk_bytes > kMaxSmem) a.x_stages = 1;
@@ -1121,8 +1118,16 @@ int gs_decode_prepare(const void* w_gate, const void* w_up, const void* w_down, 
   return check_launch("k_decode_prepare");
 }
 
+size_t gs_decode_workspace_bytes(const void* x, const void* dy, int64_t n, int d, int f, int c, int weights) {
+  if (n < 0 || gs_decode_image_bytes(d, f, c) == 0) return 0;
+  size_t bytes = fetchable(x, d) ? 0 : padded_bytes(n, d);
+  if (dy && !fetchable(dy, c)) bytes += padded_bytes(n, c);
+  if (weights) bytes += (size_t)decode_splits(n, f) * (2 * (size_t)f * d + (size_t)c * f) * sizeof(float);
+  return bytes;
+}
+
 int gs_decode_forward(const void* x, int dtype, int64_t n, int d, int f, int c, int activation, const void* image,
-                      size_t image_bytes, void* y, void* stream) {
+                      size_t image_bytes, void* y, void* workspace, size_t workspace_bytes, void* stream) {
   clear_error();
   if (int e = check_dims("gs_decode_forward", n, dtype, d, f, c)) return e;
   if (activation != GS_ACT_SILU && activation != GS_ACT_GELU)
@@ -1130,15 +1135,19 @@ int gs_decode_forward(const void* x, int dtype, int64_t n, int d, int f, int c, 
   if (n == 0) return GS_OK;
   if (!x || !y) return set_error(GS_ERR_INVALID_ARG, "gs_decode_forward: NULL pointer");
   if (int e = check_image("gs_decode_forward", image, image_bytes, d, f, c)) return e;
-  DecodeArgs a = decode_args(x, nullptr, n, d, f, c, activation, image);
+  if (int e = check_workspace("gs_decode_forward", workspace, workspace_bytes,
+                              gs_decode_workspace_bytes(x, nullptr, n, d, f, c, 0)))
+    return e;
+  cudaStream_t s = as_stream(stream);
+  DecodeArgs a = decode_args(n, d, f, c, activation, image);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const void* rows = fetchable_rows(x, n, d, &ws, s);
+  if (rows != x)
+    if (int e = check_launch("k_pad_rows")) return e;
+  if (!panel_map(&a.map_x, rows, dtype, n, d)) return set_error(GS_ERR_CUDA, "gs_decode_forward: tensor map refused");
   a.out = y;
   const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, kTile), 148);
-  return launch_decode<kFwd>(a, dtype, dim3(grid), as_stream(stream));
-}
-
-size_t gs_decode_workspace_bytes(int64_t n, int d, int f, int c) {
-  if (n < 0 || gs_decode_image_bytes(d, f, c) == 0) return 0;
-  return (size_t)decode_splits(n, f) * (2 * (size_t)f * d + (size_t)c * f) * sizeof(float);
+  return launch_decode<kFwd>(a, dtype, dim3(grid), s);
 }
 
 int gs_decode_backward(const void* x, const void* dy, int dtype, int64_t n, int d, int f, int c, int activation,
@@ -1151,29 +1160,36 @@ int gs_decode_backward(const void* x, const void* dy, int dtype, int64_t n, int 
   const bool weights = d_gate || d_up || d_down;
   if (weights && (!d_gate || !d_up || !d_down))
     return set_error(GS_ERR_INVALID_ARG, "gs_decode_backward: give all weight gradients or none");
+  if (!weights && !dx) return GS_OK;
   cudaStream_t s = as_stream(stream);
   const int64_t fd = (int64_t)f * d, cf = (int64_t)c * f;
+  int splits = 0;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (n > 0) {
     if (!x || !dy) return set_error(GS_ERR_INVALID_ARG, "gs_decode_backward: NULL pointer");
     if (int e = check_image("gs_decode_backward", image, image_bytes, d, f, c)) return e;
-  }
-  if (weights && n > 0 && (!workspace || workspace_bytes < gs_decode_workspace_bytes(n, d, f, c)))
-    return set_error(GS_ERR_CAPACITY, "gs_decode_backward: workspace too small");
-  DecodeArgs a = decode_args(x, dy, n, d, f, c, activation, image);
-  if (dx && n > 0) {
-    a.out = dx;
-    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, kTile), 148);
-    if (int e = launch_decode<kDx>(a, dtype, dim3(grid), s)) return e;
-  }
-  if (!weights) return GS_OK;
-  int splits = 0;
-  if (n > 0) {
+    if (int e = check_workspace("gs_decode_backward", workspace, workspace_bytes,
+                                gs_decode_workspace_bytes(x, dy, n, d, f, c, weights)))
+      return e;
+    DecodeArgs a = decode_args(n, d, f, c, activation, image);
+    const void* xr = fetchable_rows(x, n, d, &ws, s);
+    const void* yr = fetchable_rows(dy, n, c, &ws, s);
+    if (int e = check_launch("k_pad_rows", (xr != x) + (yr != dy))) return e;
+    if (!panel_map(&a.map_x, xr, dtype, n, d) || !panel_map(&a.map_dy, yr, dtype, n, c))
+      return set_error(GS_ERR_CUDA, "gs_decode_backward: tensor map refused");
+    if (dx) {
+      a.out = dx;
+      const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, kTile), 148);
+      if (int e = launch_decode<kDx>(a, dtype, dim3(grid), s)) return e;
+    }
+    if (!weights) return GS_OK;
     splits = decode_splits(n, f);
-    a.partials = static_cast<float*>(workspace);
+    a.partials = reinterpret_cast<float*>(ws);
     if (int e = launch_decode<kDw>(a, dtype, dim3((unsigned)splits, (unsigned)a.chunks), s)) return e;
   }
+  if (!weights) return GS_OK;
   const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(2 * fd + cf, 256), 148 * 8);
-  const float* part = static_cast<const float*>(workspace);
+  const float* part = reinterpret_cast<const float*>(ws);
   if (dtype == GS_F16)
     k_decode_reduce<__half><<<grid, 256, 0, s>>>(part, splits, fd, cf, static_cast<__half*>(d_gate),
                                                  static_cast<__half*>(d_up), static_cast<__half*>(d_down));

@@ -17,6 +17,11 @@ from .. import _native as nat
 __all__ = ["FeatureDecoder", "decode_features"]
 
 
+def _workspace(x, dy, f, c, weights):
+    size = nat.load().gs_decode_workspace_bytes(nat.ptr(x), nat.ptr(dy), x.shape[0], x.shape[1], f, c, int(weights))
+    return torch.empty((size,), device=x.device, dtype=torch.uint8) if size else None
+
+
 class _Decode(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act):
@@ -27,8 +32,9 @@ class _Decode(torch.autograd.Function):
         y = torch.empty((n, c), device=dev, dtype=x.dtype)
         nat.call_on(dev, "gs_decode_prepare", nat.ptr(w_gate), nat.ptr(w_up), nat.ptr(w_down), ty, d, f, c,
                     nat.ptr(image), image.numel())
+        ws = _workspace(x, None, f, c, False)
         nat.call_on(dev, "gs_decode_forward", nat.ptr(x), ty, n, d, f, c, act, nat.ptr(image), image.numel(),
-                    nat.ptr(y))
+                    nat.ptr(y), nat.ptr(ws), 0 if ws is None else ws.numel())
         ctx.save_for_backward(x, w_gate, w_up, w_down, image)
         ctx.act = act
         return y
@@ -42,10 +48,9 @@ class _Decode(torch.autograd.Function):
         dev = x.device
         dy = dy.contiguous()
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-        grads, ws = (None, None, None), None
-        if any(ctx.needs_input_grad[1:4]):
-            grads = tuple(torch.empty_like(w) for w in (w_gate, w_up, w_down))
-            ws = torch.empty((nat.load().gs_decode_workspace_bytes(n, d, f, c),), device=dev, dtype=torch.uint8)
+        weights = any(ctx.needs_input_grad[1:4])
+        grads = tuple(torch.empty_like(w) for w in (w_gate, w_up, w_down)) if weights else (None, None, None)
+        ws = _workspace(x, dy, f, c, weights)
         nat.call_on(dev, "gs_decode_backward", nat.ptr(x), nat.ptr(dy), nat.DTYPES[x.dtype], n, d, f, c, ctx.act,
                     nat.ptr(image), image.numel(), nat.ptr(dx), *(nat.ptr(g) for g in grads), nat.ptr(ws),
                     0 if ws is None else ws.numel())
@@ -86,6 +91,8 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
     w_gate, w_up, w_down = (nat.require_cuda(k, w, ty) for k, w in (("w_gate", w_gate), ("w_up", w_up),
                                                                    ("w_down", w_down)))
     nat.same_device(x.device, w_gate=w_gate, w_up=w_up, w_down=w_down)
+    if x.numel() // d > nat.GS_DECODE_MAX_N:
+        raise ValueError(f"features must have at most {nat.GS_DECODE_MAX_N} rows.")
     y = _Decode.apply(x.reshape(-1, d), w_gate, w_up, w_down, nat.GS_GATES[activation])
     return y.reshape(*features.shape[:-1], c)
 

@@ -177,22 +177,29 @@ def test_native_decode_rejects_bad_arguments_before_the_device():
     assert size == 2 * (16384 + 32 * 128)
     for d, f, c in ((0, 8, 8), (129, 8, 8), (8, 0, 8), (8, 65537, 8), (8, 8, 0), (8, 8, 257)):
         assert lib.gs_decode_image_bytes(d, f, c) == 0
-        assert lib.gs_decode_workspace_bytes(10, d, f, c) == 0
+        assert lib.gs_decode_workspace_bytes(16, 16, 10, d, f, c, 1) == 0
         assert lib.gs_decode_prepare(16, 16, 16, 1, d, f, c, 16, 1 << 30, None) == nat.GS_ERR_INVALID_ARG
-        assert lib.gs_decode_forward(16, 1, 4, d, f, c, 0, 16, 1 << 30, 16, None) == nat.GS_ERR_INVALID_ARG
+        assert lib.gs_decode_forward(16, 1, 4, d, f, c, 0, 16, 1 << 30, 16, None, 0, None) == nat.GS_ERR_INVALID_ARG
         assert lib.gs_decode_backward(16, 16, 1, 4, d, f, c, 0, 16, 1 << 30, 16, None, None, None, None, 0,
                                       None) == nat.GS_ERR_INVALID_ARG
     assert lib.gs_decode_prepare(16, 16, 16, 0, 32, 100, 20, 16, size, None) == nat.GS_ERR_INVALID_ARG  # float32
     assert lib.gs_decode_prepare(16, 16, 16, 1, 32, 100, 20, 16, size - 1, None) == nat.GS_ERR_CAPACITY
     assert lib.gs_decode_prepare(16, 16, 16, 1, 32, 100, 20, 8, size, None) == nat.GS_ERR_INVALID_ARG
     assert lib.gs_decode_prepare(None, 16, 16, 1, 32, 100, 20, 16, size, None) == nat.GS_ERR_INVALID_ARG
-    assert lib.gs_decode_forward(16, 1, -1, 32, 100, 20, 0, 16, size, 16, None) == nat.GS_ERR_INVALID_ARG
-    assert lib.gs_decode_forward(16, 1, 4, 32, 100, 20, 2, 16, size, 16, None) == nat.GS_ERR_INVALID_ARG
-    assert lib.gs_decode_forward(None, 1, 4, 32, 100, 20, 0, 16, size, 16, None) == nat.GS_ERR_INVALID_ARG
-    assert lib.gs_decode_forward(16, 1, 4, 32, 100, 20, 0, 16, size - 16, 16, None) == nat.GS_ERR_CAPACITY
-    assert lib.gs_decode_forward(None, 1, 0, 32, 100, 20, 0, None, 0, None, None) == nat.GS_OK
-    need = lib.gs_decode_workspace_bytes(1000, 32, 100, 20)
-    assert need >= 4 * (2 * 32 * 100 + 20 * 100)
+    assert lib.gs_decode_forward(16, 1, -1, 32, 100, 20, 0, 16, size, 16, None, 0, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(16, 1, 4, 32, 100, 20, 2, 16, size, 16, None, 0, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(None, 1, 4, 32, 100, 20, 0, 16, size, 16, None, 0, None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_forward(16, 1, 4, 32, 100, 20, 0, 16, size - 16, 16, None, 0, None) == nat.GS_ERR_CAPACITY
+    assert lib.gs_decode_forward(None, 1, 0, 32, 100, 20, 0, None, 0, None, None, 0, None) == nat.GS_OK
+    assert lib.gs_decode_forward(16, 1, nat.GS_DECODE_MAX_N + 1, 32, 100, 20, 0, 16, size, 16, None, 0,
+                                 None) == nat.GS_ERR_INVALID_ARG
+    # aligned rows need no copy; 20 classes (40 bytes a row) and unaligned addresses do
+    assert lib.gs_decode_workspace_bytes(16, None, 1000, 32, 100, 20, 0) == 0
+    assert lib.gs_decode_workspace_bytes(18, None, 1000, 32, 100, 20, 0) >= 1000 * 64
+    assert lib.gs_decode_workspace_bytes(16, 16, 1000, 32, 100, 20, 0) >= 1000 * 48
+    assert lib.gs_decode_forward(18, 1, 1000, 32, 100, 20, 0, 16, size, 16, None, 0, None) == nat.GS_ERR_CAPACITY
+    need = lib.gs_decode_workspace_bytes(16, 16, 1000, 32, 100, 20, 1)
+    assert need >= 4 * (2 * 32 * 100 + 20 * 100) + 1000 * 48
     args = (16, 16, 1, 1000, 32, 100, 20, 0, 16, size, None, 16, 16)
     assert lib.gs_decode_backward(*args, None, 16, need, None) == nat.GS_ERR_INVALID_ARG
     assert lib.gs_decode_backward(*args, 16, 16, need - 1, None) == nat.GS_ERR_CAPACITY
