@@ -36,6 +36,7 @@ enum { kFwd = 0, kDx = 1, kDw = 2 };
 
 __device__ unsigned long long g_decode_wait_failures;
 
+
 int decode_wait_failures(unsigned long long* out, int reset) {
   cudaError_t e = cudaMemcpyFromSymbol(out, g_decode_wait_failures, sizeof(*out));
   if (e == cudaSuccess && reset) {
@@ -165,8 +166,10 @@ __device__ __forceinline__ void gate2(F2 g, F2& a, F2& slope) {
   if (ACT == GS_ACT_SILU) {
     float t0, t1, p0, p1;
     split(mul(g, f2(-1.4426950408889634f)), t0, t1);
-    const F2 p = add(f2(ex2(fminf(t0, 63.0f)), ex2(fminf(t1, 63.0f))), f2(1.0f));
-    split(p, p0, p1);
+    t0 = fminf(t0, 63.0f);
+    t1 = fminf(t1, 63.0f);
+    const F2 e = f2(ex2(t0), ex2(t1));
+    split(add(e, f2(1.0f)), p0, p1);
     const float inv = rcp(p0 * p1);
     const F2 l = f2(fma_sat(inv, p1, -0x1p-62f), fma_sat(inv, p0, -0x1p-62f));
     a = mul(g, l);
@@ -292,17 +295,26 @@ __device__ __forceinline__ void init_bars(Bars* b) {
 // shifted 16-byte chunks of a row per thread or exchanged between lanes, 128 rows
 // of 150 took 5600 to 10000 cycles, against 1900 for the weight gradients' matrix
 // instructions.
+__device__ __forceinline__ void fetch_panel(uint8_t* dst, const CUtensorMap* map, int col, int row,
+                                            unsigned long long* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(smem_addr(dst)), "l"(map), "r"(col), "r"(row), "r"(smem_addr(bar))
+      : "memory");
+}
 __device__ __forceinline__ void fetch_panels(uint8_t* panels, const CUtensorMap* map, int count, int row,
                                              unsigned long long* bar) {
+  for (int p = 0; p < count; ++p) fetch_panel(panels + p * kPanel, map, p * 64, row, bar);
+}
+// Into L2 only.
+__device__ __forceinline__ void prefetch_panels(const CUtensorMap* map, int count, int row) {
   for (int p = 0; p < count; ++p)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
-        ::"r"(smem_addr(panels + p * kPanel)), "l"(map), "r"(p * 64), "r"(row), "r"(smem_addr(bar))
-        : "memory");
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(p * 64), "r"(row)
+                 : "memory");
 }
 
 // One lane's loop over this CTA's tiles.
-template <bool DY>
+template <bool DY, bool PREFETCH>
 __device__ __forceinline__ void fetch_inputs(const DecodeArgs& a, Bars* b, uint8_t* stages, int stage_bytes,
                                              int64_t first, int64_t step, int64_t tiles) {
   Ring fill;
@@ -313,6 +325,10 @@ __device__ __forceinline__ void fetch_inputs(const DecodeArgs& a, Bars* b, uint8
     mbar_arrive_expect_tx(full, stage_bytes);
     fetch_panels(xs, &a.map_x, a.nxp, (int)(t * kTile), full);
     if (DY) fetch_panels(xs + a.nxp * kPanel, &a.map_dy, a.nyp, (int)(t * kTile), full);
+    if (PREFETCH && t + step < tiles) {  // the next stage is free only when its tile is needed
+      prefetch_panels(&a.map_x, a.nxp, (int)((t + step) * kTile));
+      if (DY) prefetch_panels(&a.map_dy, a.nyp, (int)((t + step) * kTile));
+    }
     fill.next(a.x_stages);
   }
 }
@@ -352,7 +368,10 @@ struct GateIn {
 
 // 32 columns of an output row (or `left`, if fewer), in stores of `vec` bytes.
 __device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16], int left, int vec) {
-  if (vec == 16) {
+  if (vec == 4 && left >= 32) {  // (the tests below cost as much as the stores)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) *reinterpret_cast<uint32_t*>(p + 4 * e) = w[e];
+  } else if (vec == 16) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (8 * e < left)
@@ -389,9 +408,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
   Bars* b = &bars;
   constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
   constexpr uint32_t kBuf = MODE == kFwd ? 128 : 192;  // TMEM columns of a chunk: g, u (, dh)
-  constexpr uint32_t kOut = 2 * kBuf;
+  // TMEM: two chunk buffers, then the accumulators of finished tiles
   const int width = MODE == kFwd ? a.c : a.d, wp = MODE == kFwd ? a.cp : a.dp;
-  const int nout = wp <= (512 - (int)kOut) / 2 ? 2 : 1;  // accumulators of finished tiles
+  constexpr uint32_t kOut = 2 * kBuf;
+  const int nout = wp <= (512 - (int)kOut) / 2 ? 2 : 1;
   const uint32_t out_cols = (512 - kOut) / nout;
   uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
   const int stage_bytes = (a.nxp + (MODE == kFwd ? 0 : a.nyp)) * kPanel;
@@ -416,19 +436,56 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
   const bool resident = a.w_stages >= a.chunks;
 
   if (warp == 3) {
-    if (lane == 0) fetch_inputs<MODE != kFwd>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+    if (lane == 0 && resident) fetch_inputs<MODE != kFwd, false>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {  // weight chunks; all resident: loaded once
-      const int64_t loads = resident ? a.chunks : total;
-      Ring w;
-      int j = 0;
-      for (int64_t q = 0; q < loads; ++q) {
-        if (!wait_for(b, &b->wempty[w.at], w.parity ^ 1)) break;
-        mbar_arrive_expect_tx(&b->wfull[w.at], a.chunk_bytes);
-        bulk_g2s(ws + w.at * a.chunk_bytes, a.image + (size_t)j * a.chunk_bytes, a.chunk_bytes, &b->wfull[w.at]);
-        w.next(a.w_stages);
-        if (++j == a.chunks) j = 0;
+    if (lane == 0 && resident) {
+      for (int j = 0; j < a.chunks; ++j) {
+        mbar_arrive_expect_tx(&b->wfull[j], a.chunk_bytes);
+        bulk_g2s(ws + j * a.chunk_bytes, a.image + (size_t)j * a.chunk_bytes, a.chunk_bytes, &b->wfull[j]);
+      }
+    } else if (lane == 0) {
+      // Weights stream through the stages.  The copy engine serves one SM's
+      // requests in order, so the next tile's panels are spread over this
+      // tile's chunks: fetched at once they would hold up the weights.
+      constexpr bool kDy = MODE != kFwd;
+      const int panels = a.nxp + (kDy ? a.nyp : 0);
+      Ring w, x;
+      auto fetch_some = [&](int64_t i, int from, int to) {  // panels [from, to) of this CTA's tile i
+        unsigned long long* full = &b->xfull[x.at];
+        const int row = (int)((blockIdx.x + i * gridDim.x) * kTile);
+        for (int p = from; p < to; ++p) {
+          uint8_t* dst = smem + x.at * stage_bytes + p * kPanel;
+          const bool dy = p >= a.nxp;
+          fetch_panel(dst, dy ? &a.map_dy : &a.map_x, (dy ? p - a.nxp : p) * 64, row, full);
+        }
+      };
+      mbar_arrive_expect_tx(&b->xfull[0], stage_bytes);
+      fetch_some(0, 0, panels);
+      x.next(a.x_stages);
+      bool ok = true;
+      for (int64_t i = 0; i < mine && ok; ++i) {
+        bool open = false;  // the next tile's stage is free
+        int done = 0;
+        for (int j = 0; j < a.chunks; ++j) {
+          ok = wait_for(b, &b->wempty[w.at], w.parity ^ 1);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&b->wfull[w.at], a.chunk_bytes);
+          bulk_g2s(ws + w.at * a.chunk_bytes, a.image + (size_t)j * a.chunk_bytes, a.chunk_bytes, &b->wfull[w.at]);
+          w.next(a.w_stages);
+          // with one stage, this tile's first products must all be done first
+          if (i + 1 == mine || (a.x_stages == 1 && j + 1 < a.chunks)) continue;
+          if (!open) {
+            ok = wait_for(b, &b->xempty[x.at], x.parity ^ 1);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&b->xfull[x.at], stage_bytes);
+            open = true;
+          }
+          const int upto = panels * (j + 1) / a.chunks;
+          fetch_some(i + 1, done, upto);
+          done = upto;
+        }
+        x.next(a.x_stages);
       }
     }
     __syncwarp();
@@ -562,29 +619,29 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
       const uint32_t src = lanes + kOut + y.at * out_cols;
       const bool here = staged || t * kTile + row < a.n;
       uint8_t* p = staged ? os + row * a.out_pitch : static_cast<uint8_t*>(a.out) + (t * kTile + row) * width * 2;
-      // The next columns are on their way while the current ones are stored; the
-      // accumulator is given back when the last ones have been read.
-      uint32_t v[2][32];
-      tc::tmem_ld(src, v[0]);
-      if (width > 32) tc::tmem_ld(src + 32, v[1]);
-      for (int c0 = 0; c0 < width; c0 += 64, p += 128) {
-        tc::tmem_wait_ld();
-        tc::after_wait(v[0]);
-        tc::after_wait(v[1]);
-        if (c0 + 64 >= width) {
+      // Up to 160 columns are read and rounded before any is stored: the next
+      // tile's second products wait for the accumulator.
+      for (int c0 = 0; c0 < width; c0 += 160, p += 320) {
+        uint32_t w[5][16];
+#pragma unroll
+        for (int g = 0; g < 5; ++g) {
+          if (c0 + 32 * g < width) {
+            uint32_t v[32];
+            __syncwarp();
+            tc::tmem_ld(src + c0 + 32 * g, v);
+            tc::tmem_wait_ld();
+            tc::after_wait(v);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) w[g][e] = pack2<T>(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+          }
+        }
+        if (c0 + 160 >= width) {
           tc::fence_before();
           arrive(&b->yempty[y.at]);
         }
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t w[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            w[e] = pack2<T>(__uint_as_float(v[half][2 * e]), __uint_as_float(v[half][2 * e + 1]));
-          __syncwarp();
-          if (c0 + 64 + 32 * half < width) tc::tmem_ld(src + c0 + 64 + 32 * half, v[half]);
-          if (here && c0 + 32 * half < width) store_row32(p + 64 * half, w, width - c0 - 32 * half, a.out_vec);
-        }
+        for (int g = 0; g < 5; ++g)
+          if (here && c0 + 32 * g < width) store_row32(p + 64 * g, w[g], width - c0 - 32 * g, a.out_vec);
       }
       __syncwarp();
       if (a.out_bulk) {
@@ -643,9 +700,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
           v[0].load(next, next + 64, next + 128);
           have = true;
         }
-        // The results go over columns of g and u that this warp has read.
         uint32_t h[kCols / 2], dg[kCols / 2], du[kCols / 2];
         v[p & 1].template compute<T, ACT>(h, dg, du);
+        // over columns of g and u that this warp has read
         if constexpr (MODE == kFwd) {
           tc::tmem_st(buf + p * (kCols / 2), h);
         } else {
@@ -714,7 +771,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
   const int64_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;
 
   if (warp == 1) {
-    if (lane == 0) fetch_inputs<true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+    if (lane == 0) fetch_inputs<true, true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
     __syncwarp();
   } else if (warp == 0) {
     {
@@ -835,7 +892,6 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
         }
         v.template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
       }
-      // the previous tile's sums have read the panels
       if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
       if (!ok) break;
 #pragma unroll
@@ -999,6 +1055,10 @@ static bool panel_map(CUtensorMap* map, const void* base, int dtype, int64_t n, 
     return reinterpret_cast<Encode>(fn);
   }();
   if (!encode) return false;
+  // Encoding needs a current context, which a thread that has made no runtime
+  // call yet (autograd's) does not have.
+  int device;
+  if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return false;
   const cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)n}, strides[1] = {(cuuint64_t)round_up(width, 8) * 2};
   const cuuint32_t box[2] = {64, kTile}, step[2] = {1, 1};
   return encode(map, dtype == GS_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,

@@ -2,6 +2,7 @@
 
 import ctypes
 import math
+import threading
 
 import pytest
 import torch
@@ -195,3 +196,23 @@ def test_decoder_object_trains_float32_leaves():
     y.float().square().sum().backward()
     for p in dec.params.values():
         assert p.grad is not None and p.grad.dtype == torch.float32 and torch.isfinite(p.grad).all()
+
+
+def test_first_call_of_a_thread():
+    x, wg, wu, wd, dy = _inputs(300, 64, 64, 64, "bf16")
+    size = nat.load().gs_decode_image_bytes(64, 64, 64)
+    image = torch.empty((size,), device="cuda", dtype=torch.uint8)
+    nat.call("gs_decode_prepare", wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 2, 64, 64, 64, image.data_ptr(), size,
+             nat.stream())
+    leaf = x.clone().requires_grad_(True)
+    want = torch.autograd.grad(decode_features(leaf, wg, wu, wd), leaf, dy)[0]
+    dx = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    args = (x.data_ptr(), dy.data_ptr(), 2, 300, 64, 64, 64, 0, image.data_ptr(), size, dx.data_ptr(), None, None, None,
+            None, 0, None)
+    status = []
+    t = threading.Thread(target=lambda: status.append(nat.load().gs_decode_backward(*args)))  # no CUDA call before it
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert status == [nat.GS_OK] and torch.equal(dx, want)
