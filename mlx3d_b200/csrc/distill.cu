@@ -4,15 +4,34 @@
 //   q = softmax over all classes s_c / T
 //   L = w T^2 sum_k p_k (log p_k - log q_{i_k}),  dL/ds_c = w T (q_c - sum_{i_k = c} p_k)
 //
-// One warp per row; the running maximum and sum of the student's softmax are
-// kept per lane in one pass and merged over the warp, the gradient rereads the
-// row from cache.
+// Bound by memory: the logits are read once and the gradient written once.
+//   k_distill_tile  rows of up to 8 KB: a block stages a tile of rows in shared
+//                   memory with one bulk copy, groups of 4 to 32 lanes take a row
+//                   each, the gradient replaces the logits in the tile and leaves
+//                   with one bulk copy.  Several blocks per SM overlap their
+//                   copies with each other's arithmetic.
+//   k_distill_row   longer rows: one block per row, staged in shared memory while
+//                   it fits.
 #include "feature_common.cuh"
 
 namespace gs {
 
-constexpr int kDistillWarps = 8;
 constexpr int kDistillMaxBlocks = 148 * 8;
+constexpr int kTileThreads = 128, kRowThreads = 512;
+constexpr size_t kTileRowBytes = 8192;   // longest row of the tile kernel
+constexpr size_t kTileSmem = 40 * 1024;  // five blocks per SM
+constexpr size_t kRowSmem = 200 * 1024;
+
+__device__ unsigned long long g_distill_wait_failures;
+
+int distill_wait_failures(unsigned long long* out, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_distill_wait_failures, sizeof(*out));
+  if (e == cudaSuccess && reset) {
+    const unsigned long long z = 0;
+    e = cudaMemcpyToSymbol(g_distill_wait_failures, &z, sizeof(z));
+  }
+  return (int)e;
+}
 
 struct DistillArgs {
   const void* logits;
@@ -29,15 +48,32 @@ struct DistillArgs {
   void* grad;
 };
 
-__device__ __forceinline__ float warp_max(float v) {
+// Over G consecutive lanes.
+template <int G>
+__device__ __forceinline__ float group_max(float v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
+  for (int o = G / 2; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
   return v;
 }
-__device__ __forceinline__ float warp_sum(float v) {
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   return v;
+}
+// 2^x to 2 ulp.  Arguments are (difference) * (log2 e / T): three roundings,
+// each relative to the exponent.
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ int64_t teacher_row(const DistillArgs& a, int64_t r) {
+  if (!a.rec_bytes) return 0;
+  const int64_t rec = a.t.rows ? a.t.rows[r] : a.t.first_row + r;
+  return rec >= 0 && rec < a.t.n_records ? rec : -1;
 }
 
 // Entry e of row r: index -1 where absent.
@@ -67,112 +103,281 @@ __device__ __forceinline__ void teacher_entry(const DistillArgs& a, int64_t r, i
   *idx = here ? i : -1;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDistillWarps * 32) k_distill_rows(DistillArgs a) {
-  extern __shared__ float2 smem[];  // k (index, p) pairs per warp
-  __shared__ double block_sum[kDistillWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int k = a.t.k;
-  float2* ent = smem + warp * k;
-  const T* logits = static_cast<const T*>(a.logits);
-  double acc = 0.0;
-  for (int64_t r = (int64_t)blockIdx.x * kDistillWarps + warp; r < a.n; r += (int64_t)gridDim.x * kDistillWarps) {
-    const T* s = logits + r * a.classes;
-    // teacher
-    int64_t rec = 0;
-    if (a.rec_bytes) {
-      rec = a.t.rows ? a.t.rows[r] : a.t.first_row + r;
-      if (rec < 0 || rec >= a.t.n_records) rec = -1;
+// The sum of a double per thread over the block, in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ void block_partial(double v, double* out) {
+  __shared__ double part[THREADS / 32];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (int i = 0; i < THREADS / 32; ++i) t += part[i];
+    *out = t;
+  }
+}
+
+// The teacher's side of a row by a group of G lanes: entries (index, z) become
+// (index, p); returns whether any is present (in every lane of the group).
+//   term = sum_k p_k ((z_k - max z) - (s_k - m)) / T - log sum_k exp((z_k - max z) / T)
+// so that the loss is T^2 (term + log sum_c exp((s_c - m) / T)), as sum_k p_k = 1.
+template <int G, typename Logit>
+__device__ __forceinline__ bool teacher_terms(float2* ent, int k, int lane, float m, float inv_temp, Logit logit,
+                                              float& term) {
+  const float c2 = inv_temp * kLog2e;
+  float zmax = -INFINITY, any = 0.0f;
+  for (int e = lane; e < k; e += G) {
+    if (__float_as_int(ent[e].x) >= 0) any = 1.0f;
+    zmax = fmaxf(zmax, ent[e].y);
+  }
+  zmax = group_max<G>(zmax);
+  float tot = 0.0f;
+  for (int e = lane; e < k; e += G)
+    if (__float_as_int(ent[e].x) >= 0) tot += exp2_of((ent[e].y - zmax) * c2);
+  tot = group_sum<G>(tot);
+  float sum = 0.0f;
+  for (int e = lane; e < k; e += G) {
+    const int idx = __float_as_int(ent[e].x);
+    float p = 0.0f;
+    if (idx >= 0) {
+      const float z = ent[e].y - zmax;
+      p = exp2_of(z * c2) / tot;
+      if (p != 0.0f) sum += p * ((z - (logit(idx) - m)) * inv_temp);
     }
-    float zmax = -INFINITY;
-    bool any = false;
-    for (int e = lane; e < k; e += 32) {
+    ent[e].y = p;
+  }
+  term = group_sum<G>(sum) - logf(tot);
+  return group_max<G>(any) > 0.0f;
+}
+
+// Gradients of the teacher's classes, scaled: the first entry of a class holds
+// (class, f (q - sum of the class's p)), every other one (-1, -).
+template <int G, typename Logit>
+__device__ __forceinline__ void class_gradients(const float2* ent, float2* out, int k, int lane, float m, float c2,
+                                                float inv_sum, float f, Logit logit) {
+  for (int e = lane; e < k; e += G) {
+    const int idx = __float_as_int(ent[e].x);
+    int to = -1;
+    float g = 0.0f;
+    if (idx >= 0) {
+      bool first = true;
+      float p = 0.0f;
+      for (int j = 0; j < k; ++j) {
+        const float2 o = ent[j];
+        if (__float_as_int(o.x) == idx) {
+          first &= j >= e;
+          p += o.y;
+        }
+      }
+      if (first) {
+        to = idx;
+        g = (exp2_of((logit(idx) - m) * c2) * inv_sum - p) * f;
+      }
+    }
+    out[e] = make_float2(__int_as_float(to), g);
+  }
+}
+
+template <typename T, int G>
+__global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, int tile_rows, int bulk_in, int bulk_out) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ unsigned long long bar;
+  const int C = (int)a.classes, k = a.t.k;
+  T* tile = reinterpret_cast<T*>(smem);
+  float2* ents = reinterpret_cast<float2*>(smem + (((size_t)tile_rows * C * sizeof(T) + 15) & ~(size_t)15));
+  float2* fixes = ents + (size_t)tile_rows * k;
+  float2* row_w = fixes + (size_t)tile_rows * k;  // (weight, gradient factor)
+  constexpr int kGroups = kTileThreads / G;
+  const int group = threadIdx.x / G, lane = threadIdx.x % G;
+  const float c2 = a.inv_temp * kLog2e;
+  if (threadIdx.x == 0) mbar_init(&bar, 1);
+  __syncthreads();
+  unsigned phase = 0;
+  double acc = 0.0;
+  const int64_t tiles = (a.n + tile_rows - 1) / tile_rows;
+  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+    const int64_t r0 = t * tile_rows;
+    const int rows = (int)min((int64_t)tile_rows, a.n - r0);
+    const T* src = static_cast<const T*>(a.logits) + r0 * C;
+    const bool in = bulk_in && rows == tile_rows;
+    const uint32_t bytes = (uint32_t)(rows * C * sizeof(T));
+    if (threadIdx.x == 0) {
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile has left
+      if (in) {
+        mbar_arrive_expect_tx(&bar, bytes);
+        bulk_g2s(tile, src, bytes, &bar);
+      }
+    }
+    if (!in) {
+      __syncthreads();
+#pragma unroll 4
+      for (int i = threadIdx.x; i < rows * C; i += kTileThreads) tile[i] = src[i];
+    }
+    // meanwhile the teacher's entries and the weights
+    for (int r = threadIdx.x; r < rows; r += kTileThreads) {
+      const float w = a.weight ? a.weight[r0 + r] : 1.0f;
+      row_w[r] = make_float2(w, w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r0 + r : 0] : 1.0f));
+    }
+    for (int i = threadIdx.x; i < rows * k; i += kTileThreads) {
+      const int r = i / k;
+      float z;
+      int idx;
+      teacher_entry(a, r0 + r, teacher_row(a, r0 + r), i - r * k, &z, &idx);
+      ents[i] = make_float2(__int_as_float(idx), z);
+    }
+    bool ok = true;
+    if (in) {
+      ok = mbar_wait(&bar, phase);
+      phase ^= 1;
+    }
+    if (!__syncthreads_and(ok)) {
+      if (threadIdx.x == 0) atomicAdd(&g_distill_wait_failures, 1ull);
+      break;
+    }
+    for (int rr = 0; rr < rows; rr += kGroups) {
+      // Idle groups of the last round read a row like the others (the shuffles
+      // are the warp's) and write nothing.
+      const bool live = rr + group < rows;
+      const int r = live ? rr + group : rows - 1, kk = live ? k : 0;
+      T* s = tile + (size_t)r * C;
+      float2* ent = ents + (size_t)r * k;
+      float m = -INFINITY;
+#pragma unroll 4
+      for (int c = lane; c < C; c += G) m = fmaxf(m, to_f32(s[c]));
+      m = group_max<G>(m);
+      float sum = 0.0f;
+#pragma unroll 4
+      for (int c = lane; c < C; c += G) sum += exp2_of((to_f32(s[c]) - m) * c2);
+      sum = group_sum<G>(sum);
+      const float inv = 1.0f / sum;
+      auto logit = [&](int i) { return to_f32(s[i]); };
+      float term;
+      const bool any = teacher_terms<G>(ent, kk, lane, m, a.inv_temp, logit, term);
+      const float2 w = row_w[r];
+      const float loss = any ? (term + logf(sum)) * (a.temp * a.temp) * w.x : 0.0f;
+      if (live && lane == 0) {
+        if (a.row_loss) a.row_loss[r0 + r] = loss;
+        acc += (double)loss;
+      }
+      if (a.grad) {
+        __syncwarp();
+        float2* fix = fixes + (size_t)r * k;
+        class_gradients<G>(ent, fix, any ? kk : 0, lane, m, c2, inv, w.y, logit);
+        __syncwarp();
+        if (live) {
+          if (any) {
+            const float f = inv * w.y;
+#pragma unroll 4
+            for (int c = lane; c < C; c += G) s[c] = from_f32<T>(exp2_of((to_f32(s[c]) - m) * c2) * f);
+          } else {
+            for (int c = lane; c < C; c += G) s[c] = from_f32<T>(0.0f);
+          }
+        }
+        __syncwarp();
+        for (int e = lane; e < (any ? kk : 0); e += G) {
+          const float2 g = fix[e];
+          if (__float_as_int(g.x) >= 0) s[__float_as_int(g.x)] = from_f32<T>(g.y);
+        }
+      }
+    }
+    if (a.grad) {
+      T* dst = static_cast<T*>(a.grad) + r0 * C;
+      const bool out = bulk_out && rows == tile_rows;
+      if (out) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncthreads();
+      if (!out) {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < rows * C; i += kTileThreads) dst[i] = tile[i];
+        __syncthreads();
+      } else if (threadIdx.x == 0) {
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(tile)),
+                     "r"(bytes)
+                     : "memory");
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+    } else {
+      __syncthreads();
+    }
+  }
+  if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (a.partials) block_partial<kTileThreads>(acc, a.partials + blockIdx.x);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int staged) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float red[kRowThreads / 32], stats[3];
+  __shared__ float2 ent[GS_TEACHER_MAX_K], fix[GS_TEACHER_MAX_K];
+  const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  T* row = reinterpret_cast<T*>(smem);
+  const float c2 = a.inv_temp * kLog2e;
+  double acc = 0.0;
+  for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
+    const T* src = static_cast<const T*>(a.logits) + r * C;
+    const int64_t rec = teacher_row(a, r);
+    for (int e = threadIdx.x; e < k; e += kRowThreads) {
       float z;
       int idx;
       teacher_entry(a, r, rec, e, &z, &idx);
       ent[e] = make_float2(__int_as_float(idx), z);
-      any |= idx >= 0;
-      zmax = fmaxf(zmax, z);
     }
-    any = __any_sync(~0u, any);
-    T* g = static_cast<T*>(a.grad);
-    if (g) g += r * a.classes;
-    const float w = a.weight ? a.weight[r] : 1.0f;
-    if (!any) {  // nothing to learn from: no loss, no gradient
-      if (g)
-        for (int64_t c = lane; c < a.classes; c += 32) g[c] = from_f32<T>(0.0f);
-      if (a.row_loss && lane == 0) a.row_loss[r] = 0.0f;
-      __syncwarp();
-      continue;
+    float m = -INFINITY;
+#pragma unroll 8
+    for (int c = threadIdx.x; c < C; c += kRowThreads) {
+      const T v = src[c];
+      if (staged) row[c] = v;
+      m = fmaxf(m, to_f32(v));
     }
-    zmax = warp_max(zmax);
-    float tot = 0.0f;
-    for (int e = lane; e < k; e += 32)
-      if (__float_as_int(ent[e].x) >= 0) tot += expf((ent[e].y - zmax) * a.inv_temp);
-    tot = warp_sum(tot);
-    const float log_tot = logf(tot);
-    // student: running maximum and sum
-    float m = -INFINITY, sum = 0.0f;
-    for (int64_t c = lane; c < a.classes; c += 32) {
-      const float v = to_f32(s[c]);
-      if (v > m) {
-        sum = sum * expf((m - v) * a.inv_temp) + 1.0f;
-        m = v;
-      } else {
-        sum += expf((v - (m == -INFINITY ? 0.0f : m)) * a.inv_temp);
-      }
-    }
-    const float mw = warp_max(m);
-    sum = warp_sum(m == mw ? sum : sum * expf((m - mw) * a.inv_temp));
-    m = mw;
-    const float lse = logf(sum);
-    float loss = 0.0f;
-    for (int e = lane; e < k; e += 32) {
-      const int idx = __float_as_int(ent[e].x);
-      float p = 0.0f;
-      if (idx >= 0) {
-        const float zz = (ent[e].y - zmax) * a.inv_temp;
-        p = expf(zz) / tot;
-        const float logq = (to_f32(s[idx]) - m) * a.inv_temp - lse;
-        if (p != 0.0f) loss += p * (zz - log_tot - logq);
-      }
-      ent[e].y = p;
-    }
-    loss = warp_sum(loss) * (a.temp * a.temp) * w;
-    if (lane == 0) {
-      if (a.row_loss) a.row_loss[r] = loss;
-      acc += (double)loss;
-    }
-    if (g) {
-      const float f = w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r : 0] : 1.0f);
-      for (int64_t c = lane; c < a.classes; c += 32)
-        g[c] = from_f32<T>(expf((to_f32(s[c]) - m) * a.inv_temp - lse) * f);
-      __syncwarp();
-      // The teacher's classes: the first entry of a class writes q - (sum of the class's p).
-      for (int e = lane; e < k; e += 32) {
-        const int idx = __float_as_int(ent[e].x);
-        if (idx < 0) continue;
-        bool first = true;
-        float p = 0.0f;
-        for (int j = 0; j < k; ++j)
-          if (__float_as_int(ent[j].x) == idx) {
-            first &= j >= e;
-            p += ent[j].y;
-          }
-        if (first) g[idx] = from_f32<T>((expf((to_f32(s[idx]) - m) * a.inv_temp - lse) - p) * f);
-      }
-    }
-    __syncwarp();
-  }
-  if (a.partials) {
-    if (lane == 0) block_sum[warp] = acc;
+    m = group_max<32>(m);
+    if (lane == 0) red[warp] = m;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      double t = 0.0;
-      for (int i = 0; i < kDistillWarps; ++i) t += block_sum[i];
-      a.partials[blockIdx.x] = t;
+    m = group_max<32>(lane < kRowThreads / 32 ? red[lane] : -INFINITY);
+    __syncthreads();
+    const T* s = staged ? row : src;  // (staged[c] was written by this thread; other reads follow a barrier)
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int c = threadIdx.x; c < C; c += kRowThreads) sum += exp2_of((to_f32(s[c]) - m) * c2);
+    sum = group_sum<32>(sum);
+    if (lane == 0) red[warp] = sum;
+    __syncthreads();
+    const float w = a.weight ? a.weight[r] : 1.0f;
+    const float f = w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r : 0] : 1.0f);
+    if (warp == 0) {
+      sum = group_sum<32>(lane < kRowThreads / 32 ? red[lane] : 0.0f);
+      auto logit = [&](int i) { return to_f32(s[i]); };
+      float term;
+      const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
+      __syncwarp();
+      const float inv = 1.0f / sum;
+      if (a.grad) class_gradients<32>(ent, fix, any ? k : 0, lane, m, c2, inv, f, logit);
+      if (lane == 0) {
+        const float loss = any ? (term + logf(sum)) * (a.temp * a.temp) * w : 0.0f;
+        if (a.row_loss) a.row_loss[r] = loss;
+        acc += (double)loss;
+        stats[0] = inv;
+        stats[1] = any ? 1.0f : 0.0f;
+      }
     }
+    __syncthreads();
+    if (a.grad) {
+      T* g = static_cast<T*>(a.grad) + r * C;
+      const bool any = stats[1] > 0.0f;
+      const float qf = stats[0] * f;
+      if (any) {
+#pragma unroll 8
+        for (int c = threadIdx.x; c < C; c += kRowThreads) g[c] = from_f32<T>(exp2_of((to_f32(s[c]) - m) * c2) * qf);
+      } else {
+        for (int c = threadIdx.x; c < C; c += kRowThreads) g[c] = from_f32<T>(0.0f);
+      }
+      __syncthreads();
+      if (any)
+        for (int e = threadIdx.x; e < k; e += kRowThreads)
+          if (__float_as_int(fix[e].x) >= 0) g[__float_as_int(fix[e].x)] = from_f32<T>(fix[e].y);
+    }
+    __syncthreads();
   }
+  if (a.partials) block_partial<kRowThreads>(acc, a.partials + blockIdx.x);
 }
 
 __global__ void k_distill_finish(const double* partials, int n, double scale, float* loss) {
@@ -185,6 +390,44 @@ __global__ void k_distill_finish(const double* partials, int n, double scale, fl
     if (threadIdx.x < o) part[threadIdx.x] += part[threadIdx.x + o];
   }
   if (threadIdx.x == 0) *loss = (float)(part[0] * scale);
+}
+
+template <typename T, int G>
+static int launch_tile(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
+  const size_t per_row = a.classes * sizeof(T) + 16 * (size_t)a.t.k + 8;
+  // a multiple of 8 rows is a multiple of 16 bytes, and few rows still make a
+  // tile for every SM
+  int64_t rows = std::max<int64_t>(8, (int64_t)(kTileSmem / per_row) & ~7ll);
+  rows = std::min<int64_t>(rows, std::max<int64_t>(8, ceil_div(ceil_div(a.n, 148 * 4), 8) * 8));
+  const size_t smem = ((rows * a.classes * sizeof(T) + 15) & ~(size_t)15) + rows * (16 * (size_t)a.t.k + 8);
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(k_distill_tile<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_tile: %s", cudaGetErrorString(e));
+  }
+  *blocks = (unsigned)std::min<int64_t>(ceil_div(a.n, rows), kDistillMaxBlocks);
+  k_distill_tile<T, G><<<*blocks, kTileThreads, smem, st>>>(a, (int)rows, aligned(a.logits, 16), aligned(a.grad, 16));
+  return check_launch("k_distill_tile");
+}
+
+template <typename T>
+static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
+  if (a.classes * sizeof(T) > kTileRowBytes) {
+    const size_t row = (a.classes * sizeof(T) + 15) & ~(size_t)15;
+    const bool staged = row <= kRowSmem;
+    if (staged && row > 32 * 1024) {
+      cudaError_t e = cudaFuncSetAttribute(k_distill_row<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)row);
+      if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_row: %s", cudaGetErrorString(e));
+    }
+    *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
+    k_distill_row<T><<<*blocks, kRowThreads, staged ? row : 0, st>>>(a, staged);
+    return check_launch("k_distill_row");
+  }
+  // Lanes of a row: enough that a lane's share stays a few dozen classes, few
+  // enough that reductions and the teacher's entries do not outweigh it.
+  if (a.classes <= 32) return launch_tile<T, 4>(a, st, blocks);
+  if (a.classes <= 256) return launch_tile<T, 8>(a, st, blocks);
+  if (a.classes <= 1024) return launch_tile<T, 16>(a, st, blocks);
+  return launch_tile<T, 32>(a, st, blocks);
 }
 
 }  // namespace gs
@@ -234,13 +477,12 @@ int gs_distill(const void* logits, int dtype, int64_t n, int64_t classes, const 
   a.row_loss = row_loss; a.grad = grad;
   a.partials = loss ? static_cast<double*>(workspace) : nullptr;
   cudaStream_t st = as_stream(stream);
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, kDistillWarps), kDistillMaxBlocks);
-  if (grid > 0) {
-    const size_t smem = sizeof(float2) * kDistillWarps * teacher->k;
-    if (dtype == GS_F32) k_distill_rows<float><<<grid, kDistillWarps * 32, smem, st>>>(a);
-    else if (dtype == GS_F16) k_distill_rows<__half><<<grid, kDistillWarps * 32, smem, st>>>(a);
-    else k_distill_rows<__nv_bfloat16><<<grid, kDistillWarps * 32, smem, st>>>(a);
-    if (int e = check_launch("k_distill_rows")) return e;
+  unsigned grid = 0;
+  if (n > 0) {
+    const int e = dtype == GS_F32   ? launch_distill<float>(a, st, &grid)
+                  : dtype == GS_F16 ? launch_distill<__half>(a, st, &grid)
+                                    : launch_distill<__nv_bfloat16>(a, st, &grid);
+    if (e) return e;
   }
   if (loss) {
     k_distill_finish<<<1, 256, 0, st>>>(a.partials, (int)grid, scale, loss);
