@@ -5,7 +5,7 @@
 //   L = w T^2 sum_k p_k (log p_k - log q_{i_k}),  dL/ds_c = w T (q_c - sum_{i_k = c} p_k)
 //
 // Bound by memory: the logits are read once and the gradient written once.
-//   k_distill_tile  rows of up to 8 KB: a block stages a tile of rows in shared
+//   k_distill_tile  up to 1536 classes: a block stages a tile of rows in shared
 //                   memory with one bulk copy, groups of 4 to 32 lanes take a row
 //                   each, the gradient replaces the logits in the tile and leaves
 //                   with one bulk copy.  Several blocks per SM overlap their
@@ -18,8 +18,7 @@ namespace gs {
 
 constexpr int kDistillMaxBlocks = 148 * 8;
 constexpr int kTileThreads = 128, kRowThreads = 512;
-constexpr size_t kTileRowBytes = 8192;   // longest row of the tile kernel
-constexpr size_t kTileSmem = 40 * 1024;  // five blocks per SM
+constexpr size_t kTileSmem = 20 * 1024;  // shared memory of a block (or 8 rows)
 constexpr size_t kRowSmem = 200 * 1024;
 
 __device__ unsigned long long g_distill_wait_failures;
@@ -69,38 +68,52 @@ __device__ __forceinline__ float exp2_of(float x) {
   return y;
 }
 constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ int64_t teacher_row(const DistillArgs& a, int64_t r) {
-  if (!a.rec_bytes) return 0;
-  const int64_t rec = a.t.rows ? a.t.rows[r] : a.t.first_row + r;
-  return rec >= 0 && rec < a.t.n_records ? rec : -1;
+// ln x and 1 / x to 2 ulp
+__device__ __forceinline__ float ln_of(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y * 0.69314718055994531f;
+}
+__device__ __forceinline__ float rcp_of(float x) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// Entry e of row r: index -1 where absent.
-__device__ __forceinline__ void teacher_entry(const DistillArgs& a, int64_t r, int64_t rec, int e, float* z, int* idx) {
-  const gs_teacher& t = a.t;
-  int i;
-  float v;
-  if (a.rec_bytes) {
-    if (rec < 0) {
-      *z = -INFINITY;
-      *idx = -1;
-      return;
-    }
-    const uint8_t* p = static_cast<const uint8_t*>(t.records) + rec * a.rec_bytes;
-    const float2 head = *reinterpret_cast<const float2*>(p);
-    i = reinterpret_cast<const int16_t*>(p + 8)[e];
-    v = record_value(head.x, head.y, record_code(p + 8 + 2 * t.k, e, t.bits));
-  } else {
-    const int64_t at = r * t.k + e;
-    i = t.index[at];
-    v = t.values_dtype == GS_F32   ? static_cast<const float*>(t.values)[at]
-        : t.values_dtype == GS_F16 ? to_f32(static_cast<const __half*>(t.values)[at])
-                                   : to_f32(static_cast<const __nv_bfloat16*>(t.values)[at]);
+__device__ __forceinline__ float2 checked_entry(int idx, float z, int64_t classes) {
+  const bool here = idx >= 0 && idx < classes && z != -INFINITY;
+  return make_float2(__int_as_float(here ? idx : -1), here ? z : -INFINITY);
+}
+template <typename V>
+__device__ __forceinline__ void stage_arrays(const DistillArgs& a, float2* ents, int64_t at, int count) {
+  const V* z = static_cast<const V*>(a.t.values) + at;
+  const int32_t* idx = a.t.index + at;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < count; i += blockDim.x) ents[i] = checked_entry(__ldg(idx + i), to_f32(z[i]), a.classes);
+}
+
+// Teacher entries of `rows` rows from r0 as (index, z), index -1 where absent.
+__device__ __forceinline__ void stage_entries(const DistillArgs& a, float2* ents, int64_t r0, int rows) {
+  const int k = a.t.k;
+  if (!a.rec_bytes) {
+    if (a.t.values_dtype == GS_F32) stage_arrays<float>(a, ents, r0 * k, rows * k);
+    else if (a.t.values_dtype == GS_F16) stage_arrays<__half>(a, ents, r0 * k, rows * k);
+    else stage_arrays<__nv_bfloat16>(a, ents, r0 * k, rows * k);
+    return;
   }
-  const bool here = i >= 0 && i < a.classes && v != -INFINITY;
-  *z = here ? v : -INFINITY;
-  *idx = here ? i : -1;
+  const uint32_t per_k = 0xffffffffu / k + 1;  // i / k for i < 2^16
+  for (int i = threadIdx.x; i < rows * k; i += blockDim.x) {
+    const int r = k == 1 ? i : (int)__umulhi((uint32_t)i, per_k), e = i - r * k;
+    const int64_t rec = a.t.rows ? __ldg(a.t.rows + r0 + r) : a.t.first_row + r0 + r;
+    float2 v = make_float2(__int_as_float(-1), -INFINITY);
+    if (rec >= 0 && rec < a.t.n_records) {
+      const uint8_t* p = static_cast<const uint8_t*>(a.t.records) + rec * a.rec_bytes;
+      const float2 head = *reinterpret_cast<const float2*>(p);
+      v = checked_entry(reinterpret_cast<const int16_t*>(p + 8)[e],
+                        record_value(head.x, head.y, record_code(p + 8 + 2 * k, e, a.t.bits)), a.classes);
+    }
+    ents[i] = v;
+  }
 }
 
 // The sum of a double per thread over the block, in a fixed order.
@@ -126,48 +139,54 @@ template <int G, typename Logit>
 __device__ __forceinline__ bool teacher_terms(float2* ent, int k, int lane, float m, float inv_temp, Logit logit,
                                               float& term) {
   const float c2 = inv_temp * kLog2e;
-  float zmax = -INFINITY, any = 0.0f;
+  float zmax = -INFINITY;
+  bool mine = false;
   for (int e = lane; e < k; e += G) {
-    if (__float_as_int(ent[e].x) >= 0) any = 1.0f;
+    mine |= __float_as_int(ent[e].x) >= 0;
     zmax = fmaxf(zmax, ent[e].y);
   }
+  const unsigned present = __ballot_sync(~0u, mine) & (G == 32 ? ~0u : ((1u << (G & 31)) - 1) << (threadIdx.x & 31 & ~(G - 1)));
   zmax = group_max<G>(zmax);
   float tot = 0.0f;
   for (int e = lane; e < k; e += G)
     if (__float_as_int(ent[e].x) >= 0) tot += exp2_of((ent[e].y - zmax) * c2);
   tot = group_sum<G>(tot);
+  const float inv_tot = rcp_of(tot);
   float sum = 0.0f;
   for (int e = lane; e < k; e += G) {
     const int idx = __float_as_int(ent[e].x);
     float p = 0.0f;
     if (idx >= 0) {
       const float z = ent[e].y - zmax;
-      p = exp2_of(z * c2) / tot;
+      p = exp2_of(z * c2) * inv_tot;
       if (p != 0.0f) sum += p * ((z - (logit(idx) - m)) * inv_temp);
     }
     ent[e].y = p;
   }
-  term = group_sum<G>(sum) - logf(tot);
-  return group_max<G>(any) > 0.0f;
+  term = group_sum<G>(sum) - ln_of(tot);
+  return present != 0;
 }
 
 // Gradients of the teacher's classes, scaled: the first entry of a class holds
 // (class, f (q - sum of the class's p)), every other one (-1, -).
 template <int G, typename Logit>
-__device__ __forceinline__ void class_gradients(const float2* ent, float2* out, int k, int lane, float m, float c2,
-                                                float inv_sum, float f, Logit logit) {
+__device__ __forceinline__ void class_gradients(const float2* ent, float2* out, int k, bool repeats, int lane, float m,
+                                                float c2, float inv_sum, float f, Logit logit) {
   for (int e = lane; e < k; e += G) {
     const int idx = __float_as_int(ent[e].x);
     int to = -1;
     float g = 0.0f;
     if (idx >= 0) {
       bool first = true;
-      float p = 0.0f;
-      for (int j = 0; j < k; ++j) {
-        const float2 o = ent[j];
-        if (__float_as_int(o.x) == idx) {
-          first &= j >= e;
-          p += o.y;
+      float p = ent[e].y;
+      if (repeats) {
+        p = 0.0f;
+        for (int j = 0; j < k; ++j) {
+          const float2 o = ent[j];
+          if (__float_as_int(o.x) == idx) {
+            first &= j >= e;
+            p += o.y;
+          }
         }
       }
       if (first) {
@@ -179,7 +198,8 @@ __device__ __forceinline__ void class_gradients(const float2* ent, float2* out, 
   }
 }
 
-template <typename T, int G>
+// A lane holds EACH of its row's logits, G apart, in registers.
+template <typename T, int G, int EACH>
 __global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, int tile_rows, int bulk_in, int bulk_out) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ unsigned long long bar;
@@ -187,7 +207,8 @@ __global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, in
   T* tile = reinterpret_cast<T*>(smem);
   float2* ents = reinterpret_cast<float2*>(smem + (((size_t)tile_rows * C * sizeof(T) + 15) & ~(size_t)15));
   float2* fixes = ents + (size_t)tile_rows * k;
-  float2* row_w = fixes + (size_t)tile_rows * k;  // (weight, gradient factor)
+  float2* row_w = fixes + (size_t)tile_rows * k;             // (weight, gradient factor)
+  int* repeats = reinterpret_cast<int*>(row_w + tile_rows);  // a class appears twice among the row's entries
   constexpr int kGroups = kTileThreads / G;
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   const float c2 = a.inv_temp * kLog2e;
@@ -218,13 +239,19 @@ __global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, in
     for (int r = threadIdx.x; r < rows; r += kTileThreads) {
       const float w = a.weight ? a.weight[r0 + r] : 1.0f;
       row_w[r] = make_float2(w, w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r0 + r : 0] : 1.0f));
+      repeats[r] = 0;
     }
-    for (int i = threadIdx.x; i < rows * k; i += kTileThreads) {
-      const int r = i / k;
-      float z;
-      int idx;
-      teacher_entry(a, r0 + r, teacher_row(a, r0 + r), i - r * k, &z, &idx);
-      ents[i] = make_float2(__int_as_float(idx), z);
+    stage_entries(a, ents, r0, rows);
+    __syncthreads();
+    if (a.grad) {
+      const uint32_t per_k = 0xffffffffu / k + 1;
+      for (int i = threadIdx.x; i < rows * k; i += kTileThreads) {
+        const int r = k == 1 ? i : (int)__umulhi((uint32_t)i, per_k);
+        const int idx = __float_as_int(ents[i].x);
+        bool twice = false;
+        for (int j = r * k; j < i; ++j) twice |= __float_as_int(ents[j].x) == idx;
+        if (twice && idx >= 0) repeats[r] = 1;
+      }
     }
     bool ok = true;
     if (in) {
@@ -242,20 +269,27 @@ __global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, in
       const int r = live ? rr + group : rows - 1, kk = live ? k : 0;
       T* s = tile + (size_t)r * C;
       float2* ent = ents + (size_t)r * k;
-      float m = -INFINITY;
-#pragma unroll 4
-      for (int c = lane; c < C; c += G) m = fmaxf(m, to_f32(s[c]));
+      float v[EACH], m = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int c = lane + G * i;
+        v[i] = c < C ? to_f32(s[c]) : -INFINITY;
+        m = fmaxf(m, v[i]);
+      }
       m = group_max<G>(m);
       float sum = 0.0f;
-#pragma unroll 4
-      for (int c = lane; c < C; c += G) sum += exp2_of((to_f32(s[c]) - m) * c2);
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        v[i] = lane + G * i < C ? exp2_of((v[i] - m) * c2) : 0.0f;
+        sum += v[i];
+      }
       sum = group_sum<G>(sum);
-      const float inv = 1.0f / sum;
+      const float inv = rcp_of(sum);
       auto logit = [&](int i) { return to_f32(s[i]); };
       float term;
       const bool any = teacher_terms<G>(ent, kk, lane, m, a.inv_temp, logit, term);
       const float2 w = row_w[r];
-      const float loss = any ? (term + logf(sum)) * (a.temp * a.temp) * w.x : 0.0f;
+      const float loss = any ? (term + ln_of(sum)) * (a.temp * a.temp) * w.x : 0.0f;
       if (live && lane == 0) {
         if (a.row_loss) a.row_loss[r0 + r] = loss;
         acc += (double)loss;
@@ -263,16 +297,13 @@ __global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, in
       if (a.grad) {
         __syncwarp();
         float2* fix = fixes + (size_t)r * k;
-        class_gradients<G>(ent, fix, any ? kk : 0, lane, m, c2, inv, w.y, logit);
+        class_gradients<G>(ent, fix, any ? kk : 0, repeats[r] != 0, lane, m, c2, inv, w.y, logit);
         __syncwarp();
+        const float f = any ? inv * w.y : 0.0f;
         if (live) {
-          if (any) {
-            const float f = inv * w.y;
-#pragma unroll 4
-            for (int c = lane; c < C; c += G) s[c] = from_f32<T>(exp2_of((to_f32(s[c]) - m) * c2) * f);
-          } else {
-            for (int c = lane; c < C; c += G) s[c] = from_f32<T>(0.0f);
-          }
+#pragma unroll
+          for (int i = 0; i < EACH; ++i)
+            if (lane + G * i < C) s[lane + G * i] = from_f32<T>(any ? v[i] * f : 0.0f);
         }
         __syncwarp();
         for (int e = lane; e < (any ? kk : 0); e += G) {
@@ -315,13 +346,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
   double acc = 0.0;
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* src = static_cast<const T*>(a.logits) + r * C;
-    const int64_t rec = teacher_row(a, r);
-    for (int e = threadIdx.x; e < k; e += kRowThreads) {
-      float z;
-      int idx;
-      teacher_entry(a, r, rec, e, &z, &idx);
-      ent[e] = make_float2(__int_as_float(idx), z);
-    }
+    stage_entries(a, ent, r, 1);
     float m = -INFINITY;
 #pragma unroll 8
     for (int c = threadIdx.x; c < C; c += kRowThreads) {
@@ -349,10 +374,10 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
       float term;
       const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
       __syncwarp();
-      const float inv = 1.0f / sum;
-      if (a.grad) class_gradients<32>(ent, fix, any ? k : 0, lane, m, c2, inv, f, logit);
+      const float inv = rcp_of(sum);
+      if (a.grad) class_gradients<32>(ent, fix, any ? k : 0, true, lane, m, c2, inv, f, logit);
       if (lane == 0) {
-        const float loss = any ? (term + logf(sum)) * (a.temp * a.temp) * w : 0.0f;
+        const float loss = any ? (term + ln_of(sum)) * (a.temp * a.temp) * w : 0.0f;
         if (a.row_loss) a.row_loss[r] = loss;
         acc += (double)loss;
         stats[0] = inv;
@@ -392,42 +417,49 @@ __global__ void k_distill_finish(const double* partials, int n, double scale, fl
   if (threadIdx.x == 0) *loss = (float)(part[0] * scale);
 }
 
-template <typename T, int G>
+template <typename T, int G, int EACH>
 static int launch_tile(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
-  const size_t per_row = a.classes * sizeof(T) + 16 * (size_t)a.t.k + 8;
+  const size_t extra = 16 * (size_t)a.t.k + 12, per_row = a.classes * sizeof(T) + extra;
   // a multiple of 8 rows is a multiple of 16 bytes, and few rows still make a
   // tile for every SM
   int64_t rows = std::max<int64_t>(8, (int64_t)(kTileSmem / per_row) & ~7ll);
   rows = std::min<int64_t>(rows, std::max<int64_t>(8, ceil_div(ceil_div(a.n, 148 * 4), 8) * 8));
-  const size_t smem = ((rows * a.classes * sizeof(T) + 15) & ~(size_t)15) + rows * (16 * (size_t)a.t.k + 8);
+  const size_t smem = ((rows * a.classes * sizeof(T) + 15) & ~(size_t)15) + rows * extra;
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(k_distill_tile<T, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e =
+        cudaFuncSetAttribute(k_distill_tile<T, G, EACH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_tile: %s", cudaGetErrorString(e));
   }
   *blocks = (unsigned)std::min<int64_t>(ceil_div(a.n, rows), kDistillMaxBlocks);
-  k_distill_tile<T, G><<<*blocks, kTileThreads, smem, st>>>(a, (int)rows, aligned(a.logits, 16), aligned(a.grad, 16));
+  k_distill_tile<T, G, EACH>
+      <<<*blocks, kTileThreads, smem, st>>>(a, (int)rows, aligned(a.logits, 16), aligned(a.grad, 16));
   return check_launch("k_distill_tile");
 }
 
 template <typename T>
 static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
-  if (a.classes * sizeof(T) > kTileRowBytes) {
-    const size_t row = (a.classes * sizeof(T) + 15) & ~(size_t)15;
-    const bool staged = row <= kRowSmem;
-    if (staged && row > 32 * 1024) {
-      cudaError_t e = cudaFuncSetAttribute(k_distill_row<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)row);
-      if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_row: %s", cudaGetErrorString(e));
-    }
-    *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
-    k_distill_row<T><<<*blocks, kRowThreads, staged ? row : 0, st>>>(a, staged);
-    return check_launch("k_distill_row");
+  // Lanes of a row: enough that a lane's share fits in registers, few enough that
+  // the reductions and the teacher's entries do not outweigh it.
+  const int64_t c = a.classes;
+  if (c <= 16) return launch_tile<T, 4, 4>(a, st, blocks);
+  if (c <= 32) return launch_tile<T, 4, 8>(a, st, blocks);
+  if (c <= 64) return launch_tile<T, 8, 8>(a, st, blocks);
+  if (c <= 96) return launch_tile<T, 8, 12>(a, st, blocks);
+  if (c <= 128) return launch_tile<T, 8, 16>(a, st, blocks);
+  if (c <= 160) return launch_tile<T, 8, 20>(a, st, blocks);
+  if (c <= 256) return launch_tile<T, 16, 16>(a, st, blocks);
+  if (c <= 512) return launch_tile<T, 16, 32>(a, st, blocks);
+  if (c <= 1024) return launch_tile<T, 32, 32>(a, st, blocks);
+  if (c <= 1536) return launch_tile<T, 32, 48>(a, st, blocks);
+  const size_t row = (c * sizeof(T) + 15) & ~(size_t)15;
+  const bool staged = row <= kRowSmem;
+  if (staged && row > 32 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(k_distill_row<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)row);
+    if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_row: %s", cudaGetErrorString(e));
   }
-  // Lanes of a row: enough that a lane's share stays a few dozen classes, few
-  // enough that reductions and the teacher's entries do not outweigh it.
-  if (a.classes <= 32) return launch_tile<T, 4>(a, st, blocks);
-  if (a.classes <= 256) return launch_tile<T, 8>(a, st, blocks);
-  if (a.classes <= 1024) return launch_tile<T, 16>(a, st, blocks);
-  return launch_tile<T, 32>(a, st, blocks);
+  *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
+  k_distill_row<T><<<*blocks, kRowThreads, staged ? row : 0, st>>>(a, staged);
+  return check_launch("k_distill_row");
 }
 
 }  // namespace gs
