@@ -5,20 +5,21 @@
 //   L = w T^2 sum_k p_k (log p_k - log q_{i_k}),  dL/ds_c = w T (q_c - sum_{i_k = c} p_k)
 //
 // Bound by memory: the logits are read once and the gradient written once.
-//   k_distill_tile  up to 1536 classes: a block stages a tile of rows in shared
-//                   memory with one bulk copy, groups of 4 to 32 lanes take a row
-//                   each, the gradient replaces the logits in the tile and leaves
-//                   with one bulk copy.  Several blocks per SM overlap their
-//                   copies with each other's arithmetic.
+//   k_distill_warp  up to 1536 classes: every warp walks tiles of its own, loaded
+//                   and stored by bulk copies, with no block barrier; dozens of
+//                   warps per SM overlap their copies with each other's
+//                   arithmetic.  The classes of a row are shared by 4 to 32 lanes;
+//                   the teacher's few entries are worked on by one lane per row,
+//                   which needs no reductions (by the row's lanes, with one, they
+//                   were 60% of the instructions).
 //   k_distill_row   longer rows: one block per row, staged in shared memory while
 //                   it fits.
 #include "feature_common.cuh"
 
 namespace gs {
 
-constexpr int kDistillMaxBlocks = 148 * 8;
-constexpr int kTileThreads = 128, kRowThreads = 512;
-constexpr size_t kTileSmem = 20 * 1024;  // shared memory of a block (or 8 rows)
+constexpr int kDistillMaxBlocks = 148 * 16;
+constexpr int kWarpBlock = 128, kRowThreads = 512;
 constexpr size_t kRowSmem = 200 * 1024;
 
 __device__ unsigned long long g_distill_wait_failures;
@@ -84,25 +85,28 @@ __device__ __forceinline__ float2 checked_entry(int idx, float z, int64_t classe
   const bool here = idx >= 0 && idx < classes && z != -INFINITY;
   return make_float2(__int_as_float(here ? idx : -1), here ? z : -INFINITY);
 }
-template <typename V>
-__device__ __forceinline__ void stage_arrays(const DistillArgs& a, float2* ents, int64_t at, int count) {
+template <int STRIDE, typename V>
+__device__ __forceinline__ void stage_arrays(const DistillArgs& a, float2* ents, int64_t at, int count, int first) {
   const V* z = static_cast<const V*>(a.t.values) + at;
   const int32_t* idx = a.t.index + at;
-#pragma unroll 2
-  for (int i = threadIdx.x; i < count; i += blockDim.x) ents[i] = checked_entry(__ldg(idx + i), to_f32(z[i]), a.classes);
+#pragma unroll 4
+  for (int i = first; i < count; i += STRIDE) ents[i] = checked_entry(__ldg(idx + i), to_f32(z[i]), a.classes);
 }
 
-// Teacher entries of `rows` rows from r0 as (index, z), index -1 where absent.
-__device__ __forceinline__ void stage_entries(const DistillArgs& a, float2* ents, int64_t r0, int rows) {
+// Teacher entries of `rows` rows from r0 as (index, z), index -1 where absent,
+// by STRIDE threads of which this is number `first`.
+template <int STRIDE>
+__device__ __forceinline__ void stage_entries(const DistillArgs& a, float2* ents, int64_t r0, int rows, int first) {
   const int k = a.t.k;
   if (!a.rec_bytes) {
-    if (a.t.values_dtype == GS_F32) stage_arrays<float>(a, ents, r0 * k, rows * k);
-    else if (a.t.values_dtype == GS_F16) stage_arrays<__half>(a, ents, r0 * k, rows * k);
-    else stage_arrays<__nv_bfloat16>(a, ents, r0 * k, rows * k);
+    if (a.t.values_dtype == GS_F32) stage_arrays<STRIDE, float>(a, ents, r0 * k, rows * k, first);
+    else if (a.t.values_dtype == GS_F16) stage_arrays<STRIDE, __half>(a, ents, r0 * k, rows * k, first);
+    else stage_arrays<STRIDE, __nv_bfloat16>(a, ents, r0 * k, rows * k, first);
     return;
   }
   const uint32_t per_k = 0xffffffffu / k + 1;  // i / k for i < 2^16
-  for (int i = threadIdx.x; i < rows * k; i += blockDim.x) {
+#pragma unroll 4
+  for (int i = first; i < rows * k; i += STRIDE) {
     const int r = k == 1 ? i : (int)__umulhi((uint32_t)i, per_k), e = i - r * k;
     const int64_t rec = a.t.rows ? __ldg(a.t.rows + r0 + r) : a.t.first_row + r0 + r;
     float2 v = make_float2(__int_as_float(-1), -INFINITY);
@@ -117,16 +121,15 @@ __device__ __forceinline__ void stage_entries(const DistillArgs& a, float2* ents
 }
 
 // The sum of a double per thread over the block, in a fixed order.
-template <int THREADS>
 __device__ __forceinline__ void block_partial(double v, double* out) {
-  __shared__ double part[THREADS / 32];
+  __shared__ double part[32];
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   if (threadIdx.x == 0) {
     double t = 0.0;
-    for (int i = 0; i < THREADS / 32; ++i) t += part[i];
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) t += part[i];
     *out = t;
   }
 }
@@ -198,146 +201,291 @@ __device__ __forceinline__ void class_gradients(const float2* ent, float2* out, 
   }
 }
 
-// A lane holds EACH of its row's logits, G apart, in registers.
-template <typename T, int G, int EACH>
-__global__ void __launch_bounds__(kTileThreads) k_distill_tile(DistillArgs a, int tile_rows, int bulk_in, int bulk_out) {
+// What a warp keeps of a row besides its logits and entries.
+struct RowState {
+  float weight, factor;  // of the loss, of the gradient
+  float term;            // the teacher's part of the loss; NaN-free "none": any == 0
+  float m, inv;          // maximum and 1 / sum of the student's exponentials
+  int any, repeats;      // entries present; a class twice among them
+  float lse;
+};
+
+// The teacher's softmax of one row by one lane: entries (index, z) -> (index, p).
+// Up to MAX entries, in registers (MAX = 0: any number, through memory).
+template <int MAX>
+__device__ __forceinline__ void teacher_row(float2* ent, int k, float inv_temp, RowState& st) {
+  const float c2 = inv_temp * kLog2e;
+  float zmax = -INFINITY, tot = 0.0f, sum = 0.0f;
+  bool any = false, twice = false;
+  if constexpr (MAX > 0) {
+    int idx[MAX];
+    float z[MAX];
+#pragma unroll
+    for (int e = 0; e < MAX; ++e) {
+      const float2 v = e < k ? ent[e] : make_float2(__int_as_float(-1), -INFINITY);
+      idx[e] = __float_as_int(v.x);
+      z[e] = v.y;
+      zmax = fmaxf(zmax, v.y);
+      any |= idx[e] >= 0;
+#pragma unroll
+      for (int j = 0; j < e; ++j) twice |= idx[e] == idx[j] && idx[e] >= 0;
+    }
+#pragma unroll
+    for (int e = 0; e < MAX; ++e) {
+      const float d = z[e] - zmax;
+      z[e] = idx[e] >= 0 ? exp2_of(d * c2) : 0.0f;
+      if (z[e] != 0.0f) sum += z[e] * (d * inv_temp);
+      tot += z[e];
+    }
+    const float inv = rcp_of(tot);
+#pragma unroll
+    for (int e = 0; e < MAX; ++e)
+      if (e < k) ent[e].y = z[e] * inv;
+    sum *= inv;
+  } else {
+    for (int e = 0; e < k; ++e) {
+      const float2 v = ent[e];
+      const int idx = __float_as_int(v.x);
+      zmax = fmaxf(zmax, v.y);
+      any |= idx >= 0;
+      if (idx >= 0)
+        for (int j = 0; j < e; ++j) twice |= __float_as_int(ent[j].x) == idx;
+    }
+    for (int e = 0; e < k; ++e) {
+      const float2 v = ent[e];
+      float x = 0.0f;
+      if (__float_as_int(v.x) >= 0) {
+        const float d = v.y - zmax;
+        x = exp2_of(d * c2);
+        if (x != 0.0f) sum += x * (d * inv_temp);
+      }
+      tot += x;
+      ent[e].y = x;
+    }
+    const float inv = rcp_of(tot);
+    for (int e = 0; e < k; ++e) ent[e].y *= inv;
+    sum *= inv;
+  }
+  st.any = any;
+  st.repeats = twice;
+  st.term = sum - ln_of(tot);  // sum_k p_k log p_k
+}
+
+// sum_k p_k (s_k - m) / T of a row by one lane, and the gradients of the teacher's
+// classes (unless fix is NULL): the first entry of a class holds (class, factor *
+// (q - sum of the class's p)), every other one (-1, -).
+template <int MAX, typename T>
+__device__ __forceinline__ float class_row(const T* s, const float2* ent, float2* fix, int k, float inv_temp,
+                                           const RowState& st) {
+  const float c2 = inv_temp * kLog2e;
+  float cross = 0.0f;
+#pragma unroll MAX > 0 ? MAX : 1
+  for (int e = 0; e < (MAX > 0 ? MAX : k); ++e) {
+    if (MAX > 0 && e >= k) break;
+    const float2 v = ent[e];
+    const int idx = __float_as_int(v.x);
+    int to = -1;
+    float g = 0.0f;
+    if (idx >= 0) {
+      const float d = to_f32(s[idx]) - st.m;
+      if (v.y != 0.0f) cross += v.y * (d * inv_temp);
+      if (fix) {
+        bool first = true;
+        float p = v.y;
+        if (st.repeats) {
+          p = 0.0f;
+#pragma unroll 1
+          for (int j = 0; j < k; ++j) {
+            const float2 o = ent[j];
+            if (__float_as_int(o.x) == idx) {
+              first &= j >= e;
+              p += o.y;
+            }
+          }
+        }
+        if (first) {
+          to = idx;
+          g = (exp2_of(d * c2) * st.inv - p) * st.factor;
+        }
+      }
+    }
+    if (fix) fix[e] = make_float2(__int_as_float(to), g);
+  }
+  return cross;
+}
+
+// Shared memory of a warp: two tiles, then entries, fixes, row states.
+constexpr int kWarpBuffers = 2;
+__host__ __device__ inline size_t warp_tile_bytes(int rows, int64_t classes, int elem) {
+  return ((size_t)rows * classes * elem + 127) & ~(size_t)127;
+}
+__host__ __device__ inline size_t warp_smem(int rows, int64_t classes, int elem, int k) {
+  return kWarpBuffers * warp_tile_bytes(rows, classes, elem) + (((size_t)rows * (16 * k + sizeof(RowState)) + 127) & ~(size_t)127);
+}
+
+// G lanes share a row, each holding EACH of its logits, G apart, in registers; the
+// first FULL of them exist for sure.  With KEEP the exponentials of all rows of the
+// tile (KEEP rounds of 32 / G rows) stay in registers for the gradient; otherwise
+// they are computed again.
+template <typename T, int G, int EACH, int FULL, int KEEP>
+__global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int tile_rows, int bulk_in, int bulk_out) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ unsigned long long bar;
-  const int C = (int)a.classes, k = a.t.k;
-  T* tile = reinterpret_cast<T*>(smem);
-  float2* ents = reinterpret_cast<float2*>(smem + (((size_t)tile_rows * C * sizeof(T) + 15) & ~(size_t)15));
-  float2* fixes = ents + (size_t)tile_rows * k;
-  float2* row_w = fixes + (size_t)tile_rows * k;             // (weight, gradient factor)
-  int* repeats = reinterpret_cast<int*>(row_w + tile_rows);  // a class appears twice among the row's entries
-  constexpr int kGroups = kTileThreads / G;
-  const int group = threadIdx.x / G, lane = threadIdx.x % G;
+  __shared__ unsigned long long bars[kWarpBlock / 32][kWarpBuffers];
+  const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, wl = threadIdx.x & 31;
+  const int group = wl / G, lane = wl % G;
   const float c2 = a.inv_temp * kLog2e;
-  if (threadIdx.x == 0) mbar_init(&bar, 1);
-  __syncthreads();
-  unsigned phase = 0;
+  uint8_t* own = smem + warp * warp_smem(tile_rows, C, sizeof(T), k);
+  const size_t tile_bytes = warp_tile_bytes(tile_rows, C, sizeof(T));
+  float2* ents = reinterpret_cast<float2*>(own + kWarpBuffers * tile_bytes);
+  float2* fixes = ents + tile_rows * k;
+  RowState* state = reinterpret_cast<RowState*>(fixes + tile_rows * k);
+  if (wl == 0)
+    for (int i = 0; i < kWarpBuffers; ++i) mbar_init(&bars[warp][i], 1);
+  __syncwarp();
+  const int64_t tiles = (a.n + tile_rows - 1) / tile_rows, step = (int64_t)gridDim.x * (blockDim.x >> 5);
+  const T* logits = static_cast<const T*>(a.logits);
+  const uint32_t whole_bytes = (uint32_t)(tile_rows * C * sizeof(T));
+  auto fetch = [&](int64_t t, int buf) {  // whole tiles only
+    if (wl == 0 && bulk_in && (t + 1) * tile_rows <= a.n) {
+      mbar_arrive_expect_tx(&bars[warp][buf], whole_bytes);
+      bulk_g2s(own + buf * tile_bytes, logits + t * tile_rows * C, whole_bytes, &bars[warp][buf]);
+    }
+  };
   double acc = 0.0;
-  const int64_t tiles = (a.n + tile_rows - 1) / tile_rows;
-  for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
+  int buf = 0;
+  unsigned phase = 0;
+  int64_t t = blockIdx.x + (int64_t)gridDim.x * warp;
+  if (t < tiles) fetch(t, 0);
+  for (; t < tiles; t += step) {
     const int64_t r0 = t * tile_rows;
     const int rows = (int)min((int64_t)tile_rows, a.n - r0);
-    const T* src = static_cast<const T*>(a.logits) + r0 * C;
-    const bool in = bulk_in && rows == tile_rows;
-    const uint32_t bytes = (uint32_t)(rows * C * sizeof(T));
-    if (threadIdx.x == 0) {
-      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile has left
-      if (in) {
-        mbar_arrive_expect_tx(&bar, bytes);
-        bulk_g2s(tile, src, bytes, &bar);
-      }
+    const bool whole = rows == tile_rows;
+    T* tile = reinterpret_cast<T*>(own + buf * tile_bytes);
+    stage_entries<32>(a, ents, r0, rows, wl);
+    __syncwarp();
+    for (int r = wl; r < rows; r += 32) {
+      RowState st;
+      st.weight = a.weight ? a.weight[r0 + r] : 1.0f;
+      st.factor = st.weight * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r0 + r : 0] : 1.0f);
+      if (k <= 8) teacher_row<8>(ents + r * k, k, a.inv_temp, st);
+      else teacher_row<0>(ents + r * k, k, a.inv_temp, st);
+      state[r] = st;
     }
-    if (!in) {
-      __syncthreads();
+    if (wl == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile has left
+    __syncwarp();
+    if (t + step < tiles) fetch(t + step, buf ^ 1);
+    if (bulk_in && whole) {
+      if (!__all_sync(~0u, mbar_wait(&bars[warp][buf], phase))) {
+        if (wl == 0) atomicAdd(&g_distill_wait_failures, 1ull);
+        break;
+      }
+    } else {
 #pragma unroll 4
-      for (int i = threadIdx.x; i < rows * C; i += kTileThreads) tile[i] = src[i];
+      for (int i = wl; i < rows * C; i += 32) tile[i] = logits[r0 * C + i];
     }
-    // meanwhile the teacher's entries and the weights
-    for (int r = threadIdx.x; r < rows; r += kTileThreads) {
-      const float w = a.weight ? a.weight[r0 + r] : 1.0f;
-      row_w[r] = make_float2(w, w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r0 + r : 0] : 1.0f));
-      repeats[r] = 0;
-    }
-    stage_entries(a, ents, r0, rows);
-    __syncthreads();
-    if (a.grad) {
-      const uint32_t per_k = 0xffffffffu / k + 1;
-      for (int i = threadIdx.x; i < rows * k; i += kTileThreads) {
-        const int r = k == 1 ? i : (int)__umulhi((uint32_t)i, per_k);
-        const int idx = __float_as_int(ents[i].x);
-        bool twice = false;
-        for (int j = r * k; j < i; ++j) twice |= __float_as_int(ents[j].x) == idx;
-        if (twice && idx >= 0) repeats[r] = 1;
-      }
-    }
-    bool ok = true;
-    if (in) {
-      ok = mbar_wait(&bar, phase);
-      phase ^= 1;
-    }
-    if (!__syncthreads_and(ok)) {
-      if (threadIdx.x == 0) atomicAdd(&g_distill_wait_failures, 1ull);
-      break;
-    }
-    for (int rr = 0; rr < rows; rr += kGroups) {
-      // Idle groups of the last round read a row like the others (the shuffles
-      // are the warp's) and write nothing.
+    __syncwarp();
+    // the student's maximum and sum, by the rows' lanes
+    constexpr int kRounds = KEEP > 0 ? KEEP : 1;
+    float kept[kRounds][EACH];
+    auto exponentials = [&](int rr, float(&v)[EACH]) {
       const bool live = rr + group < rows;
-      const int r = live ? rr + group : rows - 1, kk = live ? k : 0;
-      T* s = tile + (size_t)r * C;
-      float2* ent = ents + (size_t)r * k;
-      float v[EACH], m = -INFINITY;
+      const int r = live ? rr + group : rows - 1;
+      const T* s = tile + r * C + lane;
+      float m = -INFINITY, sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
-        const int c = lane + G * i;
-        v[i] = c < C ? to_f32(s[c]) : -INFINITY;
+        v[i] = i < FULL || lane + G * i < C ? to_f32(s[G * i]) : -INFINITY;
         m = fmaxf(m, v[i]);
       }
       m = group_max<G>(m);
-      float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
-        v[i] = lane + G * i < C ? exp2_of((v[i] - m) * c2) : 0.0f;
+        v[i] = i < FULL || lane + G * i < C ? exp2_of((v[i] - m) * c2) : 0.0f;
         sum += v[i];
       }
       sum = group_sum<G>(sum);
-      const float inv = rcp_of(sum);
-      auto logit = [&](int i) { return to_f32(s[i]); };
-      float term;
-      const bool any = teacher_terms<G>(ent, kk, lane, m, a.inv_temp, logit, term);
-      const float2 w = row_w[r];
-      const float loss = any ? (term + ln_of(sum)) * (a.temp * a.temp) * w.x : 0.0f;
-      if (live && lane == 0) {
-        if (a.row_loss) a.row_loss[r0 + r] = loss;
-        acc += (double)loss;
+      if (lane == 0 && live) {
+        state[r].m = m;
+        state[r].inv = rcp_of(sum);
+        state[r].lse = ln_of(sum);
       }
-      if (a.grad) {
-        __syncwarp();
-        float2* fix = fixes + (size_t)r * k;
-        class_gradients<G>(ent, fix, any ? kk : 0, repeats[r] != 0, lane, m, c2, inv, w.y, logit);
-        __syncwarp();
-        const float f = any ? inv * w.y : 0.0f;
-        if (live) {
+    };
+    if constexpr (KEEP > 0) {
 #pragma unroll
-          for (int i = 0; i < EACH; ++i)
-            if (lane + G * i < C) s[lane + G * i] = from_f32<T>(any ? v[i] * f : 0.0f);
-        }
-        __syncwarp();
-        for (int e = lane; e < (any ? kk : 0); e += G) {
-          const float2 g = fix[e];
-          if (__float_as_int(g.x) >= 0) s[__float_as_int(g.x)] = from_f32<T>(g.y);
-        }
-      }
+      for (int q = 0; q < KEEP; ++q) exponentials(q * (32 / G), kept[q]);
+    } else {
+      for (int rr = 0; rr < rows; rr += 32 / G) exponentials(rr, kept[0]);
+    }
+    __syncwarp();
+    // the loss and the gradients of the teacher's classes, by one lane per row
+    for (int r = wl; r < rows; r += 32) {
+      const RowState st = state[r];
+      float2* fix = a.grad ? fixes + r * k : nullptr;
+      const float cross = k <= 8 ? class_row<8>(tile + r * C, ents + r * k, fix, k, a.inv_temp, st)
+                                 : class_row<0>(tile + r * C, ents + r * k, fix, k, a.inv_temp, st);
+      const float loss = st.any ? (st.term - cross + st.lse) * (a.temp * a.temp) * st.weight : 0.0f;
+      if (a.row_loss) a.row_loss[r0 + r] = loss;
+      acc += (double)loss;
     }
     if (a.grad) {
-      T* dst = static_cast<T*>(a.grad) + r0 * C;
-      const bool out = bulk_out && rows == tile_rows;
-      if (out) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncthreads();
-      if (!out) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < rows * C; i += kTileThreads) dst[i] = tile[i];
-        __syncthreads();
-      } else if (threadIdx.x == 0) {
-        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(tile)),
-                     "r"(bytes)
-                     : "memory");
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      __syncwarp();
+      auto gradients = [&](int rr, const float(&v)[EACH]) {
+        const int r = rr + group;
+        if (r >= rows) return;
+        const RowState st = state[r];
+        T* s = tile + r * C + lane;
+        const float f = st.inv * st.factor;
+        if (st.any) {
+#pragma unroll
+          for (int i = 0; i < EACH; ++i)
+            if (i < FULL || lane + G * i < C)
+              s[G * i] = from_f32<T>((KEEP > 0 ? v[i] : exp2_of((to_f32(s[G * i]) - st.m) * c2)) * f);
+        } else {
+#pragma unroll
+          for (int i = 0; i < EACH; ++i)
+            if (i < FULL || lane + G * i < C) s[G * i] = from_f32<T>(0.0f);
+        }
+      };
+      if constexpr (KEEP > 0) {
+#pragma unroll
+        for (int q = 0; q < KEEP; ++q) gradients(q * (32 / G), kept[q]);
+      } else {
+        for (int rr = 0; rr < rows; rr += 32 / G) gradients(rr, kept[0]);
       }
-    } else {
-      __syncthreads();
+      __syncwarp();
+      const uint32_t per_k = 0xffffffffu / k + 1;
+      for (int i = wl; i < rows * k; i += 32) {
+        const float2 g = fixes[i];
+        const int r = k == 1 ? i : (int)__umulhi((uint32_t)i, per_k);
+        if (__float_as_int(g.x) >= 0) tile[r * C + __float_as_int(g.x)] = from_f32<T>(g.y);
+      }
+      T* dst = static_cast<T*>(a.grad) + r0 * C;
+      if (bulk_out && whole) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (wl == 0) {
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(tile)),
+                       "r"(whole_bytes)
+                       : "memory");
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+      } else {
+        __syncwarp();
+#pragma unroll 4
+        for (int i = wl; i < rows * C; i += 32) dst[i] = tile[i];
+      }
     }
+    __syncwarp();
+    buf ^= 1;
+    if (buf == 0) phase ^= 1;
   }
-  if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  if (a.partials) block_partial<kTileThreads>(acc, a.partials + blockIdx.x);
+  if (wl == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (a.partials) block_partial(acc, a.partials + blockIdx.x);
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int staged) {
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float red[kRowThreads / 32], stats[3];
   __shared__ float2 ent[GS_TEACHER_MAX_K], fix[GS_TEACHER_MAX_K];
   const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -346,7 +494,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
   double acc = 0.0;
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* src = static_cast<const T*>(a.logits) + r * C;
-    stage_entries(a, ent, r, 1);
+    stage_entries<kRowThreads>(a, ent, r, 1, threadIdx.x);
     float m = -INFINITY;
 #pragma unroll 8
     for (int c = threadIdx.x; c < C; c += kRowThreads) {
@@ -402,7 +550,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
     }
     __syncthreads();
   }
-  if (a.partials) block_partial<kRowThreads>(acc, a.partials + blockIdx.x);
+  if (a.partials) block_partial(acc, a.partials + blockIdx.x);
 }
 
 __global__ void k_distill_finish(const double* partials, int n, double scale, float* loss) {
@@ -417,40 +565,39 @@ __global__ void k_distill_finish(const double* partials, int n, double scale, fl
   if (threadIdx.x == 0) *loss = (float)(part[0] * scale);
 }
 
-template <typename T, int G, int EACH>
-static int launch_tile(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
-  const size_t extra = 16 * (size_t)a.t.k + 12, per_row = a.classes * sizeof(T) + extra;
-  // a multiple of 8 rows is a multiple of 16 bytes, and few rows still make a
-  // tile for every SM
-  int64_t rows = std::max<int64_t>(8, (int64_t)(kTileSmem / per_row) & ~7ll);
-  rows = std::min<int64_t>(rows, std::max<int64_t>(8, ceil_div(ceil_div(a.n, 148 * 4), 8) * 8));
-  const size_t smem = ((rows * a.classes * sizeof(T) + 15) & ~(size_t)15) + rows * extra;
-  if (smem > 48 * 1024) {
-    cudaError_t e =
-        cudaFuncSetAttribute(k_distill_tile<T, G, EACH>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_tile: %s", cudaGetErrorString(e));
-  }
-  *blocks = (unsigned)std::min<int64_t>(ceil_div(a.n, rows), kDistillMaxBlocks);
-  k_distill_tile<T, G, EACH>
-      <<<*blocks, kTileThreads, smem, st>>>(a, (int)rows, aligned(a.logits, 16), aligned(a.grad, 16));
-  return check_launch("k_distill_tile");
+// The warps' tiles: a multiple of 8 rows, which is one of 16 bytes.
+template <typename T, int G, int EACH, int FULL, int KEEP>
+static int launch_warps(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
+  int64_t rows = 8;
+  if (KEEP > 0) rows = KEEP * (32 / G);
+  const size_t own = warp_smem((int)rows, a.classes, sizeof(T), a.t.k);
+  int warps = kWarpBlock / 32;
+  while (warps > 1 && own * warps > 100 * 1024) warps /= 2;
+  const size_t smem = own * warps;
+  auto* kernel = k_distill_warp<T, G, EACH, FULL, KEEP>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_warp: %s", cudaGetErrorString(e));
+  const int64_t resident = 148 * std::max<int64_t>(1, std::min<int64_t>(16, (227 * 1024) / (int64_t)(smem + 1024)));
+  *blocks = (unsigned)std::min<int64_t>(ceil_div(ceil_div(a.n, rows), warps), resident);
+  kernel<<<*blocks, warps * 32, smem, st>>>(a, (int)rows, aligned(a.logits, 16), aligned(a.grad, 16));
+  return check_launch("k_distill_warp");
 }
 
 template <typename T>
 static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
   // Lanes of a row: enough that a lane's share fits in registers, few enough that
-  // the reductions and the teacher's entries do not outweigh it.
+  // the reductions do not outweigh it.
   const int64_t c = a.classes;
-  if (c <= 16) return launch_tile<T, 4, 4>(a, st, blocks);
-  if (c <= 32) return launch_tile<T, 4, 8>(a, st, blocks);
-  if (c <= 64) return launch_tile<T, 8, 8>(a, st, blocks);
-  if (c <= 96) return launch_tile<T, 8, 12>(a, st, blocks);
-  if (c <= 128) return launch_tile<T, 8, 16>(a, st, blocks);
-  if (c <= 160) return launch_tile<T, 8, 20>(a, st, blocks);
-  if (c <= 256) return launch_tile<T, 16, 16>(a, st, blocks);
-  if (c <= 512) return launch_tile<T, 16, 32>(a, st, blocks);
-  if (c <= 1024) return launch_tile<T, 32, 32>(a, st, blocks);
-  if (c <= 1536) return launch_tile<T, 32, 48>(a, st, blocks);
+  if (c <= 16) return launch_warps<T, 4, 4, 0, 6>(a, st, blocks);
+  if (c <= 32) return launch_warps<T, 4, 8, 4, 4>(a, st, blocks);
+  if (c <= 64) return launch_warps<T, 8, 8, 4, 4>(a, st, blocks);
+  if (c <= 96) return launch_warps<T, 8, 12, 8, 2>(a, st, blocks);
+  if (c <= 128) return launch_warps<T, 8, 16, 12, 2>(a, st, blocks);
+  if (c <= 160) return launch_warps<T, 8, 20, 16, 2>(a, st, blocks);
+  if (c <= 256) return launch_warps<T, 16, 16, 10, 4>(a, st, blocks);
+  if (c <= 512) return launch_warps<T, 16, 32, 16, 0>(a, st, blocks);
+  if (c <= 1024) return launch_warps<T, 32, 32, 16, 0>(a, st, blocks);
+  if (c <= 1536 && a.t.k <= 64) return launch_warps<T, 32, 48, 32, 0>(a, st, blocks);
   const size_t row = (c * sizeof(T) + 15) & ~(size_t)15;
   const bool staged = row <= kRowSmem;
   if (staged && row > 32 * 1024) {
