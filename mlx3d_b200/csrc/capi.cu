@@ -44,14 +44,15 @@ int gs_set_wait_limit(int polls) {
 int gs_wait_failures(uint64_t* count, int reset) {
   gs::clear_error();
   if (!count) return gs::set_error(GS_ERR_INVALID_ARG, "count is NULL");
-  unsigned long long a = 0, b = 0, c = 0, d = 0;
+  unsigned long long a = 0, b = 0, c = 0, d = 0, t = 0;
   int e = gs::binning_wait_failures(&a, reset);
   if (e == 0) e = gs::preprocess_wait_failures(&b, reset);
   if (e == 0) e = gs::decode_wait_failures(&c, reset);
   if (e == 0) e = gs::distill_wait_failures(&d, reset);
+  if (e == 0) e = gs::teacher_wait_failures(&t, reset);
   if (e != 0)
     return gs::set_error(GS_ERR_CUDA, "gs_wait_failures: %s", cudaGetErrorString((cudaError_t)e));
-  *count = a + b + c + d;
+  *count = a + b + c + d + t;
   return GS_OK;
 }
 

@@ -40,6 +40,7 @@ int binning_set_wait_limit(int polls);
 int preprocess_wait_failures(unsigned long long* out, int reset);
 int decode_wait_failures(unsigned long long* out, int reset);
 int distill_wait_failures(unsigned long long* out, int reset);
+int teacher_wait_failures(unsigned long long* out, int reset);
 
 // ------------------------------------------------ bulk (TMA) copies
 // One-shot shared-memory mbarrier tracking bulk global->shared copies

@@ -1,21 +1,107 @@
 // Teacher cache: a row's k largest logits, kept in 8 or 4 bits.
 //
-// Writing: one warp per row.  The order is (value descending, index
-// ascending); entry j + 1 is the best one that comes after entry j in that
-// order, found by a scan of the row (from cache after the first) and a warp
-// reduction.
-// Reading: one thread per entry.
+// Writing is a selection; the order is (value descending, index ascending), held
+// in one sortable key per class.
+//   k_teacher_write_rows  few entries, short rows: one thread per row keeps its K
+//                         best keys sorted in registers and takes K classes at a
+//                         time (sorting network, then a bitonic merge), which
+//                         needs no exchange between lanes.  A block stages its
+//                         rows in shared memory with one bulk copy.
+//   k_teacher_write_warp  anything else: one warp per row.  A first pass finds
+//                         each lane's largest value; the K-th largest of these is
+//                         a bound that at least K classes reach and few others do.
+//                         A second pass collects those, 32 at a time, sorts them
+//                         across the warp and merges them into the best 32.
+// Reading is a gather of whole records, a group of lanes per record.
 #include "feature_common.cuh"
 
 namespace gs {
 
 constexpr int kWriteWarps = 8;
+constexpr int kStagedRows = 128;                // rows (threads) of a staging block
+constexpr size_t kStagedSmem = 48 * 1024;       // its shared memory at most
+
+__device__ unsigned long long g_teacher_wait_failures;
+
+int teacher_wait_failures(unsigned long long* out, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_teacher_wait_failures, sizeof(*out));
+  if (e == cudaSuccess && reset) {
+    const unsigned long long z = 0;
+    e = cudaMemcpyToSymbol(g_teacher_wait_failures, &z, sizeof(z));
+  }
+  return (int)e;
+}
 
 struct TeacherWriteArgs {
   const void* logits;
   int64_t n, classes;
   uint8_t* records;  // of first_row
   int k, bits, rec_bytes;
+};
+
+// Sortable keys: a larger key comes first.  16-bit types: the value's bits made
+// monotonic in the upper half, the inverted class below, one 32-bit word.  float:
+// the same with 32 bits each.  0 is no class.
+template <typename T>
+struct Key {
+  using Word = uint32_t;
+  static constexpr uint32_t kLow = sizeof(T) == 2 && __is_same(T, __half) ? 0x0400u : 0x0080u;   // lowest finite
+  static constexpr uint32_t kHigh = sizeof(T) == 2 && __is_same(T, __half) ? 0xfc00u : 0xff80u;  // +inf
+  static __device__ __forceinline__ Word make(T v, int c) {
+    uint32_t b = *reinterpret_cast<const uint16_t*>(&v);
+    if (b == 0x8000u) b = 0;  // -0 equals 0
+    b ^= b & 0x8000u ? 0xffffu : 0x8000u;
+    return b > kLow && b < kHigh ? (b << 16) | (0xffffu - (uint32_t)c) : 0u;
+  }
+  // Keys of neighbouring classes c and c + 1 from one word, without the test for
+  // infinities, NaN and the lowest value: in the order, -inf and the lowest value
+  // come last anyway (absent() tells them in the result), +inf and NaN first
+  // (spoilt() tells that they are there).
+  static __device__ __forceinline__ void quick(uint32_t w, uint32_t inverted, Word& k0, Word& k1) {
+    T z[2];
+    z[0] = z[1] = from_f32<T>(0.0f);
+    if constexpr (__is_same(T, __half)) {
+      const __half2 v = __hadd2(*reinterpret_cast<const __half2*>(&w), *reinterpret_cast<const __half2*>(z));
+      w = *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+      const __nv_bfloat162 v =
+          __hadd2(*reinterpret_cast<const __nv_bfloat162*>(&w), *reinterpret_cast<const __nv_bfloat162*>(z));
+      w = *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const uint32_t sign = (w >> 15) & 0x00010001u;
+    w ^= sign * 0x7fffu | 0x80008000u;
+    k0 = (w << 16) | inverted;
+    k1 = (w & 0xffff0000u) | (inverted - 1);
+  }
+  static __device__ __forceinline__ bool absent(Word w) { return w >> 16 <= kLow; }
+  static __device__ __forceinline__ bool spoilt(Word w) { return w >> 16 >= kHigh; }
+  static __device__ __forceinline__ float value(Word w) {
+    uint32_t b = w >> 16;
+    b ^= b & 0x8000u ? 0x8000u : 0xffffu;
+    const unsigned short h = (unsigned short)b;
+    return to_f32(*reinterpret_cast<const T*>(&h));
+  }
+  static __device__ __forceinline__ int index(Word w) { return (int)(0xffffu - (w & 0xffffu)); }
+  static __device__ __forceinline__ Word shuffle(Word w, int from) { return __shfl_sync(~0u, w, from); }
+  static __device__ __forceinline__ Word exchange(Word w, int mask) { return __shfl_xor_sync(~0u, w, mask); }
+};
+template <>
+struct Key<float> {
+  using Word = unsigned long long;
+  static __device__ __forceinline__ Word make(float v, int c) {
+    uint32_t b = __float_as_uint(v + 0.0f);  // -0 equals 0
+    if (!(v > -FLT_MAX && v < INFINITY)) return 0ull;
+    b ^= b & 0x80000000u ? 0xffffffffu : 0x80000000u;
+    return ((Word)b << 32) | (0xffffffffu - (uint32_t)c);
+  }
+  static __device__ __forceinline__ float value(Word w) {
+    uint32_t b = (uint32_t)(w >> 32);
+    b ^= b & 0x80000000u ? 0x80000000u : 0xffffffffu;
+    return __uint_as_float(b);
+  }
+  static __device__ __forceinline__ int index(Word w) { return (int)(0xffffffffu - (uint32_t)w); }
+  static __device__ __forceinline__ Word shuffle(Word w, int from) { return __shfl_sync(~0u, w, from); }
+  static __device__ __forceinline__ Word exchange(Word w, int mask) { return __shfl_xor_sync(~0u, w, mask); }
 };
 
 // code = (2^bits - 1) (first - v) / (first - last) to nearest, ties to even.
@@ -29,93 +115,376 @@ __device__ __forceinline__ int quantise(float first, float last, float v, float 
   return (int)rint(((double)first - (double)v) * (double)levels / ((double)first - (double)last));
 }
 
+template <typename W>
+__device__ __forceinline__ void order(W& hi, W& lo) {  // hi >= lo afterwards
+  const W a = hi, b = lo;
+  hi = a > b ? a : b;
+  lo = a > b ? b : a;
+}
+// Descending sort of N registers (Batcher's odd-even merge sort).
+template <int N, typename W>
+__device__ __forceinline__ void sort_desc(W (&v)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(v[i + j], v[i + j + k]);
+}
+// The N largest of two descending runs, descending, in `best`.
+template <int N, typename W>
+__device__ __forceinline__ void merge_desc(W (&best)[N], const W (&other)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) best[i] = best[i] > other[N - 1 - i] ? best[i] : other[N - 1 - i];
+#pragma unroll
+  for (int k = N / 2; k >= 1; k /= 2)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & k) == 0) order(best[i], best[i + k]);
+}
+
+// One thread per row, MAX >= k a power of two; the block's rows are contiguous in
+// memory and in shared memory.
+template <typename T, int MAX>
+__global__ void __launch_bounds__(kStagedRows) k_teacher_write_rows(TeacherWriteArgs a, int block_rows, int bulk) {
+  using K = Key<T>;
+  using W = typename K::Word;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ unsigned long long bar;
+  const int C = (int)a.classes, l = threadIdx.x;
+  const int64_t r0 = (int64_t)blockIdx.x * block_rows;
+  const int rows = (int)min((int64_t)block_rows, a.n - r0);
+  T* tile = reinterpret_cast<T*>(smem);
+  const T* src = static_cast<const T*>(a.logits) + r0 * C;
+  const bool whole = bulk && rows == block_rows;
+  if (l == 0) {
+    mbar_init(&bar, 1);
+    if (whole) {
+      const uint32_t bytes = (uint32_t)(rows * C * sizeof(T));
+      mbar_arrive_expect_tx(&bar, bytes);
+      bulk_g2s(tile, src, bytes, &bar);
+    }
+  }
+  if (!whole)
+#pragma unroll 4
+    for (int i = l; i < rows * C; i += blockDim.x) tile[i] = src[i];
+  __syncthreads();
+  if (whole && !mbar_wait(&bar, 0)) {
+    if (l == 0) atomicAdd(&g_teacher_wait_failures, 1ull);
+    return;
+  }
+  // Rows an even number of words apart: lane l starts at word l, so that the lanes
+  // read different banks.
+  const T* row = tile + (l < rows ? l : 0) * C;
+  constexpr int kWord = 4 / sizeof(T);
+  const bool skew = C % (2 * kWord) == 0;
+  W best[MAX];
+  auto scan = [&]() {  // any row, every test
+#pragma unroll
+    for (int i = 0; i < MAX; ++i) best[i] = 0;
+    const int turn = skew ? (l * kWord) % C : 0;
+    for (int c0 = 0; c0 < C; c0 += MAX) {
+      W next[MAX];
+#pragma unroll
+      for (int i = 0; i < MAX; ++i) {
+        int c = c0 + i + turn;
+        if (c >= C) c -= C;
+        next[i] = c0 + i < C ? K::make(row[c], c) : 0;
+      }
+      sort_desc(next);
+      merge_desc(best, next);
+    }
+  };
+  if constexpr (sizeof(T) == 2) {
+    // Rows of whole words, two classes a word, few instructions a class.
+    if (C % 2 == 0 && !skew) {
+#pragma unroll
+      for (int i = 0; i < MAX; ++i) best[i] = 0;
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(row);
+      for (int c0 = 0; c0 < C; c0 += MAX) {
+        W next[MAX];
+        const uint32_t inverted = 0xffffu - (uint32_t)c0;
+#pragma unroll
+        for (int i = 0; i < MAX; i += 2) {
+          next[i] = next[i + 1] = 0;
+          if (c0 + i < C) K::quick(words[(c0 + i) >> 1], inverted - i, next[i], next[i + 1]);
+        }
+        sort_desc(next);
+        merge_desc(best, next);
+      }
+      bool again = K::spoilt(best[0]);
+#pragma unroll
+      for (int i = 0; i < MAX; ++i)
+        if (K::absent(best[i])) best[i] = 0;
+      if (again) scan();
+    } else {
+      scan();
+    }
+  } else {
+    scan();
+  }
+  __syncthreads();  // the tile is not needed any more: records are put together in its place
+  const float first = best[0] ? K::value(best[0]) : 0.0f, levels = (float)((1 << a.bits) - 1);
+  float last = first;
+#pragma unroll
+  for (int i = 0; i < MAX; ++i)
+    if (i < a.k && best[i]) last = K::value(best[i]);
+  // records an odd number of words apart
+  const int pitch = a.rec_bytes + 4;
+  if (l < rows) {
+    uint8_t* rec = smem + l * pitch;
+    *reinterpret_cast<float*>(rec) = first;
+    *reinterpret_cast<float*>(rec + 4) = (float)(((double)first - (double)last) / (double)levels);
+    uint8_t* codes = rec + 8 + 2 * a.k;
+    int low = 0;
+#pragma unroll
+    for (int i = 0; i < MAX; ++i) {
+      if (i >= a.k) break;
+      const int code = best[i] && first > last ? quantise(first, last, K::value(best[i]), levels) : 0;
+      reinterpret_cast<int16_t*>(rec + 8)[i] = best[i] ? (int16_t)K::index(best[i]) : (int16_t)-1;
+      if (a.bits == 8) codes[i] = (uint8_t)code;
+      else if (i & 1) codes[i >> 1] = (uint8_t)(low | code << 4);
+      else if (i + 1 == a.k) codes[i >> 1] = (uint8_t)code;
+      low = code;
+    }
+    for (int b = 8 + 2 * a.k + (a.k * a.bits + 7) / 8; b < a.rec_bytes; ++b) rec[b] = 0;
+  }
+  __syncthreads();
+  const int words = a.rec_bytes / 4;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.records + r0 * a.rec_bytes);
+  for (int i = l; i < rows * words; i += blockDim.x) {
+    const int r = i / words;
+    dst[i] = *reinterpret_cast<const uint32_t*>(smem + r * pitch + 4 * (i - r * words));
+  }
+}
+
+// Across a warp: lane i's key of a descending sort of 32.
+template <typename K>
+__device__ __forceinline__ typename K::Word warp_sort(typename K::Word v, int lane) {
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+    for (int j = k / 2; j >= 1; j /= 2) {
+      const auto o = K::exchange(v, j);
+      const bool larger = ((lane & k) == 0) == ((lane & j) == 0);
+      v = (o > v) == larger ? o : v;
+    }
+  return v;
+}
+// The 32 largest of two descending runs, descending.
+template <typename K>
+__device__ __forceinline__ typename K::Word warp_merge(typename K::Word best, typename K::Word other, int lane) {
+  const auto turned = K::shuffle(other, 31 - lane);
+  best = best > turned ? best : turned;
+#pragma unroll
+  for (int j = 16; j >= 1; j /= 2) {
+    const auto o = K::exchange(best, j);
+    const bool larger = (lane & j) == 0;
+    best = (o > best) == larger ? o : best;
+  }
+  return best;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kWriteWarps * 32) k_teacher_write_rows(TeacherWriteArgs a) {
+__global__ void __launch_bounds__(kWriteWarps * 32) k_teacher_write_warp(TeacherWriteArgs a) {
+  using K = Key<T>;
+  using W = typename K::Word;
+  __shared__ W pending[kWriteWarps][64];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t r = (int64_t)blockIdx.x * kWriteWarps + warp;
   if (r >= a.n) return;
-  const T* s = static_cast<const T*>(a.logits) + r * a.classes;
-  const float low = lowest_of<T>();
-  float mine = -INFINITY;  // lane e holds entry e
-  int mine_idx = -1;
-  float prev = INFINITY;
-  int prev_idx = -1;
-  float first = 0.0f, last = 0.0f;
-  int count = 0;
-  for (int e = 0; e < a.k; ++e) {
-    float best = -INFINITY;
-    int best_idx = INT32_MAX;
-    for (int c = lane; c < a.classes; c += 32) {
-      const float v = to_f32(s[c]);
-      if (!(v > low) || v == INFINITY) continue;
-      const bool after = v < prev || (v == prev && c > prev_idx);
-      if (after && v > best) {  // ascending c: the lowest index stays
-        best = v;
-        best_idx = c;
-      }
+  const int C = (int)a.classes, k = a.k;
+  const T* s = static_cast<const T*>(a.logits) + r * C;
+  W top = 0;  // largest key of this lane
+#pragma unroll 8
+  for (int c = lane; c < C; c += 32) {
+    const W w = K::make(s[c], c);
+    top = w > top ? w : top;
+  }
+  // At least k keys reach the k-th largest of the lanes' largest.
+  W bound = K::shuffle(warp_sort<K>(top, lane), k - 1);
+  if (bound == 0) bound = 1;  // fewer than k lanes have a class at all
+  W best = 0;
+  int held = 0;
+  W* queue = pending[warp];
+  for (int c0 = 0; c0 < C; c0 += 32 * 4) {
+    W w[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int c = c0 + 32 * q + lane;
+      w[q] = c < C ? K::make(s[c], c) : 0;
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float ov = __shfl_xor_sync(~0u, best, o);
-      const int oi = __shfl_xor_sync(~0u, best_idx, o);
-      if (ov > best || (ov == best && oi < best_idx)) {
-        best = ov;
-        best_idx = oi;
+    for (int q = 0; q < 4; ++q) {
+      const unsigned take = __ballot_sync(~0u, w[q] >= bound);
+      if (take == 0) continue;
+      if (w[q] >= bound) queue[held + __popc(take & ((1u << lane) - 1))] = w[q];
+      held += __popc(take);
+      __syncwarp();
+      if (held >= 32) {  // held is the same in every lane
+        best = warp_merge<K>(best, warp_sort<K>(queue[lane], lane), lane);
+        const W kth = K::shuffle(best, k - 1);
+        if (kth >= bound) bound = kth + 1;  // keys are all different
+        const W rest = lane < held - 32 ? queue[32 + lane] : 0;
+        __syncwarp();
+        queue[lane] = rest;
+        held -= 32;
+        __syncwarp();
       }
     }
-    if (best == -INFINITY) break;
-    if (e == 0) first = best;
-    last = best;
-    prev = best;
-    prev_idx = best_idx;
-    ++count;
-    if (lane == e) {
-      mine = best;
-      mine_idx = best_idx;
-    }
   }
+  if (held > 0) best = warp_merge<K>(best, warp_sort<K>(lane < held ? queue[lane] : 0, lane), lane);
+  const bool mine = lane < k && best != 0;
+  const int count = __popc(__ballot_sync(~0u, mine));
+  const float value = mine ? K::value(best) : 0.0f;
+  const float first = __shfl_sync(~0u, value, 0), last = __shfl_sync(~0u, value, count > 0 ? count - 1 : 0);
   const float levels = (float)((1 << a.bits) - 1);
-  int code = 0;
-  if (lane < count && first > last) code = quantise(first, last, mine, levels);
+  const int code = mine && first > last ? quantise(first, last, value, levels) : 0;
   uint8_t* rec = a.records + r * a.rec_bytes;
-  if (lane == 0) {
-    const float scale = (float)(((double)first - (double)last) / (double)levels);
-    *reinterpret_cast<float2*>(rec) = make_float2(first, scale);
-  }
-  if (lane < a.k) reinterpret_cast<int16_t*>(rec + 8)[lane] = (int16_t)mine_idx;
-  uint8_t* codes = rec + 8 + 2 * a.k;
-  int used = 8 + 2 * a.k;
+  if (lane == 0)
+    *reinterpret_cast<float2*>(rec) = make_float2(first, (float)(((double)first - (double)last) / (double)levels));
+  if (lane < k) reinterpret_cast<int16_t*>(rec + 8)[lane] = mine ? (int16_t)K::index(best) : (int16_t)-1;
+  uint8_t* codes = rec + 8 + 2 * k;
+  int used = 8 + 2 * k;
   if (a.bits == 8) {
-    if (lane < a.k) codes[lane] = (uint8_t)code;
-    used += a.k;
+    if (lane < k) codes[lane] = (uint8_t)code;
+    used += k;
   } else {
     const int hi = __shfl_down_sync(~0u, code, 1);
-    if (!(lane & 1) && lane < a.k) codes[lane >> 1] = (uint8_t)(code | (lane + 1 < a.k ? hi << 4 : 0));
-    used += (a.k + 1) / 2;
+    if (!(lane & 1) && lane < k) codes[lane >> 1] = (uint8_t)(code | (lane + 1 < k ? hi << 4 : 0));
+    used += (k + 1) / 2;
   }
   for (int b = used + lane; b < a.rec_bytes; b += 32) rec[b] = 0;
 }
 
-__global__ void k_teacher_read(const uint8_t* __restrict__ records, int64_t n_records, const int64_t* rows,
-                               int64_t first_row, int64_t n, int k, int bits, int rec_bytes, float* values,
-                               int32_t* index) {
-  const int64_t total = n * k;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / k;
-    const int e = (int)(i - r * k);
-    const int64_t rec = rows ? rows[r] : first_row + r;
-    float v = -INFINITY;
-    int idx = -1;
-    if (rec >= 0 && rec < n_records) {
-      const uint8_t* p = records + rec * rec_bytes;
-      const float2 head = *reinterpret_cast<const float2*>(p);
-      idx = reinterpret_cast<const int16_t*>(p + 8)[e];
-      if (idx >= 0) v = record_value(head.x, head.y, record_code(p + 8 + 2 * k, e, bits));
-      else idx = -1;
+// LANES (a power of two >= k) lanes per record, several records in flight.
+template <int LANES>
+__global__ void __launch_bounds__(256) k_teacher_read(const uint8_t* __restrict__ records, int64_t n_records,
+                                                      const int64_t* __restrict__ rows, int64_t first_row, int64_t n,
+                                                      int k, int bits, int rec_bytes, float* __restrict__ values,
+                                                      int32_t* __restrict__ index) {
+  constexpr int kFlight = 4, kGroups = 256 / LANES;
+  const int e = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  for (int64_t r0 = (int64_t)blockIdx.x * kGroups * kFlight; r0 < n; r0 += (int64_t)gridDim.x * kGroups * kFlight) {
+    int64_t rec[kFlight];
+    float v[kFlight];
+    int idx[kFlight];
+#pragma unroll
+    for (int q = 0; q < kFlight; ++q) {
+      const int64_t r = r0 + q * kGroups + group;
+      rec[q] = r < n ? (rows ? __ldg(rows + r) : first_row + r) : -1;
     }
-    values[i] = v;
-    index[i] = idx;
+#pragma unroll
+    for (int q = 0; q < kFlight; ++q) {
+      v[q] = -INFINITY;
+      idx[q] = -1;
+      if (rec[q] >= 0 && rec[q] < n_records && e < k) {
+        const uint8_t* p = records + rec[q] * rec_bytes;
+        const float2 head = __ldg(reinterpret_cast<const float2*>(p));
+        const int i = __ldg(reinterpret_cast<const int16_t*>(p + 8) + e);
+        const int byte = __ldg(p + 8 + 2 * k + (bits == 8 ? e : e >> 1));
+        if (i >= 0) {
+          idx[q] = i;
+          v[q] = record_value(head.x, head.y, bits == 8 ? byte : (byte >> ((e & 1) * 4)) & 15);
+        }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kFlight; ++q) {
+      const int64_t r = r0 + q * kGroups + group;
+      if (r < n && e < k) {
+        values[r * k + e] = v[q];
+        index[r * k + e] = idx[q];
+      }
+    }
   }
+}
+
+// The same for K = 8, 16 or 32 entries, one thread per record: whole 16-byte units
+// in and out, a tenth of the instructions.
+template <int K, int BITS>
+__global__ void __launch_bounds__(256) k_teacher_read_whole(const uint8_t* __restrict__ records, int64_t n_records,
+                                                            const int64_t* __restrict__ rows, int64_t first_row,
+                                                            int64_t n, float* __restrict__ values,
+                                                            int32_t* __restrict__ index) {
+  constexpr int kBytes = (8 + 2 * K + K * BITS / 8 + 15) / 16 * 16;
+  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < n; r += (int64_t)gridDim.x * 256) {
+    const int64_t rec = rows ? __ldg(rows + r) : first_row + r;
+    const bool here = rec >= 0 && rec < n_records;
+    uint32_t w[kBytes / 4];
+#pragma unroll
+    for (int i = 0; i < kBytes / 16; ++i) {
+      uint4 v = make_uint4(0, 0, 0xffffffffu, 0xffffffffu);
+      if (i > 0) v.x = v.y = 0xffffffffu;
+      if (here) v = __ldg(reinterpret_cast<const uint4*>(records + rec * kBytes) + i);
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+    const float offset = __uint_as_float(w[0]), scale = __uint_as_float(w[1]);
+    float4* vo = reinterpret_cast<float4*>(values + r * K);
+    int4* io = reinterpret_cast<int4*>(index + r * K);
+#pragma unroll
+    for (int q = 0; q < K / 4; ++q) {
+      float v[4];
+      int idx[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = 4 * q + j, bit = BITS * e;
+        const int i = (int)(int16_t)(w[2 + e / 2] >> (16 * (e & 1)));
+        const int code = (int)(w[2 + K / 2 + bit / 32] >> (bit % 32)) & ((1 << BITS) - 1);
+        idx[j] = i >= 0 ? i : -1;
+        v[j] = i >= 0 ? record_value(offset, scale, code) : -INFINITY;
+      }
+      vo[q] = make_float4(v[0], v[1], v[2], v[3]);
+      io[q] = make_int4(idx[0], idx[1], idx[2], idx[3]);
+    }
+  }
+}
+
+template <int K>
+static int launch_read_whole(const void* records, int64_t n_records, const int64_t* rows, int64_t first_row, int64_t n,
+                             int bits, float* values, int32_t* index, cudaStream_t st) {
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, 256), 148 * 32);
+  auto* kernel = bits == 8 ? k_teacher_read_whole<K, 8> : k_teacher_read_whole<K, 4>;
+  kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(records), n_records, rows, first_row, n, values, index);
+  return check_launch("k_teacher_read_whole");
+}
+
+template <typename T, int MAX>
+static int launch_rows(const TeacherWriteArgs& a, cudaStream_t st) {
+  const size_t row = a.classes * sizeof(T);
+  // 128 rows, 64 or 32 (whole warps, and a multiple of 16 bytes)
+  int rows = kStagedRows;
+  while (rows > 32 && rows * row > kStagedSmem) rows /= 2;
+  const size_t smem = std::max((size_t)rows * row, (size_t)rows * (a.rec_bytes + 4));
+  auto* kernel = k_teacher_write_rows<T, MAX>;
+  if (smem > 40 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_teacher_write_rows: %s", cudaGetErrorString(e));
+  }
+  kernel<<<(unsigned)ceil_div(a.n, rows), rows, smem, st>>>(a, rows, aligned(a.logits, 16));
+  return check_launch("k_teacher_write_rows");
+}
+
+template <typename T>
+static int launch_write(const TeacherWriteArgs& a, cudaStream_t st) {
+  // A thread per row needs many rows, short ones and few entries (its network grows
+  // with k log^2 k).
+  if (a.n >= 148 * 32 && a.classes * sizeof(T) <= kStagedSmem / 32 && a.k <= 16)
+    return a.k <= 4 ? launch_rows<T, 4>(a, st) : a.k <= 8 ? launch_rows<T, 8>(a, st) : launch_rows<T, 16>(a, st);
+  k_teacher_write_warp<T><<<(unsigned)ceil_div(a.n, kWriteWarps), kWriteWarps * 32, 0, st>>>(a);
+  return check_launch("k_teacher_write_warp");
+}
+
+template <int LANES>
+static int launch_read(const void* records, int64_t n_records, const int64_t* rows, int64_t first_row, int64_t n, int k,
+                       int bits, float* values, int32_t* index, cudaStream_t st) {
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, 256 / LANES * 4), 148 * 32);
+  k_teacher_read<LANES><<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(records), n_records, rows, first_row, n, k,
+                                              bits, record_bytes(k, bits), values, index);
+  return check_launch("k_teacher_read");
 }
 
 static int check_cache(const char* who, int64_t n, const void* records, int64_t n_records, int k, int bits) {
@@ -157,12 +526,10 @@ int gs_teacher_write(const void* logits, int dtype, int64_t n, int64_t classes, 
   a.logits = logits; a.n = n; a.classes = classes; a.k = k; a.bits = bits;
   a.rec_bytes = record_bytes(k, bits);
   a.records = static_cast<uint8_t*>(records) + first_row * a.rec_bytes;
-  const unsigned grid = (unsigned)ceil_div(n, kWriteWarps);
   cudaStream_t st = as_stream(stream);
-  if (dtype == GS_F32) k_teacher_write_rows<float><<<grid, kWriteWarps * 32, 0, st>>>(a);
-  else if (dtype == GS_F16) k_teacher_write_rows<__half><<<grid, kWriteWarps * 32, 0, st>>>(a);
-  else k_teacher_write_rows<__nv_bfloat16><<<grid, kWriteWarps * 32, 0, st>>>(a);
-  return check_launch("k_teacher_write_rows");
+  if (dtype == GS_F32) return launch_write<float>(a, st);
+  if (dtype == GS_F16) return launch_write<__half>(a, st);
+  return launch_write<__nv_bfloat16>(a, st);
 }
 
 int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows, int64_t first_row, int64_t n,
@@ -171,10 +538,16 @@ int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows,
   if (int e = check_cache("gs_teacher_read", n, records, n_records, k, bits)) return e;
   if (n == 0) return GS_OK;
   if (!values || !index) return set_error(GS_ERR_INVALID_ARG, "gs_teacher_read: NULL pointer");
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * k, 256), 148 * 32);
-  k_teacher_read<<<grid, 256, 0, as_stream(stream)>>>(static_cast<const uint8_t*>(records), n_records, rows,
-                                                      first_row, n, k, bits, record_bytes(k, bits), values, index);
-  return check_launch("k_teacher_read");
+  cudaStream_t st = as_stream(stream);
+  if (aligned(values, 16) && aligned(index, 16)) {
+    if (k == 8) return launch_read_whole<8>(records, n_records, rows, first_row, n, bits, values, index, st);
+    if (k == 16) return launch_read_whole<16>(records, n_records, rows, first_row, n, bits, values, index, st);
+    if (k == 32) return launch_read_whole<32>(records, n_records, rows, first_row, n, bits, values, index, st);
+  }
+  if (k <= 4) return launch_read<4>(records, n_records, rows, first_row, n, k, bits, values, index, st);
+  if (k <= 8) return launch_read<8>(records, n_records, rows, first_row, n, k, bits, values, index, st);
+  if (k <= 16) return launch_read<16>(records, n_records, rows, first_row, n, k, bits, values, index, st);
+  return launch_read<32>(records, n_records, rows, first_row, n, k, bits, values, index, st);
 }
 
 }  // extern "C"

@@ -171,6 +171,9 @@ def _cache_logits(n, c, dtype, seed):
 @pytest.mark.parametrize("n,c,k", [
     (1, 1, 1), (1, 5, 8), (3, 2, 2), (100, 20, 5), (257, 32, 32), (300, 33, 31), (1000, 150, 8), (515, 133, 7),
     (64, 1201, 32), (31, 4096, 16), (9, 32767, 32), (4100, 64, 3), (70, 257, 1),
+    # one thread per row: many rows
+    (4736, 1, 1), (5003, 150, 8), (4801, 133, 5), (4999, 128, 16), (4750, 7, 16), (4736, 300, 12), (5000, 64, 2),
+    (4737, 384, 9), (4900, 20, 20),
 ])
 def test_write_and_read_match_the_definition(n, c, k, dtype, bits):
     z = _cache_logits(n, c, dtype, n * 7 + c)
@@ -216,21 +219,24 @@ def test_write_extreme_ranges():
         assert torch.equal(values.cpu(), read64(first, scale, want_i, code))
 
 
-def test_read_rows_in_any_order():
+@pytest.mark.parametrize("k,bits", [(7, 8), (8, 8), (8, 4), (16, 8), (16, 4), (32, 8), (32, 4), (3, 4), (1, 8), (20, 4)])
+def test_read_rows_in_any_order(k, bits):
     z = _cache_logits(500, 40, "fp32", 1)
-    cache = TeacherCache(500, 7, 40)
+    z[:100, 5:] = -math.inf  # rows with absent entries
+    cache = TeacherCache(500, k, 40, bits=bits)
     cache.write(0, z)
     all_v, all_i = cache.read(slice(None))
     rows = torch.tensor([[3, 499, 3], [0, -1, 500], [250, 1 << 40, -(1 << 50)]], device="cuda")
     v, i = cache.read(rows)
-    assert v.shape == (3, 3, 7)
+    assert v.shape == (3, 3, k)
+    assert torch.equal(all_v.cpu(), read64(*write64(z, k, bits)))
     inside = (rows >= 0) & (rows < 500)
     assert torch.equal(v[inside], all_v[rows[inside]]) and torch.equal(i[inside], all_i[rows[inside]])
     assert (v[~inside] == -math.inf).all() and (i[~inside] == -1).all()
     v32, i32 = cache.read(rows[:2].int())
     assert torch.equal(v32, v[:2]) and torch.equal(i32, i[:2])
-    assert cache.read(slice(7, 7))[0].shape == (0, 7)
-    assert cache.read(rows[:0])[0].shape == (0, 3, 7)
+    assert cache.read(slice(7, 7))[0].shape == (0, k)
+    assert cache.read(rows[:0])[0].shape == (0, 3, k)
 
 
 def test_cache_starts_empty_and_saves():
