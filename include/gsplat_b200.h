@@ -498,6 +498,14 @@ int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows,
 size_t gs_decode_image_bytes(int d, int f, int c);
 int gs_decode_prepare(const void* w_gate, const void* w_up, const void* w_down, int dtype, int d, int f, int c,
                       void* image, size_t image_bytes, void* stream);
+/* For few rows of a small block (gs_decode_is_few: at most GS_DECODE_FEW_N rows,
+ * f (2 d + c) <= GS_DECODE_FEW_WEIGHTS): y straight from the weights, in one
+ * launch, the hidden values kept in 32 bits. */
+#define GS_DECODE_FEW_N 64
+#define GS_DECODE_FEW_WEIGHTS 49152
+int gs_decode_is_few(int64_t n, int d, int f, int c);
+int gs_decode_forward_few(const void* x, const void* w_gate, const void* w_up, const void* w_down, int dtype, int64_t n,
+                          int d, int f, int c, int activation, void* y, void* stream);
 size_t gs_decode_workspace_bytes(const void* x, const void* dy, int64_t n, int d, int f, int c, int weights);
 int gs_decode_forward(const void* x, int dtype, int64_t n, int d, int f, int c, int activation, const void* image,
                       size_t image_bytes, void* y, void* workspace, size_t workspace_bytes, void* stream);

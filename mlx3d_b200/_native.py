@@ -191,6 +191,8 @@ _SIGS = {
     "gs_decode_forward": (
         c_int, [_P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, c_size_t, _P, _P, c_size_t, _P]
     ),
+    "gs_decode_is_few": (c_int, [c_int64, c_int, c_int, c_int]),
+    "gs_decode_forward_few": (c_int, [_P, _P, _P, _P, c_int, c_int64, c_int, c_int, c_int, c_int, _P, _P]),
     "gs_decode_workspace_bytes": (c_size_t, [_P, _P, c_int64, c_int, c_int, c_int, c_int]),
     "gs_decode_backward": (
         c_int,

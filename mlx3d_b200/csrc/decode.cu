@@ -951,6 +951,54 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
   if (warp == 0) tc::tmem_free(tmem, kTmemCols);
 }
 
+// A few rows of a small block (a picked point, a handful of samples): one launch
+// that reads the weights where they are, one block per row, a warp per hidden
+// unit and then per output.  h stays in 32 bits.  The matrix path's weight layout
+// and pipeline start cost more than this whole call: one row, 32-64-20, FEW_US
+// instead of 45 us.
+constexpr int kFewThreads = 256;
+template <typename T, int ACT>
+__global__ void __launch_bounds__(kFewThreads) k_decode_few(const T* __restrict__ x, const T* __restrict__ wg,
+                                                            const T* __restrict__ wu, const T* __restrict__ wd, int d,
+                                                            int f, int c, T* __restrict__ y) {
+  extern __shared__ float few[];
+  float *xs = few, *hs = few + d;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  x += (size_t)blockIdx.x * d;
+  y += (size_t)blockIdx.x * c;
+  for (int i = threadIdx.x; i < d; i += kFewThreads) xs[i] = to_f32(x[i]);
+  __syncthreads();
+#pragma unroll 4
+  for (int h = warp; h < f; h += kFewThreads / 32) {
+    float g = 0.0f, u = 0.0f;
+    for (int i = lane; i < d; i += 32) {
+      g = fmaf(xs[i], to_f32(wg[(size_t)h * d + i]), g);
+      u = fmaf(xs[i], to_f32(wu[(size_t)h * d + i]), u);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      g += __shfl_xor_sync(~0u, g, o);
+      u += __shfl_xor_sync(~0u, u, o);
+    }
+    if (lane == 0) {
+      F2 a, slope;
+      float a0, a1;
+      gate2<ACT, false>(f2(g), a, slope);
+      split(a, a0, a1);
+      hs[h] = a0 * u;
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int o = warp; o < c; o += kFewThreads / 32) {
+    float s = 0.0f;
+    for (int i = lane; i < f; i += 32) s = fmaf(hs[i], to_f32(wd[(size_t)o * f + i]), s);
+#pragma unroll
+    for (int k = 16; k; k >>= 1) s += __shfl_xor_sync(~0u, s, k);
+    if (lane == 0) y[o] = from_f32<T>(s);
+  }
+}
+
 // Sums the splits' partial weight gradients in order and rounds once.
 template <typename T>
 __global__ void k_decode_reduce(const float* __restrict__ partials, int splits, int64_t fd, int64_t cf, T* dg, T* du,
@@ -1184,6 +1232,39 @@ size_t gs_decode_workspace_bytes(const void* x, const void* dy, int64_t n, int d
   if (dy && !fetchable(dy, c)) bytes += padded_bytes(n, c);
   if (weights) bytes += (size_t)decode_splits(n, f) * (2 * (size_t)f * d + (size_t)c * f) * sizeof(float);
   return bytes;
+}
+
+int gs_decode_is_few(int64_t n, int d, int f, int c) {
+  return n >= 0 && n <= GS_DECODE_FEW_N && d >= 1 && c >= 1 && f >= 1 &&
+         (int64_t)f * (2 * (int64_t)d + c) <= GS_DECODE_FEW_WEIGHTS;
+}
+
+int gs_decode_forward_few(const void* x, const void* w_gate, const void* w_up, const void* w_down, int dtype, int64_t n,
+                          int d, int f, int c, int activation, void* y, void* stream) {
+  clear_error();
+  if (int e = check_dims("gs_decode_forward_few", n, dtype, d, f, c)) return e;
+  if (!gs_decode_is_few(n, d, f, c))
+    return set_error(GS_ERR_INVALID_ARG, "gs_decode_forward_few: more than %d rows or %d weights", GS_DECODE_FEW_N,
+                     GS_DECODE_FEW_WEIGHTS);
+  if (activation != GS_ACT_SILU && activation != GS_ACT_GELU)
+    return set_error(GS_ERR_INVALID_ARG, "gs_decode_forward_few: unknown activation %d", activation);
+  if (n == 0) return GS_OK;
+  if (!x || !w_gate || !w_up || !w_down || !y)
+    return set_error(GS_ERR_INVALID_ARG, "gs_decode_forward_few: NULL pointer");
+  const size_t smem = sizeof(float) * ((size_t)d + f);
+  auto launch = [&](auto zero) {
+    using T = decltype(zero);
+    auto* kernel = activation == GS_ACT_SILU ? k_decode_few<T, GS_ACT_SILU> : k_decode_few<T, GS_ACT_GELU>;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_decode_few: %s", cudaGetErrorString(e));
+    }
+    kernel<<<(unsigned)n, kFewThreads, smem, as_stream(stream)>>>(
+        static_cast<const T*>(x), static_cast<const T*>(w_gate), static_cast<const T*>(w_up),
+        static_cast<const T*>(w_down), d, f, c, static_cast<T*>(y));
+    return check_launch("k_decode_few");
+  };
+  return dtype == GS_F16 ? launch(__half{}) : launch(__nv_bfloat16{});
 }
 
 int gs_decode_forward(const void* x, int dtype, int64_t n, int d, int f, int c, int activation, const void* image,

@@ -237,7 +237,9 @@ def distill_loss(logits: torch.Tensor, teacher, temperature: float = 1.0, weight
     or "none" (a float32 loss per row).  With float16 logits take "sum": a mean's gradients, of the order of
     1 / rows, fall below float16's range.  No gradient flows to the teacher or to ``weight``."""
     args = _DistillArgs(logits, teacher, temperature, weight, reduction)
-    return _Distill.apply(args.logits, args)
+    if torch.is_grad_enabled() and args.logits.requires_grad:
+        return _Distill.apply(args.logits, args)
+    return args.run(args.logits)
 
 
 def distill_loss_and_grad(logits: torch.Tensor, teacher, temperature: float = 1.0,

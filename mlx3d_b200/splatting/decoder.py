@@ -22,19 +22,34 @@ def _workspace(x, dy, f, c, weights):
     return torch.empty((size,), device=x.device, dtype=torch.uint8) if size else None
 
 
+def _prepare(w_gate, w_up, w_down):
+    (f, d), c = w_gate.shape, w_down.shape[0]
+    image = torch.empty((nat.load().gs_decode_image_bytes(d, f, c),), device=w_gate.device, dtype=torch.uint8)
+    nat.call_on(w_gate.device, "gs_decode_prepare", nat.ptr(w_gate), nat.ptr(w_up), nat.ptr(w_down),
+                nat.DTYPES[w_gate.dtype], d, f, c, nat.ptr(image), image.numel())
+    return image
+
+
+def _forward(x, w_gate, w_up, w_down, act):
+    """y, and the weights' image (None where few rows were decoded without one)."""
+    n, d = x.shape
+    f, c = w_gate.shape[0], w_down.shape[0]
+    y = torch.empty((n, c), device=x.device, dtype=x.dtype)
+    if nat.load().gs_decode_is_few(n, d, f, c):
+        nat.call_on(x.device, "gs_decode_forward_few", nat.ptr(x), nat.ptr(w_gate), nat.ptr(w_up), nat.ptr(w_down),
+                    nat.DTYPES[x.dtype], n, d, f, c, act, nat.ptr(y))
+        return y, None
+    image = _prepare(w_gate, w_up, w_down)
+    ws = _workspace(x, None, f, c, False)
+    nat.call_on(x.device, "gs_decode_forward", nat.ptr(x), nat.DTYPES[x.dtype], n, d, f, c, act, nat.ptr(image),
+                image.numel(), nat.ptr(y), nat.ptr(ws), 0 if ws is None else ws.numel())
+    return y, image
+
+
 class _Decode(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, act):
-        n, d = x.shape
-        f, c = w_gate.shape[0], w_down.shape[0]
-        dev, ty = x.device, nat.DTYPES[x.dtype]
-        image = torch.empty((nat.load().gs_decode_image_bytes(d, f, c),), device=dev, dtype=torch.uint8)
-        y = torch.empty((n, c), device=dev, dtype=x.dtype)
-        nat.call_on(dev, "gs_decode_prepare", nat.ptr(w_gate), nat.ptr(w_up), nat.ptr(w_down), ty, d, f, c,
-                    nat.ptr(image), image.numel())
-        ws = _workspace(x, None, f, c, False)
-        nat.call_on(dev, "gs_decode_forward", nat.ptr(x), ty, n, d, f, c, act, nat.ptr(image), image.numel(),
-                    nat.ptr(y), nat.ptr(ws), 0 if ws is None else ws.numel())
+        y, image = _forward(x, w_gate, w_up, w_down, act)
         ctx.save_for_backward(x, w_gate, w_up, w_down, image)
         ctx.act = act
         return y
@@ -47,6 +62,8 @@ class _Decode(torch.autograd.Function):
         f, c = w_gate.shape[0], w_down.shape[0]
         dev = x.device
         dy = dy.contiguous()
+        if image is None:
+            image = _prepare(w_gate, w_up, w_down)
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         weights = any(ctx.needs_input_grad[1:4])
         grads = tuple(torch.empty_like(w) for w in (w_gate, w_up, w_down)) if weights else (None, None, None)
@@ -93,7 +110,11 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
     nat.same_device(x.device, w_gate=w_gate, w_up=w_up, w_down=w_down)
     if x.numel() // d > nat.GS_DECODE_MAX_N:
         raise ValueError(f"features must have at most {nat.GS_DECODE_MAX_N} rows.")
-    y = _Decode.apply(x.reshape(-1, d), w_gate, w_up, w_down, nat.GS_GATES[activation])
+    args = (x.reshape(-1, d), w_gate, w_up, w_down)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in args):
+        y = _Decode.apply(*args, nat.GS_GATES[activation])
+    else:
+        y = _forward(*args, nat.GS_GATES[activation])[0]
     return y.reshape(*features.shape[:-1], c)
 
 

@@ -193,6 +193,12 @@ def test_native_decode_rejects_bad_arguments_before_the_device():
     assert lib.gs_decode_forward(None, 1, 0, 32, 100, 20, 0, None, 0, None, None, 0, None) == nat.GS_OK
     assert lib.gs_decode_forward(16, 1, nat.GS_DECODE_MAX_N + 1, 32, 100, 20, 0, 16, size, 16, None, 0,
                                  None) == nat.GS_ERR_INVALID_ARG
+    assert lib.gs_decode_is_few(64, 32, 256, 100) == 1 and lib.gs_decode_is_few(65, 32, 256, 100) == 0
+    assert lib.gs_decode_is_few(1, 128, 256, 250) == 0 and lib.gs_decode_is_few(-1, 8, 8, 8) == 0
+    few = (16, 16, 16, 16, 1, 1, 32, 64, 20, 0, 16, None)
+    for at, bad in ((0, None), (3, None), (10, None), (4, 0), (5, 65), (5, -1), (6, 129), (7, 1 << 16), (9, 2)):
+        assert lib.gs_decode_forward_few(*few[:at], bad, *few[at + 1:]) == nat.GS_ERR_INVALID_ARG, at
+    assert lib.gs_decode_forward_few(None, None, None, None, 1, 0, 32, 64, 20, 0, None, None) == nat.GS_OK
     # aligned rows need no copy; 20 classes (40 bytes a row) and unaligned addresses do
     assert lib.gs_decode_workspace_bytes(16, None, 1000, 32, 100, 20, 0) == 0
     assert lib.gs_decode_workspace_bytes(18, None, 1000, 32, 100, 20, 0) >= 1000 * 64
