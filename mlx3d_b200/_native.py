@@ -248,11 +248,12 @@ def call(name: str, *args) -> None:
 def call_on(device: torch.device, name: str, *args) -> None:
     """:func:`call` on ``device`` (which need not be the current one), with
     that device's current stream as the last argument."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+            call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

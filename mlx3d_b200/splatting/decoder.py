@@ -83,7 +83,8 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
     type are rounded to it.  ``activation`` is "silu" or "gelu" (the error-function form).  Returns (..., C) in
     the weights' type.  Products are summed in 32 bits and the hidden values are rounded once to the weights'
     type; they stay on chip, forward and backward."""
-    if activation not in nat.GS_GATES:
+    act = nat.GS_GATES.get(activation)
+    if act is None:
         raise ValueError("activation must be 'silu' or 'gelu'.")
     for name, w in (("features", features), ("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
         if not isinstance(w, torch.Tensor):
@@ -92,7 +93,8 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
             raise TypeError(f"{name} must be a floating-point tensor (got {w.dtype})")
     if features.ndim < 1 or w_gate.ndim != 2 or w_down.ndim != 2:
         raise ValueError("features must have shape (..., D), w_gate and w_up (F, D), w_down (C, F).")
-    d, f, c = features.shape[-1], w_gate.shape[0], w_down.shape[0]
+    lead, d = features.shape[:-1], features.shape[-1]
+    f, c = w_gate.shape[0], w_down.shape[0]
     if w_gate.shape != (f, d) or w_up.shape != (f, d) or w_down.shape != (c, f):
         raise ValueError("features (..., D), w_gate (F, D), w_up (F, D) and w_down (C, F) must agree.")
     if not 1 <= d <= nat.GS_DECODE_MAX_D:
@@ -105,17 +107,21 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
     if ty not in (torch.float16, torch.bfloat16) or w_up.dtype != ty or w_down.dtype != ty:
         raise TypeError("w_gate, w_up and w_down must all be float16 or all bfloat16.")
     x = nat.require_cuda("features", features, ty)
-    w_gate, w_up, w_down = (nat.require_cuda(k, w, ty) for k, w in (("w_gate", w_gate), ("w_up", w_up),
-                                                                   ("w_down", w_down)))
+    w_gate = nat.require_cuda("w_gate", w_gate, ty)
+    w_up = nat.require_cuda("w_up", w_up, ty)
+    w_down = nat.require_cuda("w_down", w_down, ty)
     nat.same_device(x.device, w_gate=w_gate, w_up=w_up, w_down=w_down)
     if x.numel() // d > nat.GS_DECODE_MAX_N:
         raise ValueError(f"features must have at most {nat.GS_DECODE_MAX_N} rows.")
-    args = (x.reshape(-1, d), w_gate, w_up, w_down)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in args):
-        y = _Decode.apply(*args, nat.GS_GATES[activation])
+    flat = len(lead) == 1
+    if not flat:
+        x = x.reshape(-1, d)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
+                                    or w_down.requires_grad):
+        y = _Decode.apply(x, w_gate, w_up, w_down, act)
     else:
-        y = _forward(*args, nat.GS_GATES[activation])[0]
-    return y.reshape(*features.shape[:-1], c)
+        y = _forward(x, w_gate, w_up, w_down, act)[0]
+    return y if flat else y.reshape(*lead, c)
 
 
 class FeatureDecoder:

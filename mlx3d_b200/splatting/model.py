@@ -181,12 +181,14 @@ class GaussianModel:
         normalize: bool = False,
         antialias: bool = False,
         projection: str = "ewa",
+        decoder=None,
     ) -> dict:
-        """Arbitrary per-Gaussian features (model.py:182-203)."""
+        """Arbitrary per-Gaussian features (model.py:182-203), decoded to ``logits``
+        where a :class:`~mlx3d_b200.splatting.FeatureDecoder` is given."""
         p = self.params
         return render_gaussian_features(camera, p["means"], p["quats"], self.scales_act, self.opacities_act,
                                         features, background=background, normalize=normalize,
-                                        antialias=antialias, projection=projection)
+                                        antialias=antialias, projection=projection, decoder=decoder)
 
     def save_ply(self, path: str) -> None:
         """Save in the standard 3DGS PLY layout (model.py:338-361)."""

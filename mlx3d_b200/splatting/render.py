@@ -436,8 +436,11 @@ def render_gaussian_features(
     refine_tiles: bool = False,
     antialias: bool = False,
     projection: str = "ewa",
+    decoder=None,
 ) -> dict[str, torch.Tensor]:
-    """Composite arbitrary (N, C) features (render.py:164-220)."""
+    """Composite arbitrary (N, C) features (render.py:164-220).  With a ``decoder``
+    (:class:`~mlx3d_b200.splatting.FeatureDecoder`, an addition) the result also has
+    ``logits`` (H, W, outputs), the decoded features, in the decoder's type."""
     if features.ndim != 2:
         raise ValueError("features must have shape (N, C).")
     if features.shape[0] != means.shape[0]:
@@ -447,4 +450,6 @@ def render_gaussian_features(
     )
     out = rasterize_features(proj["means2d"], proj["conics"], features, opac, ids, ranges, camera.width,
                              camera.height, tx, ty, background=background, normalize=normalize)
+    if decoder is not None:
+        out["logits"] = decoder(out["features"])
     return _extras(out, proj)

@@ -31,9 +31,9 @@ import torch
 from .. import _native as nat
 from ..cameras import Camera
 from ..distributed import GradientReducer, world
-from ..losses import l1_dssim_loss
+from ..losses import distill_loss_and_grad, l1_dssim_loss
 from .model import GaussianModel
-from .render import _project, _render_fused, side_streams
+from .render import _project, _render_fused, render_gaussian_features, side_streams
 
 __all__ = ["TrainerConfig", "GaussianTrainer"]
 
@@ -354,6 +354,33 @@ class GaussianTrainer:
                 self._apply_method_constraints()
         opacity_reset, sh_changed = self._schedules_after_update()
         return self._info(float(loss), opacity_reset, sh_changed, densify)
+
+    def distill_view(self, camera: Camera, features: torch.Tensor, teacher, decoder=None, temperature: float = 1.0) -> dict:
+        """One view of a feature field's training (an addition): composite the
+        per-Gaussian ``features`` (N, C) over this model's geometry, which stays
+        fixed, decode them where a ``decoder`` is given, and distil the class
+        logits from ``teacher``: ``TeacherCache.at(rows)`` or ``(values, index)`` of
+        the view's H * W pixels, row by row.  A pixel counts by its alpha; the loss
+        is the mean over pixels.  Gradients are accumulated in ``features.grad`` and
+        the decoder's ``params``; the caller's optimiser applies them.  Returns
+        ``loss`` (a device scalar), ``logits`` and ``alpha``."""
+        cfg, p = self.config, self.model.params
+        if decoder is not None and decoder.dtype == torch.float16:
+            raise ValueError("distill_view takes a bfloat16 decoder: the mean's gradients, of the order of 1 / pixels, "
+                             "fall below float16's range.")
+        with torch.no_grad():
+            scales, opacities = torch.exp(p["scales"]), torch.sigmoid(p["opacities"])
+        out = render_gaussian_features(camera, p["means"].detach(), p["quats"].detach(), scales, opacities, features,
+                                       normalize=True, antialias=cfg.antialias, projection=cfg.projection,
+                                       decoder=decoder)
+        logits = out["features"] if decoder is None else out["logits"]
+        alpha = out["alpha"].detach()
+        if isinstance(teacher, (tuple, list)):
+            values, index = teacher
+            teacher = tuple(t.reshape(*alpha.shape, t.shape[-1]) for t in (values, index))
+        loss, grad = distill_loss_and_grad(logits, teacher, temperature=temperature, weight=alpha)
+        logits.backward(grad)
+        return {"loss": loss, "logits": logits.detach(), "alpha": alpha}
 
     def _views_backward(self, cameras, targets, scale: float, streams: int, first_sink=None) -> list:
         """Forward + backward of every view, gradients accumulated in .grad.

@@ -1,0 +1,99 @@
+"""A semantic feature field end to end: render, decode, distil from the teacher
+cache, gradients into the per-Gaussian features and the decoder."""
+
+import pytest
+import torch
+
+from feature_helpers import distill64
+from helpers import random_scene
+from mlx3d_b200 import splatting as gs
+from mlx3d_b200.losses import distill_loss
+from mlx3d_b200.splatting import FeatureDecoder, GaussianModel, GaussianTrainer
+from mlx3d_b200.staging import TeacherCache
+
+pytestmark = pytest.mark.gpu
+
+
+def _scene(channels):
+    cam, means, quats, scales, opac, colors = random_scene(3)
+    t = lambda a: torch.tensor(a, device="cuda")  # noqa: E731
+    n = means.shape[0]
+    params = {"means": t(means), "quats": t(quats), "scales": torch.log(t(scales)), "opacities": torch.logit(t(opac)),
+              "sh_dc": t(colors).reshape(n, 1, 3).clone(), "sh_rest": torch.zeros((n, 0, 3), device="cuda")}
+    g = torch.Generator(device="cuda").manual_seed(4)
+    feats = torch.randn((n, channels), device="cuda", generator=g).requires_grad_(True)
+    return cam, GaussianModel(params, sh_degree=0), feats, g
+
+
+@pytest.mark.parametrize("channels,hidden,classes,decoded", [(16, 40, 7, True), (12, 0, 12, False)])
+def test_distill_view_against_the_plain_pipeline(channels, hidden, classes, decoded):
+    cam, model, feats, g = _scene(channels)
+    pixels = cam.width * cam.height
+    teacher = torch.randn((2, cam.height, cam.width, classes), device="cuda", generator=g) * 3
+    cache = TeacherCache(2 * pixels, 4, classes)
+    for view in range(2):
+        cache.write(view * pixels, teacher[view])
+    dec = FeatureDecoder.create(channels, hidden, classes, generator=g) if decoded else None
+    trainer = GaussianTrainer(model)
+    rows = cache.at(slice(pixels, 2 * pixels))
+    out = trainer.distill_view(cam, feats, rows, dec, temperature=2.0)
+    assert all(p.grad is None for p in model.params.values())  # the geometry is left alone
+    got = [feats.grad] + ([dec.params[k].grad for k in ("w_gate", "w_up", "w_down")] if decoded else [])
+
+    # the same from the rendered channels on, in 64 bits
+    leaf = feats.detach().clone().requires_grad_(True)
+    r = model.render_features(cam, leaf, normalize=True)
+    x = r["features"].detach().double().requires_grad_(True)
+    ws = [dec.params[k].detach().double().requires_grad_(True) for k in ("w_gate", "w_up", "w_down")] if decoded else []
+    logits = x
+    if decoded:
+        gate = x @ ws[0].T
+        logits = (gate * torch.sigmoid(gate) * (x @ ws[1].T)) @ ws[2].T
+    values, index = cache.read(slice(pixels, 2 * pixels))
+    shape = (cam.height, cam.width, 4)
+    loss, dl = distill64(logits.detach(), values.reshape(shape), index.reshape(shape), 2.0, r["alpha"].detach())
+    grads = torch.autograd.grad(logits, [x, *ws], dl / pixels)
+    r["features"].backward(grads[0].float())
+    want = [leaf.grad, *grads[1:]]
+    # Roundings to 16 bits (half a step e = 2^-9): weights, features, h, logits, dlogits, dg or du, and the result: 8 in a
+    # row at most.  A logit's rounding changes the softmax by 2 |s| e / T.  dlogits = q - p cancels: relative to what is
+    # left, the errors of q and p grow by kappa.
+    kappa = float((dl.abs() + 2 * torch.softmax(logits.detach() / 2, -1) * r["alpha"].detach()[..., None] * 2).norm()
+                  / dl.norm())
+    tol = 2.0 ** -9 * (8 + kappa * float(logits.detach().abs().max())) if decoded else 1e-4
+    assert abs(float(out["loss"]) - float(loss.mean())) <= tol * float(loss.mean())
+    for a, b in zip(got, want):
+        assert a.shape == b.shape
+        assert float((a.double() - b.double()).norm()) <= tol * float(b.double().norm())
+
+
+def test_distill_view_accumulates_and_takes_arrays():
+    cam, model, feats, g = _scene(5)
+    trainer = GaussianTrainer(model)
+    values = torch.randn((cam.width * cam.height, 3), device="cuda", generator=g)
+    index = torch.randint(0, 5, (cam.width * cam.height, 3), device="cuda", generator=g)
+    first = trainer.distill_view(cam, feats, (values, index))
+    once = feats.grad.clone()
+    trainer.distill_view(cam, feats, (values, index))
+    assert torch.allclose(feats.grad, 2 * once, rtol=1e-4, atol=1e-9)  # (the compositor's atomics change the order)
+    shape = (cam.height, cam.width, 3)
+    again = distill_loss(first["logits"], (values.reshape(shape), index.reshape(shape)), weight=first["alpha"])
+    assert torch.equal(again, first["loss"])
+
+
+def test_render_features_decodes():
+    cam, model, feats, g = _scene(8)
+    dec = FeatureDecoder.create(8, 16, 3, activation="gelu", generator=g)
+    out = model.render_features(cam, feats, decoder=dec)
+    assert out["logits"].shape == (cam.height, cam.width, 3) and out["logits"].dtype == torch.bfloat16
+    assert torch.equal(out["logits"], dec(out["features"]))
+    plain = gs.render_gaussian_features(cam, model.params["means"], model.params["quats"], model.scales_act,
+                                        model.opacities_act, feats)
+    assert "logits" not in plain and torch.equal(plain["features"], out["features"])
+
+
+def test_distill_view_refuses_float16_decoders():
+    cam, model, feats, g = _scene(8)
+    dec = FeatureDecoder.create(8, 16, 3, dtype=torch.float16, generator=g)
+    with pytest.raises(ValueError, match="bfloat16"):
+        GaussianTrainer(model).distill_view(cam, feats, (torch.zeros(1, 1), torch.zeros(1, 1).int()), dec)
