@@ -256,6 +256,17 @@ def call_on(device: torch.device, name: str, *args) -> None:
             call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+_distill_workspace = None
+
+
+def distill_workspace_bytes() -> int:
+    """The size of every distillation call's workspace."""
+    global _distill_workspace
+    if _distill_workspace is None:
+        _distill_workspace = int(load().gs_distill_workspace_bytes())
+    return _distill_workspace
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -270,6 +281,8 @@ def require_cuda(name: str, t: torch.Tensor, dtype=torch.float32) -> torch.Tenso
     error: this package has no CPU path."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    if t.is_cuda and t.dtype == dtype and t.is_contiguous():
+        return t
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be a CUDA tensor (got device {t.device}); mlx3d_b200 has no CPU path")
     if t.dtype != dtype:
@@ -288,8 +301,9 @@ def require_float(name: str, t: torch.Tensor) -> torch.Tensor:
 
 
 def same_device(device: torch.device, **tensors) -> None:
+    index = device.index
     for name, t in tensors.items():
-        if t is not None and t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError(f"{name} must be on {device} (got {t.device})")
 
 

@@ -483,34 +483,63 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
   if (a.partials) block_partial(acc, a.partials + blockIdx.x);
 }
 
+// One block per row.  A row starts anywhere; it is moved in 16-byte units of
+// memory, the first and last of which may reach outside it and are taken element
+// by element.  `staged`: the units are kept in shared memory, else read again.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int staged) {
+__global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int staged, int vector_out) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float red[kRowThreads / 32], stats[3];
+  __shared__ float red[kRowThreads / 32], stats[2];
   __shared__ float2 ent[GS_TEACHER_MAX_K], fix[GS_TEACHER_MAX_K];
+  constexpr int kUnit = 16 / sizeof(T);
+  union Unit {
+    uint4 all;
+    T e[kUnit];
+  };
   const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  T* row = reinterpret_cast<T*>(smem);
+  Unit* kept = reinterpret_cast<Unit*>(smem);
   const float c2 = a.inv_temp * kLog2e;
   double acc = 0.0;
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
     const T* src = static_cast<const T*>(a.logits) + r * C;
+    const int lead = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));  // elements before the row
+    const int units = (lead + C + kUnit - 1) / kUnit;
+    const uint4* from = reinterpret_cast<const uint4*>(src - lead);
+    auto whole = [&](int u) { return u * kUnit >= lead && (u + 1) * kUnit <= lead + C; };
+    auto read = [&](int u) {  // elements outside the row are -inf
+      Unit v;
+      if (whole(u)) {
+        v.all = __ldg(from + u);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) {
+          const int c = u * kUnit + i - lead;
+          v.e[i] = c >= 0 && c < C ? src[c] : from_f32<T>(-INFINITY);
+        }
+      }
+      return v;
+    };
     stage_entries<kRowThreads>(a, ent, r, 1, threadIdx.x);
     float m = -INFINITY;
-#pragma unroll 8
-    for (int c = threadIdx.x; c < C; c += kRowThreads) {
-      const T v = src[c];
-      if (staged) row[c] = v;
-      m = fmaxf(m, to_f32(v));
+#pragma unroll 4
+    for (int u = threadIdx.x; u < units; u += kRowThreads) {
+      const Unit v = read(u);
+      if (staged) kept[u] = v;
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) m = fmaxf(m, to_f32(v.e[i]));
     }
     m = group_max<32>(m);
     if (lane == 0) red[warp] = m;
     __syncthreads();
     m = group_max<32>(lane < kRowThreads / 32 ? red[lane] : -INFINITY);
     __syncthreads();
-    const T* s = staged ? row : src;  // (staged[c] was written by this thread; other reads follow a barrier)
     float sum = 0.0f;
-#pragma unroll 8
-    for (int c = threadIdx.x; c < C; c += kRowThreads) sum += exp2_of((to_f32(s[c]) - m) * c2);
+#pragma unroll 2
+    for (int u = threadIdx.x; u < units; u += kRowThreads) {
+      const Unit v = staged ? kept[u] : read(u);
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) sum += exp2_of((to_f32(v.e[i]) - m) * c2);
+    }
     sum = group_sum<32>(sum);
     if (lane == 0) red[warp] = sum;
     __syncthreads();
@@ -518,7 +547,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
     const float f = w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r : 0] : 1.0f);
     if (warp == 0) {
       sum = group_sum<32>(lane < kRowThreads / 32 ? red[lane] : 0.0f);
-      auto logit = [&](int i) { return to_f32(s[i]); };
+      auto logit = [&](int i) { return to_f32(src[i]); };
       float term;
       const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
       __syncwarp();
@@ -537,11 +566,22 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
       T* g = static_cast<T*>(a.grad) + r * C;
       const bool any = stats[1] > 0.0f;
       const float qf = stats[0] * f;
-      if (any) {
-#pragma unroll 8
-        for (int c = threadIdx.x; c < C; c += kRowThreads) g[c] = from_f32<T>(exp2_of((to_f32(s[c]) - m) * c2) * qf);
-      } else {
-        for (int c = threadIdx.x; c < C; c += kRowThreads) g[c] = from_f32<T>(0.0f);
+      uint4* to = reinterpret_cast<uint4*>(g - lead);  // (vector_out: aligned as the logits)
+#pragma unroll 2
+      for (int u = threadIdx.x; u < units; u += kRowThreads) {
+        Unit v;
+        if (any) v = staged ? kept[u] : read(u);
+#pragma unroll
+        for (int i = 0; i < kUnit; ++i) v.e[i] = from_f32<T>(any ? exp2_of((to_f32(v.e[i]) - m) * c2) * qf : 0.0f);
+        if (vector_out && whole(u)) {
+          to[u] = v.all;
+        } else {
+#pragma unroll
+          for (int i = 0; i < kUnit; ++i) {
+            const int c = u * kUnit + i - lead;
+            if (c >= 0 && c < C) g[c] = v.e[i];
+          }
+        }
       }
       __syncthreads();
       if (any)
@@ -598,14 +638,15 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* block
   if (c <= 512) return launch_warps<T, 16, 32, 16, 0>(a, st, blocks);
   if (c <= 1024) return launch_warps<T, 32, 32, 16, 0>(a, st, blocks);
   if (c <= 1536 && a.t.k <= 64) return launch_warps<T, 32, 48, 32, 0>(a, st, blocks);
-  const size_t row = (c * sizeof(T) + 15) & ~(size_t)15;
+  const size_t row = (c * sizeof(T) + 47) & ~(size_t)15;  // a unit more where the row starts inside one
   const bool staged = row <= kRowSmem;
   if (staged && row > 32 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(k_distill_row<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)row);
     if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_row: %s", cudaGetErrorString(e));
   }
   *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
-  k_distill_row<T><<<*blocks, kRowThreads, staged ? row : 0, st>>>(a, staged);
+  const bool alike = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
+  k_distill_row<T><<<*blocks, kRowThreads, staged ? row : 0, st>>>(a, staged, alike);
   return check_launch("k_distill_row");
 }
 

@@ -126,6 +126,10 @@ def psnr(pred: torch.Tensor, target: torch.Tensor, max_val: float = 1.0) -> torc
     return 10.0 * torch.log10((max_val * max_val) / torch.clamp(mse, min=1e-12))
 
 
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    return t.detach() if t.requires_grad else t
+
+
 class _DistillArgs:
     """Checked arguments of one distillation call; keeps the tensors alive."""
 
@@ -170,17 +174,18 @@ class _DistillArgs:
             self.native = nat.GsTeacher(None, None, cache.records.data_ptr(), nat.ptr(teacher.rows), teacher.first,
                                         cache.num_rows, 0, cache.k, cache.bits)
         else:
-            self.values = nat.require_float("teacher values", teacher[0].detach())
+            self.values = nat.require_float("teacher values", _plain(teacher[0]))
             index = teacher[1]
             if index.dtype == torch.int64:  # out of int32's range is out of the classes' range
                 index = index.clamp(-1, 2**31 - 1)
             self.index = nat.require_cuda("teacher index", index, torch.int32)
             self.native = nat.GsTeacher(self.values.data_ptr(), self.index.data_ptr(), None, None, 0, 0,
                                         nat.DTYPES[self.values.dtype], self.values.shape[-1], 0)
-        self.weight = None if weight is None else nat.require_cuda("weight", weight.detach())
-        nat.same_device(dev, **{"teacher values": self.values, "teacher index": self.index,
-                                "the teacher cache": self.records, "teacher rows": self.row_ids,
-                                "weight": self.weight})
+        self.weight = None if weight is None else nat.require_cuda("weight", _plain(weight))
+        if self.records is None:
+            nat.same_device(dev, teacher_values=self.values, teacher_index=self.index, weight=self.weight)
+        else:
+            nat.same_device(dev, teacher=self.records, weight=self.weight)
         self.logits = logits
         self.lead = lead
         self.temperature = temperature
@@ -196,7 +201,7 @@ class _DistillArgs:
                 row_loss = torch.empty(self.lead, device=dev, dtype=torch.float32)
             else:
                 loss = torch.empty((), device=dev, dtype=torch.float32)
-                ws = torch.empty((nat.load().gs_distill_workspace_bytes(),), device=dev, dtype=torch.uint8)
+                ws = torch.empty((nat.distill_workspace_bytes(),), device=dev, dtype=torch.uint8)
         nat.call_on(dev, "gs_distill", nat.ptr(logits), nat.DTYPES[logits.dtype], self.rows, logits.shape[-1],
                     ctypes.byref(self.native), self.temperature, nat.ptr(self.weight), self.scale,
                     nat.ptr(cotangent), int(self.reduction == "none"), nat.ptr(row_loss), nat.ptr(loss),
@@ -248,7 +253,7 @@ def distill_loss_and_grad(logits: torch.Tensor, teacher, temperature: float = 1.
     """``distill_loss`` and its gradient with respect to ``logits`` (their shape and type) in one pass over the
     logits, outside autograd: hand the gradient on with ``logits.backward(grad)``.  With ``reduction="none"``
     each row's gradient is its own loss's."""
-    args = _DistillArgs(logits.detach() if isinstance(logits, torch.Tensor) else logits, teacher, temperature, weight,
+    args = _DistillArgs(_plain(logits) if isinstance(logits, torch.Tensor) else logits, teacher, temperature, weight,
                         reduction)
     grad = torch.empty_like(args.logits)
     loss = args.run(args.logits, grad=grad)

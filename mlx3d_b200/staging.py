@@ -156,7 +156,7 @@ class TeacherCache:
         start = int(start)
         if start < 0 or start + n > self.num_rows:
             raise ValueError(f"rows [{start}, {start + n}) are outside the cache of {self.num_rows} rows.")
-        logits = nat.require_float("logits", logits.detach())
+        logits = nat.require_float("logits", logits.detach() if logits.requires_grad else logits)
         nat.same_device(self.device, logits=logits)
         nat.call_on(self.device, "gs_teacher_write", nat.ptr(logits), nat.DTYPES[logits.dtype], n, self.num_classes,
                     nat.ptr(self.records), self.num_rows, start, self.k, self.bits)
