@@ -12,15 +12,13 @@
 //                   the teacher's few entries are worked on by one lane per row,
 //                   which needs no reductions (by the row's lanes, with one, they
 //                   were 60% of the instructions).
-//   k_distill_row   longer rows: one block per row, staged in shared memory while
-//                   it fits.
+//   k_distill_row   longer rows: one block per row.
 #include "feature_common.cuh"
 
 namespace gs {
 
 constexpr int kDistillMaxBlocks = 148 * 16;
-constexpr int kWarpBlock = 128, kRowThreads = 512;
-constexpr size_t kRowSmem = 200 * 1024;
+constexpr int kWarpBlock = 128, kRowThreads = 256;
 
 __device__ unsigned long long g_distill_wait_failures;
 
@@ -485,10 +483,11 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
 
 // One block per row.  A row starts anywhere; it is moved in 16-byte units of
 // memory, the first and last of which may reach outside it and are taken element
-// by element.  `staged`: the units are kept in shared memory, else read again.
+// by element.  Each of the three passes reads the row, the later ones from L2:
+// four blocks of 256 threads per SM that read again took 61 us for 1031 rows of
+// 32001, three of 512 that kept their row in shared memory 69 us.
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int staged, int vector_out) {
-  extern __shared__ __align__(128) uint8_t smem[];
+__global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int vector_out) {
   __shared__ float red[kRowThreads / 32], stats[2];
   __shared__ float2 ent[GS_TEACHER_MAX_K], fix[GS_TEACHER_MAX_K];
   constexpr int kUnit = 16 / sizeof(T);
@@ -497,7 +496,6 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
     T e[kUnit];
   };
   const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Unit* kept = reinterpret_cast<Unit*>(smem);
   const float c2 = a.inv_temp * kLog2e;
   double acc = 0.0;
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
@@ -524,7 +522,6 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
 #pragma unroll 4
     for (int u = threadIdx.x; u < units; u += kRowThreads) {
       const Unit v = read(u);
-      if (staged) kept[u] = v;
 #pragma unroll
       for (int i = 0; i < kUnit; ++i) m = fmaxf(m, to_f32(v.e[i]));
     }
@@ -536,7 +533,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
     float sum = 0.0f;
 #pragma unroll 2
     for (int u = threadIdx.x; u < units; u += kRowThreads) {
-      const Unit v = staged ? kept[u] : read(u);
+      const Unit v = read(u);
 #pragma unroll
       for (int i = 0; i < kUnit; ++i) sum += exp2_of((to_f32(v.e[i]) - m) * c2);
     }
@@ -570,7 +567,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
 #pragma unroll 2
       for (int u = threadIdx.x; u < units; u += kRowThreads) {
         Unit v;
-        if (any) v = staged ? kept[u] : read(u);
+        if (any) v = read(u);
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) v.e[i] = from_f32<T>(any ? exp2_of((to_f32(v.e[i]) - m) * c2) * qf : 0.0f);
         if (vector_out && whole(u)) {
@@ -638,15 +635,9 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* block
   if (c <= 512) return launch_warps<T, 16, 32, 16, 0>(a, st, blocks);
   if (c <= 1024) return launch_warps<T, 32, 32, 16, 0>(a, st, blocks);
   if (c <= 1536 && a.t.k <= 64) return launch_warps<T, 32, 48, 32, 0>(a, st, blocks);
-  const size_t row = (c * sizeof(T) + 47) & ~(size_t)15;  // a unit more where the row starts inside one
-  const bool staged = row <= kRowSmem;
-  if (staged && row > 32 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(k_distill_row<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)row);
-    if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_row: %s", cudaGetErrorString(e));
-  }
   *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
   const bool alike = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
-  k_distill_row<T><<<*blocks, kRowThreads, staged ? row : 0, st>>>(a, staged, alike);
+  k_distill_row<T><<<*blocks, kRowThreads, 0, st>>>(a, alike);
   return check_launch("k_distill_row");
 }
 

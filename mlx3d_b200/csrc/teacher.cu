@@ -298,36 +298,47 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_teacher_write_warp(Teacher
   if (r >= a.n) return;
   const int C = (int)a.classes, k = a.k;
   const T* s = static_cast<const T*>(a.logits) + r * C;
-  W top = 0;  // largest key of this lane
+  const float low = lowest_of<T>();
+  // Values decide until a class is taken: its key is made then.
+  auto value_at = [&](int c) {
+    const float v = to_f32(s[c]);
+    return v > low && v < INFINITY ? v : -INFINITY;
+  };
+  float top = -INFINITY;  // largest of this lane
 #pragma unroll 8
-  for (int c = lane; c < C; c += 32) {
-    const W w = K::make(s[c], c);
-    top = w > top ? w : top;
-  }
-  // At least k keys reach the k-th largest of the lanes' largest.
-  W bound = K::shuffle(warp_sort<K>(top, lane), k - 1);
-  if (bound == 0) bound = 1;  // fewer than k lanes have a class at all
+  for (int c = lane; c < C; c += 32) top = fmaxf(top, value_at(c));
+  // At least k classes reach the k-th largest of the lanes' largest.
+#pragma unroll
+  for (int j = 2; j <= 32; j *= 2)
+#pragma unroll
+    for (int d = j / 2; d >= 1; d /= 2) {
+      const float o = __shfl_xor_sync(~0u, top, d);
+      top = ((lane & j) == 0) == ((lane & d) == 0) ? fmaxf(top, o) : fminf(top, o);
+    }
+  float bound = __shfl_sync(~0u, top, k - 1);  // -inf: fewer than k lanes have a class at all
   W best = 0;
   int held = 0;
   W* queue = pending[warp];
   for (int c0 = 0; c0 < C; c0 += 32 * 4) {
-    W w[4];
+    float v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int c = c0 + 32 * q + lane;
-      w[q] = c < C ? K::make(s[c], c) : 0;
+      v[q] = c < C ? value_at(c) : -INFINITY;
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const unsigned take = __ballot_sync(~0u, w[q] >= bound);
+      const bool mine = v[q] >= bound && v[q] != -INFINITY;
+      const unsigned take = __ballot_sync(~0u, mine);
       if (take == 0) continue;
-      if (w[q] >= bound) queue[held + __popc(take & ((1u << lane) - 1))] = w[q];
+      const int c = c0 + 32 * q + lane;
+      if (mine) queue[held + __popc(take & ((1u << lane) - 1))] = K::make(s[c], c);
       held += __popc(take);
       __syncwarp();
       if (held >= 32) {  // held is the same in every lane
         best = warp_merge<K>(best, warp_sort<K>(queue[lane], lane), lane);
         const W kth = K::shuffle(best, k - 1);
-        if (kth >= bound) bound = kth + 1;  // keys are all different
+        if (kth != 0) bound = fmaxf(bound, K::value(kth));  // (equal values are sorted out by their keys)
         const W rest = lane < held - 32 ? queue[32 + lane] : 0;
         __syncwarp();
         queue[lane] = rest;
