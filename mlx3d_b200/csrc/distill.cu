@@ -321,11 +321,12 @@ __host__ __device__ inline size_t warp_smem(int rows, int64_t classes, int elem,
   return kWarpBuffers * warp_tile_bytes(rows, classes, elem) + (((size_t)rows * (16 * k + sizeof(RowState)) + 127) & ~(size_t)127);
 }
 
-// G lanes share a row, each holding EACH of its logits, G apart, in registers; the
-// first FULL of them exist for sure.  With KEEP the exponentials of all rows of the
+// G lanes share a row, each holding EACH of its logits in registers, as pairs of
+// neighbours (PAIRS: rows are a whole number of pairs) or G apart; the first FULL of
+// them exist for sure.  With KEEP the exponentials of all rows of the
 // tile (KEEP rounds of 32 / G rows) stay in registers for the gradient; otherwise
 // they are computed again.
-template <typename T, int G, int EACH, int FULL, int KEEP>
+template <typename T, int G, int EACH, int FULL, int KEEP, bool PAIRS>
 __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int tile_rows, int bulk_in, int bulk_out) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ unsigned long long bars[kWarpBlock / 32][kWarpBuffers];
@@ -384,24 +385,46 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
     __syncwarp();
     // the student's maximum and sum, by the rows' lanes
     constexpr int kRounds = KEEP > 0 ? KEEP : 1;
-    float kept[kRounds][EACH];
-    auto exponentials = [&](int rr, float(&v)[EACH]) {
+    F2 kept[kRounds][EACH / 2];
+    // the two classes of a lane's pair i
+    auto first_of = [&](int i) { return PAIRS ? 2 * (lane + G * i) : lane + G * 2 * i; };
+    constexpr int kApart = PAIRS ? 1 : G;
+    auto read = [&](const T* s, int i, float none) {
+      const int c = first_of(i);
+      if constexpr (PAIRS) {
+        return 2 * i + 1 < FULL || c < C ? load_pair(s + c) : f2(none);
+      } else {
+        return f2(2 * i < FULL || c < C ? to_f32(s[c]) : none,
+                  2 * i + 1 < FULL || c + kApart < C ? to_f32(s[c + kApart]) : none);
+      }
+    };
+    auto scaled = [&](F2 v, float m) {  // exp((v - m) / T)
+      float x, y;
+      split(mul(add(v, f2(-m)), f2(c2)), x, y);
+      return f2(exp2_of(x), exp2_of(y));
+    };
+    auto exponentials = [&](int rr, F2(&v)[EACH / 2]) {
       const bool live = rr + group < rows;
       const int r = live ? rr + group : rows - 1;
-      const T* s = tile + r * C + lane;
-      float m = -INFINITY, sum = 0.0f;
+      const T* s = tile + r * C;
+      float m = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        v[i] = i < FULL || lane + G * i < C ? to_f32(s[G * i]) : -INFINITY;
-        m = fmaxf(m, v[i]);
+      for (int i = 0; i < EACH / 2; ++i) {
+        v[i] = read(s, i, -INFINITY);
+        float x, y;
+        split(v[i], x, y);
+        m = fmaxf(m, fmaxf(x, y));
       }
       m = group_max<G>(m);
+      F2 sums = f2(0.0f);
 #pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        v[i] = i < FULL || lane + G * i < C ? exp2_of((v[i] - m) * c2) : 0.0f;
-        sum += v[i];
+      for (int i = 0; i < EACH / 2; ++i) {
+        v[i] = scaled(v[i], m);  // (0 where there is no class: m is finite, or the row is NaN)
+        sums = add(sums, v[i]);
       }
-      sum = group_sum<G>(sum);
+      float x, y;
+      split(sums, x, y);
+      const float sum = group_sum<G>(x + y);
       if (lane == 0 && live) {
         state[r].m = m;
         state[r].inv = rcp_of(sum);
@@ -427,21 +450,24 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
     }
     if (a.grad) {
       __syncwarp();
-      auto gradients = [&](int rr, const float(&v)[EACH]) {
+      auto gradients = [&](int rr, const F2(&v)[EACH / 2]) {
         const int r = rr + group;
         if (r >= rows) return;
         const RowState st = state[r];
-        T* s = tile + r * C + lane;
-        const float f = st.inv * st.factor;
-        if (st.any) {
+        T* s = tile + r * C;
+        const F2 f = f2(st.inv * st.factor);
 #pragma unroll
-          for (int i = 0; i < EACH; ++i)
-            if (i < FULL || lane + G * i < C)
-              s[G * i] = from_f32<T>((KEEP > 0 ? v[i] : exp2_of((to_f32(s[G * i]) - st.m) * c2)) * f);
-        } else {
-#pragma unroll
-          for (int i = 0; i < EACH; ++i)
-            if (i < FULL || lane + G * i < C) s[G * i] = from_f32<T>(0.0f);
+        for (int i = 0; i < EACH / 2; ++i) {
+          const int c = first_of(i);
+          const F2 g = st.any ? mul(KEEP > 0 ? v[i] : scaled(read(s, i, 0.0f), st.m), f) : f2(0.0f);
+          if constexpr (PAIRS) {
+            if (2 * i + 1 < FULL || c < C) store_pair(s + c, g);
+          } else {
+            float x, y;
+            split(g, x, y);
+            if (2 * i < FULL || c < C) s[c] = from_f32<T>(x);
+            if (2 * i + 1 < FULL || c + kApart < C) s[c + kApart] = from_f32<T>(y);
+          }
         }
       };
       if constexpr (KEEP > 0) {
@@ -611,7 +637,9 @@ static int launch_warps(const DistillArgs& a, cudaStream_t st, unsigned* blocks)
   int warps = kWarpBlock / 32;
   while (warps > 1 && own * warps > 100 * 1024) warps /= 2;
   const size_t smem = own * warps;
-  auto* kernel = k_distill_warp<T, G, EACH, FULL, KEEP>;
+  // (tiles start on 128 bytes, and a row of an even number of classes on a pair)
+  auto* kernel = a.classes % 2 == 0 ? k_distill_warp<T, G, EACH, FULL, KEEP, true>
+                                    : k_distill_warp<T, G, EACH, FULL, KEEP, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_warp: %s", cudaGetErrorString(e));
   const int64_t resident = 148 * std::max<int64_t>(1, std::min<int64_t>(16, (227 * 1024) / (int64_t)(smem + 1024)));

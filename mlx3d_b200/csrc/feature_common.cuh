@@ -35,6 +35,57 @@ __device__ __forceinline__ float lowest_of<__half>() { return -65504.0f; }
 template <>
 __device__ __forceinline__ float lowest_of<__nv_bfloat16>() { return __uint_as_float(0xff7f0000u); }
 
+// Pairs of float32 values in 64-bit registers: sm_100 multiplies and adds two at
+// once.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(uint32_t lo, uint32_t hi) { return f2(__uint_as_float(lo), __uint_as_float(hi)); }
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ void split(F2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Two neighbouring elements (p aligned to both) as floats, and back.
+__device__ __forceinline__ F2 load_pair(const float* p) { return *reinterpret_cast<const F2*>(p); }
+__device__ __forceinline__ F2 load_pair(const __half* p) {
+  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(p));
+  return f2(v.x, v.y);
+}
+__device__ __forceinline__ F2 load_pair(const __nv_bfloat16* p) {
+  const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+  return f2(w << 16, w & 0xffff0000u);
+}
+__device__ __forceinline__ void store_pair(float* p, F2 v) { *reinterpret_cast<F2*>(p) = v; }
+__device__ __forceinline__ void store_pair(__half* p, F2 v) {
+  float lo, hi;
+  split(v, lo, hi);
+  *reinterpret_cast<__half2*>(p) = __floats2half2_rn(lo, hi);
+}
+__device__ __forceinline__ void store_pair(__nv_bfloat16* p, F2 v) {
+  float lo, hi;
+  split(v, lo, hi);
+  *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(lo, hi);
+}
+
 inline int elem_size(int dtype) { return dtype == GS_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == GS_F32 || dtype == GS_F16 || dtype == GS_BF16; }
 
