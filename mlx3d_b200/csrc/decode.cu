@@ -278,15 +278,9 @@ __device__ __forceinline__ void fetch_panels(uint8_t* panels, const CUtensorMap*
                                              unsigned long long* bar) {
   for (int p = 0; p < count; ++p) fetch_panel(panels + p * kPanel, map, p * 64, row, bar);
 }
-// Into L2 only.
-__device__ __forceinline__ void prefetch_panels(const CUtensorMap* map, int count, int row) {
-  for (int p = 0; p < count; ++p)
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(map), "r"(p * 64), "r"(row)
-                 : "memory");
-}
 
 // One lane's loop over this CTA's tiles.
-template <bool DY, bool PREFETCH>
+template <bool DY>
 __device__ __forceinline__ void fetch_inputs(const DecodeArgs& a, Bars* b, uint8_t* stages, int stage_bytes,
                                              int64_t first, int64_t step, int64_t tiles) {
   Ring fill;
@@ -297,10 +291,6 @@ __device__ __forceinline__ void fetch_inputs(const DecodeArgs& a, Bars* b, uint8
     mbar_arrive_expect_tx(full, stage_bytes);
     fetch_panels(xs, &a.map_x, a.nxp, (int)(t * kTile), full);
     if (DY) fetch_panels(xs + a.nxp * kPanel, &a.map_dy, a.nyp, (int)(t * kTile), full);
-    if (PREFETCH && t + step < tiles) {  // the next stage is free only when its tile is needed
-      prefetch_panels(&a.map_x, a.nxp, (int)((t + step) * kTile));
-      if (DY) prefetch_panels(&a.map_dy, a.nyp, (int)((t + step) * kTile));
-    }
     fill.next(a.x_stages);
   }
 }
@@ -408,7 +398,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
   const bool resident = a.w_stages >= a.chunks;
 
   if (warp == 3) {
-    if (lane == 0 && resident) fetch_inputs<MODE != kFwd, false>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+    if (lane == 0 && resident) fetch_inputs<MODE != kFwd>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && resident) {
@@ -743,7 +733,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
   const int64_t mine = (tiles - blockIdx.x + gridDim.x - 1) / gridDim.x;
 
   if (warp == 1) {
-    if (lane == 0) fetch_inputs<true, true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
+    if (lane == 0) fetch_inputs<true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
     __syncwarp();
   } else if (warp == 0) {
     {
@@ -797,20 +787,35 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
       if (ok) dh_products();
       const uint32_t tgu = tc::uniform(tmem + col_gu), tdd = tc::uniform(tmem + col_dd);
       for (int64_t i = 0; i < mine && ok; ++i) {
-        // The next tile's first products go before this one's sums if its inputs are there.
-        const bool ahead = i + 1 < mine && nbuf == 2 && __all_sync(~0u, passed(&b->xfull[xg.at], xg.parity));
-        if (ahead) gu_products();
-        // tile i's g, u and dh have been read
+        // The next tile's first products go before this one's sums as soon as its
+        // inputs are there: [g | u] at once with two buffers, else, like dh, when
+        // this tile's have been read.
+        const bool more_tiles = i + 1 < mine;
+        auto ready = [&]() { return more_tiles && __all_sync(~0u, passed(&b->xfull[xg.at], xg.parity)); };
+        bool ahead = false;
+        if (nbuf == 2 && ready()) {
+          gu_products();
+          ahead = true;
+        }
         ok &= wait_for(b, &b->dhread, (unsigned)i & 1);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
+        if (!ahead && ready()) {
+          gu_products();
+          ahead = true;
+        }
         if (ahead) dh_products();
         // its panels are written
         ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         tc::fence_after();
+        if (!ahead && ready()) {
+          gu_products();
+          dh_products();
+          ahead = true;
+        }
         const uint32_t xd = tc::uniform(xn0 + xs.at * xstep), yd = xd + ypart;
         const bool more = __all_sync(~0u, i > 0);
         if (tc::elect_one()) {
@@ -832,7 +837,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
         }
         __syncwarp();
         xs.next(a.x_stages);
-        if (!ahead && i + 1 < mine) {
+        if (!ahead && more_tiles) {
           gu_products();
           if (ok) dh_products();
         }
@@ -864,6 +869,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
         }
         v.template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
       }
+      // the previous tile's sums have read the panels
       if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
       if (!ok) break;
 #pragma unroll
