@@ -240,11 +240,13 @@ int gs_bin_end(const float* means2d, const float* radii, int64_t n, int64_t d, i
 
 /* Bounded device-side waits: the radix passes and the offsets scan of
  * gs_bin_begin / gs_bin_end (blocks wait for earlier blocks' counts) and the
- * bulk (TMA) staging of gs_preprocess_forward / _backward (threads wait for
- * the copy engine).  A wait that runs out leaves that block's output
- * unwritten and is counted on the device; this reads the total for the
- * current device (synchronous; reset != 0 clears it).  Always 0 unless a
- * GPU stalls for far longer than a kernel takes.  No counterpart in the
+ * bulk (TMA) staging of gs_preprocess_forward / _backward, gs_distill,
+ * gs_teacher_write and gs_decode_forward / _backward (threads wait for the
+ * copy engine, in the decoder also for the tensor core and for each other).
+ * A wait that runs out leaves that block's output unwritten and is counted on
+ * the device; this reads the total for the current device (synchronous; reset
+ * != 0 clears it).  Always 0 unless a GPU stalls for far longer than a kernel
+ * takes.  No counterpart in the
  * reference (its sort is mx.argsort; MLX stages nothing). */
 int gs_wait_failures(uint64_t* count, int reset);
 
@@ -429,6 +431,7 @@ typedef struct gs_teacher {
   int32_t k;    /* 1 .. GS_TEACHER_MAX_K (arrays), 1 .. GS_CACHE_MAX_K (cache) */
   int32_t bits; /* 8 or 4: cache; 0: arrays */
 } gs_teacher;
+#define GS_DISTILL_MAX_CLASSES 2147483631
 #define GS_TEACHER_MAX_K 256
 #define GS_CACHE_MAX_K 32
 #define GS_CACHE_MAX_CLASSES 32767

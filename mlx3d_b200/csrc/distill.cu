@@ -9,9 +9,10 @@
 //                   and stored by bulk copies, with no block barrier; dozens of
 //                   warps per SM overlap their copies with each other's
 //                   arithmetic.  The classes of a row are shared by 4 to 32 lanes;
-//                   the teacher's few entries are worked on by one lane per row,
-//                   which needs no reductions (by the row's lanes, with one, they
-//                   were 60% of the instructions).
+//                   the teacher's few entries by as many as make the tile's rows a
+//                   whole warp.  Instructions bound it: 1920x1080x150 in float32
+//                   takes 466 us (67% of DRAM's rate), with one lane per row for
+//                   the entries (8 of 32 busy) 536.
 //   k_distill_row   longer rows: one block per row.
 #include "feature_common.cuh"
 
@@ -208,10 +209,13 @@ struct RowState {
   float lse;
 };
 
-// The teacher's softmax of one row by one lane: entries (index, z) -> (index, p).
-// Up to MAX entries, in registers (MAX = 0: any number, through memory).
-template <int MAX>
-__device__ __forceinline__ void teacher_row(float2* ent, int k, float inv_temp, RowState& st) {
+// Over the L neighbouring lanes that share a row's entries; lane `sub` of them has
+// entries sub, sub + L, ...: with MAX > 0 up to MAX of them, in registers, otherwise
+// any number, through memory.
+//
+// The teacher's softmax of one row: entries (index, z) -> (index, p).
+template <int L, int MAX>
+__device__ __forceinline__ void teacher_row(float2* ent, int k, int sub, float inv_temp, RowState& st) {
   const float c2 = inv_temp * kLog2e;
   float zmax = -INFINITY, tot = 0.0f, sum = 0.0f;
   bool any = false, twice = false;
@@ -219,29 +223,41 @@ __device__ __forceinline__ void teacher_row(float2* ent, int k, float inv_temp, 
     int idx[MAX];
     float z[MAX];
 #pragma unroll
-    for (int e = 0; e < MAX; ++e) {
+    for (int i = 0; i < MAX; ++i) {
+      const int e = sub + L * i;
       const float2 v = e < k ? ent[e] : make_float2(__int_as_float(-1), -INFINITY);
-      idx[e] = __float_as_int(v.x);
-      z[e] = v.y;
+      idx[i] = __float_as_int(v.x);
+      z[i] = v.y;
       zmax = fmaxf(zmax, v.y);
-      any |= idx[e] >= 0;
+      any |= idx[i] >= 0;
+      idx[i] = idx[i] >= 0 ? idx[i] : -1 - e;  // absent entries differ from each other
 #pragma unroll
-      for (int j = 0; j < e; ++j) twice |= idx[e] == idx[j] && idx[e] >= 0;
+      for (int j = 0; j < i; ++j) twice |= idx[i] == idx[j];
     }
 #pragma unroll
-    for (int e = 0; e < MAX; ++e) {
-      const float d = z[e] - zmax;
-      z[e] = idx[e] >= 0 ? exp2_of(d * c2) : 0.0f;
-      if (z[e] != 0.0f) sum += z[e] * (d * inv_temp);
-      tot += z[e];
+    for (int d = 1; d < L; ++d)
+#pragma unroll
+      for (int i = 0; i < MAX; ++i) {
+        const int other = __shfl_xor_sync(~0u, idx[i], d);
+#pragma unroll
+        for (int j = 0; j < MAX; ++j) twice |= other == idx[j];
+      }
+    zmax = group_max<L>(zmax);
+#pragma unroll
+    for (int i = 0; i < MAX; ++i) {
+      const float d = z[i] - zmax;
+      z[i] = idx[i] >= 0 ? exp2_of(d * c2) : 0.0f;
+      if (z[i] != 0.0f) sum += z[i] * (d * inv_temp);
+      tot += z[i];
     }
+    tot = group_sum<L>(tot);
     const float inv = rcp_of(tot);
 #pragma unroll
-    for (int e = 0; e < MAX; ++e)
-      if (e < k) ent[e].y = z[e] * inv;
-    sum *= inv;
+    for (int i = 0; i < MAX; ++i)
+      if (sub + L * i < k) ent[sub + L * i].y = z[i] * inv;
+    sum = group_sum<L>(sum) * inv;
   } else {
-    for (int e = 0; e < k; ++e) {
+    for (int e = sub; e < k; e += L) {
       const float2 v = ent[e];
       const int idx = __float_as_int(v.x);
       zmax = fmaxf(zmax, v.y);
@@ -249,7 +265,8 @@ __device__ __forceinline__ void teacher_row(float2* ent, int k, float inv_temp, 
       if (idx >= 0)
         for (int j = 0; j < e; ++j) twice |= __float_as_int(ent[j].x) == idx;
     }
-    for (int e = 0; e < k; ++e) {
+    zmax = group_max<L>(zmax);
+    for (int e = sub; e < k; e += L) {
       const float2 v = ent[e];
       float x = 0.0f;
       if (__float_as_int(v.x) >= 0) {
@@ -260,26 +277,31 @@ __device__ __forceinline__ void teacher_row(float2* ent, int k, float inv_temp, 
       tot += x;
       ent[e].y = x;
     }
+    tot = group_sum<L>(tot);
     const float inv = rcp_of(tot);
-    for (int e = 0; e < k; ++e) ent[e].y *= inv;
-    sum *= inv;
+    for (int e = sub; e < k; e += L) ent[e].y *= inv;
+    sum = group_sum<L>(sum) * inv;
   }
-  st.any = any;
-  st.repeats = twice;
+  int found = (any ? 1 : 0) | (twice ? 2 : 0);
+#pragma unroll
+  for (int o = L / 2; o; o >>= 1) found |= __shfl_xor_sync(~0u, found, o);
+  st.any = found & 1;
+  st.repeats = found & 2;
   st.term = sum - ln_of(tot);  // sum_k p_k log p_k
 }
 
-// sum_k p_k (s_k - m) / T of a row by one lane, and the gradients of the teacher's
-// classes (unless fix is NULL): the first entry of a class holds (class, factor *
-// (q - sum of the class's p)), every other one (-1, -).
-template <int MAX, typename T>
-__device__ __forceinline__ float class_row(const T* s, const float2* ent, float2* fix, int k, float inv_temp,
+// sum_k p_k (s_k - m) / T of a row, this lane's part, and the gradients of the
+// teacher's classes (unless fix is NULL): the first entry of a class holds (class,
+// factor * (q - sum of the class's p)), every other one (-1, -).
+template <int L, int MAX, typename T>
+__device__ __forceinline__ float class_row(const T* s, const float2* ent, float2* fix, int k, int sub, float inv_temp,
                                            const RowState& st) {
   const float c2 = inv_temp * kLog2e;
   float cross = 0.0f;
 #pragma unroll MAX > 0 ? MAX : 1
-  for (int e = 0; e < (MAX > 0 ? MAX : k); ++e) {
-    if (MAX > 0 && e >= k) break;
+  for (int i = 0; i < (MAX > 0 ? MAX : k); ++i) {
+    const int e = sub + L * i;
+    if (e >= k) break;
     const float2 v = ent[e];
     const int idx = __float_as_int(v.x);
     int to = -1;
@@ -314,6 +336,9 @@ __device__ __forceinline__ float class_row(const T* s, const float2* ent, float2
 
 // Shared memory of a warp: two tiles, then entries, fixes, row states.
 constexpr int kWarpBuffers = 2;
+// Rows of a tile whose exponentials are not kept (all tiles have a multiple of 8
+// rows, which is one of 16 bytes).
+constexpr int kTileRows = 8;
 __host__ __device__ inline size_t warp_tile_bytes(int rows, int64_t classes, int elem) {
   return ((size_t)rows * classes * elem + 127) & ~(size_t)127;
 }
@@ -322,12 +347,16 @@ __host__ __device__ inline size_t warp_smem(int rows, int64_t classes, int elem,
 }
 
 // G lanes share a row, each holding EACH of its logits in registers, as pairs of
-// neighbours (PAIRS: rows are a whole number of pairs) or G apart; the first FULL of
-// them exist for sure.  With KEEP the exponentials of all rows of the
+// neighbours; the first FULL of them exist for sure.  Pairs are aligned: with an ODD
+// number of classes every second row starts inside one, and shares its first and last
+// pair with the rows beside it.  With KEEP the exponentials of all rows of the
 // tile (KEEP rounds of 32 / G rows) stay in registers for the gradient; otherwise
 // they are computed again.
-template <typename T, int G, int EACH, int FULL, int KEEP, bool PAIRS>
-__global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int tile_rows, int bulk_in, int bulk_out) {
+template <typename T, int G, int EACH, int FULL, int KEEP, bool ODD>
+__global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int bulk_in, int bulk_out) {
+  constexpr int tile_rows = KEEP > 0 ? KEEP * (32 / G) : kTileRows;
+  // lanes per row for the teacher's entries, and entries of a lane where k <= 8
+  constexpr int L = tile_rows >= 32 ? 1 : 32 / tile_rows, kFew = 8 / L;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ unsigned long long bars[kWarpBlock / 32][kWarpBuffers];
   const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, wl = threadIdx.x & 31;
@@ -362,20 +391,29 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
     T* tile = reinterpret_cast<T*>(own + buf * tile_bytes);
     stage_entries<32>(a, ents, r0, rows, wl);
     __syncwarp();
-    for (int r = wl; r < rows; r += 32) {
+    const int sub = wl % L;
+    for (int rr = 0; rr < rows; rr += 32 / L) {
+      const int r = rr + wl / L;
+      if (L == 1 && r >= rows) break;
+      const int held = L == 1 || r < rows ? k : 0;  // (every lane takes part in the exchanges)
       RowState st;
-      st.weight = a.weight ? a.weight[r0 + r] : 1.0f;
-      st.factor = st.weight * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r0 + r : 0] : 1.0f);
-      if (k <= 8) teacher_row<8>(ents + r * k, k, a.inv_temp, st);
-      else teacher_row<0>(ents + r * k, k, a.inv_temp, st);
-      state[r] = st;
+      st.weight = a.weight && r < rows ? a.weight[r0 + r] : 1.0f;
+      st.factor = st.weight * a.grad_scale * (a.cot && r < rows ? a.cot[a.cot_per_row ? r0 + r : 0] : 1.0f);
+      if (k <= 8) teacher_row<L, kFew>(ents + r * k, held, sub, a.inv_temp, st);
+      else teacher_row<L, 0>(ents + r * k, held, sub, a.inv_temp, st);
+      if (sub == 0 && r < rows) state[r] = st;
     }
     if (wl == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the last tile has left
     __syncwarp();
     if (t + step < tiles) fetch(t + step, buf ^ 1);
     if (bulk_in && whole) {
       if (!__all_sync(~0u, mbar_wait(&bars[warp][buf], phase))) {
-        if (wl == 0) atomicAdd(&g_distill_wait_failures, 1ull);
+        // copies in flight must end before the block does (bounded)
+        if (wl == 0) {
+          atomicAdd(&g_distill_wait_failures, 1ull);
+          mbar_wait(&bars[warp][buf], phase);
+        }
+        if (wl == 0 && t + step < tiles) mbar_wait(&bars[warp][buf ^ 1], buf ? phase ^ 1 : phase);
         break;
       }
     } else {
@@ -386,16 +424,19 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
     // the student's maximum and sum, by the rows' lanes
     constexpr int kRounds = KEEP > 0 ? KEEP : 1;
     F2 kept[kRounds][EACH / 2];
-    // the two classes of a lane's pair i
-    auto first_of = [&](int i) { return PAIRS ? 2 * (lane + G * i) : lane + G * 2 * i; };
-    constexpr int kApart = PAIRS ? 1 : G;
-    auto read = [&](const T* s, int i, float none) {
-      const int c = first_of(i);
-      if constexpr (PAIRS) {
-        return 2 * i + 1 < FULL || c < C ? load_pair(s + c) : f2(none);
+    // the first class of a lane's pair i; -1 for the first pair of a row that starts inside it
+    auto first_of = [&](int i, int lead) { return 2 * (lane + G * i) - lead; };
+    auto lead_of = [&](int r) { return ODD ? r & 1 : 0; };
+    auto read = [&](const T* s, int i, int lead, float none) {
+      const int c = first_of(i, lead);
+      if constexpr (ODD) {
+        if (i > 0 && 2 * i + 1 < FULL) return load_pair(s + c);
+        if (c >= C) return f2(none);
+        float x, y;
+        split(load_pair(s + c), x, y);
+        return f2(i > 0 || c >= 0 ? x : none, 2 * i + 1 < FULL || c + 1 < C ? y : none);
       } else {
-        return f2(2 * i < FULL || c < C ? to_f32(s[c]) : none,
-                  2 * i + 1 < FULL || c + kApart < C ? to_f32(s[c + kApart]) : none);
+        return 2 * i + 1 < FULL || c < C ? load_pair(s + c) : f2(none);
       }
     };
     auto scaled = [&](F2 v, float m) {  // exp((v - m) / T)
@@ -410,7 +451,7 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
       float m = -INFINITY;
 #pragma unroll
       for (int i = 0; i < EACH / 2; ++i) {
-        v[i] = read(s, i, -INFINITY);
+        v[i] = read(s, i, lead_of(r), -INFINITY);
         float x, y;
         split(v[i], x, y);
         m = fmaxf(m, fmaxf(x, y));
@@ -438,15 +479,21 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
       for (int rr = 0; rr < rows; rr += 32 / G) exponentials(rr, kept[0]);
     }
     __syncwarp();
-    // the loss and the gradients of the teacher's classes, by one lane per row
-    for (int r = wl; r < rows; r += 32) {
-      const RowState st = state[r];
+    // the loss and the gradients of the teacher's classes
+    for (int rr = 0; rr < rows; rr += 32 / L) {
+      const int r = rr + wl / L;
+      if (L == 1 && r >= rows) break;
+      const int held = L == 1 || r < rows ? k : 0;
+      const RowState st = state[L == 1 ? r : min(r, rows - 1)];
       float2* fix = a.grad ? fixes + r * k : nullptr;
-      const float cross = k <= 8 ? class_row<8>(tile + r * C, ents + r * k, fix, k, a.inv_temp, st)
-                                 : class_row<0>(tile + r * C, ents + r * k, fix, k, a.inv_temp, st);
-      const float loss = st.any ? (st.term - cross + st.lse) * (a.temp * a.temp) * st.weight : 0.0f;
-      if (a.row_loss) a.row_loss[r0 + r] = loss;
-      acc += (double)loss;
+      float cross = k <= 8 ? class_row<L, kFew>(tile + r * C, ents + r * k, fix, held, sub, a.inv_temp, st)
+                           : class_row<L, 0>(tile + r * C, ents + r * k, fix, held, sub, a.inv_temp, st);
+      cross = group_sum<L>(cross);
+      if (sub == 0 && r < rows) {
+        const float loss = st.any ? (st.term - cross + st.lse) * (a.temp * a.temp) * st.weight : 0.0f;
+        if (a.row_loss) a.row_loss[r0 + r] = loss;
+        acc += (double)loss;
+      }
     }
     if (a.grad) {
       __syncwarp();
@@ -456,17 +503,22 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
         const RowState st = state[r];
         T* s = tile + r * C;
         const F2 f = f2(st.inv * st.factor);
+        const int lead = lead_of(r);
 #pragma unroll
         for (int i = 0; i < EACH / 2; ++i) {
-          const int c = first_of(i);
-          const F2 g = st.any ? mul(KEEP > 0 ? v[i] : scaled(read(s, i, 0.0f), st.m), f) : f2(0.0f);
-          if constexpr (PAIRS) {
-            if (2 * i + 1 < FULL || c < C) store_pair(s + c, g);
+          const int c = first_of(i, lead);
+          const F2 g = st.any ? mul(KEEP > 0 ? v[i] : scaled(read(s, i, lead, 0.0f), st.m), f) : f2(0.0f);
+          if constexpr (ODD) {
+            const bool low = i > 0 || c >= 0, high = 2 * i + 1 < FULL || c + 1 < C;
+            if (low && high) {
+              store_pair(s + c, g);
+            } else if (c < C) {  // the other half is a neighbouring row's
+              float x, y;
+              split(g, x, y);
+              s[low ? c : c + 1] = from_f32<T>(low ? x : y);
+            }
           } else {
-            float x, y;
-            split(g, x, y);
-            if (2 * i < FULL || c < C) s[c] = from_f32<T>(x);
-            if (2 * i + 1 < FULL || c + kApart < C) s[c + kApart] = from_f32<T>(y);
+            if (2 * i + 1 < FULL || c < C) store_pair(s + c, g);
           }
         }
       };
@@ -628,23 +680,20 @@ __global__ void k_distill_finish(const double* partials, int n, double scale, fl
   if (threadIdx.x == 0) *loss = (float)(part[0] * scale);
 }
 
-// The warps' tiles: a multiple of 8 rows, which is one of 16 bytes.
 template <typename T, int G, int EACH, int FULL, int KEEP>
 static int launch_warps(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
-  int64_t rows = 8;
-  if (KEEP > 0) rows = KEEP * (32 / G);
+  const int64_t rows = KEEP > 0 ? KEEP * (32 / G) : kTileRows;
   const size_t own = warp_smem((int)rows, a.classes, sizeof(T), a.t.k);
   int warps = kWarpBlock / 32;
   while (warps > 1 && own * warps > 100 * 1024) warps /= 2;
   const size_t smem = own * warps;
-  // (tiles start on 128 bytes, and a row of an even number of classes on a pair)
-  auto* kernel = a.classes % 2 == 0 ? k_distill_warp<T, G, EACH, FULL, KEEP, true>
-                                    : k_distill_warp<T, G, EACH, FULL, KEEP, false>;
+  auto* kernel = a.classes % 2 ? k_distill_warp<T, G, EACH, FULL, KEEP, true>
+                               : k_distill_warp<T, G, EACH, FULL, KEEP, false>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_warp: %s", cudaGetErrorString(e));
   const int64_t resident = 148 * std::max<int64_t>(1, std::min<int64_t>(16, (227 * 1024) / (int64_t)(smem + 1024)));
   *blocks = (unsigned)std::min<int64_t>(ceil_div(ceil_div(a.n, rows), warps), resident);
-  kernel<<<*blocks, warps * 32, smem, st>>>(a, (int)rows, aligned(a.logits, 16), aligned(a.grad, 16));
+  kernel<<<*blocks, warps * 32, smem, st>>>(a, aligned(a.logits, 16), aligned(a.grad, 16));
   return check_launch("k_distill_warp");
 }
 
@@ -683,8 +732,9 @@ int gs_distill(const void* logits, int dtype, int64_t n, int64_t classes, const 
                size_t workspace_bytes, void* stream) {
   clear_error();
   if (!dtype_ok(dtype)) return set_error(GS_ERR_INVALID_ARG, "gs_distill: unknown dtype %d", dtype);
-  if (n < 0 || classes < 1 || classes > INT32_MAX)
-    return set_error(GS_ERR_INVALID_ARG, "gs_distill: logits must be (n >= 0, 1 <= classes < 2^31)");
+  if (n < 0 || classes < 1 || classes > GS_DISTILL_MAX_CLASSES)
+    return set_error(GS_ERR_INVALID_ARG, "gs_distill: logits must be (n >= 0, 1 <= classes <= %d)",
+                     GS_DISTILL_MAX_CLASSES);
   if (!teacher) return set_error(GS_ERR_INVALID_ARG, "gs_distill: teacher is NULL");
   const bool cached = teacher->bits != 0;
   const int max_k = cached ? GS_CACHE_MAX_K : GS_TEACHER_MAX_K;

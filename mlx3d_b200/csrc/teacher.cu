@@ -111,7 +111,8 @@ struct Key<float> {
 __device__ __forceinline__ int quantise(float first, float last, float v, float levels) {
   const float q = (first - v) * levels / (first - last);
   const float near = rintf(q);
-  if (fabsf(q - near) < 0.499f) return (int)near;  // |error of q| < 255 * 3 * 2^-24 < 1e-4
+  // |error of q| < 255 * 3 * 2^-24 < 1e-4, unless the span overflows
+  if (fabsf(q - near) < 0.499f && first - last <= FLT_MAX) return (int)near;
   return (int)rint(((double)first - (double)v) * (double)levels / ((double)first - (double)last));
 }
 
@@ -174,6 +175,7 @@ __global__ void __launch_bounds__(kStagedRows) k_teacher_write_rows(TeacherWrite
   __syncthreads();
   if (whole && !mbar_wait(&bar, 0)) {
     if (l == 0) atomicAdd(&g_teacher_wait_failures, 1ull);
+    mbar_wait(&bar, 0);  // the copy in flight must end before the block does (bounded)
     return;
   }
   // Rows an even number of words apart: lane l starts at word l, so that the lanes

@@ -78,6 +78,8 @@ def test_native_distill_rejects_bad_arguments_before_the_device():
     assert call(n=-1) == nat.GS_ERR_INVALID_ARG
     assert call(classes=0) == nat.GS_ERR_INVALID_ARG
     assert call(classes=1 << 31) == nat.GS_ERR_INVALID_ARG
+    assert call(classes=nat.GS_DISTILL_MAX_CLASSES + 1) == nat.GS_ERR_INVALID_ARG  # 16 bytes of a row stay countable
+    assert b"classes" in lib.gs_last_error()
     assert call(t=_native_teacher(k=0)) == nat.GS_ERR_INVALID_ARG
     assert call(t=_native_teacher(k=33)) == nat.GS_ERR_INVALID_ARG  # a cache's limit
     assert call(t=_native_teacher(bits=0, k=257)) == nat.GS_ERR_INVALID_ARG

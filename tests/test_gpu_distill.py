@@ -61,6 +61,29 @@ def test_distill_matches_the_definition(n, c, k, t, dtype):
     assert torch.equal(leaf.grad, grad)
 
 
+@pytest.mark.parametrize("k", [1, 3, 8, 9, 40])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_every_split_of_a_row(dtype, k):
+    """Class counts on both sides of every split; odd ones start every second row inside a pair of classes."""
+    for c in (1, 2, 3, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 97, 127, 128, 129, 159, 160, 161, 255, 257, 511, 513,
+              1023, 1025, 1535, 1536, 1537):
+        s, v, i, w = _inputs(75, c, k, dtype, dtype, seed=c)
+        loss, grad = distill_loss_and_grad(s, (v, i), temperature=1.0, weight=w, reduction="none")
+        _check(s, v, i, w, 1.0, loss, grad)
+
+
+@pytest.mark.parametrize("c", [3, 31, 133, 301, 1201])
+def test_odd_rows_do_not_see_their_neighbours(c):
+    for dtype in ("fp32", "bf16"):
+        s, v, i, w = _inputs(41, c, 5, dtype, dtype)
+        want_l, want_g = distill_loss_and_grad(s, (v, i), weight=w, reduction="none")
+        s[1::2] = math.nan
+        loss, grad = distill_loss_and_grad(s, (v, i), weight=w, reduction="none")
+        assert torch.equal(loss[::2], want_l[::2]) and torch.equal(grad[::2], want_g[::2])
+        here = ((i >= 0) & (i < c)).any(1)[1::2]
+        assert loss[1::2][here].isnan().all() and (loss[1::2][~here] == 0).all()
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum"])
 def test_reductions_and_cotangents(reduction):
     n, c, k = 1031, 77, 6
@@ -217,6 +240,33 @@ def test_write_extreme_ranges():
         first, scale, want_i, code = write64(z, 4, bits)
         assert torch.equal(index.cpu(), want_i)
         assert torch.equal(values.cpu(), read64(first, scale, want_i, code))
+
+
+def test_write_a_span_beyond_float32():
+    # last - first overflows; the second entry lies 0.9 of a step below the first
+    z = torch.tensor([[3.3e38, 3.3e38 - 0.9 * 6.6e38 / 255, 1e38, -3.3e38]], device="cuda")
+    for rows in (1, 5000):  # both ways of writing
+        cache = TeacherCache(rows, 4, 4)
+        cache.write(0, z.repeat(rows, 1))
+        values, index = cache.read(slice(rows - 1, rows))
+        first, scale, want_i, code = write64(z, 4, 8)
+        assert code[0, 1] == 1 and torch.equal(index.cpu(), want_i)
+        assert torch.equal(values.cpu(), read64(first, scale, want_i, code))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_write_subnormals_and_signed_zeros_in_order(dtype):
+    """Even rows of 16-bit logits in their many: the quick path has to order what rounds and flushes easily."""
+    t = torch.finfo(DTYPES[dtype])
+    tiny = t.smallest_normal * t.eps
+    line = torch.tensor([-0.0, 0.0, tiny, -tiny, 2 * tiny, t.min, t.max, -t.smallest_normal, t.smallest_normal, -1.0],
+                        device="cuda", dtype=DTYPES[dtype])
+    assert (line[2] > 0) and (line[4] > line[2])
+    z = line.repeat(5000, 1)
+    cache = TeacherCache(5000, 9, 10)
+    cache.write(0, z)
+    _, index = cache.read(slice(None))
+    assert (index == torch.tensor([6, 8, 4, 2, 0, 1, 3, 7, 9], device="cuda")).all()
 
 
 @pytest.mark.parametrize("k,bits", [(7, 8), (8, 8), (8, 4), (16, 8), (16, 4), (32, 8), (32, 4), (3, 4), (1, 8), (20, 4)])
