@@ -36,7 +36,6 @@ enum { kFwd = 0, kDx = 1, kDw = 2 };
 
 __device__ unsigned long long g_decode_wait_failures;
 
-
 int decode_wait_failures(unsigned long long* out, int reset) {
   cudaError_t e = cudaMemcpyFromSymbol(out, g_decode_wait_failures, sizeof(*out));
   if (e == cudaSuccess && reset) {
@@ -62,6 +61,7 @@ struct DecodeArgs {
   int out_pitch;           // bytes of a row of the output stage, 0: rows stored from registers
   int out_vec;             // bytes of a store to the output stage
   int out_bulk;            // the output stage is stored by one bulk copy
+  int bars_at;             // the barriers' place, behind the stages
 };
 
 __host__ __device__ __forceinline__ int round_up(int v, int m) { return (v + m - 1) / m * m; }
@@ -102,7 +102,6 @@ __global__ void k_decode_prepare(const T* __restrict__ wg, const T* __restrict__
     *reinterpret_cast<uint4*>(out + off) = *reinterpret_cast<const uint4*>(v);
   }
 }
-
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -241,6 +240,14 @@ __device__ __forceinline__ void arrive(unsigned long long* bar) {
   asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// Panels start on 1024-byte boundaries of shared memory, which the kernels declare
+// for their base; a launch where it is not so is counted as failed.
+__device__ __forceinline__ bool panels_aligned(const uint8_t* smem) {
+  const bool ok = (smem_addr(smem) & 1023) == 0;
+  if (!ok && threadIdx.x == 0) atomicAdd(&g_decode_wait_failures, 1ull);
+  return ok;
+}
+
 __device__ __forceinline__ void init_bars(Bars* b) {
   for (int i = 0; i < kMaxXStages; ++i) {
     mbar_init(&b->xfull[i], 1);
@@ -365,9 +372,7 @@ __device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16],
 // the registers would write one sector per thread and instruction.
 template <typename T, int MODE, int ACT>
 __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_constant__ DecodeArgs a) {
-  extern __shared__ uint8_t raw[];
-  __shared__ Bars bars;
-  Bars* b = &bars;
+  extern __shared__ __align__(1024) uint8_t smem[];
   constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
   constexpr uint32_t kBuf = MODE == kFwd ? 128 : 192;  // TMEM columns of a chunk: g, u (, dh)
   // TMEM: two chunk buffers, then the accumulators of finished tiles
@@ -375,10 +380,11 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
   constexpr uint32_t kOut = 2 * kBuf;
   const int nout = wp <= (512 - (int)kOut) / 2 ? 2 : 1;
   const uint32_t out_cols = (512 - kOut) / nout;
-  uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
   const int stage_bytes = (a.nxp + (MODE == kFwd ? 0 : a.nyp)) * kPanel;
   uint8_t* ws = smem + a.x_stages * stage_bytes;
   uint8_t* os = ws + a.w_stages * a.chunk_bytes;
+  Bars* b = reinterpret_cast<Bars*>(smem + a.bars_at);
+  if (!panels_aligned(smem)) return;
 
   const int warp = __shfl_sync(~0u, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // warp: uniform
   if (warp == 0) tc::tmem_alloc(&b->tmem, kTmemCols);
@@ -452,95 +458,93 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
     }
     __syncwarp();
   } else if (warp == 0) {
-    {
-      // This warp's instructions bound short tiles: counters instead of
-      // divisions, and all operands of the matrix instructions made uniform
-      // before the elected lane issues them.
-      Ring x, w1, w2, y;
-      int j1 = 0, j2 = 0;
-      bool ok = true, wait_w = true;
-      const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
-      const uint32_t id2 = tc::instr_desc(kBf16, wp, false, MODE == kDx);
-      const uint32_t x0 = tc::desc_k(smem_addr(smem)), wk0 = tc::desc_k(smem_addr(ws));
-      const uint32_t wn0 = tc::desc_mn(smem_addr(ws), kPanel);
-      const uint32_t xstep = stage_bytes >> 4, wstep = a.chunk_bytes >> 4, wdn = a.nxp * (kPanel >> 4);
-      const int k1 = a.dp / 16, kh = a.cp / 16;
-      auto first_products = [&](uint32_t buf_, unsigned long long* done) {
-        if (j1 == 0) ok &= wait_for(b, &b->xfull[x.at], x.parity);
-        if (wait_w) ok &= wait_for(b, &b->wfull[w1.at], w1.parity);
-        ok = __all_sync(~0u, ok);
-        if (!ok) return;
-        tc::fence_after();
-        const uint32_t buf = tc::uniform(buf_), xd = tc::uniform(x0 + x.at * xstep);
-        const uint32_t wk = tc::uniform(wk0 + w1.at * wstep), wn = tc::uniform(wn0 + w1.at * wstep + wdn);
-        const bool last = j1 + 1 == a.chunks;
-        if (tc::elect_one()) {
-          tc::mma_ss(buf, xd, wk, id1, false);
+    // This warp's instructions bound short tiles: counters instead of
+    // divisions, and all operands of the matrix instructions made uniform
+    // before the elected lane issues them.
+    Ring x, w1, w2, y;
+    int j1 = 0, j2 = 0;
+    bool ok = true, wait_w = true;
+    const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
+    const uint32_t id2 = tc::instr_desc(kBf16, wp, false, MODE == kDx);
+    const uint32_t x0 = tc::desc_k(smem_addr(smem)), wk0 = tc::desc_k(smem_addr(ws));
+    const uint32_t wn0 = tc::desc_mn(smem_addr(ws), kPanel);
+    const uint32_t xstep = stage_bytes >> 4, wstep = a.chunk_bytes >> 4, wdn = a.nxp * (kPanel >> 4);
+    const int k1 = a.dp / 16, kh = a.cp / 16;
+    auto first_products = [&](uint32_t buf_, unsigned long long* done) {
+      if (j1 == 0) ok &= wait_for(b, &b->xfull[x.at], x.parity);
+      if (wait_w) ok &= wait_for(b, &b->wfull[w1.at], w1.parity);
+      ok = __all_sync(~0u, ok);
+      if (!ok) return;
+      tc::fence_after();
+      const uint32_t buf = tc::uniform(buf_), xd = tc::uniform(x0 + x.at * xstep);
+      const uint32_t wk = tc::uniform(wk0 + w1.at * wstep), wn = tc::uniform(wn0 + w1.at * wstep + wdn);
+      const bool last = j1 + 1 == a.chunks;
+      if (tc::elect_one()) {
+        tc::mma_ss(buf, xd, wk, id1, false);
 #pragma unroll
-          for (int k = 1; k < GS_DECODE_MAX_D / 16; ++k)
-            if (k < k1)
-              tc::mma_ss(buf, xd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wk + (k >> 2) * (kPanel >> 4) + (k & 3) * 2,
-                         id1, true);
-          if (MODE == kDx) {
-            const uint32_t yd = xd + wdn;
-            tc::mma_ss(buf + 128, yd, wn, idh, false);
+        for (int k = 1; k < GS_DECODE_MAX_D / 16; ++k)
+          if (k < k1)
+            tc::mma_ss(buf, xd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wk + (k >> 2) * (kPanel >> 4) + (k & 3) * 2,
+                       id1, true);
+        if (MODE == kDx) {
+          const uint32_t yd = xd + wdn;
+          tc::mma_ss(buf + 128, yd, wn, idh, false);
 #pragma unroll
-            for (int k = 1; k < GS_DECODE_MAX_C / 16; ++k)
-              if (k < kh)
-                tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, true);
-          }
-          tc::commit(done);
-          if (last) tc::commit(&b->xempty[x.at]);
+          for (int k = 1; k < GS_DECODE_MAX_C / 16; ++k)
+            if (k < kh)
+              tc::mma_ss(buf + 128, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, true);
         }
-        __syncwarp();
-        w1.next(a.w_stages);
-        ++j1;
-        if (last) {
-          x.next(a.x_stages);
-          j1 = 0;
-          if (resident) wait_w = false;
-        }
-      };
-      first_products(tmem, &b->gfull[0]);
-      unsigned qb = 0, qphase = 0;  // chunk's buffer and its phase
-      for (int64_t q = 0; q < total && ok; ++q) {
-        if (q + 1 < total) first_products(tmem + (qb ^ 1) * kBuf, &b->gfull[qb ^ 1]);
-        if (j2 == 0) ok &= wait_for(b, &b->yempty[y.at], y.parity ^ 1);
-        ok &= wait_for(b, &b->hfull[qb], qphase);
-        ok = __all_sync(~0u, ok);
-        if (!ok) break;
-        tc::fence_after();
-        const uint32_t buf = tc::uniform(tmem + qb * kBuf), out = tc::uniform(tmem + kOut + y.at * out_cols);
-        const uint32_t wk = tc::uniform(wk0 + w2.at * wstep + wdn), wn = tc::uniform(wn0 + w2.at * wstep);
-        const bool last = j2 + 1 == a.chunks, more = __all_sync(~0u, j2 > 0);
-        if (tc::elect_one()) {
-          if (MODE == kFwd) {
-            tc::mma_ts(out, buf, wk, id2, more);
-#pragma unroll
-            for (int k = 1; k < 4; ++k)  // h in the columns of g, 16 of each 32
-              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wk + k * 2, id2, true);
-          } else {
-            tc::mma_ts(out, buf, wn, id2, more);
-#pragma unroll
-            for (int k = 1; k < 8; ++k)  // dg in the columns of g, du in those of u
-              tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wn + k * 128, id2, true);
-          }
-          if (!resident) tc::commit(&b->wempty[w2.at]);
-          if (last) tc::commit(&b->yfull[y.at]);
-        }
-        __syncwarp();
-        w2.next(a.w_stages);
-        ++j2;
-        if (last) {
-          y.next(nout);
-          j2 = 0;
-        }
-        qb ^= 1;
-        if (qb == 0) qphase ^= 1;
+        tc::commit(done);
+        if (last) tc::commit(&b->xempty[x.at]);
       }
-      // Every issued instruction has finished when this phase completes.
-      if (!ok && tc::elect_one()) tc::commit(&b->sfree);
+      __syncwarp();
+      w1.next(a.w_stages);
+      ++j1;
+      if (last) {
+        x.next(a.x_stages);
+        j1 = 0;
+        if (resident) wait_w = false;
+      }
+    };
+    first_products(tmem, &b->gfull[0]);
+    unsigned qb = 0, qphase = 0;  // chunk's buffer and its phase
+    for (int64_t q = 0; q < total && ok; ++q) {
+      if (q + 1 < total) first_products(tmem + (qb ^ 1) * kBuf, &b->gfull[qb ^ 1]);
+      if (j2 == 0) ok &= wait_for(b, &b->yempty[y.at], y.parity ^ 1);
+      ok &= wait_for(b, &b->hfull[qb], qphase);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      tc::fence_after();
+      const uint32_t buf = tc::uniform(tmem + qb * kBuf), out = tc::uniform(tmem + kOut + y.at * out_cols);
+      const uint32_t wk = tc::uniform(wk0 + w2.at * wstep + wdn), wn = tc::uniform(wn0 + w2.at * wstep);
+      const bool last = j2 + 1 == a.chunks, more = __all_sync(~0u, j2 > 0);
+      if (tc::elect_one()) {
+        if (MODE == kFwd) {
+          tc::mma_ts(out, buf, wk, id2, more);
+#pragma unroll
+          for (int k = 1; k < 4; ++k)  // h in the columns of g, 16 of each 32
+            tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wk + k * 2, id2, true);
+        } else {
+          tc::mma_ts(out, buf, wn, id2, more);
+#pragma unroll
+          for (int k = 1; k < 8; ++k)  // dg in the columns of g, du in those of u
+            tc::mma_ts(out, buf + (k >> 1) * 32 + (k & 1) * 8, wn + k * 128, id2, true);
+        }
+        if (!resident) tc::commit(&b->wempty[w2.at]);
+        if (last) tc::commit(&b->yfull[y.at]);
+      }
+      __syncwarp();
+      w2.next(a.w_stages);
+      ++j2;
+      if (last) {
+        y.next(nout);
+        j2 = 0;
+      }
+      qb ^= 1;
+      if (qb == 0) qphase ^= 1;
     }
+    // Every issued instruction has finished when this phase completes.
+    if (!ok && tc::elect_one()) tc::commit(&b->sfree);
     __syncwarp();
   } else if (warp == 2) {
     if (a.out_bulk) {  // finished tiles: output stage -> global memory
@@ -551,15 +555,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
         if (!__all_sync(~0u, wait_for(b, &b->ofull, (unsigned)i & 1))) break;
         const int rows = (int)min((int64_t)kTile, a.n - t * kTile);
         uint8_t* dst = out + t * kTile * row_bytes;
-        {
-          const int bytes = rows * row_bytes & ~15;
-          if (lane == 0 && bytes > 0)
-            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(os)),
-                         "r"(bytes)
-                         : "memory");
-          for (int e = bytes + 2 * lane; e < rows * row_bytes; e += 64)
-            *reinterpret_cast<uint16_t*>(dst + e) = *reinterpret_cast<const uint16_t*>(os + e);
-        }
+        const int bytes = rows * row_bytes & ~15;
+        if (lane == 0 && bytes > 0)
+          asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(smem_addr(os)),
+                       "r"(bytes)
+                       : "memory");
+        for (int e = bytes + 2 * lane; e < rows * row_bytes; e += 64)
+          *reinterpret_cast<uint16_t*>(dst + e) = *reinterpret_cast<const uint16_t*>(os + e);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
@@ -703,14 +705,13 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
 // tile's [g | u] is issued before this tile's sums.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_constant__ DecodeArgs a) {
-  extern __shared__ uint8_t raw[];
-  __shared__ Bars bars;
-  Bars* b = &bars;
+  extern __shared__ __align__(1024) uint8_t smem[];
   constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
-  uint8_t* smem = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
   const int stage_bytes = (a.nxp + a.nyp) * kPanel;
   uint8_t* ws = smem + a.x_stages * stage_bytes;
   uint8_t* st = ws + a.chunk_bytes;  // dg, du, h panels
+  Bars* b = reinterpret_cast<Bars*>(smem + a.bars_at);
+  if (!panels_aligned(smem)) return;
   const int mblocks = (a.c + 127) / 128;
   const int acc_cols = (a.dp > 64 ? 128 : 64) + mblocks * 64;
   const int nbuf = acc_cols <= 192 ? 2 : 1;  // [g | u] buffers
@@ -736,116 +737,114 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
     if (lane == 0) fetch_inputs<true>(a, b, smem, stage_bytes, blockIdx.x, gridDim.x, tiles);
     __syncwarp();
   } else if (warp == 0) {
-    {
-      bool ok = true;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&b->wfull[0], a.chunk_bytes);
-        bulk_g2s(ws, a.image + (size_t)blockIdx.y * a.chunk_bytes, a.chunk_bytes, &b->wfull[0]);
+    bool ok = true;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&b->wfull[0], a.chunk_bytes);
+      bulk_g2s(ws, a.image + (size_t)blockIdx.y * a.chunk_bytes, a.chunk_bytes, &b->wfull[0]);
+    }
+    __syncwarp();
+    ok = wait_for(b, &b->wfull[0], 0);
+    const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
+    const uint32_t idg = tc::instr_desc(kBf16, a.dp, true, true), idd = tc::instr_desc(kBf16, 64, true, true);
+    const uint32_t xstep = stage_bytes >> 4, ypart = a.nxp * (kPanel >> 4);
+    const uint32_t xk0 = tc::desc_k(smem_addr(smem)), xn0 = tc::desc_mn(smem_addr(smem), kPanel);
+    const uint32_t wk = tc::uniform(tc::desc_k(smem_addr(ws))), sn = tc::uniform(tc::desc_mn(smem_addr(st), kPanel));
+    const uint32_t wn = tc::uniform(tc::desc_mn(smem_addr(ws), kPanel) + ypart);
+    const int k1 = a.dp / 16, kh = a.cp / 16;
+    Ring xg, xh, xs;  // stages of the next [g | u], dh and sums
+    unsigned gb = 0;
+    auto gu_products = [&]() {
+      ok &= wait_for(b, &b->xfull[xg.at], xg.parity);
+      ok = __all_sync(~0u, ok);
+      if (!ok) return;
+      tc::fence_after();
+      const uint32_t xd = tc::uniform(xk0 + xg.at * xstep), buf = tc::uniform(tmem + gb * 128);
+      if (tc::elect_one()) {
+        tc::mma_ss(buf, xd, wk, id1, false);
+#pragma unroll
+        for (int k = 1; k < GS_DECODE_MAX_D / 16; ++k)
+          if (k < k1)
+            tc::mma_ss(buf, xd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wk + (k >> 2) * (kPanel >> 4) + (k & 3) * 2,
+                       id1, true);
       }
       __syncwarp();
-      ok = wait_for(b, &b->wfull[0], 0);
-      const uint32_t id1 = tc::instr_desc(kBf16, 128, false, false), idh = tc::instr_desc(kBf16, 64, false, true);
-      const uint32_t idg = tc::instr_desc(kBf16, a.dp, true, true), idd = tc::instr_desc(kBf16, 64, true, true);
-      const uint32_t xstep = stage_bytes >> 4, ypart = a.nxp * (kPanel >> 4);
-      const uint32_t xk0 = tc::desc_k(smem_addr(smem)), xn0 = tc::desc_mn(smem_addr(smem), kPanel);
-      const uint32_t wk = tc::uniform(tc::desc_k(smem_addr(ws))), sn = tc::uniform(tc::desc_mn(smem_addr(st), kPanel));
-      const uint32_t wn = tc::uniform(tc::desc_mn(smem_addr(ws), kPanel) + ypart);
-      const int k1 = a.dp / 16, kh = a.cp / 16;
-      Ring xg, xh, xs;  // stages of the next [g | u], dh and sums
-      unsigned gb = 0;
-      auto gu_products = [&]() {
-        ok &= wait_for(b, &b->xfull[xg.at], xg.parity);
-        ok = __all_sync(~0u, ok);
-        if (!ok) return;
-        tc::fence_after();
-        const uint32_t xd = tc::uniform(xk0 + xg.at * xstep), buf = tc::uniform(tmem + gb * 128);
-        if (tc::elect_one()) {
-          tc::mma_ss(buf, xd, wk, id1, false);
+      xg.next(a.x_stages);
+      if (nbuf == 2) gb ^= 1;
+    };
+    auto dh_products = [&]() {
+      const uint32_t yd = tc::uniform(xk0 + xh.at * xstep + ypart), buf = tc::uniform(tmem + col_dh);
+      if (tc::elect_one()) {
+        tc::mma_ss(buf, yd, wn, idh, false);
 #pragma unroll
-          for (int k = 1; k < GS_DECODE_MAX_D / 16; ++k)
-            if (k < k1)
-              tc::mma_ss(buf, xd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wk + (k >> 2) * (kPanel >> 4) + (k & 3) * 2,
-                         id1, true);
-        }
-        __syncwarp();
-        xg.next(a.x_stages);
-        if (nbuf == 2) gb ^= 1;
-      };
-      auto dh_products = [&]() {
-        const uint32_t yd = tc::uniform(xk0 + xh.at * xstep + ypart), buf = tc::uniform(tmem + col_dh);
-        if (tc::elect_one()) {
-          tc::mma_ss(buf, yd, wn, idh, false);
-#pragma unroll
-          for (int k = 1; k < GS_DECODE_MAX_C / 16; ++k)
-            if (k < kh) tc::mma_ss(buf, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, true);
-          tc::commit(&b->dhfull);
-        }
-        __syncwarp();
-        xh.next(a.x_stages);
-      };
-      gu_products();
-      if (ok) dh_products();
-      const uint32_t tgu = tc::uniform(tmem + col_gu), tdd = tc::uniform(tmem + col_dd);
-      for (int64_t i = 0; i < mine && ok; ++i) {
-        // The next tile's first products go before this one's sums as soon as its
-        // inputs are there: [g | u] at once with two buffers, else, like dh, when
-        // this tile's have been read.
-        const bool more_tiles = i + 1 < mine;
-        auto ready = [&]() { return more_tiles && __all_sync(~0u, passed(&b->xfull[xg.at], xg.parity)); };
-        bool ahead = false;
-        if (nbuf == 2 && ready()) {
-          gu_products();
-          ahead = true;
-        }
-        ok &= wait_for(b, &b->dhread, (unsigned)i & 1);
-        ok = __all_sync(~0u, ok);
-        if (!ok) break;
-        tc::fence_after();
-        if (!ahead && ready()) {
-          gu_products();
-          ahead = true;
-        }
-        if (ahead) dh_products();
-        // its panels are written
-        ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
-        ok = __all_sync(~0u, ok);
-        if (!ok) break;
-        tc::fence_after();
-        if (!ahead && ready()) {
-          gu_products();
-          dh_products();
-          ahead = true;
-        }
-        const uint32_t xd = tc::uniform(xn0 + xs.at * xstep), yd = xd + ypart;
-        const bool more = __all_sync(~0u, i > 0);
-        if (tc::elect_one()) {
-          tc::mma_ss(tgu, sn, xd, idg, more);
-#pragma unroll
-          for (int k = 1; k < 8; ++k) tc::mma_ss(tgu, sn + k * 128, xd + k * 128, idg, true);
-          // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
-          const uint32_t hn = sn + 2 * (kPanel >> 4);
-#pragma unroll
-          for (int m = 0; m < GS_DECODE_MAX_C / 128; ++m) {
-            if (m >= mblocks) break;
-            const uint32_t ym = yd + m * 2 * (kPanel >> 4);
-            tc::mma_ss(tdd + m * 64, ym, hn, idd, more);
-#pragma unroll
-            for (int k = 1; k < 8; ++k) tc::mma_ss(tdd + m * 64, ym + k * 128, hn + k * 128, idd, true);
-          }
-          tc::commit(&b->sfree);
-          tc::commit(&b->xempty[xs.at]);
-        }
-        __syncwarp();
-        xs.next(a.x_stages);
-        if (!ahead && more_tiles) {
-          gu_products();
-          if (ok) dh_products();
-        }
+        for (int k = 1; k < GS_DECODE_MAX_C / 16; ++k)
+          if (k < kh) tc::mma_ss(buf, yd + (k >> 2) * (kPanel >> 4) + (k & 3) * 2, wn + k * 128, idh, true);
+        tc::commit(&b->dhfull);
       }
-      if (!ok) {
-        mbar_wait(&b->wfull[0], 0);
-        if (tc::elect_one()) tc::commit(&b->yfull[0]);
+      __syncwarp();
+      xh.next(a.x_stages);
+    };
+    gu_products();
+    if (ok) dh_products();
+    const uint32_t tgu = tc::uniform(tmem + col_gu), tdd = tc::uniform(tmem + col_dd);
+    for (int64_t i = 0; i < mine && ok; ++i) {
+      // The next tile's first products go before this one's sums as soon as its
+      // inputs are there: [g | u] at once with two buffers, else, like dh, when
+      // this tile's have been read.
+      const bool more_tiles = i + 1 < mine;
+      auto ready = [&]() { return more_tiles && __all_sync(~0u, passed(&b->xfull[xg.at], xg.parity)); };
+      bool ahead = false;
+      if (nbuf == 2 && ready()) {
+        gu_products();
+        ahead = true;
       }
+      ok &= wait_for(b, &b->dhread, (unsigned)i & 1);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      tc::fence_after();
+      if (!ahead && ready()) {
+        gu_products();
+        ahead = true;
+      }
+      if (ahead) dh_products();
+      // its panels are written
+      ok &= wait_for(b, &b->hfull[0], (unsigned)i & 1);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      tc::fence_after();
+      if (!ahead && ready()) {
+        gu_products();
+        dh_products();
+        ahead = true;
+      }
+      const uint32_t xd = tc::uniform(xn0 + xs.at * xstep), yd = xd + ypart;
+      const bool more = __all_sync(~0u, i > 0);
+      if (tc::elect_one()) {
+        tc::mma_ss(tgu, sn, xd, idg, more);
+#pragma unroll
+        for (int k = 1; k < 8; ++k) tc::mma_ss(tgu, sn + k * 128, xd + k * 128, idg, true);
+        // A dy panel past nyp is other shared memory: it only reaches rows >= c of the sums, which are not read.
+        const uint32_t hn = sn + 2 * (kPanel >> 4);
+#pragma unroll
+        for (int m = 0; m < GS_DECODE_MAX_C / 128; ++m) {
+          if (m >= mblocks) break;
+          const uint32_t ym = yd + m * 2 * (kPanel >> 4);
+          tc::mma_ss(tdd + m * 64, ym, hn, idd, more);
+#pragma unroll
+          for (int k = 1; k < 8; ++k) tc::mma_ss(tdd + m * 64, ym + k * 128, hn + k * 128, idd, true);
+        }
+        tc::commit(&b->sfree);
+        tc::commit(&b->xempty[xs.at]);
+      }
+      __syncwarp();
+      xs.next(a.x_stages);
+      if (!ahead && more_tiles) {
+        gu_products();
+        if (ok) dh_products();
+      }
+    }
+    if (!ok) {
+      mbar_wait(&b->wfull[0], 0);
+      if (tc::elect_one()) tc::commit(&b->yfull[0]);
     }
     __syncwarp();
   } else if (warp >= 4) {
@@ -858,17 +857,15 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
       if (!ok) break;
       tc::fence_after();
       uint32_t pg[8], pu[8], ph[8];
+      GateIn<kDw, 8> v[2];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        GateIn<kDw, 8> v;
-        v.load(buf + 8 * p, buf + 64 + 8 * p, dhc + 8 * p);
-        v.settle();
-        if (p == 1) {
-          tc::fence_before();
-          arrive(&b->dhread);
-        }
-        v.template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
-      }
+      for (int p = 0; p < 2; ++p) v[p].load(buf + 8 * p, buf + 64 + 8 * p, dhc + 8 * p);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) v[p].settle();
+      tc::fence_before();
+      arrive(&b->dhread);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) v[p].template compute<T, ACT>(ph + 4 * p, pg + 4 * p, pu + 4 * p);
       // the previous tile's sums have read the panels
       if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
       if (!ok) break;
@@ -932,8 +929,8 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
 // A few rows of a small block (a picked point, a handful of samples): one launch
 // that reads the weights where they are, one block per row, a warp per hidden
 // unit and then per output.  h stays in 32 bits.  The matrix path's weight layout
-// and pipeline start cost more than this whole call: one row, 32-64-20, FEW_US
-// instead of 45 us.
+// and pipeline start cost more than this whole call: one row, 32-64-20, 15 us
+// from Python instead of 45.
 constexpr int kFewThreads = 256;
 template <typename T, int ACT>
 __global__ void __launch_bounds__(kFewThreads) k_decode_few(const T* __restrict__ x, const T* __restrict__ wg,
@@ -984,6 +981,7 @@ __global__ void k_decode_reduce(const float* __restrict__ partials, int splits, 
   const int64_t total = 2 * fd + cf;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     float s = 0.0f;
+#pragma unroll 8
     for (int p = 0; p < splits; ++p) s += partials[p * total + i];
     T* out = i < fd ? dg + i : i < 2 * fd ? du + (i - fd) : dd + (i - 2 * fd);
     *out = from_f32<T>(s);
@@ -1105,50 +1103,62 @@ static DecodeArgs decode_args(int64_t n, int d, int f, int c, int act, const voi
   return a;
 }
 
-// Shared memory of a launch: input stages, weight stages, output stage.  Weight
-// chunks are kept resident if they all fit beside two input stages; else at
-// least two stages stream them.  What is left goes to further input stages.
+// Shared memory of a launch: input stages, weight stages, output stage, barriers.
+// Weight chunks are kept resident if they all fit beside two input stages.  Else three
+// stages stream them; where only two would fit, resident weights beside a single input
+// stage are better (dx of 1600x1060 rows, 64-256-152: 505 us, streamed 531; with three
+// stages, 64-256-128: 432 us, streamed 401).  The largest blocks stream them through two
+// stages.  What is left goes to further input stages.
 template <int MODE>
 static size_t plan_smem(DecodeArgs& a) {
-  const size_t fixed = 1024 + sizeof(Bars) + 64;
+  constexpr size_t kMost = kMaxSmem - sizeof(Bars);
   const size_t in = (size_t)(a.nxp + (MODE == kFwd ? 0 : a.nyp)) * kPanel;
   if (MODE == kDw) {
-    const size_t own = fixed + a.chunk_bytes + 3 * (size_t)kPanel;
+    const size_t own = a.chunk_bytes + 3 * (size_t)kPanel;
     a.w_stages = 1;
-    a.x_stages = (int)std::min<size_t>(kMaxXStages, (kMaxSmem - own) / in);
-    return own + a.x_stages * in - sizeof(Bars);
+    a.x_stages = (int)std::min<size_t>(kMaxXStages, (kMost - own) / in);
+    a.bars_at = (int)(own + a.x_stages * in);
+    return a.bars_at + sizeof(Bars);
   }
   const int width = MODE == kFwd ? a.c : a.d, row = width * 2;
   // The stage has the output's own layout where its rows are an odd number of
   // out_vec bytes apart, so that a column's stores hit all banks: one bulk copy
   // a tile.  An even number of 16-byte units is padded by one, and the drain
-  // warps copy the rows themselves (128 bulk copies a tile, one a row, took
-  // 5000 cycles: 64 classes 498 us for 1600x1060 instead of DRAIN_US).
+  // warps copy the rows themselves (one bulk copy a row took 5000 cycles a tile:
+  // forward, 1600x1060 rows of 64 classes, 498 us instead of 283).
   a.out_vec = width % 8 == 0 ? 16 : width % 4 == 0 ? 8 : width % 2 == 0 ? 4 : 2;
   a.out_pitch = width % 8 == 0 ? (row / 16 | 1) * 16 : row;
-  const bool fits = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-  a.out_bulk = fits && a.out_pitch == row;
-  size_t out = fits ? ((size_t)kTile * a.out_pitch + 15) & ~(size_t)15 : 0;
-  const int need = std::min(a.chunks, 2);
-  a.x_stages = 2;
-  if (fixed + out + 2 * in + (size_t)need * a.chunk_bytes > kMaxSmem) a.x_stages = 1;
-  if (fixed + out + in + (size_t)need * a.chunk_bytes > kMaxSmem) {
-    out = 0;
-    a.x_stages = fixed + 2 * in + (size_t)need * a.chunk_bytes > kMaxSmem ? 1 : 2;
+  bool staged = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  a.out_bulk = staged && a.out_pitch == row;
+  size_t out = staged ? ((size_t)kTile * a.out_pitch + 127) & ~(size_t)127 : 0;
+  const size_t all = (size_t)a.chunks * a.chunk_bytes, two = (size_t)std::min(a.chunks, 2) * a.chunk_bytes;
+  const bool fit = a.chunks <= kMaxWStages;  // the barriers
+  if (fit && out + 2 * in + all <= kMost) {
+    a.x_stages = 2;
+  } else if (out + 2 * in + two + a.chunk_bytes <= kMost) {
+    a.x_stages = 2;
+  } else if (fit && out + in + all <= kMost) {
+    a.x_stages = 1;
+  } else {
+    if (out + in + two > kMost) {
+      out = 0;
+      staged = false;
+    }
+    a.x_stages = out + 2 * in + two <= kMost ? 2 : 1;
   }
-  if (!out) {
+  if (!staged) {
     a.out_pitch = 0;
     a.out_bulk = 0;
     // rows of the caller's own output: its alignment bounds the store size
     const uintptr_t at = reinterpret_cast<uintptr_t>(a.out);
     while (a.out_vec > 2 && at % a.out_vec) a.out_vec /= 2;
   }
-  const size_t left = kMaxSmem - fixed - out - a.x_stages * in;
-  a.w_stages = (int)std::min<size_t>(std::min(a.chunks, kMaxWStages), left / a.chunk_bytes);
+  a.w_stages = (int)std::min<size_t>(std::min(a.chunks, kMaxWStages), (kMost - out - a.x_stages * in) / a.chunk_bytes);
   while (a.x_stages >= 2 && a.x_stages < kMaxXStages &&
-         fixed + out + (a.x_stages + 1) * in + (size_t)a.w_stages * a.chunk_bytes <= kMaxSmem)
+         out + (a.x_stages + 1) * in + (size_t)a.w_stages * a.chunk_bytes <= kMost)
     ++a.x_stages;
-  return fixed - sizeof(Bars) + out + a.x_stages * in + (size_t)a.w_stages * a.chunk_bytes;
+  a.bars_at = (int)(a.x_stages * in + (size_t)a.w_stages * a.chunk_bytes + out);
+  return a.bars_at + sizeof(Bars);
 }
 
 template <typename T, int MODE, int ACT>

@@ -86,7 +86,6 @@ __device__ __forceinline__ void store_pair(__nv_bfloat16* p, F2 v) {
   *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(lo, hi);
 }
 
-inline int elem_size(int dtype) { return dtype == GS_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == GS_F32 || dtype == GS_F16 || dtype == GS_BF16; }
 
 // A teacher cache record: [offset f32][scale f32][index int16 x k][codes],

@@ -19,10 +19,6 @@ constexpr int kPanelRow = 128;  // bytes of a panel row
 __device__ __forceinline__ uint32_t panel_offset(int row, int unit) {
   return (uint32_t)(row * kPanelRow + ((unit ^ (row & 7)) << 4));
 }
-// Byte offset of element `col` (< 64) of `row`.
-__device__ __forceinline__ uint32_t panel_elem(int row, int col) {
-  return panel_offset(row, col >> 3) + (uint32_t)((col & 7) << 1);
-}
 
 // Shared-memory matrix descriptor, 128-byte swizzle: bits 0-13 address / 16,
 // 16-29 leading byte offset / 16, 32-45 stride byte offset / 16, bits 46-48 =
@@ -128,14 +124,6 @@ __device__ __forceinline__ void after_wait(uint32_t (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(v[i]));
 }
 
-__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
-      " %16};" ::"r"(addr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&v)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(v[0]),
                "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])

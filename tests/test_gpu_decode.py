@@ -216,3 +216,35 @@ def test_first_call_of_a_thread():
     t.join()
     torch.cuda.synchronize()
     assert status == [nat.GS_OK] and torch.equal(dx, want)
+
+
+@pytest.mark.parametrize("f,d,c", [(256, 64, 152), (256, 64, 128), (256, 128, 256), (1100, 40, 24), (64, 128, 200)])
+def test_many_tiles_of_every_plan(f, d, c):
+    """Several tiles per SM, with weights resident beside one or more input stages, or streamed through three or two."""
+    x, wg, wu, wd, dy = _inputs(60001, d, f, c, "bf16", seed=f + c)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = decode_features(*leaves)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    with torch.no_grad():
+        want, tol = decode64(x, wg, wu, wd, "silu", dy), decode_tolerances(x, wg, wu, wd, "silu", dy)
+        for g, w, t in zip(got, want, tol):
+            _within(g, w, t)
+    assert _wait_failures() == 0
+
+
+@pytest.mark.parametrize("c", [7, 64, 150])
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+def test_outputs_at_any_element_leave_their_surroundings(c, offset):
+    n, d, f = 1301, 24, 96
+    x, wg, wu, wd, _ = _inputs(n, d, f, c, "bf16")
+    want = decode_features(x, wg, wu, wd)
+    lib = nat.load()
+    size = lib.gs_decode_image_bytes(d, f, c)
+    image = torch.empty((size,), device="cuda", dtype=torch.uint8)
+    nat.call("gs_decode_prepare", wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), 2, d, f, c, image.data_ptr(), size,
+             nat.stream())
+    flat = torch.full((n * c + 64,), 5.0, device="cuda", dtype=torch.bfloat16)
+    nat.call("gs_decode_forward", x.data_ptr(), 2, n, d, f, c, 0, image.data_ptr(), size,
+             flat.data_ptr() + 2 * offset, None, 0, nat.stream())
+    assert torch.equal(flat[offset:offset + n * c].reshape(n, c), want)
+    assert (flat[:offset] == 5.0).all() and (flat[offset + n * c:] == 5.0).all()
