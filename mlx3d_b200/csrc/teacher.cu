@@ -104,23 +104,44 @@ struct Key<float> {
   static __device__ __forceinline__ Word exchange(Word w, int mask) { return __shfl_xor_sync(~0u, w, mask); }
 };
 
-// code = (2^bits - 1) (first - v) / (first - last) to nearest, ties to even.
-// The 32-bit quotient decides except next to a border, where the exact
-// differences do: with few mantissa bits in the logits many quotients lie
-// exactly between two codes.
-__device__ __forceinline__ int quantise(float first, float last, float v, float levels) {
-  const float q = (first - v) * levels / (first - last);
-  const float near = rintf(q);
-  // |error of q| < 255 * 3 * 2^-24 < 1e-4, unless the span overflows
-  if (fabsf(q - near) < 0.499f && first - last <= FLT_MAX) return (int)near;
-  return (int)rint(((double)first - (double)v) * (double)levels / ((double)first - (double)last));
+// code = levels (first - v) / (first - last) to nearest, ties to even, levels =
+// 2^bits - 1.  The 32-bit quotient decides except next to a border, where the exact
+// differences do (with few mantissa bits in the logits many quotients lie exactly
+// between two codes): levels (first - v) against code and a half times the span, in
+// 64 bits.  Spans that overflow, or whose reciprocal does, are scaled by a power of
+// two first.
+struct Quantiser {
+  float scale, first, last, inv;
+  __device__ __forceinline__ Quantiser(float f, float l, float levels) {
+    const float span = f - l;
+    scale = span > FLT_MAX ? 0.25f : span < 0x1p-60f ? 0x1p80f : 1.0f;
+    first = f * scale;
+    last = l * scale;
+    inv = levels / (first - last);
+  }
+  __device__ __forceinline__ int operator()(float v, float levels) const {
+    v *= scale;
+    const float q = (first - v) * inv, near = rintf(q);
+    if (fabsf(q - near) < 0.499f) return (int)near;  // |error of q| < 255 * 4 * 2^-24 < 1e-4
+    const float low = floorf(q);
+    const double twice = ((double)first - (double)v) * (double)(2.0f * levels);
+    const double border = ((double)first - (double)last) * (double)(2.0f * low + 1.0f);
+    return (int)low + (twice > border || (twice == border && ((int)low & 1)) ? 1 : 0);
+  }
+};
+// (first - last) / levels, rounded once: the 64-bit product with 1 / levels, corrected
+// by its remainder.
+__device__ __forceinline__ float step_of(float first, float last, int bits) {
+  const double span = (double)first - (double)last, levels = (double)((1 << bits) - 1);
+  const double inv = bits == 8 ? 1.0 / 255.0 : 1.0 / 15.0, q = span * inv;
+  return (float)__fma_rn(__fma_rn(-q, levels, span), inv, q);
 }
 
 template <typename W>
 __device__ __forceinline__ void order(W& hi, W& lo) {  // hi >= lo afterwards
   const W a = hi, b = lo;
-  hi = a > b ? a : b;
-  lo = a > b ? b : a;
+  hi = max(a, b);
+  lo = min(a, b);
 }
 // Descending sort of N registers (Batcher's odd-even merge sort).
 template <int N, typename W>
@@ -139,7 +160,7 @@ __device__ __forceinline__ void sort_desc(W (&v)[N]) {
 template <int N, typename W>
 __device__ __forceinline__ void merge_desc(W (&best)[N], const W (&other)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) best[i] = best[i] > other[N - 1 - i] ? best[i] : other[N - 1 - i];
+  for (int i = 0; i < N; ++i) best[i] = max(best[i], other[N - 1 - i]);
 #pragma unroll
   for (int k = N / 2; k >= 1; k /= 2)
 #pragma unroll
@@ -239,13 +260,14 @@ __global__ void __launch_bounds__(kStagedRows) k_teacher_write_rows(TeacherWrite
   if (l < rows) {
     uint8_t* rec = smem + l * pitch;
     *reinterpret_cast<float*>(rec) = first;
-    *reinterpret_cast<float*>(rec + 4) = (float)(((double)first - (double)last) / (double)levels);
+    *reinterpret_cast<float*>(rec + 4) = step_of(first, last, a.bits);
+    const Quantiser quantise(first, last, levels);
     uint8_t* codes = rec + 8 + 2 * a.k;
     int low = 0;
 #pragma unroll
     for (int i = 0; i < MAX; ++i) {
       if (i >= a.k) break;
-      const int code = best[i] && first > last ? quantise(first, last, K::value(best[i]), levels) : 0;
+      const int code = best[i] && first > last ? quantise(K::value(best[i]), levels) : 0;
       reinterpret_cast<int16_t*>(rec + 8)[i] = best[i] ? (int16_t)K::index(best[i]) : (int16_t)-1;
       if (a.bits == 8) codes[i] = (uint8_t)code;
       else if (i & 1) codes[i >> 1] = (uint8_t)(low | code << 4);
@@ -355,10 +377,10 @@ __global__ void __launch_bounds__(kWriteWarps * 32) k_teacher_write_warp(Teacher
   const float value = mine ? K::value(best) : 0.0f;
   const float first = __shfl_sync(~0u, value, 0), last = __shfl_sync(~0u, value, count > 0 ? count - 1 : 0);
   const float levels = (float)((1 << a.bits) - 1);
-  const int code = mine && first > last ? quantise(first, last, value, levels) : 0;
+  const int code = mine && first > last ? Quantiser(first, last, levels)(value, levels) : 0;
   uint8_t* rec = a.records + r * a.rec_bytes;
   if (lane == 0)
-    *reinterpret_cast<float2*>(rec) = make_float2(first, (float)(((double)first - (double)last) / (double)levels));
+    *reinterpret_cast<float2*>(rec) = make_float2(first, step_of(first, last, a.bits));
   if (lane < k) reinterpret_cast<int16_t*>(rec + 8)[lane] = mine ? (int16_t)K::index(best) : (int16_t)-1;
   uint8_t* codes = rec + 8 + 2 * k;
   int used = 8 + 2 * k;
