@@ -438,42 +438,53 @@ __global__ void __launch_bounds__(256) k_teacher_read(const uint8_t* __restrict_
   }
 }
 
-// The same for K = 8, 16 or 32 entries, one thread per record: whole 16-byte units
-// in and out, a tenth of the instructions.
+// The same for K = 8, 16 or 32 entries: K / 4 lanes per record, four entries each, so
+// that a warp's results are whole contiguous lines; two records in flight per lane.
 template <int K, int BITS>
 __global__ void __launch_bounds__(256) k_teacher_read_whole(const uint8_t* __restrict__ records, int64_t n_records,
                                                             const int64_t* __restrict__ rows, int64_t first_row,
                                                             int64_t n, float* __restrict__ values,
                                                             int32_t* __restrict__ index) {
-  constexpr int kBytes = (8 + 2 * K + K * BITS / 8 + 15) / 16 * 16;
-  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < n; r += (int64_t)gridDim.x * 256) {
-    const int64_t rec = rows ? __ldg(rows + r) : first_row + r;
-    const bool here = rec >= 0 && rec < n_records;
-    uint32_t w[kBytes / 4];
+  constexpr int kBytes = (8 + 2 * K + K * BITS / 8 + 15) / 16 * 16, kLanes = K / 4, kFlight = 2;
+  constexpr int kGroups = 256 / kLanes;
+  const int q = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  for (int64_t r0 = (int64_t)blockIdx.x * kGroups * kFlight; r0 < n; r0 += (int64_t)gridDim.x * kGroups * kFlight) {
+    int64_t rec[kFlight];
 #pragma unroll
-    for (int i = 0; i < kBytes / 16; ++i) {
-      uint4 v = make_uint4(0, 0, 0xffffffffu, 0xffffffffu);
-      if (i > 0) v.x = v.y = 0xffffffffu;
-      if (here) v = __ldg(reinterpret_cast<const uint4*>(records + rec * kBytes) + i);
-      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    for (int i = 0; i < kFlight; ++i) {
+      const int64_t r = r0 + i * kGroups + group;
+      rec[i] = r < n ? (rows ? __ldg(rows + r) : first_row + r) : -1;
     }
-    const float offset = __uint_as_float(w[0]), scale = __uint_as_float(w[1]);
-    float4* vo = reinterpret_cast<float4*>(values + r * K);
-    int4* io = reinterpret_cast<int4*>(index + r * K);
+    float2 head[kFlight];
+    uint2 idx[kFlight];
+    uint32_t codes[kFlight];
 #pragma unroll
-    for (int q = 0; q < K / 4; ++q) {
+    for (int i = 0; i < kFlight; ++i) {
+      head[i] = make_float2(0.0f, 0.0f);
+      idx[i] = make_uint2(0xffffffffu, 0xffffffffu);
+      codes[i] = 0;
+      if (rec[i] >= 0 && rec[i] < n_records) {
+        const uint8_t* p = records + rec[i] * kBytes;
+        head[i] = __ldg(reinterpret_cast<const float2*>(p));
+        idx[i] = __ldg(reinterpret_cast<const uint2*>(p + 8) + q);
+        if (BITS == 8) codes[i] = __ldg(reinterpret_cast<const uint32_t*>(p + 8 + 2 * K) + q);
+        else codes[i] = __ldg(reinterpret_cast<const uint16_t*>(p + 8 + 2 * K) + q);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kFlight; ++i) {
+      const int64_t r = r0 + i * kGroups + group;
       float v[4];
-      int idx[4];
+      int c[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int e = 4 * q + j, bit = BITS * e;
-        const int i = (int)(int16_t)(w[2 + e / 2] >> (16 * (e & 1)));
-        const int code = (int)(w[2 + K / 2 + bit / 32] >> (bit % 32)) & ((1 << BITS) - 1);
-        idx[j] = i >= 0 ? i : -1;
-        v[j] = i >= 0 ? record_value(offset, scale, code) : -INFINITY;
+        c[j] = max((int)(int16_t)((j < 2 ? idx[i].x : idx[i].y) >> (16 * (j & 1))), -1);
+        v[j] = c[j] >= 0 ? record_value(head[i].x, head[i].y, (int)(codes[i] >> (BITS * j)) & ((1 << BITS) - 1)) : -INFINITY;
       }
-      vo[q] = make_float4(v[0], v[1], v[2], v[3]);
-      io[q] = make_int4(idx[0], idx[1], idx[2], idx[3]);
+      if (r < n) {
+        *(reinterpret_cast<float4*>(values + r * K) + q) = make_float4(v[0], v[1], v[2], v[3]);
+        *(reinterpret_cast<int4*>(index + r * K) + q) = make_int4(c[0], c[1], c[2], c[3]);
+      }
     }
   }
 }
@@ -481,7 +492,7 @@ __global__ void __launch_bounds__(256) k_teacher_read_whole(const uint8_t* __res
 template <int K>
 static int launch_read_whole(const void* records, int64_t n_records, const int64_t* rows, int64_t first_row, int64_t n,
                              int bits, float* values, int32_t* index, cudaStream_t st) {
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, 256), 148 * 32);
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n, 256 / (K / 4) * 2), 148 * 32);
   auto* kernel = bits == 8 ? k_teacher_read_whole<K, 8> : k_teacher_read_whole<K, 4>;
   kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(records), n_records, rows, first_row, n, values, index);
   return check_launch("k_teacher_read_whole");
