@@ -248,3 +248,18 @@ def test_outputs_at_any_element_leave_their_surroundings(c, offset):
              flat.data_ptr() + 2 * offset, None, 0, nat.stream())
     assert torch.equal(flat[offset:offset + n * c].reshape(n, c), want)
     assert (flat[:offset] == 5.0).all() and (flat[offset + n * c:] == 5.0).all()
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 outputs, and gradients of them through padded rows: the last rows are those of a call of their own."""
+    n, d, f, c = 14_400_003, 15, 64, 150
+    _, wg, wu, wd, _ = _inputs(1, d, f, c, "bf16")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.empty((n, d), device="cuda", dtype=torch.bfloat16).normal_(generator=g).requires_grad_(True)
+    y = decode_features(x, wg, wu, wd)
+    dy = y.detach() * 0.5
+    dx, = torch.autograd.grad(y, x, dy)
+    tail = x.detach()[-999:].clone().requires_grad_(True)
+    own = decode_features(tail, wg, wu, wd)
+    assert torch.equal(y.detach()[-999:], own.detach())
+    assert torch.equal(dx[-999:], torch.autograd.grad(own, tail, dy[-999:])[0])

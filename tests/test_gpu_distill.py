@@ -391,3 +391,22 @@ def test_kernels_are_counted():
     cache = TeacherCache(4, 2, 5)
     cache.write(0, torch.zeros((4, 5), device="cuda"))
     assert lib.gs_kernel_launch_count() > before
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 logits: the last rows are those of a call of their own."""
+    n, c, k = 14_400_003, 150, 8
+    s = torch.empty((n, c), device="cuda", dtype=torch.bfloat16).normal_(generator=_gen(1))
+    cache = TeacherCache(n, k, c)
+    cache.write(0, s)
+    v, i = cache.read(slice(n - 999, n))
+    own = TeacherCache(999, k, c)
+    own.write(0, s[-999:])
+    want_v, want_i = own.read(slice(None))
+    assert torch.equal(v, want_v) and torch.equal(i, want_i)
+    picked = torch.arange(n - 999, n, device="cuda")
+    assert torch.equal(cache.read(picked)[1], want_i)
+    s.mul_(-0.5)  # not the teacher's own logits
+    loss, grad = distill_loss_and_grad(s, cache.at(slice(0, n)), 2.0, reduction="none")
+    want_l, want_g = distill_loss_and_grad(s[-999:], own.at(slice(0, 999)), 2.0, reduction="none")
+    assert torch.equal(loss[-999:], want_l) and torch.equal(grad[-999:], want_g)
