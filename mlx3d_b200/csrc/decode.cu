@@ -1166,7 +1166,8 @@ static int launch_decode_as(DecodeArgs a, dim3 grid, cudaStream_t s) {
   // one CTA per SM: each takes all of TMEM
   const size_t smem = std::max<size_t>(plan_smem<MODE>(a), 120 * 1024);
   auto* kernel = MODE == kDw ? k_decode_dw<T, ACT> : k_decode<T, MODE == kDx ? kDx : kFwd, ACT>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // (always the same limit: threads may launch different sizes at once)
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMaxSmem);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_decode: %s", cudaGetErrorString(e));
   kernel<<<grid, MODE == kDw ? kDwThreads : kDecodeThreads, smem, s>>>(a);
   return check_launch("k_decode");
@@ -1244,7 +1245,8 @@ int gs_decode_forward_few(const void* x, const void* w_gate, const void* w_up, c
     using T = decltype(zero);
     auto* kernel = activation == GS_ACT_SILU ? k_decode_few<T, GS_ACT_SILU> : k_decode_few<T, GS_ACT_GELU>;
     if (smem > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+      const int most = 4 * (GS_DECODE_MAX_D + GS_DECODE_FEW_WEIGHTS / 3);  // of any call
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_decode_few: %s", cudaGetErrorString(e));
     }
     kernel<<<(unsigned)n, kFewThreads, smem, as_stream(stream)>>>(

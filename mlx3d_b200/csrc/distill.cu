@@ -689,7 +689,8 @@ static int launch_warps(const DistillArgs& a, cudaStream_t st, unsigned* blocks)
   const size_t smem = own * warps;
   auto* kernel = a.classes % 2 ? k_distill_warp<T, G, EACH, FULL, KEEP, true>
                                : k_distill_warp<T, G, EACH, FULL, KEEP, false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  // (always the same limit, what the static part leaves: threads may launch different sizes at once)
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_warp: %s", cudaGetErrorString(e));
   const int64_t resident = 148 * std::max<int64_t>(1, std::min<int64_t>(16, (227 * 1024) / (int64_t)(smem + 1024)));
   *blocks = (unsigned)std::min<int64_t>(ceil_div(ceil_div(a.n, rows), warps), resident);

@@ -508,7 +508,7 @@ static int launch_rows(const TeacherWriteArgs& a, cudaStream_t st) {
   const size_t smem = std::max((size_t)rows * row, (size_t)rows * (a.rec_bytes + 4));
   auto* kernel = k_teacher_write_rows<T, MAX>;
   if (smem > 40 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kStagedSmem);
     if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_teacher_write_rows: %s", cudaGetErrorString(e));
   }
   kernel<<<(unsigned)ceil_div(a.n, rows), rows, smem, st>>>(a, rows, aligned(a.logits, 16));

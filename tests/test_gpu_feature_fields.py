@@ -1,14 +1,16 @@
 """A semantic feature field end to end: render, decode, distil from the teacher
 cache, gradients into the per-Gaussian features and the decoder."""
 
+import threading
+
 import pytest
 import torch
 
 from feature_helpers import distill64
 from helpers import random_scene
 from mlx3d_b200 import splatting as gs
-from mlx3d_b200.losses import distill_loss
-from mlx3d_b200.splatting import FeatureDecoder, GaussianModel, GaussianTrainer
+from mlx3d_b200.losses import distill_loss, distill_loss_and_grad
+from mlx3d_b200.splatting import FeatureDecoder, GaussianModel, GaussianTrainer, decode_features
 from mlx3d_b200.staging import TeacherCache
 
 pytestmark = pytest.mark.gpu
@@ -97,3 +99,43 @@ def test_distill_view_refuses_float16_decoders():
     dec = FeatureDecoder.create(8, 16, 3, dtype=torch.float16, generator=g)
     with pytest.raises(ValueError, match="bfloat16"):
         GaussianTrainer(model).distill_view(cam, feats, (torch.zeros(1, 1), torch.zeros(1, 1).int()), dec)
+
+
+def test_calls_of_several_threads_at_once():
+    """Different sizes of every operator from threads with streams of their own, again and again."""
+    def work(seed, n, d, f, c, k):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rnd = lambda *s: torch.randn(s, device="cuda", generator=g).to(torch.bfloat16)  # noqa: E731
+        leaves = [t.requires_grad_(True) for t in (rnd(n, d), rnd(f, d), rnd(f, d), rnd(c, f))]
+        cache = TeacherCache(n, k, c)
+        cache.write(0, rnd(n, c))
+
+        def once():
+            y = decode_features(*leaves)
+            loss, grad = distill_loss_and_grad(y.detach(), cache.at(slice(0, n)))
+            return [loss, *torch.autograd.grad(y, leaves, grad)]
+        return once
+
+    jobs = [work(1, 3000, 64, 256, 150, 8), work(2, 700, 16, 64, 20, 5), work(3, 5000, 128, 128, 250, 32),
+            work(4, 40, 9, 30, 201, 3)]
+    wants = [job() for job in jobs]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(job, want):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(60):
+                    got = job()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    failed.append("different results")
+        except Exception as e:  # noqa: BLE001
+            failed.append(repr(e))
+
+    threads = [threading.Thread(target=run, args=a) for a in zip(jobs, wants)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
