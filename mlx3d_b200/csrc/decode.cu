@@ -335,8 +335,14 @@ struct GateIn {
   }
 };
 
-// 32 columns of an output row (or `left`, if fewer), in stores of `vec` bytes.
-__device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16], int left, int vec) {
+// 32 columns of an output row (or `left`, if fewer), in stores of `vec` bytes.  Rows
+// of 2-byte alignment are written in words all the same: a row that starts inside one
+// (`odd`) stores its columns (2e - 1, 2e) together, `before` being the word of the two
+// columns before these (first: there are none), and single columns at its ends: column
+// by column, the drain warps held up everything else (forward of 1600x1060 rows,
+// 32-128-151: 373 us instead of 262).
+__device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16], int left, int vec, bool odd,
+                                            uint32_t before, bool first) {
   if (vec == 4 && left >= 32) {  // (the tests below cost as much as the stores)
 #pragma unroll
     for (int e = 0; e < 16; ++e) *reinterpret_cast<uint32_t*>(p + 4 * e) = w[e];
@@ -354,9 +360,25 @@ __device__ __forceinline__ void store_row32(uint8_t* p, const uint32_t (&w)[16],
     for (int e = 0; e < 16; ++e)
       if (2 * e < left) *reinterpret_cast<uint32_t*>(p + 4 * e) = w[e];
   } else {
+    // (no branches: lanes of both kinds sit side by side)
+    uint8_t* q = odd ? p - 2 : p;
+    const uint32_t bytes = odd ? 0x5432 : 0x7654;
+    if (odd ? !first : left > 1) *reinterpret_cast<uint32_t*>(q) = __byte_perm(before, w[0], bytes);
+    if (odd && first) *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    if (left > 32) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (e < left) *reinterpret_cast<uint16_t*>(p + 2 * e) = (uint16_t)(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]);
+      for (int e = 1; e < 16; ++e) *reinterpret_cast<uint32_t*>(q + 4 * e) = __byte_perm(w[e - 1], w[e], bytes);
+    } else {
+      const int words = odd ? left : left - 1;
+      uint32_t last = w[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) {
+        if (2 * e < words) *reinterpret_cast<uint32_t*>(q + 4 * e) = __byte_perm(w[e - 1], w[e], bytes);
+        if (2 * e < left) last = w[e];
+      }
+      if ((left & 1) != (odd ? 1 : 0))
+        *reinterpret_cast<uint16_t*>(p + 2 * left - 2) = (uint16_t)(left & 1 ? last : last >> 16);
+    }
   }
 }
 
@@ -585,6 +607,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
       uint8_t* p = staged ? os + row * a.out_pitch : static_cast<uint8_t*>(a.out) + (t * kTile + row) * width * 2;
       // Up to 160 columns are read and rounded before any is stored: the next
       // tile's second products wait for the accumulator.
+      const bool odd = reinterpret_cast<uintptr_t>(p) & 2;
+      uint32_t before = 0;
       for (int c0 = 0; c0 < width; c0 += 160, p += 320) {
         uint32_t w[5][16];
 #pragma unroll
@@ -605,7 +629,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 1) k_decode(const __grid_const
         }
 #pragma unroll
         for (int g = 0; g < 5; ++g)
-          if (here && c0 + 32 * g < width) store_row32(p + 64 * g, w[g], width - c0 - 32 * g, a.out_vec);
+          if (here && c0 + 32 * g < width)
+            store_row32(p + 64 * g, w[g], width - c0 - 32 * g, a.out_vec, odd, g > 0 ? w[g > 0 ? g - 1 : 0][15] : before,
+                        c0 + g == 0);
+        before = w[4][15];
       }
       __syncwarp();
       if (a.out_bulk) {
