@@ -232,7 +232,7 @@ def test_many_tiles_of_every_plan(f, d, c):
     assert _wait_failures() == 0
 
 
-@pytest.mark.parametrize("c", [7, 64, 150])
+@pytest.mark.parametrize("c", [1, 2, 7, 33, 64, 150, 161, 163, 192, 225, 255])
 @pytest.mark.parametrize("offset", [1, 2, 4, 8])
 def test_outputs_at_any_element_leave_their_surroundings(c, offset):
     n, d, f = 1301, 24, 96
