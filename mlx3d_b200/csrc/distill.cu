@@ -5,7 +5,7 @@
 //   L = w T^2 sum_k p_k (log p_k - log q_{i_k}),  dL/ds_c = w T (q_c - sum_{i_k = c} p_k)
 //
 // Bound by memory: the logits are read once and the gradient written once.
-//   k_distill_warp  up to 1536 classes: every warp walks tiles of its own, loaded
+//   k_distill_warp  up to 256 classes: every warp walks tiles of its own, loaded
 //                   and stored by bulk copies, with no block barrier; dozens of
 //                   warps per SM overlap their copies with each other's
 //                   arithmetic.  The classes of a row are shared by 4 to 32 lanes;
@@ -13,6 +13,7 @@
 //                   whole warp.  Instructions bound it: 1920x1080x150 in float32
 //                   takes 466 us (67% of DRAM's rate), with one lane per row for
 //                   the entries (8 of 32 busy) 536.
+//   k_distill_long  rows that fit in a warp's registers: one warp per row.
 //   k_distill_row   longer rows: one block per row.
 #include "feature_common.cuh"
 
@@ -336,9 +337,6 @@ __device__ __forceinline__ float class_row(const T* s, const float2* ent, float2
 
 // Shared memory of a warp: two tiles, then entries, fixes, row states.
 constexpr int kWarpBuffers = 2;
-// Rows of a tile whose exponentials are not kept (all tiles have a multiple of 8
-// rows, which is one of 16 bytes).
-constexpr int kTileRows = 8;
 __host__ __device__ inline size_t warp_tile_bytes(int rows, int64_t classes, int elem) {
   return ((size_t)rows * classes * elem + 127) & ~(size_t)127;
 }
@@ -349,12 +347,12 @@ __host__ __device__ inline size_t warp_smem(int rows, int64_t classes, int elem,
 // G lanes share a row, each holding EACH of its logits in registers, as pairs of
 // neighbours; the first FULL of them exist for sure.  Pairs are aligned: with an ODD
 // number of classes every second row starts inside one, and shares its first and last
-// pair with the rows beside it.  With KEEP the exponentials of all rows of the
-// tile (KEEP rounds of 32 / G rows) stay in registers for the gradient; otherwise
-// they are computed again.
-template <typename T, int G, int EACH, int FULL, int KEEP, bool ODD>
-__global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int bulk_in, int bulk_out) {
-  constexpr int tile_rows = KEEP > 0 ? KEEP * (32 / G) : kTileRows;
+// pair with the rows beside it.  The exponentials of all rows of the tile (ROUNDS
+// times 32 / G, a multiple of 8, which is one of 16 bytes) stay in registers for the
+// gradient.
+template <typename T, int G, int EACH, int FULL, int ROUNDS, bool ODD>
+__global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int bulk_in, int bulk_out) {
+  constexpr int tile_rows = ROUNDS * (32 / G);
   // lanes per row for the teacher's entries, and entries of a lane where k <= 8
   constexpr int L = tile_rows >= 32 ? 1 : 32 / tile_rows, kFew = 8 / L;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -422,8 +420,7 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
     }
     __syncwarp();
     // the student's maximum and sum, by the rows' lanes
-    constexpr int kRounds = KEEP > 0 ? KEEP : 1;
-    F2 kept[kRounds][EACH / 2];
+    F2 kept[ROUNDS][EACH / 2];
     // the first class of a lane's pair i; -1 for the first pair of a row that starts inside it
     auto first_of = [&](int i, int lead) { return 2 * (lane + G * i) - lead; };
     auto lead_of = [&](int r) { return ODD ? r & 1 : 0; };
@@ -472,12 +469,8 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
         state[r].lse = ln_of(sum);
       }
     };
-    if constexpr (KEEP > 0) {
 #pragma unroll
-      for (int q = 0; q < KEEP; ++q) exponentials(q * (32 / G), kept[q]);
-    } else {
-      for (int rr = 0; rr < rows; rr += 32 / G) exponentials(rr, kept[0]);
-    }
+    for (int q = 0; q < ROUNDS; ++q) exponentials(q * (32 / G), kept[q]);
     __syncwarp();
     // the loss and the gradients of the teacher's classes
     for (int rr = 0; rr < rows; rr += 32 / L) {
@@ -507,7 +500,7 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
 #pragma unroll
         for (int i = 0; i < EACH / 2; ++i) {
           const int c = first_of(i, lead);
-          const F2 g = st.any ? mul(KEEP > 0 ? v[i] : scaled(read(s, i, lead, 0.0f), st.m), f) : f2(0.0f);
+          const F2 g = st.any ? mul(v[i], f) : f2(0.0f);
           if constexpr (ODD) {
             const bool low = i > 0 || c >= 0, high = 2 * i + 1 < FULL || c + 1 < C;
             if (low && high) {
@@ -522,12 +515,8 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
           }
         }
       };
-      if constexpr (KEEP > 0) {
 #pragma unroll
-        for (int q = 0; q < KEEP; ++q) gradients(q * (32 / G), kept[q]);
-      } else {
-        for (int rr = 0; rr < rows; rr += 32 / G) gradients(rr, kept[0]);
-      }
+      for (int q = 0; q < ROUNDS; ++q) gradients(q * (32 / G), kept[q]);
       __syncwarp();
       const uint32_t per_k = 0xffffffffu / k + 1;
       for (int i = wl; i < rows * k; i += 32) {
@@ -559,6 +548,122 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * KEEP >= 40 ? 5 : 6) k_disti
   if (a.partials) block_partial(acc, a.partials + blockIdx.x);
 }
 
+// A row in 16-byte units of memory, the first and last of which may reach outside it.
+template <typename T>
+struct RowUnits {
+  static constexpr int kUnit = 16 / sizeof(T);
+  union Unit {
+    uint4 all;
+    T e[kUnit];
+  };
+  const T* src;
+  int classes, lead, units;  // lead: elements before the row in its first unit
+  __device__ __forceinline__ RowUnits(const T* s, int c) : src(s), classes(c) {
+    lead = (int)((reinterpret_cast<uintptr_t>(s) & 15) / sizeof(T));
+    units = (lead + c + kUnit - 1) / kUnit;
+  }
+  __device__ __forceinline__ bool whole(int u) const {
+    return u * kUnit >= lead && (u + 1) * kUnit <= lead + classes;
+  }
+  __device__ __forceinline__ Unit read(int u) const {  // elements outside the row are -inf
+    Unit v;
+    if (whole(u)) {
+      v.all = __ldg(reinterpret_cast<const uint4*>(src - lead) + u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) {
+        const int c = u * kUnit + i - lead;
+        v.e[i] = c >= 0 && c < classes ? src[c] : from_f32<T>(-INFINITY);
+      }
+    }
+    return v;
+  }
+  // vector: g starts in a unit where the row does
+  __device__ __forceinline__ void write(T* g, int u, const Unit& v, bool vector) const {
+    if (vector && whole(u)) {
+      reinterpret_cast<uint4*>(g - lead)[u] = v.all;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kUnit; ++i) {
+        const int c = u * kUnit + i - lead;
+        if (c >= 0 && c < classes) g[c] = v.e[i];
+      }
+    }
+  }
+};
+
+// One warp per row, the row in its registers: UNITS 16-byte units a lane, straight
+// from global memory, which is read once.  Tiles of 8 such rows in shared memory left
+// four warps per SM: 200000 rows of 1000 in float16, 32 entries, loss and gradient
+// 1008 us instead of 346; 153846 of 1300 in float32 2037 instead of 364.
+constexpr int kLongBlock = 128;
+template <typename T, int UNITS>
+__global__ void __launch_bounds__(kLongBlock, UNITS == 4 ? 6 : UNITS == 8 ? 5 : 4) k_distill_long(DistillArgs a, int vector_out) {
+  extern __shared__ float2 entries[];
+  using Units = RowUnits<T>;
+  const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float2 *ent = entries + warp * 2 * k, *fix = ent + k;
+  const float c2 = a.inv_temp * kLog2e;
+  double acc = 0.0;
+  for (int64_t r = (int64_t)blockIdx.x * (kLongBlock / 32) + warp; r < a.n; r += (int64_t)gridDim.x * (kLongBlock / 32)) {
+    const Units row(static_cast<const T*>(a.logits) + r * C, C);
+    typename Units::Unit v[UNITS];
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i) v[i] = row.read(lane + 32 * i);
+    stage_entries<32>(a, ent, r, 1, lane);
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+      for (int e = 0; e < Units::kUnit; ++e) m = fmaxf(m, to_f32(v[i].e[e]));
+    m = group_max<32>(m);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+      for (int e = 0; e < Units::kUnit; ++e) sum += exp2_of((to_f32(v[i].e[e]) - m) * c2);
+    sum = group_sum<32>(sum);
+    __syncwarp();
+    const float w = a.weight ? a.weight[r] : 1.0f;
+    const float f = w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r : 0] : 1.0f);
+    auto logit = [&](int i) { return to_f32(row.src[i]); };
+    float term;
+    const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
+    const float inv = rcp_of(sum);
+    if (lane == 0) {
+      const float loss = any ? (term + ln_of(sum)) * (a.temp * a.temp) * w : 0.0f;
+      if (a.row_loss) a.row_loss[r] = loss;
+      acc += (double)loss;
+    }
+    __syncwarp();
+    if (a.grad) {
+      T* g = static_cast<T*>(a.grad) + r * C;
+      bool repeats = k > 32;  // (looked for entry by entry there)
+      if (!repeats) {
+        const int idx = lane < k ? __float_as_int(ent[lane].x) : -1;
+        const unsigned same = __match_any_sync(~0u, idx >= 0 ? idx : -1 - lane);
+        repeats = __any_sync(~0u, (same & (same - 1)) != 0);
+      }
+      class_gradients<32>(ent, fix, any ? k : 0, repeats, lane, m, c2, inv, f, logit);
+      const float qf = inv * f;
+#pragma unroll
+      for (int i = 0; i < UNITS; ++i) {
+        const int u = lane + 32 * i;
+#pragma unroll
+        for (int e = 0; e < Units::kUnit; ++e)
+          v[i].e[e] = from_f32<T>(any ? exp2_of((to_f32(v[i].e[e]) - m) * c2) * qf : 0.0f);
+        if (u < row.units) row.write(g, u, v[i], vector_out);
+      }
+      __syncwarp();
+      if (any)
+        for (int e = lane; e < k; e += 32)
+          if (__float_as_int(fix[e].x) >= 0) g[__float_as_int(fix[e].x)] = from_f32<T>(fix[e].y);
+    }
+    __syncwarp();
+  }
+  if (a.partials) block_partial(acc, a.partials + blockIdx.x);
+}
+
 // One block per row.  A row starts anywhere; it is moved in 16-byte units of
 // memory, the first and last of which may reach outside it and are taken element
 // by element.  Each of the three passes reads the row, the later ones from L2:
@@ -568,38 +673,19 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int vector_out) {
   __shared__ float red[kRowThreads / 32], stats[2];
   __shared__ float2 ent[GS_TEACHER_MAX_K], fix[GS_TEACHER_MAX_K];
-  constexpr int kUnit = 16 / sizeof(T);
-  union Unit {
-    uint4 all;
-    T e[kUnit];
-  };
+  using Units = RowUnits<T>;
+  constexpr int kUnit = Units::kUnit;
   const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float c2 = a.inv_temp * kLog2e;
   double acc = 0.0;
   for (int64_t r = blockIdx.x; r < a.n; r += gridDim.x) {
-    const T* src = static_cast<const T*>(a.logits) + r * C;
-    const int lead = (int)((reinterpret_cast<uintptr_t>(src) & 15) / sizeof(T));  // elements before the row
-    const int units = (lead + C + kUnit - 1) / kUnit;
-    const uint4* from = reinterpret_cast<const uint4*>(src - lead);
-    auto whole = [&](int u) { return u * kUnit >= lead && (u + 1) * kUnit <= lead + C; };
-    auto read = [&](int u) {  // elements outside the row are -inf
-      Unit v;
-      if (whole(u)) {
-        v.all = __ldg(from + u);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kUnit; ++i) {
-          const int c = u * kUnit + i - lead;
-          v.e[i] = c >= 0 && c < C ? src[c] : from_f32<T>(-INFINITY);
-        }
-      }
-      return v;
-    };
+    const Units row(static_cast<const T*>(a.logits) + r * C, C);
+    const int units = row.units;
     stage_entries<kRowThreads>(a, ent, r, 1, threadIdx.x);
     float m = -INFINITY;
 #pragma unroll 4
     for (int u = threadIdx.x; u < units; u += kRowThreads) {
-      const Unit v = read(u);
+      const typename Units::Unit v = row.read(u);
 #pragma unroll
       for (int i = 0; i < kUnit; ++i) m = fmaxf(m, to_f32(v.e[i]));
     }
@@ -611,7 +697,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
     float sum = 0.0f;
 #pragma unroll 2
     for (int u = threadIdx.x; u < units; u += kRowThreads) {
-      const Unit v = read(u);
+      const typename Units::Unit v = row.read(u);
 #pragma unroll
       for (int i = 0; i < kUnit; ++i) sum += exp2_of((to_f32(v.e[i]) - m) * c2);
     }
@@ -622,7 +708,7 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
     const float f = w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r : 0] : 1.0f);
     if (warp == 0) {
       sum = group_sum<32>(lane < kRowThreads / 32 ? red[lane] : 0.0f);
-      auto logit = [&](int i) { return to_f32(src[i]); };
+      auto logit = [&](int i) { return to_f32(row.src[i]); };
       float term;
       const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
       __syncwarp();
@@ -641,22 +727,13 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
       T* g = static_cast<T*>(a.grad) + r * C;
       const bool any = stats[1] > 0.0f;
       const float qf = stats[0] * f;
-      uint4* to = reinterpret_cast<uint4*>(g - lead);  // (vector_out: aligned as the logits)
 #pragma unroll 2
       for (int u = threadIdx.x; u < units; u += kRowThreads) {
-        Unit v;
-        if (any) v = read(u);
+        typename Units::Unit v;
+        if (any) v = row.read(u);
 #pragma unroll
         for (int i = 0; i < kUnit; ++i) v.e[i] = from_f32<T>(any ? exp2_of((to_f32(v.e[i]) - m) * c2) * qf : 0.0f);
-        if (vector_out && whole(u)) {
-          to[u] = v.all;
-        } else {
-#pragma unroll
-          for (int i = 0; i < kUnit; ++i) {
-            const int c = u * kUnit + i - lead;
-            if (c >= 0 && c < C) g[c] = v.e[i];
-          }
-        }
+        row.write(g, u, v, vector_out);
       }
       __syncthreads();
       if (any)
@@ -680,15 +757,15 @@ __global__ void k_distill_finish(const double* partials, int n, double scale, fl
   if (threadIdx.x == 0) *loss = (float)(part[0] * scale);
 }
 
-template <typename T, int G, int EACH, int FULL, int KEEP>
+template <typename T, int G, int EACH, int FULL, int ROUNDS>
 static int launch_warps(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
-  const int64_t rows = KEEP > 0 ? KEEP * (32 / G) : kTileRows;
+  const int64_t rows = ROUNDS * (32 / G);
   const size_t own = warp_smem((int)rows, a.classes, sizeof(T), a.t.k);
   int warps = kWarpBlock / 32;
   while (warps > 1 && own * warps > 100 * 1024) warps /= 2;
   const size_t smem = own * warps;
-  auto* kernel = a.classes % 2 ? k_distill_warp<T, G, EACH, FULL, KEEP, true>
-                               : k_distill_warp<T, G, EACH, FULL, KEEP, false>;
+  auto* kernel = a.classes % 2 ? k_distill_warp<T, G, EACH, FULL, ROUNDS, true>
+                               : k_distill_warp<T, G, EACH, FULL, ROUNDS, false>;
   // (always the same limit, what the static part leaves: threads may launch different sizes at once)
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
   if (e != cudaSuccess) return set_error(GS_ERR_CUDA, "k_distill_warp: %s", cudaGetErrorString(e));
@@ -710,11 +787,18 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* block
   if (c <= 128) return launch_warps<T, 8, 16, 12, 2>(a, st, blocks);
   if (c <= 160) return launch_warps<T, 8, 20, 16, 2>(a, st, blocks);
   if (c <= 256) return launch_warps<T, 16, 16, 10, 4>(a, st, blocks);
-  if (c <= 512) return launch_warps<T, 16, 32, 16, 0>(a, st, blocks);
-  if (c <= 1024) return launch_warps<T, 32, 32, 16, 0>(a, st, blocks);
-  if (c <= 1536 && a.t.k <= 64) return launch_warps<T, 32, 48, 32, 0>(a, st, blocks);
-  *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
   const bool alike = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
+  // Longer rows that fit in a warp's registers from wherever they start.
+  constexpr int kUnit = 16 / sizeof(T), kPerUnit = 32 * kUnit;
+  if (c <= 12 * kPerUnit - (kUnit - 1)) {
+    *blocks = (unsigned)std::min<int64_t>(ceil_div(a.n, kLongBlock / 32), kDistillMaxBlocks);
+    auto* kernel = c <= 4 * kPerUnit - (kUnit - 1)   ? k_distill_long<T, 4>
+                   : c <= 8 * kPerUnit - (kUnit - 1) ? k_distill_long<T, 8>
+                                                     : k_distill_long<T, 12>;
+    kernel<<<*blocks, kLongBlock, kLongBlock / 32 * 2 * sizeof(float2) * a.t.k, st>>>(a, alike);
+    return check_launch("k_distill_long");
+  }
+  *blocks = (unsigned)std::min<int64_t>(a.n, kDistillMaxBlocks);
   k_distill_row<T><<<*blocks, kRowThreads, 0, st>>>(a, alike);
   return check_launch("k_distill_row");
 }

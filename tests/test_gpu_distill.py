@@ -65,8 +65,8 @@ def test_distill_matches_the_definition(n, c, k, t, dtype):
 @pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 def test_every_split_of_a_row(dtype, k):
     """Class counts on both sides of every split; odd ones start every second row inside a pair of classes."""
-    for c in (1, 2, 3, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 97, 127, 128, 129, 159, 160, 161, 255, 257, 511, 513,
-              1023, 1025, 1535, 1536, 1537):
+    for c in (1, 2, 3, 15, 16, 17, 31, 32, 33, 63, 64, 65, 95, 97, 127, 128, 129, 159, 160, 161, 255, 257, 509, 510, 513,
+              1017, 1018, 1021, 1022, 1025, 1533, 1534, 1537, 2041, 2043):
         s, v, i, w = _inputs(75, c, k, dtype, dtype, seed=c)
         loss, grad = distill_loss_and_grad(s, (v, i), temperature=1.0, weight=w, reduction="none")
         _check(s, v, i, w, 1.0, loss, grad)
