@@ -5,7 +5,7 @@
 //   L = w T^2 sum_k p_k (log p_k - log q_{i_k}),  dL/ds_c = w T (q_c - sum_{i_k = c} p_k)
 //
 // Bound by memory: the logits are read once and the gradient written once.
-//   k_distill_warp  up to 256 classes: every warp walks tiles of its own, loaded
+//   k_distill_warp  short rows: every warp walks tiles of its own, loaded
 //                   and stored by bulk copies, with no block barrier; dozens of
 //                   warps per SM overlap their copies with each other's
 //                   arithmetic.  The classes of a row are shared by 4 to 32 lanes;
@@ -337,6 +337,7 @@ __device__ __forceinline__ float class_row(const T* s, const float2* ent, float2
 
 // Shared memory of a warp: two tiles, then entries, fixes, row states.
 constexpr int kWarpBuffers = 2;
+constexpr int kTileRows = 8;
 __host__ __device__ inline size_t warp_tile_bytes(int rows, int64_t classes, int elem) {
   return ((size_t)rows * classes * elem + 127) & ~(size_t)127;
 }
@@ -349,10 +350,10 @@ __host__ __device__ inline size_t warp_smem(int rows, int64_t classes, int elem,
 // number of classes every second row starts inside one, and shares its first and last
 // pair with the rows beside it.  The exponentials of all rows of the tile (ROUNDS
 // times 32 / G, a multiple of 8, which is one of 16 bytes) stay in registers for the
-// gradient.
+// gradient; with ROUNDS = 0 a tile has kTileRows rows and they are computed again.
 template <typename T, int G, int EACH, int FULL, int ROUNDS, bool ODD>
 __global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_distill_warp(DistillArgs a, int bulk_in, int bulk_out) {
-  constexpr int tile_rows = ROUNDS * (32 / G);
+  constexpr int tile_rows = ROUNDS > 0 ? ROUNDS * (32 / G) : kTileRows;
   // lanes per row for the teacher's entries, and entries of a lane where k <= 8
   constexpr int L = tile_rows >= 32 ? 1 : 32 / tile_rows, kFew = 8 / L;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_dis
     }
     __syncwarp();
     // the student's maximum and sum, by the rows' lanes
-    F2 kept[ROUNDS][EACH / 2];
+    F2 kept[ROUNDS > 0 ? ROUNDS : 1][EACH / 2];
     // the first class of a lane's pair i; -1 for the first pair of a row that starts inside it
     auto first_of = [&](int i, int lead) { return 2 * (lane + G * i) - lead; };
     auto lead_of = [&](int r) { return ODD ? r & 1 : 0; };
@@ -469,8 +470,12 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_dis
         state[r].lse = ln_of(sum);
       }
     };
+    if constexpr (ROUNDS > 0) {
 #pragma unroll
-    for (int q = 0; q < ROUNDS; ++q) exponentials(q * (32 / G), kept[q]);
+      for (int q = 0; q < ROUNDS; ++q) exponentials(q * (32 / G), kept[q]);
+    } else {
+      for (int rr = 0; rr < rows; rr += 32 / G) exponentials(rr, kept[0]);
+    }
     __syncwarp();
     // the loss and the gradients of the teacher's classes
     for (int rr = 0; rr < rows; rr += 32 / L) {
@@ -500,7 +505,7 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_dis
 #pragma unroll
         for (int i = 0; i < EACH / 2; ++i) {
           const int c = first_of(i, lead);
-          const F2 g = st.any ? mul(v[i], f) : f2(0.0f);
+          const F2 g = st.any ? mul(ROUNDS > 0 ? v[i] : scaled(read(s, i, lead, 0.0f), st.m), f) : f2(0.0f);
           if constexpr (ODD) {
             const bool low = i > 0 || c >= 0, high = 2 * i + 1 < FULL || c + 1 < C;
             if (low && high) {
@@ -515,8 +520,12 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_dis
           }
         }
       };
+      if constexpr (ROUNDS > 0) {
 #pragma unroll
-      for (int q = 0; q < ROUNDS; ++q) gradients(q * (32 / G), kept[q]);
+        for (int q = 0; q < ROUNDS; ++q) gradients(q * (32 / G), kept[q]);
+      } else {
+        for (int rr = 0; rr < rows; rr += 32 / G) gradients(rr, kept[0]);
+      }
       __syncwarp();
       const uint32_t per_k = 0xffffffffu / k + 1;
       for (int i = wl; i < rows * k; i += 32) {
@@ -595,10 +604,10 @@ struct RowUnits {
 // One warp per row, the row in its registers: UNITS 16-byte units a lane, straight
 // from global memory, which is read once.  Tiles of 8 such rows in shared memory left
 // four warps per SM: 200000 rows of 1000 in float16, 32 entries, loss and gradient
-// 1008 us instead of 346; 153846 of 1300 in float32 2037 instead of 364.
+// 1008 us instead of 342; 153846 of 1300 in float32 2037 instead of 364.
 constexpr int kLongBlock = 128;
 template <typename T, int UNITS>
-__global__ void __launch_bounds__(kLongBlock, UNITS == 4 ? 6 : UNITS == 8 ? 5 : 4) k_distill_long(DistillArgs a, int vector_out) {
+__global__ void __launch_bounds__(kLongBlock, UNITS == 4 ? 8 : UNITS == 8 && sizeof(T) == 4 ? 6 : 4) k_distill_long(DistillArgs a, int vector_out) {
   extern __shared__ float2 entries[];
   using Units = RowUnits<T>;
   const int C = (int)a.classes, k = a.t.k, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -759,7 +768,7 @@ __global__ void k_distill_finish(const double* partials, int n, double scale, fl
 
 template <typename T, int G, int EACH, int FULL, int ROUNDS>
 static int launch_warps(const DistillArgs& a, cudaStream_t st, unsigned* blocks) {
-  const int64_t rows = ROUNDS * (32 / G);
+  const int64_t rows = ROUNDS > 0 ? ROUNDS * (32 / G) : kTileRows;
   const size_t own = warp_smem((int)rows, a.classes, sizeof(T), a.t.k);
   int warps = kWarpBlock / 32;
   while (warps > 1 && own * warps > 100 * 1024) warps /= 2;
@@ -788,6 +797,10 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* block
   if (c <= 160) return launch_warps<T, 8, 20, 16, 2>(a, st, blocks);
   if (c <= 256) return launch_warps<T, 16, 16, 10, 4>(a, st, blocks);
   const bool alike = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
+  // Rows of little more than a kilobyte keep too few of a warp's loads in flight below:
+  // loss and gradient of 666667 rows of 300 in float16 take 376 us here, 1019 there; 500000
+  // of 400 in float32 701 here, 487 there.
+  if (c <= 512 && c * sizeof(T) <= 1280) return launch_warps<T, 16, 32, 16, 0>(a, st, blocks);
   // Longer rows that fit in a warp's registers from wherever they start.
   constexpr int kUnit = 16 / sizeof(T), kPerUnit = 32 * kUnit;
   if (c <= 12 * kPerUnit - (kUnit - 1)) {
