@@ -410,3 +410,17 @@ def test_offsets_beyond_32_bits():
     loss, grad = distill_loss_and_grad(s, cache.at(slice(0, n)), 2.0, reduction="none")
     want_l, want_g = distill_loss_and_grad(s[-999:], own.at(slice(0, 999)), 2.0, reduction="none")
     assert torch.equal(loss[-999:], want_l) and torch.equal(grad[-999:], want_g)
+
+
+@pytest.mark.parametrize("c", [300, 700, 1201, 2041, 5001])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+def test_long_rows_off_their_vectors(dtype, c):
+    """Logits one element off a 16-byte boundary, the gradient on one."""
+    n, k = 37, 9
+    s, v, i, w = _inputs(n, c, k, dtype, dtype, seed=c)
+    flat = torch.zeros((n * c + 1,), device="cuda", dtype=s.dtype)
+    flat[1:] = s.reshape(-1)
+    off = flat[1:].reshape(n, c)
+    loss, grad = distill_loss_and_grad(off, (v, i), weight=w, reduction="none")
+    assert off.data_ptr() % 16 and grad.data_ptr() % 16 == 0
+    _check(s, v, i, w, 1.0, loss, grad)
