@@ -547,6 +547,8 @@ __global__ void __launch_bounds__(kWarpBlock, EACH * ROUNDS >= 40 ? 5 : 6) k_dis
         __syncwarp();
 #pragma unroll 4
         for (int i = wl; i < rows * C; i += 32) dst[i] = tile[i];
+        // the buffer's next bulk copy comes after these ordinary writes and reads of it
+        if (bulk_in) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
     }
     __syncwarp();

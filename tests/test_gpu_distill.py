@@ -1,5 +1,6 @@
 """Distillation loss and teacher cache on the GPU against plain 64-bit forms."""
 
+import ctypes
 import math
 
 import pytest
@@ -424,3 +425,24 @@ def test_long_rows_off_their_vectors(dtype, c):
     loss, grad = distill_loss_and_grad(off, (v, i), weight=w, reduction="none")
     assert off.data_ptr() % 16 and grad.data_ptr() % 16 == 0
     _check(s, v, i, w, 1.0, loss, grad)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
+@pytest.mark.parametrize("n,c", [(1_000_003, 20), (300_001, 133), (300_001, 150), (150_001, 300)])
+def test_gradients_off_their_vectors(n, c, dtype):
+    """Logits on a 16-byte boundary, the gradient one element off one, several tiles a warp: what is written over a
+    tile must not meet the copy that fills its buffer next."""
+    k = 4
+    s, v, i, w = _inputs(n, c, k, dtype, dtype, seed=c)
+    want_l, want_g = distill_loss_and_grad(s, (v, i), weight=w, reduction="none")
+    flat = torch.full((n * c + 64,), 5.0, device="cuda", dtype=s.dtype)
+    out = flat[1:1 + n * c].view(n, c)
+    loss = torch.empty((n,), device="cuda")
+    teacher = nat.GsTeacher(v.data_ptr(), i.data_ptr(), None, None, 0, 0, nat.DTYPES[v.dtype], k, 0)
+    for _ in range(3):
+        out.zero_()
+        assert s.data_ptr() % 16 == 0 and out.data_ptr() % 16 == s.element_size()
+        nat.call("gs_distill", s.data_ptr(), nat.DTYPES[s.dtype], n, c, ctypes.byref(teacher), 1.0, w.data_ptr(), 1.0,
+                 None, 1, loss.data_ptr(), None, out.data_ptr(), None, 0, nat.stream())
+        assert torch.equal(loss, want_l) and torch.equal(out, want_g)
+    assert flat[0] == 5.0 and (flat[1 + n * c:] == 5.0).all()
