@@ -28,6 +28,13 @@ constexpr int kPanel = kTile * 128;     // bytes of a 128-row panel
 // fetches, 4-19 (four warpgroups) activate.
 constexpr int kDecodeThreads = 512, kEpilogue = 256, kDrain = 128;
 constexpr int kDwThreads = 640, kDwEpilogue = 512;
+// Tiles of one sum in TMEM, 8 instructions each.  A matrix instruction cuts its products to
+// the last bit of a float32 accumulator, always towards zero: a sum of like-signed terms
+// loses 2^-22.2 of itself an instruction (measured: 1.4 % of the result after 16384 tiles).
+// Longer walks move their sums to 64-bit partial sums every 256 tiles, which leaves 2.1e-4,
+// less than half of float16's half step, and costs 1 % of the weight gradients' time for
+// 1600x1060 rows, 64-256-152; every 128 tiles 1.1e-4 and 3 %.
+constexpr int kSumTiles = 256;
 constexpr int kMaxXStages = 4, kMaxWStages = 16;
 constexpr uint32_t kTmemCols = 512;
 constexpr size_t kMaxSmem = 232448;     // 227 KB
@@ -49,7 +56,8 @@ struct DecodeArgs {
   CUtensorMap map_x, map_dy;  // x and dy in boxes of 128 rows of one panel
   const uint8_t* image;
   void* out;        // y or dx
-  float* partials;  // weight gradients: [split][gate f*d | up f*d | down c*f]
+  void* partials;   // weight gradients: [split][chunk][column of the sums in TMEM][row], float or (wide) double
+  int wide;         // some CTA sums over more than kSumTiles tiles
   int64_t n;
   int d, f, c;
   int dp, cp;    // d, c rounded up to 16
@@ -70,6 +78,10 @@ __host__ __device__ __forceinline__ int round_up(int v, int m) { return (v + m -
 // (gate first) of ceil(d / 64) panels, then Wd's columns of these hidden units
 // as one panel of cp rows.
 static int chunk_bytes_of(int d, int c) { return (d + 63) / 64 * kPanel + round_up(c, 16) * tc::kPanelRow; }
+
+// Columns of the weight gradients' sums: 128 rows of [dWg ; dWu] (64 or 128 columns), then
+// dWd in blocks of 128 rows and 64 columns.
+__host__ __device__ __forceinline__ int dw_columns(int d, int c) { return (d > 64 ? 128 : 64) + (c + 127) / 128 * 64; }
 
 template <typename T>
 __global__ void k_decode_prepare(const T* __restrict__ wg, const T* __restrict__ wu, const T* __restrict__ wd, int d,
@@ -740,7 +752,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
   Bars* b = reinterpret_cast<Bars*>(smem + a.bars_at);
   if (!panels_aligned(smem)) return;
   const int mblocks = (a.c + 127) / 128;
-  const int acc_cols = (a.dp > 64 ? 128 : 64) + mblocks * 64;
+  const int acc_cols = dw_columns(a.d, a.c);
   const int nbuf = acc_cols <= 192 ? 2 : 1;  // [g | u] buffers
   // TMEM: [g | u] at 0 (and 128), dh, the sums
   const uint32_t col_dh = nbuf * 128, col_gu = col_dh + 64, col_dd = col_gu + (a.dp > 64 ? 128 : 64);
@@ -844,7 +856,7 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
         ahead = true;
       }
       const uint32_t xd = tc::uniform(xn0 + xs.at * xstep), yd = xd + ypart;
-      const bool more = __all_sync(~0u, i > 0);
+      const bool more = __all_sync(~0u, i % kSumTiles != 0);
       if (tc::elect_one()) {
         tc::mma_ss(tgu, sn, xd, idg, more);
 #pragma unroll
@@ -877,6 +889,27 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
   } else if (warp >= 4) {
     const int wg = (warp >> 2) - 1, row = (warp & 3) * 32 + lane;  // 16 hidden units a thread
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    // The sums in TMEM to this CTA's partial sums (more: added to them), as they lie, so that
+    // a warp's 32 rows are neighbours in memory.
+    auto put_sums = [&](auto* partials, bool more) {
+      tc::fence_after();
+      auto* part = partials + ((size_t)blockIdx.x * gridDim.y + blockIdx.y) * dw_columns(a.d, a.c) * kTile + row;
+      auto put = [&](int col) {
+        uint32_t v[16];
+        __syncwarp();
+        tc::tmem_ld(lanes + col_gu + col, v);
+        tc::tmem_wait_ld();
+        tc::after_wait(v);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          auto* to = part + (col + e) * kTile;
+          *to = more ? *to + __uint_as_float(v[e]) : __uint_as_float(v[e]);
+        }
+      };
+      for (int c0 = wg * 16; c0 < a.dp; c0 += 64) put(c0);
+      for (int m = 0; m < mblocks; ++m) put((int)(col_dd - col_gu) + m * 64 + wg * 16);
+      tc::fence_before();
+    };
     bool ok = true;
     for (int64_t i = 0; i < mine; ++i) {
       const uint32_t buf = lanes + (nbuf == 2 ? (uint32_t)(i & 1) * 128 : 0) + wg * 16, dhc = lanes + col_dh + wg * 16;
@@ -896,6 +929,8 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
       // the previous tile's sums have read the panels
       if (i > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(i - 1) & 1));
       if (!ok) break;
+      // (this tile's sums, which start anew, wait for its panels, hence for these reads)
+      if (i > 0 && i % kSumTiles == 0) put_sums(static_cast<double*>(a.partials), i > kSumTiles);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const uint32_t off = tc::panel_offset(row, wg * 2 + q);
@@ -909,35 +944,8 @@ __global__ void __launch_bounds__(kDwThreads, 1) k_decode_dw(const __grid_consta
     }
     if (ok && mine > 0) ok = __all_sync(~0u, wait_for(b, &b->sfree, (unsigned)(mine - 1) & 1));
     if (ok && mine > 0) {
-      tc::fence_after();
-      const size_t fd = (size_t)a.f * a.d;
-      float* part = a.partials + (size_t)blockIdx.x * (2 * fd + (size_t)a.c * a.f);
-      const int h = blockIdx.y * kChunk + (row & 63);
-      float* gu = part + (row < 64 ? 0 : fd) + (size_t)h * a.d;
-      for (int c0 = wg * 16; c0 < a.d; c0 += 64) {
-        uint32_t v[16];
-        __syncwarp();
-        tc::tmem_ld(lanes + col_gu + c0, v);
-        tc::tmem_wait_ld();
-        tc::after_wait(v);
-        if (h < a.f)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (c0 + e < a.d) gu[c0 + e] = __uint_as_float(v[e]);
-      }
-      for (int m = 0; m < mblocks; ++m) {
-        uint32_t v[16];
-        __syncwarp();
-        tc::tmem_ld(lanes + col_dd + m * 64 + wg * 16, v);
-        tc::tmem_wait_ld();
-        tc::after_wait(v);
-        const int c = m * 128 + row, h0 = blockIdx.y * kChunk + wg * 16;
-        if (c < a.c)
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            if (h0 + e < a.f) part[2 * fd + (size_t)c * a.f + h0 + e] = __uint_as_float(v[e]);
-      }
-      tc::fence_before();
+      if (a.wide) put_sums(static_cast<double*>(a.partials), mine > kSumTiles);
+      else put_sums(static_cast<float*>(a.partials), false);
     }
   }
   __syncthreads();
@@ -1001,17 +1009,30 @@ __global__ void __launch_bounds__(kFewThreads) k_decode_few(const T* __restrict_
   }
 }
 
-// Sums the splits' partial weight gradients in order and rounds once.
-template <typename T>
-__global__ void k_decode_reduce(const float* __restrict__ partials, int splits, int64_t fd, int64_t cf, T* dg, T* du,
+// Sums the splits' partial weight gradients (P) in order, in 64 bits, and rounds.  Threads
+// follow the partial sums' layout, of which each is read once.
+template <typename T, typename P>
+__global__ void k_decode_reduce(const P* __restrict__ partials, int splits, int chunks, int d, int f, int c, T* dg, T* du,
                                 T* dd) {
-  const int64_t total = 2 * fd + cf;
+  const int columns = dw_columns(d, c), first_dd = d > 64 ? 128 : 64;
+  const int64_t total = (int64_t)chunks * columns * kTile;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    float s = 0.0f;
+    const int row = (int)(i % kTile), col = (int)(i / kTile % columns);
+    const int h0 = (int)(i / kTile / columns) * kChunk;
+    T* out;
+    if (col < first_dd) {
+      const int h = h0 + (row & 63);
+      if (col >= d || h >= f) continue;
+      out = (row < 64 ? dg : du) + (size_t)h * d + col;
+    } else {
+      const int o = (col - first_dd) / 64 * 128 + row, h = h0 + (col & 63);
+      if (o >= c || h >= f) continue;
+      out = dd + (size_t)o * f + h;
+    }
+    double s = 0.0;
 #pragma unroll 8
     for (int p = 0; p < splits; ++p) s += partials[p * total + i];
-    T* out = i < fd ? dg + i : i < 2 * fd ? du + (i - fd) : dd + (i - 2 * fd);
-    *out = from_f32<T>(s);
+    *out = from_f32<T>((float)s);
   }
 }
 
@@ -1020,6 +1041,8 @@ static int decode_splits(int64_t n, int f) {
   const int64_t tiles = ceil_div(n, kTile);
   return (int)std::max<int64_t>(1, std::min<int64_t>(tiles, std::max(1, 148 / chunks)));
 }
+
+static bool decode_wide(int64_t n, int f) { return ceil_div(ceil_div(n, kTile), decode_splits(n, f)) > kSumTiles; }
 
 static int check_dims(const char* who, int64_t n, int dtype, int d, int f, int c) {
   if (dtype != GS_F16 && dtype != GS_BF16)
@@ -1246,7 +1269,9 @@ size_t gs_decode_workspace_bytes(const void* x, const void* dy, int64_t n, int d
   if (n < 0 || gs_decode_image_bytes(d, f, c) == 0) return 0;
   size_t bytes = fetchable(x, d) ? 0 : padded_bytes(n, d);
   if (dy && !fetchable(dy, c)) bytes += padded_bytes(n, c);
-  if (weights) bytes += (size_t)decode_splits(n, f) * (2 * (size_t)f * d + (size_t)c * f) * sizeof(float);
+  if (weights)
+    bytes += (size_t)decode_splits(n, f) * ((f + kChunk - 1) / kChunk) * dw_columns(d, c) * kTile *
+             (decode_wide(n, f) ? sizeof(double) : sizeof(float));
   return bytes;
 }
 
@@ -1320,8 +1345,9 @@ int gs_decode_backward(const void* x, const void* dy, int dtype, int64_t n, int 
     return set_error(GS_ERR_INVALID_ARG, "gs_decode_backward: give all weight gradients or none");
   if (!weights && !dx) return GS_OK;
   cudaStream_t s = as_stream(stream);
-  const int64_t fd = (int64_t)f * d, cf = (int64_t)c * f;
+  const int chunks = (f + kChunk - 1) / kChunk;
   int splits = 0;
+  bool wide = false;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (n > 0) {
     if (!x || !dy) return set_error(GS_ERR_INVALID_ARG, "gs_decode_backward: NULL pointer");
@@ -1342,19 +1368,23 @@ int gs_decode_backward(const void* x, const void* dy, int dtype, int64_t n, int 
     }
     if (!weights) return GS_OK;
     splits = decode_splits(n, f);
-    a.partials = reinterpret_cast<float*>(ws);
+    a.partials = ws;
+    a.wide = wide = decode_wide(n, f);
     if (int e = launch_decode<kDw>(a, dtype, dim3((unsigned)splits, (unsigned)a.chunks), s)) return e;
   }
   if (!weights) return GS_OK;
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(2 * fd + cf, 256), 148 * 8);
-  const float* part = reinterpret_cast<const float*>(ws);
-  if (dtype == GS_F16)
-    k_decode_reduce<__half><<<grid, 256, 0, s>>>(part, splits, fd, cf, static_cast<__half*>(d_gate),
-                                                 static_cast<__half*>(d_up), static_cast<__half*>(d_down));
-  else
-    k_decode_reduce<__nv_bfloat16><<<grid, 256, 0, s>>>(part, splits, fd, cf, static_cast<__nv_bfloat16*>(d_gate),
-                                                        static_cast<__nv_bfloat16*>(d_up),
-                                                        static_cast<__nv_bfloat16*>(d_down));
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div((int64_t)chunks * dw_columns(d, c) * kTile, 256), 148 * 8);
+  auto reduce = [&](auto zero, const auto* part) {
+    using T = decltype(zero);
+    k_decode_reduce<<<grid, 256, 0, s>>>(part, splits, chunks, d, f, c, static_cast<T*>(d_gate), static_cast<T*>(d_up),
+                                         static_cast<T*>(d_down));
+  };
+  auto reduce_as = [&](auto zero) {
+    if (wide) reduce(zero, reinterpret_cast<const double*>(ws));
+    else reduce(zero, reinterpret_cast<const float*>(ws));
+  };
+  if (dtype == GS_F16) reduce_as(__half{});
+  else reduce_as(__nv_bfloat16{});
   return check_launch("k_decode_reduce");
 }
 

@@ -263,3 +263,39 @@ def test_offsets_beyond_32_bits():
     own = decode_features(tail, wg, wu, wd)
     assert torch.equal(y.detach()[-999:], own.detach())
     assert torch.equal(dx[-999:], torch.autograd.grad(own, tail, dy[-999:])[0])
+
+
+def test_weight_gradients_of_like_signed_sums():
+    """One CTA sums 16384 equal tiles of positive terms: the sums must not drift away from 16384 times one tile's.
+
+    A matrix instruction takes 2^-22.2 of a float32 accumulator away, 8 instructions a tile, sums of at most 256 tiles
+    in a row: 256 * 8 / 2 * 2^-22.2 = 2.1e-4 < 2^-12, always in one direction.  Rounding the results to float16
+    averages out over thousands of elements; a single one is off by half a step (2^-11) on either side besides."""
+    d, f, c, times = 8, 4800, 8, 16384
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda lo, hi, *s: (torch.rand(s, device="cuda", generator=g) * (hi - lo) + lo).half()  # noqa: E731
+    x = rnd(0.5, 1.0, 128, d)
+    leaves = [w.requires_grad_(True) for w in (rnd(0.1, 0.2, f, d), rnd(0.1, 0.2, f, d), rnd(0.1, 0.2, c, f))]
+    dy = rnd(0.5, 1.5, 128, c) * 2.0 ** -10
+    one = torch.autograd.grad(decode_features(x, *leaves), leaves, dy)
+    all_ = torch.autograd.grad(decode_features(x.repeat(times, 1), *leaves), leaves, dy.repeat(times, 1))
+    for a, b in zip(all_, one):
+        off = a.double() / (times * b.double()) - 1.0
+        assert abs(float(off.mean())) <= 2.0 ** -12 + 2.0 ** -16
+        assert float(off.abs().max()) <= 2.0 ** -12 + 2 * 2.0 ** -11 + 2.0 ** -16
+    assert _wait_failures() == 0
+
+
+def test_weight_gradients_of_long_walks():
+    """Every tile of a walk of more than 256 counts once: first, around the places where sums leave TMEM, last."""
+    n, d, f, c = 128 * 1600 + 77, 40, 4800, 24
+    x, wg, wu, wd, dy = _inputs(n, d, f, c, "bf16", seed=3)
+    leaves = [w.requires_grad_(True) for w in (wg, wu, wd)]
+    for tile in (0, 255, 256, 257, 511, 512, 1023, 1024, 1300, 1599, 1600):
+        rows = slice(128 * tile, min(n, 128 * (tile + 1)))
+        only = torch.zeros_like(dy)
+        only[rows] = dy[rows]
+        got = torch.autograd.grad(decode_features(x, *leaves), leaves, only)
+        want = torch.autograd.grad(decode_features(x[rows], *leaves), leaves, dy[rows])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), tile
+    assert _wait_failures() == 0
