@@ -13,6 +13,7 @@ from ctypes import POINTER, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgsplat_b200.so"
 
@@ -299,6 +300,16 @@ def require_float(name: str, t: torch.Tensor) -> torch.Tensor:
     if not t.is_floating_point():
         raise TypeError(f"{name} must be a floating-point tensor (got {t.dtype})")
     return require_cuda(name, t, t.dtype if t.dtype in DTYPES else torch.float32)
+
+
+def differentiated(*tensors: torch.Tensor) -> bool:
+    """Whether autograd has to see a call on ``tensors``.  A forward-mode tangent
+    does not show in ``requires_grad``: while a dual level is open every call
+    goes to autograd, which refuses inputs that carry one (there are no
+    forward-mode derivatives)."""
+    if forward_ad._current_level >= 0:
+        return True
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
 
 
 def same_device(device: torch.device, **tensors) -> None:

@@ -228,7 +228,7 @@ class _Distill(torch.autograd.Function):
 
 def distill_loss(logits: torch.Tensor, teacher, temperature: float = 1.0, weight: torch.Tensor | None = None,
                  reduction: str = "mean") -> torch.Tensor:
-    """Distillation from a teacher's largest logits; differentiable in ``logits``.
+    """Distillation from a teacher's largest logits; differentiable (reverse mode) in ``logits``.
 
     ``logits`` (..., C), float32, float16 or bfloat16: class logits of rendered pixels (for instance
     ``render_features(...)["logits"]``).  ``teacher`` is ``(values, index)``, both (..., K) with K <= 256, or
@@ -242,7 +242,7 @@ def distill_loss(logits: torch.Tensor, teacher, temperature: float = 1.0, weight
     or "none" (a float32 loss per row).  With float16 logits take "sum": a mean's gradients, of the order of
     1 / rows, fall below float16's range.  No gradient flows to the teacher or to ``weight``."""
     args = _DistillArgs(logits, teacher, temperature, weight, reduction)
-    if torch.is_grad_enabled() and args.logits.requires_grad:
+    if nat.differentiated(args.logits):
         return _Distill.apply(args.logits, args)
     return args.run(args.logits)
 

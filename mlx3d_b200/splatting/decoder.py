@@ -76,7 +76,7 @@ class _Decode(torch.autograd.Function):
 
 def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
                     activation: str = "silu") -> torch.Tensor:
-    """``(act(x w_gate^T) * (x w_up^T)) w_down^T`` per pixel; differentiable in all four tensors.
+    """``(act(x w_gate^T) * (x w_up^T)) w_down^T`` per pixel; differentiable (reverse mode) in all four tensors.
 
     ``features`` (..., D) with D <= 128, ``w_gate`` and ``w_up`` (F, D), ``w_down`` (C, F) with C <= 256; the
     weights are all float16 or all bfloat16 and set the type of the computation: features of another floating
@@ -116,8 +116,7 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
     flat = len(lead) == 1
     if not flat:
         x = x.reshape(-1, d)
-    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad
-                                    or w_down.requires_grad):
+    if nat.differentiated(x, w_gate, w_up, w_down):
         y = _Decode.apply(x, w_gate, w_up, w_down, act)
     else:
         y = _forward(x, w_gate, w_up, w_down, act)[0]

@@ -6,6 +6,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from feature_helpers import decode64, distill64
 from mlx3d_b200 import _native as nat
@@ -230,3 +231,13 @@ def test_plain_decoder_gradients_against_differences(act):
             t.view(-1)[i] = keep
             # third derivatives are below 1e3 here: remainder 2e-10; cancellation 2^-52 * 100 / h = 2e-8
             assert abs(float((up - down) / (2 * h) - grad.view(-1)[i])) < 1e-7
+
+
+def test_differentiated_sees_leaves_and_tangents():
+    a, leaf = torch.zeros(3), torch.zeros(3, requires_grad=True)
+    assert not nat.differentiated(a) and nat.differentiated(a, leaf)
+    with torch.no_grad():
+        assert not nat.differentiated(leaf)
+        with fwAD.dual_level():
+            assert nat.differentiated(fwAD.make_dual(a, torch.ones(3)))
+    assert not nat.differentiated(a)

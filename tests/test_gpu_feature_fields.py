@@ -5,6 +5,7 @@ import threading
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 from feature_helpers import distill64
 from helpers import random_scene
@@ -139,3 +140,33 @@ def test_calls_of_several_threads_at_once():
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+def test_forward_mode_is_refused():
+    """There are no forward-mode derivatives: a tangent must not get lost on the way."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=g)  # noqa: E731
+    for n in (5, 300):  # both ways of decoding
+        args = [rnd(n, 8).bfloat16(), rnd(16, 8).bfloat16(), rnd(16, 8).bfloat16(), rnd(4, 16).bfloat16()]
+        logits, teacher = rnd(n, 4), (rnd(n, 2), torch.zeros((n, 2), device="cuda", dtype=torch.int32))
+        want = decode_features(*args), distill_loss(logits, teacher)
+        with fwAD.dual_level():
+            assert torch.equal(decode_features(*args), want[0])  # no tangents: as ever
+            assert torch.equal(distill_loss(logits, teacher), want[1])
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad):
+                    for at in range(4):
+                        dual = [fwAD.make_dual(t, torch.ones_like(t)) if i == at else t for i, t in enumerate(args)]
+                        with pytest.raises(NotImplementedError, match="forward mode"):
+                            decode_features(*dual)
+                    with pytest.raises(NotImplementedError, match="forward mode"):
+                        distill_loss(fwAD.make_dual(logits, torch.ones_like(logits)), teacher)
+
+
+def test_calls_without_gradients_bypass_autograd():
+    x, w = torch.zeros((3, 8), device="cuda").bfloat16(), torch.zeros((16, 8), device="cuda").bfloat16()
+    down = torch.zeros((4, 16), device="cuda").bfloat16()
+    assert not decode_features(x, w, w, down).requires_grad
+    assert decode_features(x, w.clone().requires_grad_(True), w, down).requires_grad
+    with torch.no_grad():
+        assert not decode_features(x, w.clone().requires_grad_(True), w, down).requires_grad
