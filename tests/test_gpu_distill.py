@@ -2,6 +2,7 @@
 
 import ctypes
 import math
+from fractions import Fraction
 
 import pytest
 import torch
@@ -446,3 +447,28 @@ def test_gradients_off_their_vectors(n, c, dtype):
                  None, 1, loss.data_ptr(), None, out.data_ptr(), None, 0, nat.stream())
         assert torch.equal(loss, want_l) and torch.equal(out, want_g)
     assert flat[0] == 5.0 and (flat[1 + n * c:] == 5.0).all()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("rows", [3, 5001])  # both ways of writing
+def test_codes_next_to_a_border_by_far_less_than_64_bits_hold(rows, dtype, bits):
+    """The quotients of the exact differences decide: halves go to the even code, less than a half does not."""
+    tiny = {"fp32": 2.0 ** -149, "bf16": 2.0 ** -133}[dtype]
+    line = []
+    for big in (1.0, 2.0 ** 127, 2.0 ** -60):
+        for mid in (0.0, tiny, -tiny, 2.0 ** -100, -(2.0 ** -100)):
+            line.append([big, mid, -big])
+            line.append([big, mid + big / 2, -big])  # (on the code's own value: far from a border)
+    z = torch.tensor(line, device="cuda", dtype=torch.float64).to(DTYPES[dtype])
+    z = z.repeat((rows + len(line) - 1) // len(line), 1)[:rows] if rows > 3 else z
+    cache = TeacherCache(z.shape[0], 3, 3, bits=bits)
+    cache.write(0, z)
+    levels = 2 ** bits - 1
+    at = 8 + 2 * 3
+    codes = cache.records[:, at:at + (3 * bits + 7) // 8].cpu()
+    for r in range(min(z.shape[0], len(line))):
+        first, mid, last = (Fraction(float(v)) for v in z[r].cpu())
+        want = round((first - mid) * levels / (first - last))  # (halves to even)
+        got = int(codes[r, 1]) if bits == 8 else int(codes[r, 0]) >> 4
+        assert got == want, (r, z[r].tolist())
