@@ -464,7 +464,8 @@ int gs_distill(const void* logits, int dtype, int64_t n, int64_t classes, const 
  * gs_teacher_write fills records [first_row, first_row + n) from logits
  * (n, classes), contiguous, of type dtype: the largest first, ties to the
  * lowest index; +-inf, NaN and the type's lowest value are never taken.
- *   scale = (z_1 - z_last) / (2^bits - 1), code_k = the quotient
+ *   scale = (z_1 - z_last) / (2^bits - 1) (the next smaller float where the last
+ *   code's value would not be finite), code_k = the quotient
  *   (2^bits - 1) (z_1 - z_k) / (z_1 - z_last) rounded to nearest, ties to
  *   even (the quotient of the exact differences).
  * gs_teacher_read writes values (n, k) float (-inf where absent) and index

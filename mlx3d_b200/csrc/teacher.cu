@@ -139,11 +139,14 @@ struct Quantiser {
   }
 };
 // (first - last) / levels, rounded once: the 64-bit product with 1 / levels, corrected
-// by its remainder.
+// by its remainder.  Where rounding up would take the last code's value out of float32's
+// range, which stands for an absent entry, the step below.
 __device__ __forceinline__ float step_of(float first, float last, int bits) {
   const double span = (double)first - (double)last, levels = (double)((1 << bits) - 1);
   const double inv = bits == 8 ? 1.0 / 255.0 : 1.0 / 15.0, q = span * inv;
-  return (float)__fma_rn(__fma_rn(-q, levels, span), inv, q);
+  const float step = (float)__fma_rn(__fma_rn(-q, levels, span), inv, q);
+  const bool lost = record_value(first, step, (1 << bits) - 1) == -INFINITY;
+  return __uint_as_float(__float_as_uint(step) - (lost ? 1u : 0u));
 }
 
 template <typename W>

@@ -472,3 +472,22 @@ def test_codes_next_to_a_border_by_far_less_than_64_bits_hold(rows, dtype, bits)
         want = round((first - mid) * levels / (first - last))  # (halves to even)
         got = int(codes[r, 1]) if bits == 8 else int(codes[r, 0]) >> 4
         assert got == want, (r, z[r].tolist())
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("rows", [2000, 5000])  # both ways of writing
+def test_write_the_whole_range_of_float32(rows, bits):
+    """From next to the largest float32 to next to the lowest: nothing that is kept reads as absent."""
+    big = torch.finfo(torch.float32).max
+    z = torch.zeros((rows, 3), device="cuda")
+    z[:, 0] = (big - torch.arange(rows, device="cuda", dtype=torch.float64) * 2.0 ** 105).float()
+    z[:, 2] = -(big - 2.0 ** 104)  # the lowest value that is kept
+    cache = TeacherCache(rows, 3, 3, bits=bits)
+    cache.write(0, z)
+    values, index = cache.read(slice(None))
+    assert (index == torch.arange(3, device="cuda")).all()
+    assert torch.equal(values[:, 0], z[:, 0])
+    # the step's half a rounding (or one, where it was taken down), 2^bits - 1 times; the value's own half
+    tol = z[:, 0].double() * 2 * (2.0 ** -23 + 2.0 ** -24)
+    assert ((values[:, 2].double() - z[:, 2].double()).abs() <= tol).all()
+    assert torch.isfinite(values).all()
