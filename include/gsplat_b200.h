@@ -432,6 +432,8 @@ typedef struct gs_teacher {
   int32_t bits; /* 8 or 4: cache; 0: arrays */
 } gs_teacher;
 #define GS_DISTILL_MAX_CLASSES 2147483631
+#define GS_DISTILL_MIN_TEMPERATURE 1e-18f
+#define GS_DISTILL_MAX_TEMPERATURE 1e18f
 #define GS_TEACHER_MAX_K 256
 #define GS_CACHE_MAX_K 32
 #define GS_CACHE_MAX_CLASSES 32767
@@ -443,7 +445,8 @@ typedef struct gs_teacher {
  *   L = weight T^2 sum_k p_k (log p_k - log q_{i_k})
  *   dL/ds_c = weight T (q_c - sum_{k: i_k = c} p_k)
  * (0 log 0 = 0; a row without entries has L = 0 and gradient 0; weight (n) or
- * NULL for 1.)  Writes what is not NULL of
+ * NULL for 1; T from GS_DISTILL_MIN_TEMPERATURE to GS_DISTILL_MAX_TEMPERATURE,
+ * as T^2 is a 32-bit factor.)  Writes what is not NULL of
  *   row_loss (n)   L
  *   loss     (1)   scale * sum L, summed in a fixed order in 64 bits
  *   grad     (n, classes) of type dtype: g * scale * dL/ds, with g = 1 if

@@ -72,6 +72,8 @@ GS_ADAM_MAX_GROUPS = 8
 # Element types of the feature-field entry points.
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 GS_DISTILL_MAX_CLASSES = 2147483631
+GS_DISTILL_MIN_TEMPERATURE = 1e-18
+GS_DISTILL_MAX_TEMPERATURE = 1e18
 GS_TEACHER_MAX_K = 256
 GS_CACHE_MAX_K = 32
 GS_CACHE_MAX_CLASSES = 32767

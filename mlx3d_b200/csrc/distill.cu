@@ -840,8 +840,10 @@ int gs_distill(const void* logits, int dtype, int64_t n, int64_t classes, const 
   const int max_k = cached ? GS_CACHE_MAX_K : GS_TEACHER_MAX_K;
   if (teacher->k < 1 || teacher->k > max_k)
     return set_error(GS_ERR_INVALID_ARG, "gs_distill: k must be in [1, %d] (got %d)", max_k, teacher->k);
-  if (!(temperature > 0.0f) || temperature > FLT_MAX || 1.0f / temperature > FLT_MAX)
-    return set_error(GS_ERR_INVALID_ARG, "gs_distill: temperature must be positive and finite");
+  // The loss has the factor T^2, the exponents 1 / T: both must be normal float32 numbers.
+  if (!(temperature >= GS_DISTILL_MIN_TEMPERATURE && temperature <= GS_DISTILL_MAX_TEMPERATURE))
+    return set_error(GS_ERR_INVALID_ARG, "gs_distill: temperature must be in [%g, %g]", GS_DISTILL_MIN_TEMPERATURE,
+                     GS_DISTILL_MAX_TEMPERATURE);
   if (cached) {
     if (teacher->bits != 8 && teacher->bits != 4)
       return set_error(GS_ERR_INVALID_ARG, "gs_distill: bits must be 8 or 4 (got %d)", teacher->bits);

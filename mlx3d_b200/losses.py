@@ -137,8 +137,9 @@ class _DistillArgs:
         if reduction not in ("mean", "sum", "none"):
             raise ValueError("reduction must be 'mean', 'sum' or 'none'.")
         temperature = float(temperature)
-        if not (temperature > 0.0 and math.isfinite(temperature)):
-            raise ValueError("temperature must be positive and finite.")
+        if not nat.GS_DISTILL_MIN_TEMPERATURE <= temperature <= nat.GS_DISTILL_MAX_TEMPERATURE:
+            raise ValueError(f"temperature must be in [{nat.GS_DISTILL_MIN_TEMPERATURE:g}, "
+                             f"{nat.GS_DISTILL_MAX_TEMPERATURE:g}].")
         if not isinstance(logits, torch.Tensor) or logits.ndim < 1 or logits.shape[-1] < 1:
             raise ValueError("logits must have shape (..., C) with C >= 1.")
         lead = logits.shape[:-1]
@@ -237,8 +238,8 @@ def distill_loss(logits: torch.Tensor, teacher, temperature: float = 1.0, weight
 
         L = weight * T^2 * sum_k p_k (log p_k - log q[index_k])
 
-    An entry whose index is outside [0, C) or whose value is -inf is absent; a row without entries (an unlabelled
-    pixel) has loss and gradient 0.  Entries of one class add up.  ``reduction`` is "mean" (over all rows), "sum"
+    with 1e-18 <= T <= 1e18 (T^2 is a 32-bit factor).  An entry whose index is outside [0, C) or whose value is
+    -inf is absent; a row without entries (an unlabelled pixel) has loss and gradient 0.  Entries of one class add up.  ``reduction`` is "mean" (over all rows), "sum"
     or "none" (a float32 loss per row).  With float16 logits take "sum": a mean's gradients, of the order of
     1 / rows, fall below float16's range.  No gradient flows to the teacher or to ``weight``."""
     args = _DistillArgs(logits, teacher, temperature, weight, reduction)

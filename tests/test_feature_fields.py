@@ -241,3 +241,21 @@ def test_differentiated_sees_leaves_and_tangents():
         with fwAD.dual_level():
             assert nat.differentiated(fwAD.make_dual(a, torch.ones(3)))
     assert not nat.differentiated(a)
+
+
+def test_temperatures_whose_square_is_no_normal_number_are_refused():
+    """T^2 would be 0 or infinite in 32 bits and the loss 0 or NaN instead of its value."""
+    lib, (v, i) = nat.load(), _teacher()
+    for t in (1e-39, 3e-39, 1e-30, 1e-23, 9e-19, 1.1e18, 2e19, 1e30, 3e38):
+        for fn in (distill_loss, distill_loss_and_grad):
+            with pytest.raises(ValueError, match="temperature"):
+                fn(torch.zeros(3, 5), (v, i), temperature=t)
+        status = lib.gs_distill(None, 0, 2, 5, ctypes.byref(_native_teacher()), t, None, 1.0, None, 0, None, None, None,
+                                None, 0, None)
+        assert status == nat.GS_ERR_INVALID_ARG and b"temperature" in lib.gs_last_error()
+    for t in (1e-18, 1e18):  # the limits are allowed (and refused for the CPU tensor)
+        with pytest.raises(ValueError, match="CUDA"):
+            distill_loss(torch.zeros(3, 5), (v, i), temperature=t)
+        lib.gs_distill(None, 0, 2, 5, ctypes.byref(_native_teacher()), t, None, 1.0, None, 0, None, None, None, None, 0,
+                       None)
+        assert b"NULL" in lib.gs_last_error()

@@ -491,3 +491,12 @@ def test_write_the_whole_range_of_float32(rows, bits):
     tol = z[:, 0].double() * 2 * (2.0 ** -23 + 2.0 ** -24)
     assert ((values[:, 2].double() - z[:, 2].double()).abs() <= tol).all()
     assert torch.isfinite(values).all()
+
+
+@pytest.mark.parametrize("t", [1e-18, 1e-9, 1e9, 1e18])
+@pytest.mark.parametrize("c,k", [(20, 5), (401, 9), (5001, 40)])
+def test_temperatures_far_from_one(c, k, t):
+    s, v, i, w = _inputs(70, c, k, "fp32", "fp32", seed=c)
+    t = float(torch.tensor(t))  # as the kernels have it
+    loss, grad = distill_loss_and_grad(s * t, (v * t, i), temperature=t, weight=w, reduction="none")
+    _check(s * t, v * t, i, w, t, loss, grad)
