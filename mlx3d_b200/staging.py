@@ -121,8 +121,11 @@ class TeacherCache:
             raise ValueError(f"device must be a CUDA device (got {device}); mlx3d_b200 has no CPU path")
         self.num_rows, self.k, self.num_classes, self.bits = rows, k, num_classes, int(bits)
         self.record_bytes = int(nat.load().gs_teacher_record_bytes(k, self.bits))
-        self.records = torch.zeros((rows, self.record_bytes), dtype=torch.uint8, device=device)
-        self.records[:, 8:8 + 2 * k] = 255  # index -1: absent
+        # An ordinary tensor even where the cache is made beside a teacher that runs in inference mode: losses save
+        # it for their backward.
+        with torch.inference_mode(False):
+            self.records = torch.zeros((rows, self.record_bytes), dtype=torch.uint8, device=device)
+            self.records[:, 8:8 + 2 * k] = 255  # index -1: absent
         self.device = self.records.device
 
     def __len__(self) -> int:

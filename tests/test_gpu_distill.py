@@ -500,3 +500,21 @@ def test_temperatures_far_from_one(c, k, t):
     t = float(torch.tensor(t))  # as the kernels have it
     loss, grad = distill_loss_and_grad(s * t, (v * t, i), temperature=t, weight=w, reduction="none")
     _check(s * t, v * t, i, w, t, loss, grad)
+
+
+def test_cache_made_in_inference_mode():
+    """The teacher runs in inference mode, the student trains: the cache serves both."""
+    s = torch.randn((6, 9), device="cuda", requires_grad=True)
+    with torch.inference_mode():
+        cache = TeacherCache(6, 3, 9)
+        cache.write(0, torch.randn((6, 9), device="cuda", generator=_gen(1)))
+        saved = cache.state_dict()
+    want, want_g = distill_loss_and_grad(s.detach(), cache.read(slice(None)))
+    loss = distill_loss(s, cache.at(slice(0, 6)))
+    loss.backward()
+    assert torch.equal(loss.detach(), want) and torch.equal(s.grad, want_g)
+    loss = distill_loss(s, cache.at(slice(0, 6)))
+    with torch.inference_mode():
+        cache.load_state_dict(saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
