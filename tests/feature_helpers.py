@@ -136,3 +136,18 @@ def decode_tolerances(x, w_gate, w_up, w_down, act, dy=None):
     out.append(edu.T @ ax + acc_n * (mdu.T @ ax) + e * dwu.abs() + sub)
     out.append(ady.T @ (eh + sub) + acc_n * (ady.T @ (a * u.abs())) + e * dwd.abs() + sub)
     return out
+
+
+def decode_norm_bound(dtype) -> float:
+    """Bound of |error| / |value| (Frobenius norms) of y and of each gradient, for rows of random signs.
+
+    Every term of a sum has one factor rounded to 16 bits, by at most half a step e of itself, e / sqrt(3) in the root
+    mean square, independently; so has every sum at the end.  Terms of random signs add up like their errors: the
+    ratio of the norms is at most e sqrt(2 / 3), with what float32 accumulators lose (2.1e-4 of a stretch of like
+    signs, far less here) below e.  Twice that is allowed.  A walk that loses one tile of 128 rows out of n is off by
+    sqrt(128 / n)."""
+    return 2 * half_step(dtype)
+
+
+def norm_off(got, want) -> float:
+    return float((got.double() - want.double()).norm() / want.double().norm())

@@ -8,7 +8,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from feature_helpers import decode64, distill64
+from feature_helpers import DTYPES, decode64, decode_norm_bound, distill64, norm_off
 from mlx3d_b200 import _native as nat
 from mlx3d_b200.losses import distill_loss, distill_loss_and_grad
 from mlx3d_b200.splatting import FeatureDecoder, decode_features
@@ -259,3 +259,23 @@ def test_temperatures_whose_square_is_no_normal_number_are_refused():
         lib.gs_distill(None, 0, 2, 5, ctypes.byref(_native_teacher()), t, None, 1.0, None, 0, None, None, None, None, 0,
                        None)
         assert b"NULL" in lib.gs_last_error()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,d,f,c", [(20001, 33, 70, 31), (60001, 16, 24, 9)])
+def test_norm_bound_tells_a_lost_tile(n, d, f, c, dtype):
+    """Planted in the plain form: gradients without one tile, the first, a middle or the ragged last one, or with a
+    tile counted twice, are out of the bound the GPU tests use; gradients rounded as the kernels round are within."""
+    g = torch.Generator().manual_seed(7)
+    ty = DTYPES[dtype]
+    r = lambda *s: torch.randn(*s, generator=g).to(ty)  # noqa: E731
+    x, wg, wu, wd, dy = r(n, d), r(f, d) / d ** 0.5, r(f, d) / d ** 0.5, r(c, f) / f ** 0.5, r(n, c)
+    full = decode64(x, wg, wu, wd, "silu", dy)[2:]
+    bound = decode_norm_bound(ty)
+    for w in full:
+        assert norm_off(w.to(ty), w) <= bound / 2
+    for tile in (0, n // 256, n // 128):
+        rows = slice(128 * tile, min(n, 128 * tile + 128))
+        part = decode64(x[rows], wg, wu, wd, "silu", dy[rows])[2:]
+        for w, p in zip(full, part):
+            assert norm_off(w - p, w) > 2 * bound and norm_off(w + p, w) > 2 * bound

@@ -7,7 +7,7 @@ import threading
 import pytest
 import torch
 
-from feature_helpers import DTYPES, decode64, decode_tolerances
+from feature_helpers import DTYPES, decode64, decode_norm_bound, decode_tolerances, norm_off
 from mlx3d_b200 import _native as nat
 from mlx3d_b200.splatting import FeatureDecoder, decode_features
 
@@ -299,3 +299,79 @@ def test_weight_gradients_of_long_walks():
         want = torch.autograd.grad(decode_features(x[rows], *leaves), leaves, dy[rows])
         assert all(torch.equal(a, b) for a, b in zip(got, want)), tile
     assert _wait_failures() == 0
+
+
+LONG = [(20001, 33, 70, 31), (40000, 64, 128, 150), (60001, 64, 256, 152), (60001, 64, 256, 128), (60001, 128, 256, 256),
+        (60001, 40, 1100, 24), (60001, 128, 64, 200)]
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,d,f,c", LONG)
+def test_gradients_of_many_tiles_by_norm(n, d, f, c, dtype, act):
+    """Bounds element by element grow with n, the gradients with its root: by norm, one lost tile shows."""
+    x, wg, wu, wd, dy = _inputs(n, d, f, c, dtype, seed=n + f)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = decode_features(*leaves, act)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    want = decode64(*(t.detach() for t in leaves), act, dy)
+    for a, b in zip(got, want):
+        assert norm_off(a, b) <= decode_norm_bound(a.dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("n,d,f,c", LONG)
+def test_every_tile_of_a_walk_counts_once(n, d, f, c, dtype):
+    """All of dy but one tile is zero: the weights' gradients are those of a call on that tile alone (the other tiles
+    add exact zeros), wherever it lies in its CTA's walk."""
+    x, wg, wu, wd, dy = _inputs(n, d, f, c, dtype, seed=n + c)
+    x = torch.randn((n, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(n)).to(x.dtype)
+    leaves = [w.requires_grad_(True) for w in (wg, wu, wd)]
+    y = decode_features(x, *leaves)
+    chunks, tiles = (f + 63) // 64, (n + 127) // 128
+    splits = 148 // chunks
+    for tile in {0, 1, splits - 1, splits, 2 * splits + 1, tiles // 2, tiles - splits, tiles - 2, tiles - 1}:
+        if not 0 <= tile < tiles:
+            continue
+        rows = slice(128 * tile, min(n, 128 * (tile + 1)))
+        only = torch.zeros_like(dy)
+        only[rows] = dy[rows]
+        got = torch.autograd.grad(y, leaves, only, retain_graph=True)
+        want = torch.autograd.grad(decode_features(x[rows], *leaves), leaves, dy[rows])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), tile
+        assert all((w != 0).any() for w in want)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_one_feature_vector(dtype, act):
+    x, wg, wu, wd, _ = _inputs(600, 24, 50, 11, dtype, seed=4)
+    for row in (77, 599):  # covered pixels
+        one = x[row]
+        assert (one != 0).all()
+        y = decode_features(one, wg, wu, wd, act)
+        assert y.shape == (11,) and (y != 0).any()
+        _within(y, decode64(one[None], wg, wu, wd, act)[0], decode_tolerances(one[None], wg, wu, wd, act)[0])
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_large_gates_in_many_rows(act):
+    """As many rows as the matrix kernels take: gates of 300 and -300, bf16, every output and gradient."""
+    n = 300
+    sign = torch.ones((n, 1), device="cuda", dtype=torch.bfloat16)
+    sign[1::3], sign[2::3] = -1.0, 0.0
+    x = (300.0 * sign).requires_grad_(True)
+    one = lambda: torch.ones((1, 1), device="cuda", dtype=torch.bfloat16).requires_grad_(True)  # noqa: E731
+    wg, wu, wd = one(), one(), one()
+    y = decode_features(x, wg, wu, wd, act)
+    grads = torch.autograd.grad(y, (x, wg, wu, wd), torch.ones_like(y))
+    up = sign[:, 0] > 0
+    assert (y[up, 0] == 90112.0).all() and (y[~up] == 0).all()  # 300^2 rounded to bf16
+    # up: h = 90000 (bf16 90112), dg = u = 300, du = 300; below and at zero nothing is left
+    assert (grads[0][up] == 600.0).all() and (grads[0][~up] == 0).all()
+    # Sums of 100 rows are whole numbers below 2^24, exact in 32 bits, and rounded once: 9000000 lies between 137 and
+    # 138 steps of 2^16 (bf16 has 8 bits), nearer the first, 8978432, off by 2.4e-3 <= 2^-8.
+    rows = int(up.sum())
+    want = [300.0 * 300.0 * rows, 300.0 * 300.0 * rows, 90112.0 * rows]
+    for g, w in zip(grads[1:], want):
+        assert float(g.detach()) == float(torch.tensor(w).bfloat16())
