@@ -518,3 +518,25 @@ def test_cache_made_in_inference_mode():
         cache.load_state_dict(saved)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("off", [0, 1])
+@pytest.mark.parametrize("dtype,sizes", [
+    ("fp32", (319, 320, 321, 508, 509, 510, 511, 512, 1020, 1021, 1022, 1532, 1533, 1534)),
+    ("fp16", (511, 512, 513, 639, 640, 641, 1016, 1017, 1018, 2040, 2041, 2042, 3063, 3064, 3065, 3066, 3067)),
+    ("bf16", (511, 512, 513, 640, 641, 1017, 1018, 2041, 2042, 3064, 3065, 3066)),
+])
+def test_both_sides_of_every_limit_of_long_rows(dtype, sizes, off):
+    """The last and first row lengths of the tiles, of 4, 8 and 12 units a lane, of a block a row; logits on a 16-byte
+    boundary and one element off it."""
+    for c in sizes:
+        n, k = 70, 9
+        s, v, i, w = _inputs(n, c, k, dtype, dtype, seed=c)
+        if off:
+            flat = torch.zeros((n * c + 1,), device="cuda", dtype=s.dtype)
+            flat[1:] = s.reshape(-1)
+            s = flat[1:].view(n, c)
+        loss, grad = distill_loss_and_grad(s, (v, i), weight=w, reduction="none")
+        _check(s, v, i, w, 1.0, loss, grad)
+        alone = distill_loss(s, (v, i), weight=w, reduction="none")
+        assert torch.equal(alone, loss)
