@@ -1072,8 +1072,8 @@ static int check_image(const char* who, const void* image, size_t image_bytes, i
 }
 
 // Rows of `width` elements to rows of `padded` (a multiple of 8), zeros behind:
-// one thread per 16 bytes written, reading `PART` bytes at a time (the largest
-// power of two that divides a row and the address).
+// one thread per 16 bytes written, reading `Part`s, the largest of 2, 4 and 8 bytes
+// that divides a row and the address.
 template <typename Part>
 __global__ void k_pad_rows(const Part* __restrict__ src, int64_t n, int width, int per_row, uint4* __restrict__ dst) {
   constexpr int kParts = 16 / sizeof(Part), kElems = sizeof(Part) / 2;
@@ -1107,8 +1107,7 @@ static const void* fetchable_rows(const void* p, int64_t n, int width, uint8_t**
   const int per_row = round_up(width, 8) / 8;
   const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(n * per_row, 256), 148 * 64);
   const uintptr_t m = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(width * 2);
-  if (m % 16 == 0) k_pad_rows<uint4><<<grid, 256, 0, s>>>(static_cast<const uint4*>(p), n, width, per_row, out);
-  else if (m % 8 == 0) k_pad_rows<uint2><<<grid, 256, 0, s>>>(static_cast<const uint2*>(p), n, width, per_row, out);
+  if (m % 8 == 0) k_pad_rows<uint2><<<grid, 256, 0, s>>>(static_cast<const uint2*>(p), n, width, per_row, out);
   else if (m % 4 == 0) k_pad_rows<uint32_t><<<grid, 256, 0, s>>>(static_cast<const uint32_t*>(p), n, width, per_row, out);
   else k_pad_rows<uint16_t><<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(p), n, width, per_row, out);
   return out;

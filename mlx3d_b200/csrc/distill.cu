@@ -134,29 +134,28 @@ __device__ __forceinline__ void block_partial(double v, double* out) {
   }
 }
 
-// The teacher's side of a row by a group of G lanes: entries (index, z) become
-// (index, p); returns whether any is present (in every lane of the group).
+// The teacher's side of a row by a warp: entries (index, z) become
+// (index, p); returns whether any is present (in every lane).
 //   term = sum_k p_k ((z_k - max z) - (s_k - m)) / T - log sum_k exp((z_k - max z) / T)
 // so that the loss is T^2 (term + log sum_c exp((s_c - m) / T)), as sum_k p_k = 1.
-template <int G, typename Logit>
+template <typename Logit>
 __device__ __forceinline__ bool teacher_terms(float2* ent, int k, int lane, float m, float inv_temp, Logit logit,
                                               float& term) {
   const float c2 = inv_temp * kLog2e;
   float zmax = -INFINITY;
   bool mine = false;
-  for (int e = lane; e < k; e += G) {
+  for (int e = lane; e < k; e += 32) {
     mine |= __float_as_int(ent[e].x) >= 0;
     zmax = fmaxf(zmax, ent[e].y);
   }
-  const unsigned present = __ballot_sync(~0u, mine) & (G == 32 ? ~0u : ((1u << (G & 31)) - 1) << (threadIdx.x & 31 & ~(G - 1)));
-  zmax = group_max<G>(zmax);
+  zmax = group_max<32>(zmax);
   float tot = 0.0f;
-  for (int e = lane; e < k; e += G)
+  for (int e = lane; e < k; e += 32)
     if (__float_as_int(ent[e].x) >= 0) tot += exp2_of((ent[e].y - zmax) * c2);
-  tot = group_sum<G>(tot);
+  tot = group_sum<32>(tot);
   const float inv_tot = rcp_of(tot);
   float sum = 0.0f;
-  for (int e = lane; e < k; e += G) {
+  for (int e = lane; e < k; e += 32) {
     const int idx = __float_as_int(ent[e].x);
     float p = 0.0f;
     if (idx >= 0) {
@@ -166,16 +165,16 @@ __device__ __forceinline__ bool teacher_terms(float2* ent, int k, int lane, floa
     }
     ent[e].y = p;
   }
-  term = group_sum<G>(sum) - ln_of(tot);
-  return present != 0;
+  term = group_sum<32>(sum) - ln_of(tot);
+  return __any_sync(~0u, mine);
 }
 
 // Gradients of the teacher's classes, scaled: the first entry of a class holds
 // (class, f (q - sum of the class's p)), every other one (-1, -).
-template <int G, typename Logit>
+template <typename Logit>
 __device__ __forceinline__ void class_gradients(const float2* ent, float2* out, int k, bool repeats, int lane, float m,
                                                 float c2, float inv_sum, float f, Logit logit) {
-  for (int e = lane; e < k; e += G) {
+  for (int e = lane; e < k; e += 32) {
     const int idx = __float_as_int(ent[e].x);
     int to = -1;
     float g = 0.0f;
@@ -639,7 +638,7 @@ __global__ void __launch_bounds__(kLongBlock, UNITS == 4 ? 8 : UNITS == 8 && siz
     const float f = w * a.grad_scale * (a.cot ? a.cot[a.cot_per_row ? r : 0] : 1.0f);
     auto logit = [&](int i) { return to_f32(row.src[i]); };
     float term;
-    const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
+    const bool any = teacher_terms(ent, k, lane, m, a.inv_temp, logit, term);
     const float inv = rcp_of(sum);
     if (lane == 0) {
       const float loss = any ? (term + ln_of(sum)) * (a.temp * a.temp) * w : 0.0f;
@@ -655,7 +654,7 @@ __global__ void __launch_bounds__(kLongBlock, UNITS == 4 ? 8 : UNITS == 8 && siz
         const unsigned same = __match_any_sync(~0u, idx >= 0 ? idx : -1 - lane);
         repeats = __any_sync(~0u, (same & (same - 1)) != 0);
       }
-      class_gradients<32>(ent, fix, any ? k : 0, repeats, lane, m, c2, inv, f, logit);
+      class_gradients(ent, fix, any ? k : 0, repeats, lane, m, c2, inv, f, logit);
       const float qf = inv * f;
 #pragma unroll
       for (int i = 0; i < UNITS; ++i) {
@@ -721,10 +720,10 @@ __global__ void __launch_bounds__(kRowThreads) k_distill_row(DistillArgs a, int 
       sum = group_sum<32>(lane < kRowThreads / 32 ? red[lane] : 0.0f);
       auto logit = [&](int i) { return to_f32(row.src[i]); };
       float term;
-      const bool any = teacher_terms<32>(ent, k, lane, m, a.inv_temp, logit, term);
+      const bool any = teacher_terms(ent, k, lane, m, a.inv_temp, logit, term);
       __syncwarp();
       const float inv = rcp_of(sum);
-      if (a.grad) class_gradients<32>(ent, fix, any ? k : 0, true, lane, m, c2, inv, f, logit);
+      if (a.grad) class_gradients(ent, fix, any ? k : 0, true, lane, m, c2, inv, f, logit);
       if (lane == 0) {
         const float loss = any ? (term + ln_of(sum)) * (a.temp * a.temp) * w : 0.0f;
         if (a.row_loss) a.row_loss[r] = loss;
