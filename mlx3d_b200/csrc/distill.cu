@@ -148,6 +148,7 @@ __device__ __forceinline__ bool teacher_terms(float2* ent, int k, int lane, floa
     mine |= __float_as_int(ent[e].x) >= 0;
     zmax = fmaxf(zmax, ent[e].y);
   }
+  const unsigned present = __ballot_sync(~0u, mine);
   zmax = group_max<32>(zmax);
   float tot = 0.0f;
   for (int e = lane; e < k; e += 32)
@@ -166,7 +167,7 @@ __device__ __forceinline__ bool teacher_terms(float2* ent, int k, int lane, floa
     ent[e].y = p;
   }
   term = group_sum<32>(sum) - ln_of(tot);
-  return __any_sync(~0u, mine);
+  return present != 0;
 }
 
 // Gradients of the teacher's classes, scaled: the first entry of a class holds
