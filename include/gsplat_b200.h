@@ -484,13 +484,14 @@ int gs_teacher_read(const void* records, int64_t n_records, const int64_t* rows,
  * (pixels); x (n, d), Wg and Wu (f, d), Wd (c, f), y (n, c), all contiguous and
  * of one type, GS_F16 or GS_BF16.  1 <= d <= GS_DECODE_MAX_D, f >= 1,
  * 1 <= c <= GS_DECODE_MAX_C.  Products are summed in 32 bits; the hidden
- * values are rounded to the type as operands of the second product.
+ * values, and their gradients, are rounded to the type as operands of the
+ * second products.
  *
  * gs_decode_prepare lays the weights out for the kernels in `image`
  * (gs_decode_image_bytes, 16-byte aligned); forward and backward read only
  * that.  gs_decode_backward writes dx (n, d) unless NULL, and d_gate, d_up
  * (f, d), d_down (c, f) unless all three are NULL, from dy (n, c); sums over
- * rows are taken in a fixed order.
+ * rows are taken in a fixed order, in 64 bits past 32768 rows of one block.
  * gs_decode_workspace_bytes is the scratch (16-byte aligned) of a forward call
  * (dy NULL, weights 0) or a backward call (weights: whether the weight gradients
  * are wanted).  It depends on the alignment of x and dy: rows that are no

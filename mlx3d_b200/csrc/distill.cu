@@ -11,8 +11,9 @@
 //                   arithmetic.  The classes of a row are shared by 4 to 32 lanes;
 //                   the teacher's few entries by as many as make the tile's rows a
 //                   whole warp.  Instructions bound it: 1920x1080x150 in float32
-//                   takes 466 us (67% of DRAM's rate), with one lane per row for
-//                   the entries (8 of 32 busy) 536.
+//                   takes 492 us (its bytes at a copy's rate: 396) with 8 entries,
+//                   with one lane per row for the entries (8 of 32 busy) 15 % more.
+//                   More than 8 entries a row are compared pair by pair: 16 take 1251.
 //   k_distill_long  rows that fit in a warp's registers: one warp per row.
 //   k_distill_row   longer rows: one block per row.
 #include "feature_common.cuh"
@@ -799,9 +800,11 @@ static int launch_distill(const DistillArgs& a, cudaStream_t st, unsigned* block
   if (c <= 160) return launch_warps<T, 8, 20, 16, 2>(a, st, blocks);
   if (c <= 256) return launch_warps<T, 16, 16, 10, 4>(a, st, blocks);
   const bool alike = ((reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad)) & 15) == 0;
-  // Rows of little more than a kilobyte keep too few of a warp's loads in flight below:
-  // loss and gradient of 666667 rows of 300 in float16 take 376 us here, 1019 there; 500000
-  // of 400 in float32 701 here, 487 there.
+  // Rows of little more than a kilobyte keep too few of a warp's loads in flight below: loss
+  // and gradient of 666667 rows of 300 with 8 entries take 378 us here in float16, 990 there,
+  // in float32 607 and 609; 400000 rows of 500 in float32 486 here, 382 there.  (With 32
+  // entries, compared pair by pair here, 300 in float16 take 1336 and 1271, in float32 2038
+  // and 804.)
   if (c <= 512 && c * sizeof(T) <= 1280) return launch_warps<T, 16, 32, 16, 0>(a, st, blocks);
   // Longer rows that fit in a warp's registers from wherever they start.
   constexpr int kUnit = 16 / sizeof(T), kPerUnit = 32 * kUnit;

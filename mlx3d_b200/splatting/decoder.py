@@ -2,7 +2,7 @@
 
 Compositing cost grows with the number of feature channels, so a semantic
 scene carries few (16 to 128) and a small gated block per pixel turns them
-into class logits or a 2D network's features.  An addition to the reference,
+into class logits, or other values of a 2D network, 256 at most.  An addition to the reference,
 whose feature rendering (src/mlx3d/splatting/render.py:164-220) ends at the
 composited channels.
 """
@@ -81,8 +81,12 @@ def decode_features(features: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Te
     ``features`` (..., D) with D <= 128, ``w_gate`` and ``w_up`` (F, D), ``w_down`` (C, F) with C <= 256; the
     weights are all float16 or all bfloat16 and set the type of the computation: features of another floating
     type are rounded to it.  ``activation`` is "silu" or "gelu" (the error-function form).  Returns (..., C) in
-    the weights' type.  Products are summed in 32 bits and the hidden values are rounded once to the weights'
-    type; they stay on chip, forward and backward."""
+    the weights' type.
+
+    Products are summed in 32 bits.  The hidden values, and their gradients in the backward pass, are rounded to
+    the weights' type as operands of the next products (the forward of at most 64 rows of a small block keeps them
+    in 32 bits); they stay on chip.  In float16 a hidden value above 65504 becomes infinite and a hidden gradient
+    below 2^-25 zero: scale ``features`` and the loss accordingly, or take bfloat16."""
     act = nat.GS_GATES.get(activation)
     if act is None:
         raise ValueError("activation must be 'silu' or 'gelu'.")
