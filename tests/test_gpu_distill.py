@@ -540,3 +540,20 @@ def test_both_sides_of_every_limit_of_long_rows(dtype, sizes, off):
         _check(s, v, i, w, 1.0, loss, grad)
         alone = distill_loss(s, (v, i), weight=w, reduction="none")
         assert torch.equal(alone, loss)
+
+
+@pytest.mark.parametrize("k", [128, 255, 256])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_more_teacher_entries_than_classes(dtype, k):
+    """As many entries as there may be, most classes several times: the largest tiles, one warp a block."""
+    for c in (1, 5, 16, 17, 32, 33, 64, 96, 150, 256, 300, 700, 4001):
+        n = 100
+        s, v, i, w = _inputs(n, c, k, dtype, dtype, seed=c + k)
+        loss, grad = distill_loss_and_grad(s, (v, i), weight=w, reduction="none")
+        want_l, want_g = distill64(s, v, i, 1.0, w)
+        tol_l, rel = distill_tolerance(s, v, 1.0, k)
+        # the entries of one class are added one by one, and the row's on as few as one lane: k roundings more
+        tol_l, rel = tol_l + 2.0 ** -24 * k * (1 + tol_l / rel), rel + 2.0 ** -24 * k
+        assert ((loss.double() - want_l).abs() <= w * tol_l + 2.0 ** -22 * want_l.abs()).all()
+        tol = (w * 2 * rel)[:, None] + want_g.abs() * (half_step(s.dtype) + 2.0 ** -21)
+        assert ((grad.double() - want_g).abs() <= tol).all()
